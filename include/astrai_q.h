@@ -472,6 +472,53 @@ int aq_rope_prefill_attn_paged_ahead(const void *q, int64_t q_stride, const floa
                                      int64_t n_pages, void *out, float scale, int64_t B, int64_t S, int64_t Hq,
                                      int64_t Hkv, int64_t D, const aq_span *ahead, int n_ahead, void *stream);
 
+/* Decode attention of a batch whose sequences begin with the same pages (samples of one prompt, beams, requests behind one system
+ * prompt: what the reference's prefix cache maps into every sequence's table, astrai/inference/core/cache.py:68-185): the arguments and the
+ * meaning of aq_paged_attn_decode, and the promise that the entries of page_table for positions 0 .. shared_len - 1 are the same in
+ * every row.  Those positions are read once, through row 0, and multiplied with the queries of all sequences at once on the matrix core;
+ * the others through each sequence's own row.  shared_len may be anything from 0 (nothing is shared: aq_paged_attn_decode) on;
+ * what lies past total_len counts for nothing.  A promise that does not hold gives the values of row 0's pages.
+ * Results agree with aq_paged_attn_decode within bf16 rounding (probabilities of shared positions are rounded to bf16, sums are
+ * fp32 in another order).  seq_lens as there, a sequence may end inside the shared positions; positions that no sequence
+ * attends to may hold anything.  total_len at most 2^30, B Hq at most 2^24 (AQ_E_RANGE).
+ * workspace: 16-byte aligned, aq_paged_attn_decode_shared_workspace_bytes(..) bytes for the same sizes (0: may be NULL); two calls that
+ * overlap in time must not share it. */
+int64_t aq_paged_attn_decode_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t total_len,
+                                                    int64_t shared_len);
+int aq_paged_attn_decode_shared(const void *q, const void *k_cache, const void *v_cache, const int64_t *page_table,
+                                int64_t P, int64_t total_len, int64_t shared_len, const int64_t *seq_lens,
+                                int64_t page_size, int64_t n_pages, float scale, void *out, int64_t B, int64_t Hq,
+                                int64_t Hkv, int64_t D, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ---- pages between steps.  Caches of `layers` layers [n_pages, page_size, row_bytes], layer_bytes apart (any type; row_bytes, of
+ * one token's heads, and layer_bytes multiples of 16), refs[n_pages] int32: how many hold each page (rows of the table and whoever
+ * else, such as a cache of prompts), 0: free.  Table entries outside 0 .. n_pages - 1 are unmapped.  Outputs must not overlap inputs.
+ * The reference does this on the host (Allocator and the page lists of its tasks, astrai/inference/core/cache.py:18-185).
+ *
+ * aq_fork_pages: row i of new_table [R, P] becomes a fork of row parents[i] of page_table [B, P] (a parent outside 0 .. B - 1: an
+ * empty row, all -1).  n = total_len, or seq_lens[parent] (device int64 [B], cut to 0 .. total_len), positions of the parent are
+ * written.  Its first child goes on in all of its pages.  Every other child holds the pages that n fills, and gets a page of its own for
+ * a page that is partly filled: the written rows of all layers' keys and values are copied there, the rows behind them are left as
+ * they were; its later entries are -1.  new_refs = max(refs - entries of the old rows, 0) + entries of the new rows, so rows without a child
+ * let go of their pages, and the pages that are then free are handed out lowest first, to the rows in order.  missing[0]: rows that
+ * found none (their entry is -1).  Sources are held, destinations free: the copies touch no page in use.
+ * workspace: aq_fork_pages_workspace_bytes(n_pages, R) bytes, 4-byte aligned.
+ *
+ * aq_compact_pages: live[0] = number of pages with refs > 0; the held pages past place live[0] - 1 are moved into the free ones in front of
+ * it, the last one held into the first hole, and so on.  where[x] (int64 [n_pages]): where held page x is now, -1 if it is free;
+ * new_table: page_table's entries through where; new_refs likewise.  workspace: aq_compact_pages_workspace_bytes(n_pages) bytes, 4-byte
+ * aligned. */
+int64_t aq_fork_pages_workspace_bytes(int64_t n_pages, int64_t R);
+int aq_fork_pages(const int64_t *page_table, int64_t B, int64_t P, const int32_t *refs, const int64_t *parents, int64_t R,
+                  int64_t total_len, const int64_t *seq_lens, void *k_layers, void *v_layers, int64_t layers,
+                  int64_t layer_bytes, int64_t n_pages, int64_t page_size, int64_t row_bytes, int64_t *new_table,
+                  int32_t *new_refs, int32_t *missing, void *workspace, int64_t workspace_bytes, void *stream);
+int64_t aq_compact_pages_workspace_bytes(int64_t n_pages);
+int aq_compact_pages(const int64_t *page_table, int64_t entries, const int32_t *refs, void *k_layers, void *v_layers,
+                     int64_t layers, int64_t layer_bytes, int64_t n_pages, int64_t page_size, int64_t row_bytes,
+                     int64_t *new_table, int32_t *new_refs, int64_t *where, int32_t *live, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -90,6 +90,14 @@ SYMBOLS = {
                                                  _i64, _i64, _i64, _i64, _i64, _vp, _int, _vp]),
     "aq_rope_prefill_attn_paged_ahead": (_int, [_vp, _i64, _vp, _i64, _vp, ctypes.c_float, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp,
                                                 ctypes.c_float, _i64, _i64, _i64, _i64, _i64, _vp, _int, _vp]),
+    "aq_paged_attn_decode_shared_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "aq_paged_attn_decode_shared": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64, ctypes.c_float, _vp, _i64, _i64,
+                                           _i64, _i64, _vp, _i64, _vp]),
+    "aq_fork_pages_workspace_bytes": (_i64, [_i64, _i64]),
+    "aq_fork_pages": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp,
+                             _i64, _vp]),
+    "aq_compact_pages_workspace_bytes": (_i64, [_i64]),
+    "aq_compact_pages": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
 }
 
 # csrc/aq_lab.h: the lab library's additions (measurement probes, the tile-forcing test hook)

@@ -8,8 +8,9 @@ reference makes.  Two KV caches offer the two methods attention needs (``write``
 the ``KvcacheView`` interface, astrai/inference/core/cache.py:277-290): a
 contiguous per-sequence buffer, and a paged one with the storage layout and the
 write / gather semantics of the reference's ``Storage`` (cache.py:187-274).
-Page allocation, prefix sharing and eviction belong to the serving layer and are
-not restated: the page table is handed in.
+Page allocation and eviction belong to the serving layer and are not restated: the page table is handed in.
+Sequences may share pages: ``PagedKV.fork`` and ``compact`` make and renumber such tables on the device, and a decode step reads
+what all sequences share once.
 """
 from __future__ import annotations
 
@@ -89,7 +90,10 @@ class PagedKV:
     ``make_table_tensor`` produces for every step.
     ``seq_lens`` (int64 ``[B]`` on the device, optional): the positions each sequence may attend to
     in a single-token step whose sequences sit at different positions; the attention kernels apply it as
-    the reference's position mask (transformer.py:40-46)."""
+    the reference's position mask (transformer.py:40-46).
+    ``bind(share_prefix=True)``: the leading pages that all rows of the table have in common (found on the host copy) are
+    read once per single-token step for all sequences, by the paged-cache kernels; results within bf16 rounding of reading them per
+    sequence.  It holds until the next ``bind``."""
 
     def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device, dtype,
                  n_layers: int = 1):
@@ -101,14 +105,18 @@ class PagedKV:
         self._mapped = None      # host bool [B, P]
         self._safe = None        # device table with -1 replaced by 0
         self._invalid = None     # device bool [B, P * page_size] or None when everything is mapped
+        self._host = None        # host copy of the table
+        self._common = None      # leading columns that are the same in all of its rows, once asked for
         self.total_len = 0
+        self.shared_len = 0      # leading positions that a single-token step reads once for all sequences
         self.seq_lens: Optional[Tensor] = None
 
     def bind(self, page_table: Optional[Tensor] = None, total_len: int = 0, seq_lens: Optional[Tensor] = None,
-             refresh: bool = False) -> "PagedKV":
+             refresh: bool = False, share_prefix: bool = False) -> "PagedKV":
         if page_table is not None and (refresh or page_table is not self.page_table):
             host = page_table.detach().cpu()
             self.page_table = page_table
+            self._host, self._common = host, None
             self._mapped = host >= 0
             self._safe = page_table.clamp(min=0)
             self._invalid = None
@@ -119,7 +127,25 @@ class PagedKV:
             raise ValueError("bind() needs a page table")
         self.total_len = total_len
         self.seq_lens = seq_lens
+        self.shared_len = 0
+        if share_prefix and self._host.shape[0] > 1:
+            if self._common is None:
+                self._common = int((self._host == self._host[:1]).all(0).long().cumprod(0).sum())
+            self.shared_len = max(0, min(self._common * self.page_size, total_len - 1))  # the new token's page is its own
         return self
+
+    def fork(self, refs: Tensor, parents: Tensor, seq_lens: Optional[Tensor] = None) -> "ops.ForkedPages":
+        """Rows for the next step, forks of the bound table's (``ops.fork_pages``): row i goes on from row ``parents[i]``,
+        whose first ``total_len`` (or ``seq_lens``) positions are written.  Bind the table it returns."""
+        if self.page_table is None:
+            raise ValueError("fork() needs a bound page table")
+        return ops.fork_pages(self.page_table, refs, parents, self.k_layers, self.v_layers, self.total_len, seq_lens)
+
+    def compact(self, refs: Tensor) -> "ops.CompactedPages":
+        """The held pages moved to the front of the cache (``ops.compact_pages``).  Bind the table it returns."""
+        if self.page_table is None:
+            raise ValueError("compact() needs a bound page table")
+        return ops.compact_pages(self.page_table, refs, self.k_layers, self.v_layers)
 
     def attn_workspace(self, n_heads: int) -> Optional[Tensor]:
         """Scratch for the decode attention kernel's partial results, sized once for the longest
@@ -284,6 +310,12 @@ class GQA(nn.Module):
         if (self._decode_attention and S == 1 and attn_mask is None and isinstance(cache, PagedKV) and x.is_cuda
                 and x.dtype == torch.bfloat16):
             qkv = self._project_qkv(x, codes, norm)
+            if cache.shared_len > 0:  # the first positions of all sequences are the same pages: read once
+                kc, vc = cache.k_layers[self.layer_id], cache.v_layers[self.layer_id]
+                q = ops.rope_kv_write(qkv.view(B, -1), rotary_emb.reshape(B, -1), cache.page_table, cache.total_len - 1,
+                                      kc, vc, self.n_heads, self.n_kv_heads, qk_norm=self._qk_norm())
+                out = ops.paged_attn_decode_shared(q, kc, vc, cache.page_table, cache.total_len, cache.shared_len, seq_lens=cache.seq_lens)
+                return self._out(self._gated(out.view(B, 1, -1), x, norm, codes), residual)
             # the output projection combines the attention's position slices itself when the step is small
             # enough for its in-kernel quantiser: one launch less
             split = (isinstance(self.o_proj, QuantLinear) and not self.use_gated_attention
@@ -432,7 +464,8 @@ class DecoderBlock(nn.Module):
 
     def forward(self, x: Tensor, rotary_emb: Tensor, attention_mask: Optional[Tensor] = None,
                 cache=None) -> Tensor:
-        if self._norm_quant and self._residual_adds and attention_mask is None and cache is not None:
+        if (self._norm_quant and self._residual_adds and attention_mask is None and cache is not None
+                and not getattr(cache, "shared_len", 0)):
             # everything fused, over a paged cache: the same launches, queued by native code in one call
             y = (_host or _native())(self, x, rotary_emb, cache)
             if y is not None:

@@ -1,0 +1,55 @@
+// What the attention kernels on the matrix core share: rows of keys and values brought into LDS, and the two launches of
+// attn_decode.hip that other files queue.
+#pragma once
+#include "aq_common.h"
+
+namespace aq {
+
+typedef __bf16 pa_bf16x8 __attribute__((ext_vector_type(8)));
+typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
+typedef float pa_f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void pa_lds_void;
+typedef __attribute__((address_space(3))) pa_s16x4 pa_lds_s16x4;
+
+__device__ const uint4 pa_zero_row[16] = {};  // what a row of an unmapped page reads as
+
+// 16 bytes per lane from memory to LDS, 1 KiB in lane order from byte `at` (wavefront-uniform).  Written out because the compiler,
+// given the builtin, waits for every such load in flight before the next LDS read of any kind -- here the other buffer's,
+// requested a moment earlier.  The kernel waits itself, before the barrier that hands a buffer over.
+__device__ __forceinline__ void load_row_lds(const uint16_t* src, uint32_t at) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(at) : "memory");  // m0 needs a wait state
+}
+
+// The 16-byte piece of row r that sits in slot s of the row is s ^ row_key(r): the low bits of r, reversed.  16 rows
+// reading the same piece (K) fall on all slots of the bank lines; the 8 neighbouring rows x 64 bytes of a transposing
+// read (V) are told apart by their lowest bits, which reversed move a row's pieces by 64 bytes and more.
+template <int D>
+__device__ __forceinline__ int row_key(int row) {
+  if constexpr (D == 64)  // 128-byte rows: two to a bank line
+    return (int)(__builtin_bitreverse32((uint32_t)(row >> 1) & 7u) >> 29);
+  else
+    return (int)(__builtin_bitreverse32((uint32_t)row & 15u) >> 28);
+}
+
+// Attention of one query per sequence over positions t0 .. T - 1 (t0 a multiple of 64) of its own pages, left as partial results
+// [D + 4] in slots slot0, slot0 + 1 .. of the NS slots of each (sequence, query head) in ws: attn_tail_slices(T - t0) of them.
+// Positions from lens[b] on weigh nothing, whatever is stored there; a sequence without any length weighs all of its positions alike.
+struct AttnTail {
+  const void *q, *kc, *vc;
+  const int64_t *table, *lens;
+  float* ws;
+  int64_t P, t0, T, page, n_pages, B, Hq, Hkv, D;
+  float scale;
+  int NS, slot0;
+};
+int64_t attn_tail_slices(int64_t positions);
+int attn_tail(const AttnTail& t, hipStream_t st);
+// Combines the NS slots of every (sequence, query head) into out [B, Hq, D].
+int attn_merge(const float* ws, void* out, int64_t B, int64_t Hq, int NS, int64_t D, hipStream_t st);
+// Query heads per KV head that the decode kernels are made for.
+inline bool attn_group_ok(int64_t G) { return G == 1 || G == 2 || G == 3 || G == 4 || G == 6 || G == 8; }
+constexpr int ATT_MAX_D = 128;
+// Floats of a slot, sized for the larger head dimension so that sizes do not depend on D.
+inline int64_t attn_workspace_bytes(int64_t B, int64_t Hq, int64_t ns) { return B * Hq * ns * (ATT_MAX_D + 4) * (int64_t)sizeof(float); }
+
+}  // namespace aq

@@ -778,6 +778,137 @@ def paged_attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     return out
 
 
+def paged_attn_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                             total_len: int, shared_len: int, scale: Optional[float] = None,
+                             workspace: Optional[torch.Tensor] = None, seq_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_attn_decode`` for sequences that begin with the same pages: the entries of ``page_table`` for the first
+    ``shared_len`` positions are the same in every row (the caller's promise; row 0's pages are read).  Those positions
+    are read once and multiplied with all sequences' queries at once.  The results agree with ``paged_attn_decode`` within bf16
+    rounding; ``seq_lens`` as there.  ``workspace``: a contiguous device tensor to reuse across calls, of
+    ``paged_attn_shared_workspace_bytes`` bytes; allocated per call when omitted or too small."""
+    _need_gpu(q, k_cache, v_cache, page_table)
+    if q.dtype != torch.bfloat16 or k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
+        raise ValueError("paged_attn_decode_shared takes bfloat16 tensors")
+    if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape or q.shape[2] != k_cache.shape[3]:
+        raise ValueError("q must be [B, Hq, D] and the caches [n_pages, page, Hkv, D]")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("caches must be contiguous")
+    B, Hq, D = q.shape
+    n_pages, page, Hkv, _ = k_cache.shape
+    if page_table.dtype != torch.int64 or page_table.dim() != 2 or page_table.shape[0] != B:
+        raise ValueError("page_table must be int64 [B, P]")
+    total_len, shared_len = int(total_len), int(shared_len)
+    lens_ptr = _seq_lens_ptr(seq_lens, B, q.device)
+    page_table, q = page_table.contiguous(), q.contiguous()
+    out = torch.empty_like(q)
+    if B:
+        ws_ptr, ws_bytes = _attn_workspace(workspace, paged_attn_shared_workspace_bytes(B, Hq, Hkv, D, total_len, shared_len, q.device),
+                                           q.device)
+        with _OnDevice(q.device):
+            rc = _abi.load().aq_paged_attn_decode_shared(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
+                                                         page_table.shape[1], total_len, shared_len, lens_ptr, page, n_pages,
+                                                         float(scale if scale is not None else D ** -0.5), out.data_ptr(),
+                                                         B, Hq, Hkv, D, ws_ptr, ws_bytes, _stream(q))
+        _abi.check(rc, "aq_paged_attn_decode_shared")
+    return out
+
+
+def paged_attn_shared_workspace_bytes(B: int, n_heads: int, n_kv_heads: int, head_dim: int, total_len: int, shared_len: int, device) -> int:
+    """Bytes of device workspace ``paged_attn_decode_shared`` needs for these sizes on ``device`` (0: none)."""
+    with _OnDevice(torch.device(device)):  # the positions are cut by the device's compute units
+        return int(_abi.load().aq_paged_attn_decode_shared_workspace_bytes(B, n_heads, n_kv_heads, head_dim, int(total_len), int(shared_len)))
+
+
+class ForkedPages(NamedTuple):
+    """What ``fork_pages`` gives: the new rows ``[R, P]``, the pages' new counts ``[n_pages]``, and how many rows found no
+    free page for their copy (``missing`` int32 ``[1]``; that entry of theirs is -1)."""
+    page_table: torch.Tensor
+    refs: torch.Tensor
+    missing: torch.Tensor
+
+
+class CompactedPages(NamedTuple):
+    """What ``compact_pages`` gives: the renumbered table and counts, where each held page is now (``where`` int64
+    ``[n_pages]``, -1: it was free), and how many are held (``live`` int32 ``[1]``: pages 0 .. live - 1)."""
+    page_table: torch.Tensor
+    refs: torch.Tensor
+    where: torch.Tensor
+    live: torch.Tensor
+
+
+def _pages_args(page_table, refs, k_layers, v_layers, what):
+    """Checked caches ``[layers, n_pages, page, Hkv, D]`` (or one layer's) with their table and counts ->
+    (table, refs, (k, v, layers, layer_bytes, n_pages, page, row_bytes))."""
+    if k_layers.dtype != v_layers.dtype or k_layers.shape != v_layers.shape or k_layers.dim() not in (4, 5):
+        raise ValueError(f"{what}: the caches must be [layers, n_pages, page, Hkv, D], or one layer's, alike")
+    k, v = (c.unsqueeze(0) if c.dim() == 4 else c for c in (k_layers, v_layers))
+    layers, n_pages, page, heads, dim = k.shape
+    if layers == 0 or k[0].numel() == 0:
+        raise ValueError(f"{what}: the caches hold nothing")
+    if not (k[0].is_contiguous() and v[0].is_contiguous()) or (layers > 1 and k.stride(0) != v.stride(0)):
+        raise ValueError(f"{what}: a layer's pages must be contiguous, and the layers of both caches as far apart")
+    if page_table.dtype != torch.int64 or page_table.dim() != 2 or page_table.shape[1] == 0:
+        raise ValueError(f"{what}: page_table must be int64 [B, P]")
+    if refs.dtype != torch.int32 or refs.shape != (n_pages,):
+        raise ValueError(f"{what}: refs must be int32 [{n_pages}]")
+    size = k.element_size()
+    if heads * dim * size % 16:
+        raise ValueError(f"{what}: a token's row of a layer must be a multiple of 16 bytes, got {heads * dim * size}")
+    return page_table.contiguous(), refs.contiguous(), (k.data_ptr(), v.data_ptr(), layers, k.stride(0) * size if layers > 1 else 0,
+                                                        n_pages, page, heads * dim * size)
+
+
+def fork_pages(page_table: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, k_layers: torch.Tensor, v_layers: torch.Tensor,
+               total_len: int, seq_lens: Optional[torch.Tensor] = None) -> ForkedPages:
+    """New rows of a page table, each a fork of an old one: row i of the result goes on from row ``parents[i]`` (int64 ``[R]``;
+    outside ``0 .. B - 1``: an empty row).  Whole pages are held together; the first child of a row goes on in its pages, the others
+    get a free page with a copy of what is written of a page that is not full (``total_len`` positions are written, or
+    ``seq_lens`` int64 ``[B]`` of them, in all layers' caches).  Old rows without a child let go of their pages: dropping beams, ending
+    sequences and sampling several continuations are one call, and no call waits for the device.  ``refs`` int32
+    ``[n_pages]`` counts who holds each page.  The table and the counts given are left as they are; the caches (any type, of 16-byte
+    rows) are written in place, free pages only."""
+    _need_gpu(page_table, refs, parents, k_layers, v_layers)
+    page_table, refs, caches = _pages_args(page_table, refs, k_layers, v_layers, "fork_pages")
+    (B, P), n_pages, dev = page_table.shape, refs.numel(), refs.device
+    if parents.dtype != torch.int64 or parents.dim() != 1:
+        raise ValueError("parents must be int64 [R]")
+    total_len = int(total_len)
+    if not 0 <= total_len <= P * caches[5]:
+        raise ValueError(f"{total_len} positions fall outside the page table")
+    lens_ptr = _seq_lens_ptr(seq_lens, B, dev)
+    parents, R = parents.contiguous(), parents.numel()
+    table = torch.empty((R, P), dtype=torch.int64, device=dev)
+    counts = torch.empty_like(refs)
+    missing = torch.empty((1,), dtype=torch.int32, device=dev)
+    lib = _abi.load()
+    ws = torch.empty((lib.aq_fork_pages_workspace_bytes(n_pages, R) // 4,), dtype=torch.int32, device=dev)
+    with _OnDevice(dev):
+        rc = lib.aq_fork_pages(page_table.data_ptr(), B, P, refs.data_ptr(), parents.data_ptr(), R, total_len, lens_ptr, *caches,
+                               table.data_ptr(), counts.data_ptr(), missing.data_ptr(), ws.data_ptr(), ws.numel() * 4, _stream(refs))
+    _abi.check(rc, "aq_fork_pages")
+    return ForkedPages(table, counts, missing)
+
+
+def compact_pages(page_table: torch.Tensor, refs: torch.Tensor, k_layers: torch.Tensor, v_layers: torch.Tensor) -> CompactedPages:
+    """Moves the pages that are held (``refs`` int32 ``[n_pages]`` above 0) to the front of all layers' caches, in place, and
+    renumbers the table's entries: the last page held goes into the first free place, and so on, until pages 0 .. live - 1 are held.
+    Entries that name a free page become -1.  The table and the counts given are left as they are; ``where`` tells other holders
+    of pages where theirs went."""
+    _need_gpu(page_table, refs, k_layers, v_layers)
+    page_table, refs, caches = _pages_args(page_table, refs, k_layers, v_layers, "compact_pages")
+    n_pages, dev = refs.numel(), refs.device
+    table, counts = torch.empty_like(page_table), torch.empty_like(refs)
+    where = torch.empty((n_pages,), dtype=torch.int64, device=dev)
+    live = torch.empty((1,), dtype=torch.int32, device=dev)
+    lib = _abi.load()
+    ws = torch.empty((lib.aq_compact_pages_workspace_bytes(n_pages) // 4,), dtype=torch.int32, device=dev)
+    with _OnDevice(dev):
+        rc = lib.aq_compact_pages(page_table.data_ptr(), page_table.numel(), refs.data_ptr(), *caches, table.data_ptr(), counts.data_ptr(),
+                                  where.data_ptr(), live.data_ptr(), ws.data_ptr(), ws.numel() * 4, _stream(refs))
+    _abi.check(rc, "aq_compact_pages")
+    return CompactedPages(table, counts, where, live)
+
+
 def linear_fp8(xq, sx, wq, sw, bias=None, out_dtype=torch.bfloat16, residual=None) -> torch.Tensor:
     """FP8 e4m3fn GEMM with fp32 accumulation: y = (acc * sx[0]) * sw[0] (+ bias), cast, (+ residual)."""
     y = (_host or _native()).linear_fp8(xq, sx, wq, sw, bias, out_dtype, residual)
