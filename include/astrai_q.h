@@ -502,12 +502,12 @@ int aq_paged_attn_decode_shared(const void *q, const void *k_cache, const void *
  * they were; its later entries are -1.  new_refs = max(refs - entries of the old rows, 0) + entries of the new rows, so rows without a child
  * let go of their pages, and the pages that are then free are handed out lowest first, to the rows in order.  missing[0]: rows that
  * found none (their entry is -1).  Sources are held, destinations free: the copies touch no page in use.
- * workspace: aq_fork_pages_workspace_bytes(n_pages, R) bytes, 4-byte aligned.
+ * workspace: aq_fork_pages_workspace_bytes(n_pages, R) bytes.  It and refs are 16-byte aligned.
  *
  * aq_compact_pages: live[0] = number of pages with refs > 0; the held pages past place live[0] - 1 are moved into the free ones in front of
  * it, the last one held into the first hole, and so on.  where[x] (int64 [n_pages]): where held page x is now, -1 if it is free;
  * new_table: page_table's entries through where; new_refs likewise.  workspace: aq_compact_pages_workspace_bytes(n_pages) bytes, 4-byte
- * aligned. */
+ * aligned; refs 16-byte aligned. */
 int64_t aq_fork_pages_workspace_bytes(int64_t n_pages, int64_t R);
 int aq_fork_pages(const int64_t *page_table, int64_t B, int64_t P, const int32_t *refs, const int64_t *parents, int64_t R,
                   int64_t total_len, const int64_t *seq_lens, void *k_layers, void *v_layers, int64_t layers,

@@ -8,8 +8,13 @@
 
 namespace aq {
 
-constexpr int PG_THREADS = 256, PG_PAGES = 4096;  // pages of a workgroup that numbers them: 16 to a thread
-constexpr int PG_UNIT = 16 * 1024;                // bytes of a copying workgroup's turn: 4 x 16 to a thread
+constexpr int PG_THREADS = 1024, PG_PAGES = 4 * PG_THREADS;  // of a workgroup that numbers pages: 4 to a thread
+constexpr int PG_COPY = 256, PG_UNIT = 8 * 1024;              // a copying workgroup, and the bytes of its turn: 2 x 16 to a thread
+
+// A copy that a row needs: the page, its written positions, the row, and the entry of the row that gets the new page.
+struct ForkCopy {
+  int32_t source, rows, row, column;
+};
 
 struct ForkArgs {
   const int64_t* table;    // [B, P]
@@ -19,38 +24,28 @@ struct ForkArgs {
   int64_t* new_table;      // [R, P]
   int32_t* new_refs;       // [n_pages]
   int32_t* missing;        // [1]
+  ForkCopy* wants;         // [R] of a row, source -1: none
+  ForkCopy* copies;        // [R] the same, the rows that need one only
+  int32_t* fresh;          // [R] the pages they get, ascending
+  int32_t* got;            // [1] rows that get one
   int32_t* gone;           // [n_pages] entries of the old rows that name the page
   int32_t* come;           // [n_pages] entries of the new rows that name it
-  int32_t* source;         // [R] the page that the row needs a copy of, or -1
-  int32_t* wanting;        // [R] rows that need one, ascending
-  int32_t* fresh;          // [R] the pages they get, ascending
-  int32_t* counts;         // [2] rows that need a page, rows that get one
   uint8_t *k, *v;          // [layers][n_pages][page][row_bytes]
-  int64_t layer_bytes, row_bytes, page, T, n_pages;
-  int B, R, P, layers;
+  int64_t layer_bytes, row_bytes, page_bytes, T, n_pages;
+  int B, R, P, layers, page;
+  UDiv by_p;  // (one-workgroup form)
 };
-
-// Sum over the workgroup, in every thread.
-__device__ __forceinline__ int wg_sum(int v, int* s) {
-  const int tid = threadIdx.x;
-  __syncthreads();
-#pragma unroll
-  for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off, 64);
-  if ((tid & 63) == 0) s[tid >> 6] = v;
-  __syncthreads();
-  return s[0] + s[1] + s[2] + s[3];
-}
 
 // Sum over the threads before this one; *all: over all of them.
 __device__ __forceinline__ int wg_before(int v, int* s, int* all) {
   const int tid = threadIdx.x, lane = tid & 63;
-  __syncthreads();
   int x = v;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const int y = __shfl_up(x, off, 64);
     if (lane >= off) x += y;
   }
+  __syncthreads();  // s may still be read by an earlier call
   if (lane == 63) s[tid >> 6] = x;
   __syncthreads();
   int base = 0, sum = 0;
@@ -63,219 +58,378 @@ __device__ __forceinline__ int wg_before(int v, int* s, int* all) {
   return base + x - v;
 }
 
-__global__ __launch_bounds__(PG_THREADS) void fork_clear_kernel(int32_t* p, int64_t n) {
+// f(x, count of the pages x .. x + 3 that are there) summed over the workgroup, x = 4 i for i in [i0, i1); several loads in flight.
+template <class F>
+__device__ __forceinline__ int wg_count(int64_t i0, int64_t i1, int* s, F&& f) {
+  int n = 0;
+#pragma unroll 8
+  for (int64_t i = i0 + threadIdx.x; i < i1; i += PG_THREADS) n += f(i);
+  int all;
+  wg_before(n, s, &all);
+  return all;
+}
+
+__device__ __forceinline__ int fork_entry(const ForkArgs& a, int row, int l) {
+  const int64_t e = a.table[(int64_t)row * a.P + l];
+  return e >= 0 && e < a.n_pages ? (int)e : -1;
+}
+
+__device__ __forceinline__ int64_t fork_length(const ForkArgs& a, int row) {
+  const int64_t n = a.lens ? a.lens[row] : a.T;
+  return n < 0 ? 0 : n > a.T ? a.T : n;
+}
+
+// refs, with the old rows' entries taken away (none is left at least) and the new rows' added
+__device__ __forceinline__ int fork_count(int refs, int gone, int come) {
+  return (refs > gone ? refs - gone : 0) + come;
+}
+
+// Four pages' new counts: the free ones among them get numbers from `at` on, the first `need` of which are handed out.
+__device__ __forceinline__ void fork_hand_out(const ForkArgs& a, int64_t x, int (&c)[4], int at, int need) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if (x + u >= a.n_pages) break;
+    if (c[u] == 0) {
+      if (at < need) {
+        a.fresh[at] = (int)(x + u);
+        c[u] = 1;
+      }
+      ++at;
+    }
+    a.new_refs[x + u] = c[u];
+  }
+}
+
+__global__ __launch_bounds__(PG_THREADS) void fork_clear_kernel(v4i* p, int64_t n) {
   const int64_t i = (int64_t)blockIdx.x * PG_THREADS + threadIdx.x;
-  if (i < n) p[i] = 0;
+  if (i < n) p[i] = v4i{0, 0, 0, 0};
 }
 
-// A row of the old table (the workgroups from R on: whose pages they let go), or of the new one.  Counts are whole numbers: the order of
-// the atomics changes nothing.
-__global__ __launch_bounds__(PG_THREADS) void fork_rows_kernel(ForkArgs a) {
+// ROWS rows of the new table, or (the workgroups behind those) of the old one, whose pages are let go; a thread has a column, so that
+// neighbouring rows with the same page (what sequences share) are one atomic.  (256 old and 300 new rows of 129 columns, 63 of them
+// alike: 9.5 us with one row to a workgroup, most of it 556 atomics on each shared page in turn.)  Counts are whole numbers: the order
+// of the atomics changes nothing.
+constexpr int FORK_ROWS = 16;
+__global__ __launch_bounds__(PG_COPY) void fork_rows_kernel(ForkArgs a, int new_wgs, int chunks) {
+  __shared__ int parent_s[FORK_ROWS], whole_s[FORK_ROWS], rest_s[FORK_ROWS], later_s[FORK_ROWS];
   const int tid = threadIdx.x;
-  auto entry = [&](int row, int l) -> int {
-    const int64_t e = a.table[(int64_t)row * a.P + l];
-    return e >= 0 && e < a.n_pages ? (int)e : -1;
-  };
-  if ((int)blockIdx.x >= a.R) {
-    const int row = (int)blockIdx.x - a.R;
-    for (int l = tid; l < a.P; l += PG_THREADS) {
-      const int e = entry(row, l);
-      if (e >= 0) atomicAdd(a.gone + e, 1);
+  const bool old = (int)blockIdx.x >= new_wgs;
+  const int wg = old ? (int)blockIdx.x - new_wgs : (int)blockIdx.x, rows = old ? a.B : a.R;
+  const int i0 = wg / chunks * FORK_ROWS, l = (wg - wg / chunks * chunks) * PG_COPY + tid;
+  const int n_rows = rows - i0 < FORK_ROWS ? rows - i0 : FORK_ROWS;
+  if (!old) {
+    if (tid < n_rows) {
+      const int64_t p = a.parents[i0 + tid];
+      const bool known = p >= 0 && p < a.B;
+      parent_s[tid] = known ? (int)p : -1;
+      const int64_t n = known ? fork_length(a, (int)p) : 0;
+      whole_s[tid] = (int)(n / a.page);
+      rest_s[tid] = (int)(n - n / a.page * a.page);
+      later_s[tid] = 0;
     }
-    return;
+    __syncthreads();
+    for (int j = tid; j < i0 + n_rows; j += PG_COPY) {  // which rows have an earlier sibling
+      const int64_t p = a.parents[j];
+#pragma unroll
+      for (int r = 0; r < FORK_ROWS; ++r)
+        if (r < n_rows && j < i0 + r && p == parent_s[r]) later_s[r] = 1;
+    }
+    __syncthreads();
   }
-  const int i = (int)blockIdx.x;
-  const int64_t parent = a.parents[i];
-  const bool known = parent >= 0 && parent < a.B;
-  int before = 0;  // an earlier child of the same parent
-  for (int j = tid; j < i; j += PG_THREADS) before |= a.parents[j] == parent;
-  const bool first = known && !__syncthreads_or(before);
-  const int p = known ? (int)parent : 0;
-  int64_t n = a.lens ? a.lens[p] : a.T;
-  n = n < 0 ? 0 : n > a.T ? a.T : n;
-  const int64_t whole = n / a.page, rest = n - whole * a.page;
-  for (int l = tid; l < a.P; l += PG_THREADS) {
-    const int e = known && (first || l < whole) ? entry(p, l) : -1;
-    a.new_table[(int64_t)i * a.P + l] = e;
-    if (e >= 0) atomicAdd(a.come + e, 1);
+  if (l >= a.P) return;
+  int e[FORK_ROWS];  // all requested before any is used
+#pragma unroll
+  for (int r = 0; r < FORK_ROWS; ++r) {
+    const int p = old ? i0 + r : r < n_rows ? parent_s[r] : -1;
+    e[r] = r < n_rows && p >= 0 ? fork_entry(a, p, l) : -1;
   }
-  if (tid == 0) a.source[i] = known && !first && rest > 0 && whole < a.P ? entry(p, (int)whole) : -1;
+  int at = -1, run = 0;
+  int32_t* const counts = old ? a.gone : a.come;
+#pragma unroll
+  for (int r = 0; r < FORK_ROWS; ++r) {
+    if (r >= n_rows) break;
+    if (!old) {
+      const int i = i0 + r;
+      if (l == whole_s[r]) a.wants[i] = {later_s[r] && rest_s[r] > 0 ? e[r] : -1, rest_s[r], i, l};
+      if (l == 0 && whole_s[r] >= a.P) a.wants[i] = {-1, 0, i, 0};
+      if (later_s[r] && l >= whole_s[r]) e[r] = -1;
+      a.new_table[(int64_t)i * a.P + l] = e[r];
+    }
+    if (e[r] != at) {
+      if (at >= 0) atomicAdd(counts + at, run);
+      at = e[r];
+      run = 0;
+    }
+    ++run;
+  }
+  if (at >= 0) atomicAdd(counts + at, run);
 }
 
-// The new counts, and the free pages for the rows that need one: the k-th free page to the k-th row.  Every workgroup counts the free
-// pages in front of its own by itself.  The last workgroup numbers the rows.
-__global__ __launch_bounds__(PG_THREADS) void fork_refs_kernel(ForkArgs a, int groups) {
-  __shared__ int s[PG_THREADS / 64];
-  const int tid = threadIdx.x;
-  if ((int)blockIdx.x == groups) {
-    int done = 0;
-    for (int i0 = 0; i0 < a.R; i0 += PG_THREADS) {
-      const int i = i0 + tid;
-      const int want = i < a.R && a.source[i] >= 0;
-      int all;
-      const int at = done + wg_before(want, s, &all);
-      if (want) a.wanting[at] = i;
-      done += all;
-    }
-    if (tid == 0) a.counts[0] = done;
-    return;
-  }
-  int need = 0;
-  for (int i = tid; i < a.R; i += PG_THREADS) need += a.source[i] >= 0;
-  need = wg_sum(need, s);
-  auto count = [&](int64_t x) -> int {
-    const int left = a.refs[x] - a.gone[x];
-    return (left > 0 ? left : 0) + a.come[x];
-  };
-  const int64_t x0 = (int64_t)blockIdx.x * PG_PAGES;
-  int base = 0;
-  for (int64_t x = tid; x < x0; x += PG_THREADS) base += count(x) == 0;
-  base = wg_sum(base, s);
-  for (int64_t x = x0 + tid; x - tid < x0 + PG_PAGES; x += PG_THREADS) {
-    int c = x < a.n_pages ? count(x) : 1;
-    const int is_free = c == 0;
+// The rows that need a page, numbered: returns how many.
+__device__ __forceinline__ int fork_number(const ForkArgs& a, int* s, bool write) {
+  int done = 0;
+  for (int i0 = 0; i0 < a.R; i0 += PG_THREADS) {
+    const int i = i0 + (int)threadIdx.x;
+    ForkCopy w = {-1, 0, 0, 0};
+    if (i < a.R) w = a.wants[i];
     int all;
-    const int at = base + wg_before(is_free, s, &all);
-    if (is_free && at < need) {
-      a.fresh[at] = (int)x;
-      c = 1;
-    }
-    if (x < a.n_pages) a.new_refs[x] = c;
-    base += all;
+    const int at = done + wg_before(w.source >= 0, s, &all);
+    if (write && w.source >= 0) a.copies[at] = w;
+    done += all;
   }
-  if ((int)blockIdx.x == groups - 1 && tid == 0) {
-    a.counts[1] = need < base ? need : base;
+  return done;
+}
+
+// The new counts, and the free pages for the rows that need one: the k-th free page to the k-th row.  Every workgroup counts the rows, and
+// the free pages in front of its own, by itself (40000 pages: 53 us with a load of each count at a time by 256 threads).
+__global__ __launch_bounds__(PG_THREADS) void fork_refs_kernel(ForkArgs a) {
+  __shared__ int s[PG_THREADS / 64];
+  const int64_t i0 = (int64_t)blockIdx.x * PG_THREADS, i = i0 + threadIdx.x, x = 4 * i;
+  int base = wg_count(0, i0, s, [&](int64_t i) {
+    const v4i r = reinterpret_cast<const v4i*>(a.refs)[i], g = reinterpret_cast<const v4i*>(a.gone)[i], n = reinterpret_cast<const v4i*>(a.come)[i];
+    return (fork_count(r.x, g.x, n.x) == 0) + (fork_count(r.y, g.y, n.y) == 0) + (fork_count(r.z, g.z, n.z) == 0) + (fork_count(r.w, g.w, n.w) == 0);
+  });
+  const int need = fork_number(a, s, blockIdx.x == 0);
+  int c[4] = {1, 1, 1, 1};
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (x + u < a.n_pages) c[u] = fork_count(a.refs[x + u], a.gone[x + u], a.come[x + u]);
+  int all;
+  const int at = base + wg_before((c[0] == 0) + (c[1] == 0) + (c[2] == 0) + (c[3] == 0), s, &all);
+  fork_hand_out(a, x, c, at, need);
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+    base += all;
+    a.got[0] = need < base ? need : base;
     a.missing[0] = need > base ? need - base : 0;
   }
 }
 
-// 16 bytes a thread at a time, four in flight.
-__device__ __forceinline__ void copy_unit(const uint8_t* from, uint8_t* to, int64_t bytes) {
-  uint4 x[PG_UNIT / 16 / PG_THREADS];
-#pragma unroll
-  for (int u = 0; u < PG_UNIT / 16 / PG_THREADS; ++u) {
-    const int64_t at = (int64_t)(u * PG_THREADS + threadIdx.x) * 16;
-    if (at < bytes) x[u] = *reinterpret_cast<const uint4*>(from + at);
+// All of the above by one workgroup, its counts in LDS, for small tables and caches: one launch instead of three.
+constexpr int FORK_ONE_PAGES = 8192, FORK_ONE_ROWS = 4096, FORK_ONE_ENTRIES = 32768;
+__global__ __launch_bounds__(PG_THREADS) void fork_one_kernel(ForkArgs a) {
+  __shared__ int s[PG_THREADS / 64];
+  extern __shared__ __align__(16) int pg_lds[];
+  const int tid = threadIdx.x, pages = ((int)a.n_pages + 3) & ~3;
+  int *const gone = pg_lds, *const come = gone + pages, *const first_of = come + pages;
+  for (int x = tid; x < 2 * pages; x += PG_THREADS) gone[x] = 0;
+  for (int p = tid; p < a.B; p += PG_THREADS) first_of[p] = a.R;
+  __syncthreads();
+  for (int i = tid; i < a.R; i += PG_THREADS) {
+    const int64_t p = a.parents[i];
+    if (p >= 0 && p < a.B) atomicMin(first_of + p, i);
   }
+#pragma unroll 2
+  for (int x = tid; x < a.B * a.P; x += PG_THREADS) {
+    const int64_t e = a.table[x];
+    if (e >= 0 && e < a.n_pages) atomicAdd(gone + e, 1);
+  }
+  __syncthreads();
+#pragma unroll 2
+  for (int x = tid; x < a.R * a.P; x += PG_THREADS) {
+    const int i = a.by_p((uint32_t)x), l = x - i * a.P;
+    const int64_t parent = a.parents[i];
+    const bool known = parent >= 0 && parent < a.B;
+    const int p = known ? (int)parent : 0;
+    const int64_t n = known ? fork_length(a, p) : 0;
+    const int whole = (int)(n / a.page), mine = known ? fork_entry(a, p, l) : -1;
+    const bool first = known && first_of[p] == i;
+    const int e = first || l < whole ? mine : -1;
+    a.new_table[x] = e;
+    if (e >= 0) atomicAdd(come + e, 1);
+    const int rest = (int)(n - (int64_t)whole * a.page);
+    if (l == whole) a.wants[i] = {!first && rest > 0 ? mine : -1, rest, i, whole};
+    if (l == 0 && whole >= a.P) a.wants[i] = {-1, 0, i, 0};
+  }
+  __syncthreads();
+  const int need = fork_number(a, s, true);
+  int base = 0;
+  for (int x0 = 0; x0 < pages; x0 += PG_PAGES) {
+    const int x = x0 + 4 * tid;
+    int c[4] = {1, 1, 1, 1};
 #pragma unroll
-  for (int u = 0; u < PG_UNIT / 16 / PG_THREADS; ++u) {
-    const int64_t at = (int64_t)(u * PG_THREADS + threadIdx.x) * 16;
-    if (at < bytes) *reinterpret_cast<uint4*>(to + at) = x[u];
+    for (int u = 0; u < 4; ++u)
+      if (x + u < (int)a.n_pages) c[u] = fork_count(a.refs[x + u], gone[x + u], come[x + u]);
+    int all;
+    const int at = base + wg_before((c[0] == 0) + (c[1] == 0) + (c[2] == 0) + (c[3] == 0), s, &all);
+    fork_hand_out(a, x, c, at, need);
+    base += all;
+  }
+  if (tid == 0) {
+    a.got[0] = need < base ? need : base;
+    a.missing[0] = need > base ? need - base : 0;
   }
 }
 
-// The copies' first rest positions, in units of PG_UNIT bytes of one layer's keys or values, and their entries of the table.
-__global__ __launch_bounds__(PG_THREADS) void fork_copy_kernel(ForkArgs a) {
-  const int got = a.counts[1];
-  const int64_t per_page = (a.page * a.row_bytes + PG_UNIT - 1) / PG_UNIT, per_copy = per_page * 2 * a.layers;
-  for (int64_t u = blockIdx.x; u < got * per_copy; u += gridDim.x) {
-    const int c = (int)(u / per_copy);
-    const int64_t w = u - c * per_copy, lkv = w / per_page, chunk = w - lkv * per_page;
-    const int i = a.wanting[c], p = (int)a.parents[i];
-    int64_t n = a.lens ? a.lens[p] : a.T;
-    n = n < 0 ? 0 : n > a.T ? a.T : n;
-    const int64_t whole = n / a.page, bytes = (n - whole * a.page) * a.row_bytes - chunk * PG_UNIT;
-    if (w == 0 && threadIdx.x == 0) a.new_table[(int64_t)i * a.P + whole] = a.fresh[c];
-    if (bytes <= 0) continue;
-    uint8_t* const base = (lkv & 1 ? a.v : a.k) + (lkv >> 1) * a.layer_bytes + chunk * PG_UNIT;
-    const int64_t page_bytes = a.page * a.row_bytes;
-    copy_unit(base + a.source[i] * page_bytes, base + a.fresh[c] * page_bytes, bytes < PG_UNIT ? bytes : PG_UNIT);
+// 16 bytes a thread at a time, two in flight, past the L2: what is copied is not read again soon (1920 copies of 56 KB, two at a time
+// and four: 42.0 and 45 us, through the L2 46 and 50).  Of HIP's uint4 the compiler makes an array in LDS, three times slower.
+__device__ __forceinline__ void copy_unit(const uint8_t* from, uint8_t* to, int bytes) {
+  v4i x[PG_UNIT / 16 / PG_COPY];
+#pragma unroll
+  for (int u = 0; u < PG_UNIT / 16 / PG_COPY; ++u) {
+    const int at = (u * PG_COPY + (int)threadIdx.x) * 16;
+    if (at < bytes) x[u] = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(from + at));
   }
+#pragma unroll
+  for (int u = 0; u < PG_UNIT / 16 / PG_COPY; ++u) {
+    const int at = (u * PG_COPY + (int)threadIdx.x) * 16;
+    if (at < bytes) __builtin_nontemporal_store(x[u], reinterpret_cast<v4i*>(to + at));
+  }
+}
+
+// How the units (chunks of PG_UNIT bytes, of keys and of values, of each layer) of a page fall on workgroups: unit w of page c follows unit
+// w - 1, the workgroups take turns, and turn (pages, rest) is what one turn of all of them is, so that none divides.
+struct CopyPlan {
+  int units, chunks, turn_pages, turn_rest;
+  UDiv by_units, by_chunks;
+};
+
+// f(c, layer, values?, offset into the page) for every unit of pages 0 .. n - 1 that is this workgroup's; the first one's page: copy_first.
+__device__ __forceinline__ int copy_first(const CopyPlan& p) { return (int)p.by_units(blockIdx.x); }
+template <class F>
+__device__ __forceinline__ void each_unit(const CopyPlan& p, int c0, int n, F&& f) {
+  int c = c0, w = (int)blockIdx.x - c0 * p.units;
+  while (c < n) {
+    const int lkv = p.by_chunks(w);
+    f(c, lkv >> 1, lkv & 1, (int64_t)(w - lkv * p.chunks) * PG_UNIT);
+    c += p.turn_pages;
+    w += p.turn_rest;
+    if (w >= p.units) {
+      w -= p.units;
+      ++c;
+    }
+  }
+}
+
+// The copies' written positions, and their entries of the table.
+__global__ __launch_bounds__(PG_COPY) void fork_copy_kernel(ForkArgs a, CopyPlan plan) {
+  const int c0 = copy_first(plan), got = a.got[0];
+  const ForkCopy w0 = a.copies[c0];  // requested with the count, one round trip less: not looked at if it is not one
+  const int fresh0 = a.fresh[c0];
+  each_unit(plan, c0, got, [&](int c, int64_t layer, int values, int64_t at) {
+    const ForkCopy w = c == c0 ? w0 : a.copies[c];
+    const int fresh = c == c0 ? fresh0 : a.fresh[c];
+    if (layer == 0 && !values && at == 0 && threadIdx.x == 0) a.new_table[(int64_t)w.row * a.P + w.column] = fresh;
+    const int64_t bytes = w.rows * a.row_bytes - at;
+    if (bytes <= 0) return;
+    uint8_t* const base = (values ? a.v : a.k) + layer * a.layer_bytes + at;
+    copy_unit(base + w.source * a.page_bytes, base + fresh * a.page_bytes, (int)(bytes < PG_UNIT ? bytes : PG_UNIT));
+  });
 }
 
 struct CompactArgs {
-  const int64_t* table;  // [B, P] entries in all
+  const int64_t* table;  // entries in all
   const int32_t* refs;
   int64_t* new_table;
   int32_t* new_refs;
-  int64_t* where;  // [n_pages] where a held page went, -1: free
-  int32_t* live;   // [1]
+  int64_t* where;   // [n_pages] where a held page went, -1: free
+  int32_t* live;    // [1]
   int32_t* source;  // [n_pages] of the k-th move: the k-th page held from the top,
   int32_t* hole;    // [n_pages] the k-th free one from the bottom
   int32_t* move;    // [n_pages] of a held page past the last place: which move is its own
   int32_t* moves;   // [1]
   uint8_t *k, *v;
   int64_t layer_bytes, page_bytes, n_pages, entries;
-  int layers;
+  int layers, copy_wgs;
 };
 
 // Numbers the pages: live of them are held, places 0 .. live - 1 are to hold them.  Every workgroup counts what lies in front of its own
-// pages, and all, by itself.
+// pages, and all, by itself (60000 pages: 96 us with a load at a time by 256 threads).
 __global__ __launch_bounds__(PG_THREADS) void compact_rank_kernel(CompactArgs a) {
   __shared__ int s[PG_THREADS / 64];
-  const int tid = threadIdx.x;
-  const int64_t x0 = (int64_t)blockIdx.x * PG_PAGES;
-  int before = 0, rest = 0;
-  for (int64_t x = tid; x < x0; x += PG_THREADS) before += a.refs[x] > 0;
-  for (int64_t x = x0 + tid; x < a.n_pages; x += PG_THREADS) rest += a.refs[x] > 0;
-  before = wg_sum(before, s);
-  const int live = before + wg_sum(rest, s);
-  int base = before;
-  for (int64_t x = x0 + tid; x - tid < x0 + PG_PAGES; x += PG_THREADS) {
-    const int r = x < a.n_pages ? a.refs[x] : 0;
-    const int held = r > 0;
-    int all;
-    const int at = base + wg_before(held, s, &all);  // held pages in front of x
-    base += all;
-    if (x >= a.n_pages) continue;
-    a.where[x] = held && x < live ? x : -1;  // moved pages: their move says
-    a.new_refs[x] = held && x < live ? r : 0;
-    if (held && x >= live) {
-      a.source[live - 1 - at] = (int)x;
-      a.move[x] = live - 1 - at;
+  const int64_t i0 = (int64_t)blockIdx.x * PG_THREADS, i = i0 + threadIdx.x, x = 4 * i, whole = a.n_pages / 4;
+  auto held4 = [&](int64_t i) {
+    const v4i r = reinterpret_cast<const v4i*>(a.refs)[i];
+    return (r.x > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0);
+  };
+  int r[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (x + u < a.n_pages) r[u] = a.refs[x + u];
+  const int before = wg_count(0, i0, s, held4);
+  int rest = wg_count(i0 + PG_THREADS, whole, s, held4), mine;
+  int at = before + wg_before((r[0] > 0) + (r[1] > 0) + (r[2] > 0) + (r[3] > 0), s, &mine);  // held pages in front of x
+  if (i0 + PG_THREADS <= whole)  // the pages behind the last whole four
+    for (int64_t y = 4 * whole; y < a.n_pages; ++y) rest += a.refs[y] > 0;
+  const int live = before + mine + rest;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t y = x + u;
+    if (y >= a.n_pages) break;
+    const bool held = r[u] > 0;
+    a.where[y] = held && y < live ? y : -1;  // moved pages: their move says
+    a.new_refs[y] = held && y < live ? r[u] : 0;
+    if (held && y >= live) {
+      a.source[live - 1 - at] = (int)y;
+      a.move[y] = live - 1 - at;
     }
-    if (!held && x < live) a.hole[x - at] = (int)x;
-    if (x == live - 1) a.moves[0] = live - (at + held);  // free pages among the first live
+    if (!held && y < live) a.hole[y - at] = (int)y;
+    at += held;
+    if (y == live - 1) a.moves[0] = live - at;  // free pages among the first live
   }
-  if (blockIdx.x == 0 && tid == 0) {
+  if (x == 0) {
     a.live[0] = live;
     if (live == 0) a.moves[0] = 0;
   }
 }
 
-// Moves the pages, in units of PG_UNIT bytes of one layer's keys or values, and renumbers the table.  Sources lie behind the last place,
-// holes in front of it: no page is both.
-__global__ __launch_bounds__(PG_THREADS) void compact_move_kernel(CompactArgs a) {
-  const int moves = a.moves[0], live = a.live[0];
-  const int64_t stride = (int64_t)gridDim.x * PG_THREADS, me = (int64_t)blockIdx.x * PG_THREADS + threadIdx.x;
-  for (int64_t i = me; i < a.entries; i += stride) {
-    const int64_t e = a.table[i];
-    int64_t to = -1;
-    if (e >= 0 && e < a.n_pages && a.refs[e] > 0) to = e < live ? e : a.hole[a.move[e]];
-    a.new_table[i] = to;
+// Moves the pages; the workgroups behind those renumber the table and fill in the counts.  Sources lie behind the last place, holes in
+// front of it: no page is both.
+__global__ __launch_bounds__(PG_COPY) void compact_move_kernel(CompactArgs a, CopyPlan plan) {
+  const int moves = a.moves[0];
+  if ((int)blockIdx.x >= a.copy_wgs) {
+    const int live = a.live[0];
+    const int64_t stride = (int64_t)(gridDim.x - a.copy_wgs) * PG_COPY, me = (int64_t)((int)blockIdx.x - a.copy_wgs) * PG_COPY + threadIdx.x;
+    for (int64_t i = me; i < a.entries; i += stride) {
+      const int64_t e = a.table[i];
+      int64_t to = -1;
+      if (e >= 0 && e < a.n_pages && a.refs[e] > 0) to = e < live ? e : a.hole[a.move[e]];
+      a.new_table[i] = to;
+    }
+    for (int64_t i = me; i < moves; i += stride) {
+      const int from = a.source[i], to = a.hole[i];
+      a.where[from] = to;
+      a.new_refs[to] = a.refs[from];
+    }
+    return;
   }
-  for (int64_t i = me; i < moves; i += stride) {
-    const int from = a.source[i], to = a.hole[i];
-    a.where[from] = to;
-    a.new_refs[to] = a.refs[from];
-  }
-  const int64_t per_page = (a.page_bytes + PG_UNIT - 1) / PG_UNIT, per_move = per_page * 2 * a.layers;
-  for (int64_t u = blockIdx.x; u < moves * per_move; u += gridDim.x) {
-    const int c = (int)(u / per_move);
-    const int64_t w = u - c * per_move, lkv = w / per_page, chunk = w - lkv * per_page, left = a.page_bytes - chunk * PG_UNIT;
-    uint8_t* const base = (lkv & 1 ? a.v : a.k) + (lkv >> 1) * a.layer_bytes + chunk * PG_UNIT;
-    copy_unit(base + a.source[c] * a.page_bytes, base + a.hole[c] * a.page_bytes, left < PG_UNIT ? left : PG_UNIT);
-  }
+  const int c0 = copy_first(plan), source0 = a.source[c0], hole0 = a.hole[c0];  // requested with the count
+  each_unit(plan, c0, moves, [&](int c, int64_t layer, int values, int64_t at) {
+    const int64_t left = a.page_bytes - at;
+    uint8_t* const base = (values ? a.v : a.k) + layer * a.layer_bytes + at;
+    copy_unit(base + (c == c0 ? source0 : a.source[c]) * a.page_bytes, base + (c == c0 ? hole0 : a.hole[c]) * a.page_bytes, (int)(left < PG_UNIT ? left : PG_UNIT));
+  });
+}
+
+// At most `most` pages are copied; 8 workgroups fill a compute unit.  Returns the workgroups.
+static unsigned copy_plan(CopyPlan& p, int64_t most, int64_t layers, int64_t page_bytes) {
+  const int64_t chunks = (page_bytes + PG_UNIT - 1) / PG_UNIT, units = 2 * layers * chunks, room = (int64_t)device_cus() * 8;
+  const int64_t wgs = most < 1 ? 1 : most < room / units + 1 && most * units < room ? most * units : room;
+  p.units = (int)units;
+  p.chunks = (int)chunks;
+  p.turn_pages = (int)(wgs / units);
+  p.turn_rest = (int)(wgs - wgs / units * units);
+  p.by_units = UDiv::of((uint32_t)units);
+  p.by_chunks = UDiv::of((uint32_t)chunks);
+  return (unsigned)wgs;
 }
 
 static int check_caches(const void* k, const void* v, int64_t layers, int64_t layer_bytes, int64_t n_pages, int64_t page_size, int64_t row_bytes) {
   if (layers <= 0 || n_pages <= 0 || page_size <= 0 || row_bytes <= 0) return AQ_E_SHAPE;
-  if (layers > 65535 || n_pages > 0x7fffffff - PG_PAGES || page_size > (1 << 30) || row_bytes > (1 << 30)) return AQ_E_RANGE;
+  if (layers > 4096 || n_pages > 0x7fffffff - PG_PAGES || page_size > (1 << 30) || row_bytes > (1 << 30) || page_size * row_bytes > (int64_t)1 << 31)
+    return AQ_E_RANGE;  // (units of a copied page: 31 bits)
   if ((row_bytes & 15) || (layer_bytes & 15)) return AQ_E_ALIGN;
   if (layers > 1 && layer_bytes / row_bytes / page_size < n_pages) return AQ_E_SHAPE;  // layers that overlap
   if (!k || !v) return AQ_E_NULL;
   return check_ptr16(k) || check_ptr16(v) ? AQ_E_ALIGN : AQ_OK;
 }
 
-static unsigned copy_groups(int64_t units) {
-  const int64_t most = (int64_t)device_cus() * 8;  // 8 workgroups of 256 threads fill a compute unit
-  return (unsigned)(units < 1 ? 1 : units < most ? units : most);
-}
+// Workspace of a fork: the list of copies, then the counts.
+static int64_t fork_words(int64_t n_pages, int64_t R) { return 8 * R + (R + 4) / 4 * 4 + 2 * ((n_pages + 3) / 4 * 4); }
 
 }  // namespace aq
 
 extern "C" int64_t aq_fork_pages_workspace_bytes(int64_t n_pages, int64_t R) {
-  return n_pages <= 0 || R < 0 ? 0 : (2 * n_pages + 3 * R + 2) * (int64_t)sizeof(int32_t);
+  return n_pages <= 0 || R < 0 ? 0 : aq::fork_words(n_pages, R) * (int64_t)sizeof(int32_t);
 }
 
 extern "C" int aq_fork_pages(const int64_t* page_table, int64_t B, int64_t P, const int32_t* refs, const int64_t* parents, int64_t R,
@@ -285,9 +439,10 @@ extern "C" int aq_fork_pages(const int64_t* page_table, int64_t B, int64_t P, co
   if (B < 0 || R < 0 || P <= 0 || total_len < 0) return AQ_E_SHAPE;
   if (const int rc = aq::check_caches(k_layers, v_layers, layers, layer_bytes, n_pages, page_size, row_bytes)) return rc;
   if (B > (1 << 24) || R > (1 << 24) || P > 0x7fffffff) return AQ_E_RANGE;
+  if (total_len > P * page_size) return AQ_E_SHAPE;  // positions the page table does not cover
   if ((B > 0 && !page_table) || (R > 0 && (!parents || !new_table)) || !refs || !new_refs || !missing || !workspace) return AQ_E_NULL;
   if (aq::check_ptr(page_table, 8) || aq::check_ptr(parents, 8) || aq::check_ptr(seq_lens, 8) || aq::check_ptr(new_table, 8) ||
-      aq::check_ptr(refs, 4) || aq::check_ptr(new_refs, 4) || aq::check_ptr(missing, 4) || aq::check_ptr(workspace, 4))
+      aq::check_ptr16(refs) || aq::check_ptr(new_refs, 4) || aq::check_ptr(missing, 4) || aq::check_ptr16(workspace))
     return AQ_E_ALIGN;
   if (workspace_bytes < aq_fork_pages_workspace_bytes(n_pages, R)) return AQ_E_WORKSPACE;
   aq::ForkArgs a{};
@@ -298,17 +453,18 @@ extern "C" int aq_fork_pages(const int64_t* page_table, int64_t B, int64_t P, co
   a.new_table = new_table;
   a.new_refs = new_refs;
   a.missing = missing;
-  a.gone = static_cast<int32_t*>(workspace);
-  a.come = a.gone + n_pages;
-  a.source = a.come + n_pages;
-  a.wanting = a.source + R;
-  a.fresh = a.wanting + R;
-  a.counts = a.fresh + R;
+  a.wants = static_cast<aq::ForkCopy*>(workspace);
+  a.copies = a.wants + R;
+  a.fresh = reinterpret_cast<int32_t*>(a.copies + R);
+  a.got = a.fresh + R;
+  a.gone = a.fresh + (R + 4) / 4 * 4;
+  a.come = a.gone + (n_pages + 3) / 4 * 4;
   a.k = static_cast<uint8_t*>(k_layers);
   a.v = static_cast<uint8_t*>(v_layers);
   a.layer_bytes = layer_bytes;
   a.row_bytes = row_bytes;
-  a.page = page_size;
+  a.page_bytes = page_size * row_bytes;
+  a.page = (int)page_size;
   a.T = total_len;
   a.n_pages = n_pages;
   a.B = (int)B;
@@ -316,14 +472,24 @@ extern "C" int aq_fork_pages(const int64_t* page_table, int64_t B, int64_t P, co
   a.P = (int)P;
   a.layers = (int)layers;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 block(aq::PG_THREADS);
-  const int groups = (int)((n_pages + aq::PG_PAGES - 1) / aq::PG_PAGES);
-  aq::queue_kernel(aq::fork_clear_kernel, dim3((unsigned)((2 * n_pages + aq::PG_THREADS - 1) / aq::PG_THREADS)), block, 0, st, a.gone, 2 * n_pages);
-  if (R + B > 0) aq::queue_kernel(aq::fork_rows_kernel, dim3((unsigned)(R + B)), block, 0, st, a);
-  aq::queue_kernel(aq::fork_refs_kernel, dim3((unsigned)(groups + 1)), block, 0, st, a, groups);
+  const dim3 one(aq::PG_THREADS);
+  if (n_pages <= aq::FORK_ONE_PAGES && B <= aq::FORK_ONE_ROWS && R <= aq::FORK_ONE_ROWS && (B + R) * P <= aq::FORK_ONE_ENTRIES) {
+    a.by_p = aq::UDiv::of((uint32_t)P);
+    aq::queue_kernel(aq::fork_one_kernel, dim3(1), one, (size_t)(2 * ((n_pages + 3) / 4 * 4) + B) * sizeof(int), st, a);
+  } else {
+    const int64_t quads = (n_pages + 3) / 4 * 2, groups = (n_pages + aq::PG_PAGES - 1) / aq::PG_PAGES;
+    aq::queue_kernel(aq::fork_clear_kernel, dim3((unsigned)((quads + aq::PG_THREADS - 1) / aq::PG_THREADS)), one, 0, st,
+                     reinterpret_cast<v4i*>(a.gone), quads);
+    const int64_t chunks = (P + aq::PG_COPY - 1) / aq::PG_COPY, new_wgs = (R + aq::FORK_ROWS - 1) / aq::FORK_ROWS * chunks;
+    const int64_t wgs = new_wgs + (B + aq::FORK_ROWS - 1) / aq::FORK_ROWS * chunks;
+    if (wgs > 0x7fffffff) return AQ_E_RANGE;
+    if (wgs > 0) aq::queue_kernel(aq::fork_rows_kernel, dim3((unsigned)wgs), dim3(aq::PG_COPY), 0, st, a, (int)new_wgs, (int)chunks);
+    aq::queue_kernel(aq::fork_refs_kernel, dim3((unsigned)groups), one, 0, st, a);
+  }
   if (R > 1) {  // (a single row is its parent's first child)
-    const int64_t units = (R - 1) * 2 * layers * ((page_size * row_bytes + aq::PG_UNIT - 1) / aq::PG_UNIT);
-    aq::queue_kernel(aq::fork_copy_kernel, dim3(aq::copy_groups(units)), block, 0, st, a);
+    aq::CopyPlan plan;
+    const unsigned wgs = aq::copy_plan(plan, R - 1, layers, a.page_bytes);
+    aq::queue_kernel(aq::fork_copy_kernel, dim3(wgs), dim3(aq::PG_COPY), 0, st, a, plan);
   }
   return (int)hipGetLastError();
 }
@@ -337,7 +503,7 @@ extern "C" int aq_compact_pages(const int64_t* page_table, int64_t entries, cons
   if (entries < 0) return AQ_E_SHAPE;
   if (const int rc = aq::check_caches(k_layers, v_layers, layers, layer_bytes, n_pages, page_size, row_bytes)) return rc;
   if ((entries > 0 && (!page_table || !new_table)) || !refs || !new_refs || !where || !live || !workspace) return AQ_E_NULL;
-  if (aq::check_ptr(page_table, 8) || aq::check_ptr(new_table, 8) || aq::check_ptr(where, 8) || aq::check_ptr(refs, 4) ||
+  if (aq::check_ptr(page_table, 8) || aq::check_ptr(new_table, 8) || aq::check_ptr(where, 8) || aq::check_ptr16(refs) ||
       aq::check_ptr(new_refs, 4) || aq::check_ptr(live, 4) || aq::check_ptr(workspace, 4))
     return AQ_E_ALIGN;
   if (workspace_bytes < aq_compact_pages_workspace_bytes(n_pages)) return AQ_E_WORKSPACE;
@@ -360,9 +526,10 @@ extern "C" int aq_compact_pages(const int64_t* page_table, int64_t entries, cons
   a.entries = entries;
   a.layers = (int)layers;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 block(aq::PG_THREADS);
-  aq::queue_kernel(aq::compact_rank_kernel, dim3((unsigned)((n_pages + aq::PG_PAGES - 1) / aq::PG_PAGES)), block, 0, st, a);
-  const int64_t units = n_pages / 2 * 2 * layers * ((a.page_bytes + aq::PG_UNIT - 1) / aq::PG_UNIT), rows = (entries + aq::PG_THREADS - 1) / aq::PG_THREADS;
-  aq::queue_kernel(aq::compact_move_kernel, dim3(aq::copy_groups(units > rows ? units : rows)), block, 0, st, a);
+  aq::queue_kernel(aq::compact_rank_kernel, dim3((unsigned)((n_pages + aq::PG_PAGES - 1) / aq::PG_PAGES)), dim3(aq::PG_THREADS), 0, st, a);
+  aq::CopyPlan plan;
+  a.copy_wgs = (int)aq::copy_plan(plan, n_pages / 2, layers, a.page_bytes);
+  const int64_t work = entries > n_pages / 2 ? entries : n_pages / 2, rest = (work + aq::PG_COPY - 1) / aq::PG_COPY;
+  aq::queue_kernel(aq::compact_move_kernel, dim3((unsigned)(a.copy_wgs + (rest < 1 ? 1 : rest < 256 ? rest : 256))), dim3(aq::PG_COPY), 0, st, a, plan);
   return (int)hipGetLastError();
 }

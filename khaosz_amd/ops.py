@@ -854,7 +854,10 @@ def _pages_args(page_table, refs, k_layers, v_layers, what):
     size = k.element_size()
     if heads * dim * size % 16:
         raise ValueError(f"{what}: a token's row of a layer must be a multiple of 16 bytes, got {heads * dim * size}")
-    return page_table.contiguous(), refs.contiguous(), (k.data_ptr(), v.data_ptr(), layers, k.stride(0) * size if layers > 1 else 0,
+    refs = refs.contiguous()
+    if refs.data_ptr() % 16:
+        refs = refs.clone()
+    return page_table.contiguous(), refs, (k.data_ptr(), v.data_ptr(), layers, k.stride(0) * size if layers > 1 else 0,
                                                         n_pages, page, heads * dim * size)
 
 

@@ -112,7 +112,9 @@ def test_fork_small(page, total, parents):
 
 
 @pytest.mark.parametrize("B,R,P,page,n_pages,layers,seed", [(64, 64, 23, 16, 2000, 2, 0), (1, 300, 5, 64, 400, 1, 1), (200, 40, 30, 4, 6100, 1, 2),
-                                                           (256, 300, 17, 16, 9000, 3, 3), (2, 2, 2049, 2, 4200, 1, 4)])
+                                                           (256, 300, 17, 16, 9000, 3, 3), (2, 2, 2049, 2, 4200, 1, 4),
+                                                           (70, 90, 200, 4, 14500, 1, 5), (4, 9, 3, 16, 8193, 1, 6), (300, 5000, 2, 4, 5700, 1, 7),
+                                                           (5, 7, 4, 16, 8190, 1, 8), (64, 2100, 3, 4, 4097, 2, 9)])
 def test_fork_rows_at_lengths_of_their_own(B, R, P, page, n_pages, layers, seed):
     _say("fork lens", B, R, P, page, n_pages)
     table, refs, k, v = _state(B, P, n_pages, page, layers=layers, seed=seed, common=min(3, P - 1), heads=1)
@@ -268,6 +270,16 @@ def test_pages_beyond_32_bits():
     c = ops.compact_pages(f.page_table, f.refs, k, v)
     assert c.live.item() == n_pages - 4 and c.page_table.tolist() == [[n_pages - 5, n_pages - 6], [n_pages - 5, to]]
     assert torch.equal(k[n_pages - 6], ka[1]) and torch.equal(k[n_pages - 5], ka[0]) and torch.equal(v[n_pages - 6], va[1])
+
+
+def test_counts_at_any_address():
+    table, refs, k, v = _state(3, 4, 40, 16)
+    want = _forked(table, refs, torch.tensor([0, 0, 2]), k, v, 50)
+    kd, vd = k.to(DEV), v.to(DEV)
+    odd = torch.zeros(43, dtype=torch.int32, device=DEV)[3:]
+    odd.copy_(refs)
+    got = ops.fork_pages(table.to(DEV), odd, torch.tensor([0, 0, 2], device=DEV), kd, vd, 50)
+    _equal(got, want, kd, vd)
 
 
 def test_refusals():
