@@ -71,7 +71,13 @@ namespace {
   X(aq_prefill_attn_causal_ahead)                                                                                \
   X(aq_prefill_attn_paged_ahead)                                                                                 \
   X(aq_rope_prefill_attn_causal_ahead)                                                                           \
-  X(aq_rope_prefill_attn_paged_ahead)
+  X(aq_rope_prefill_attn_paged_ahead)                                                                            \
+  X(aq_paged_attn_decode_shared_workspace_bytes)                                                                 \
+  X(aq_paged_attn_decode_shared)                                                                                 \
+  X(aq_fork_pages_workspace_bytes)                                                                               \
+  X(aq_fork_pages)                                                                                               \
+  X(aq_compact_pages_workspace_bytes)                                                                            \
+  X(aq_compact_pages)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -408,6 +414,144 @@ PyObject* quant_tensor_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                            static_cast<uint32_t*>(ws.mutable_data_ptr()), AQ_FP8_AMAX_WS_BYTES, c.stream);
   });
   return rc ? fail(rc, state ? "aq_quant_tensor_fp8_onepass" : "aq_quant_tensor_fp8") : pair(q, s);
+  END_HANDLE_TH_ERRORS
+}
+
+// a Python int
+bool whole(PyObject* o, int64_t* v) {
+  if (!PyLong_CheckExact(o)) return false;
+  int over = 0;
+  *v = PyLong_AsLongLongAndOverflow(o, &over);
+  return over == 0;
+}
+
+// None, or lengths int64 [B]
+bool lens_of(PyObject* o, int64_t B, int dev, const int64_t** p) {
+  *p = nullptr;
+  if (o == Py_None) return true;
+  const Tensor* t = unpack(o);
+  if (!t || !plain(*t, ScalarType::Long, dev) || t->dim() != 1 || t->size(0) != B) return false;
+  *p = t->const_data_ptr<int64_t>();
+  return true;
+}
+
+// paged_attn_decode_shared(q, k_cache, v_cache, page_table, total_len, shared_len, scale or None, seq_lens or None) -> out
+PyObject* paged_attn_decode_shared(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS AQ_ARGS(8);
+  const Tensor *q = unpack(args[0]), *k = unpack(args[1]), *v = unpack(args[2]), *t = unpack(args[3]);
+  Call c;
+  if (!q || !k || !v || !t || !c.at(*q) || !plain(*q, ScalarType::BFloat16, c.dev) || !plain(*k, ScalarType::BFloat16, c.dev) ||
+      !plain(*v, ScalarType::BFloat16, c.dev) || !plain(*t, ScalarType::Long, c.dev))
+    return none();
+  if (q->dim() != 3 || k->dim() != 4 || t->dim() != 2 || k->sizes() != v->sizes() || q->size(2) != k->size(3) || t->size(0) != q->size(0) ||
+      q->size(0) < 1)
+    return none();
+  const int64_t B = q->size(0), Hq = q->size(1), D = q->size(2), n_pages = k->size(0), page = k->size(1), Hkv = k->size(2), P = t->size(1);
+  int64_t total, shared;
+  const int64_t* lens;
+  if (!whole(args[4], &total) || !whole(args[5], &shared) || !lens_of(args[7], B, c.dev, &lens)) return none();
+  double scale = 1.0 / std::sqrt(static_cast<double>(D));
+  if (args[6] != Py_None) {
+    scale = PyFloat_AsDouble(args[6]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+  }
+  c.current_stream();
+  const int64_t need = lib.aq_paged_attn_decode_shared_workspace_bytes(B, Hq, Hkv, D, total, shared);
+  Tensor y = c.empty(q->sizes(), ScalarType::BFloat16), ws;
+  if (need) ws = c.empty({need}, ScalarType::Byte);
+  const int rc = queued([&] {
+    return lib.aq_paged_attn_decode_shared(q->const_data_ptr(), k->const_data_ptr(), v->const_data_ptr(), t->const_data_ptr<int64_t>(), P, total,
+                                           shared, lens, page, n_pages, static_cast<float>(scale), y.mutable_data_ptr(), B, Hq, Hkv, D,
+                                           need ? ws.mutable_data_ptr() : nullptr, need, c.stream);
+  });
+  return rc ? fail(rc, "aq_paged_attn_decode_shared") : THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+struct Pages {  // a table, the pages' counts and the caches of one layer or of several
+  const Tensor *table, *refs;
+  void *k, *v;
+  int64_t layers, layer_bytes, n_pages, page, row_bytes, B, P;
+};
+bool pages_of(PyObject* table, PyObject* refs, PyObject* k_layers, PyObject* v_layers, Call* c, Pages* p) {
+  const Tensor *k = unpack(k_layers), *v = unpack(v_layers);
+  p->table = unpack(table);
+  p->refs = unpack(refs);
+  if (!k || !v || !p->table || !p->refs || !c->at(*k) || !plain(*k, k->scalar_type(), c->dev) || !plain(*v, k->scalar_type(), c->dev) ||
+      !plain(*p->table, ScalarType::Long, c->dev) || !plain(*p->refs, ScalarType::Int, c->dev))
+    return false;
+  const int64_t d = k->dim();
+  if ((d != 4 && d != 5) || k->sizes() != v->sizes() || k->numel() == 0 || p->table->dim() != 2 || p->table->size(1) == 0 ||
+      p->refs->dim() != 1 || p->refs->size(0) != k->size(d - 4) || !aligned16(p->refs->const_data_ptr()))
+    return false;
+  const int64_t size = static_cast<int64_t>(k->element_size());
+  p->k = k->mutable_data_ptr();
+  p->v = v->mutable_data_ptr();
+  p->layers = d == 5 ? k->size(0) : 1;
+  p->n_pages = k->size(d - 4);
+  p->page = k->size(d - 3);
+  p->row_bytes = k->size(d - 2) * k->size(d - 1) * size;
+  p->layer_bytes = p->layers > 1 ? p->n_pages * p->page * p->row_bytes : 0;
+  p->B = p->table->size(0);
+  p->P = p->table->size(1);
+  return p->row_bytes % 16 == 0;
+}
+
+// objects of tensors, as a tuple
+PyObject* tuple_of(std::initializer_list<const Tensor*> tensors) {
+  PyObject* r = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+  Py_ssize_t i = 0;
+  for (const Tensor* t : tensors) {
+    PyObject* o = r ? THPVariable_Wrap(*t) : nullptr;
+    if (!o) {
+      Py_XDECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i++, o);
+  }
+  return r;
+}
+
+// fork_pages(page_table, refs, parents, k_layers, v_layers, total_len, seq_lens or None) -> (table, refs, missing)
+PyObject* fork_pages(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS AQ_ARGS(7);
+  Call c;
+  Pages p;
+  const Tensor* parents = unpack(args[2]);
+  int64_t total;
+  const int64_t* lens;
+  if (!parents || !pages_of(args[0], args[1], args[3], args[4], &c, &p) || !plain(*parents, ScalarType::Long, c.dev) || parents->dim() != 1 ||
+      !whole(args[5], &total) || total < 0 || total > p.P * p.page || !lens_of(args[6], p.B, c.dev, &lens))
+    return none();
+  c.current_stream();
+  const int64_t R = parents->numel(), need = lib.aq_fork_pages_workspace_bytes(p.n_pages, R);
+  Tensor table = c.empty({R, p.P}, ScalarType::Long), refs = c.empty({p.n_pages}, ScalarType::Int), missing = c.empty({1}, ScalarType::Int),
+         ws = c.empty({need}, ScalarType::Byte);
+  const int rc = queued([&] {
+    return lib.aq_fork_pages(p.table->const_data_ptr<int64_t>(), p.B, p.P, p.refs->const_data_ptr<int32_t>(), parents->const_data_ptr<int64_t>(),
+                             R, total, lens, p.k, p.v, p.layers, p.layer_bytes, p.n_pages, p.page, p.row_bytes, table.mutable_data_ptr<int64_t>(),
+                             refs.mutable_data_ptr<int32_t>(), missing.mutable_data_ptr<int32_t>(), ws.mutable_data_ptr(), need, c.stream);
+  });
+  return rc ? fail(rc, "aq_fork_pages") : tuple_of({&table, &refs, &missing});
+  END_HANDLE_TH_ERRORS
+}
+
+// compact_pages(page_table, refs, k_layers, v_layers) -> (table, refs, where, live)
+PyObject* compact_pages(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS AQ_ARGS(4);
+  Call c;
+  Pages p;
+  if (!pages_of(args[0], args[1], args[2], args[3], &c, &p)) return none();
+  c.current_stream();
+  const int64_t need = lib.aq_compact_pages_workspace_bytes(p.n_pages);
+  Tensor table = c.empty({p.B, p.P}, ScalarType::Long), refs = c.empty({p.n_pages}, ScalarType::Int), where = c.empty({p.n_pages}, ScalarType::Long),
+         live = c.empty({1}, ScalarType::Int), ws = c.empty({need}, ScalarType::Byte);
+  const int rc = queued([&] {
+    return lib.aq_compact_pages(p.table->const_data_ptr<int64_t>(), p.B * p.P, p.refs->const_data_ptr<int32_t>(), p.k, p.v, p.layers, p.layer_bytes,
+                                p.n_pages, p.page, p.row_bytes, table.mutable_data_ptr<int64_t>(), refs.mutable_data_ptr<int32_t>(),
+                                where.mutable_data_ptr<int64_t>(), live.mutable_data_ptr<int32_t>(), ws.mutable_data_ptr(), need, c.stream);
+  });
+  return rc ? fail(rc, "aq_compact_pages") : tuple_of({&table, &refs, &where, &live});
   END_HANDLE_TH_ERRORS
 }
 
@@ -1083,6 +1227,9 @@ PyMethodDef methods[] = {
     AQ_METHOD(quant_tensor_fp8),
     AQ_METHOD(gemv_fp8_decode),
     AQ_METHOD(linear_fp8),
+    AQ_METHOD(paged_attn_decode_shared),
+    AQ_METHOD(fork_pages),
+    AQ_METHOD(compact_pages),
     AQ_METHOD(block_forward),
     {nullptr, nullptr, 0, nullptr},
 };

@@ -786,6 +786,10 @@ def paged_attn_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     are read once and multiplied with all sequences' queries at once.  The results agree with ``paged_attn_decode`` within bf16
     rounding; ``seq_lens`` as there.  ``workspace``: a contiguous device tensor to reuse across calls, of
     ``paged_attn_shared_workspace_bytes`` bytes; allocated per call when omitted or too small."""
+    if workspace is None:
+        y = (_host or _native()).paged_attn_decode_shared(q, k_cache, v_cache, page_table, total_len, shared_len, scale, seq_lens)
+        if y is not None:
+            return y
     _need_gpu(q, k_cache, v_cache, page_table)
     if q.dtype != torch.bfloat16 or k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
         raise ValueError("paged_attn_decode_shared takes bfloat16 tensors")
@@ -870,6 +874,9 @@ def fork_pages(page_table: torch.Tensor, refs: torch.Tensor, parents: torch.Tens
     sequences and sampling several continuations are one call, and no call waits for the device.  ``refs`` int32
     ``[n_pages]`` counts who holds each page.  The table and the counts given are left as they are; the caches (any type, of 16-byte
     rows) are written in place, free pages only."""
+    r = (_host or _native()).fork_pages(page_table, refs, parents, k_layers, v_layers, total_len, seq_lens)
+    if r is not None:
+        return ForkedPages(*r)
     _need_gpu(page_table, refs, parents, k_layers, v_layers)
     page_table, refs, caches = _pages_args(page_table, refs, k_layers, v_layers, "fork_pages")
     (B, P), n_pages, dev = page_table.shape, refs.numel(), refs.device
@@ -897,6 +904,9 @@ def compact_pages(page_table: torch.Tensor, refs: torch.Tensor, k_layers: torch.
     renumbers the table's entries: the last page held goes into the first free place, and so on, until pages 0 .. live - 1 are held.
     Entries that name a free page become -1.  The table and the counts given are left as they are; ``where`` tells other holders
     of pages where theirs went."""
+    r = (_host or _native()).compact_pages(page_table, refs, k_layers, v_layers)
+    if r is not None:
+        return CompactedPages(*r)
     _need_gpu(page_table, refs, k_layers, v_layers)
     page_table, refs, caches = _pages_args(page_table, refs, k_layers, v_layers, "compact_pages")
     n_pages, dev = refs.numel(), refs.device
