@@ -1,5 +1,4 @@
-// What the attention kernels on the matrix core share: rows of keys and values brought into LDS, and the two launches of
-// attn_decode.hip that other files queue.
+// What the attention kernels share that bring rows of keys and values into LDS and multiply them on the matrix core.
 #pragma once
 #include "aq_common.h"
 
@@ -31,25 +30,7 @@ __device__ __forceinline__ int row_key(int row) {
     return (int)(__builtin_bitreverse32((uint32_t)row & 15u) >> 28);
 }
 
-// Attention of one query per sequence over positions t0 .. T - 1 (t0 a multiple of 64) of its own pages, left as partial results
-// [D + 4] in slots slot0, slot0 + 1 .. of the NS slots of each (sequence, query head) in ws: attn_tail_slices(T - t0) of them.
-// Positions from lens[b] on weigh nothing, whatever is stored there; a sequence without any length weighs all of its positions alike.
-struct AttnTail {
-  const void *q, *kc, *vc;
-  const int64_t *table, *lens;
-  float* ws;
-  int64_t P, t0, T, page, n_pages, B, Hq, Hkv, D;
-  float scale;
-  int NS, slot0;
-};
-int64_t attn_tail_slices(int64_t positions);
-int attn_tail(const AttnTail& t, hipStream_t st);
-// Combines the NS slots of every (sequence, query head) into out [B, Hq, D].
-int attn_merge(const float* ws, void* out, int64_t B, int64_t Hq, int NS, int64_t D, hipStream_t st);
 // Query heads per KV head that the decode kernels are made for.
 inline bool attn_group_ok(int64_t G) { return G == 1 || G == 2 || G == 3 || G == 4 || G == 6 || G == 8; }
-constexpr int ATT_MAX_D = 128;
-// Floats of a slot, sized for the larger head dimension so that sizes do not depend on D.
-inline int64_t attn_workspace_bytes(int64_t B, int64_t Hq, int64_t ns) { return B * Hq * ns * (ATT_MAX_D + 4) * (int64_t)sizeof(float); }
 
 }  // namespace aq

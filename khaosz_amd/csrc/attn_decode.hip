@@ -18,7 +18,6 @@
 // bf16 tensors, head dimension 64 or 128, fp32 arithmetic.  Unmapped pages
 // (table entry < 0 or out of range) are skipped on write and read as zero keys
 // and values, as the reference's gather does.
-#include "aq_attn.h"
 #include "aq_common.h"
 #include "aq_rope.h"
 #include "aq_rows.h"
@@ -100,13 +99,12 @@ struct AttnArgs {
   int page_shift;  // log2 of a page of 64, 128, 256 .. positions, otherwise 62
   const int64_t* lens_at;  // lens, or without them anything of B numbers (the table): read without asking, beside the table
   UDiv by_hkv, by_ns, by_page;  // by_page: pages of other sizes, of launches whose positions it takes (mul 0: a division)
-  int64_t t0;            // TAIL kernels: the first position, a multiple of 64,
-  int tail_ns, slot0;    // the slices from there on, the first one's slot among the NS
 };
 
 constexpr int ATT_WAVES = 4;
 constexpr int ATT_KPW = 64;                  // positions per wavefront
 constexpr int ATT_KPG = ATT_WAVES * ATT_KPW; // positions per workgroup
+constexpr int ATT_MAX_D = 128;
 constexpr float ATT_MASKED = -1.0e30f;  // score (exp2 domain) of a cached position the sequence may not attend to
 
 // maximum / sum over each row of 16 consecutive lanes, result in all of them
@@ -164,8 +162,7 @@ typedef float attn_f32x4 __attribute__((ext_vector_type(4)));
 // chunk_sumsq) before they are used and stored: what rope_kv_write_kernel does with gains, same bits.  A head
 // vector's chunk c = 4 ks + kq sits in register ks of the lane with that kq.
 // WHOLE: pages of 64, 128, 256 .. positions: a wavefront's rows lie in one page.
-// TAIL: positions from t0 on only, partial results into slots of their own (attn_tail).
-template <int G, int D, bool WHOLE, bool ROPE, bool QKN = false, bool TAIL = false>
+template <int G, int D, bool WHOLE, bool ROPE, bool QKN = false>
 __global__ __launch_bounds__(ATT_WAVES * 64) void paged_attn_decode_kernel(AttnArgs p) {
   static_assert(!QKN || ROPE, "qk-norm belongs to the kernels that rotate");
   constexpr int CPR = D / 8;     // 16-byte chunks per row: 16 or 8
@@ -187,9 +184,9 @@ __global__ __launch_bounds__(ATT_WAVES * 64) void paged_attn_decode_kernel(AttnA
   // the KV heads of one slice are neighbours in the launch order: together they read whole
   // [position][Hkv][D] stretches of the pages at about the same time
   const int bs = p.by_hkv(blockIdx.x), kvh = blockIdx.x - bs * p.Hkv;
-  const int b = p.by_ns(bs), split = bs - b * (TAIL ? p.tail_ns : p.NS);
+  const int b = p.by_ns(bs), split = bs - b * p.NS;
   const int64_t T = p.T;
-  const int64_t t0 = (TAIL ? p.t0 : 0) + (int64_t)split * KPG + wave * KPW;  // first position of this wavefront
+  const int64_t t0 = (int64_t)split * KPG + wave * KPW;  // first position of this wavefront
   // Where the rows are.  WHOLE: one lookup, and every load's address is that plus the lane's own offset.  The table's entry
   // (otherwise its first, not used) and the sequence's length are requested before anything else and first used behind the
   // queries' requests (8 x 544 positions, 16/4 heads of 128: 9.46 us; 9.60 with divisions by the numbers of heads and slices, a
@@ -285,9 +282,6 @@ __global__ __launch_bounds__(ATT_WAVES * 64) void paged_attn_decode_kernel(AttnA
     // waited for each load before issuing the next).
     uint4 kb[4][KS], vv[NL];
     uint64_t there;  // bit per position: its row is there
-    // TAIL: rows behind the sequence's length are taken as zeros, so that nothing stored there (an infinity times a weight of zero)
-    // reaches the sums
-    const int64_t seen = TAIL && vis > 0 ? vis : T;
     if constexpr (WHOLE) {
       // (20 lookups by shuffle, with 64-bit arithmetic each, took 0.3 us of the launch at head dimension 64, and 0.1 to 0.2 at 128, where
       // 32 loads of 1 KiB wait for each other to be taken)
@@ -299,7 +293,7 @@ __global__ __launch_bounds__(ATT_WAVES * 64) void paged_attn_decode_kernel(AttnA
         for (int ks = 0; ks < KS; ++ks) kb[t][ks] = *reinterpret_cast<const uint4*>(ks0 + t * 16 * rstep + ks * 32);
 #pragma unroll
       for (int i = 0; i < NL; ++i) vv[i] = *reinterpret_cast<const uint4*>(vs0 + i * RPL * rstep);
-      there = first < 0 ? 0 : ~0ull >> (t0 + KPW > seen ? (int)(t0 + KPW - seen) : 0);
+      there = first < 0 ? 0 : ~0ull >> (t0 + KPW > T ? (int)(t0 + KPW - T) : 0);
     } else {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -313,7 +307,7 @@ __global__ __launch_bounds__(ATT_WAVES * 64) void paged_attn_decode_kernel(AttnA
         const int64_t r = row_of(i * RPL + sub);
         vv[i] = *reinterpret_cast<const uint4*>(p.vc + (r >= 0 ? r : 0) + ch * 8);
       }
-      there = __builtin_amdgcn_ballot_w64(row >= 0 && (!TAIL || t0 + lane < seen));
+      there = __builtin_amdgcn_ballot_w64(row >= 0);
     }
     __builtin_amdgcn_sched_barrier(0);  // nothing that waits for a load may move above the last load's issue
     if (there != ~0ull) {  // wavefront-uniform; rare: a hole, or the wavefront that holds T - 1
@@ -576,11 +570,11 @@ __global__ __launch_bounds__(ATT_WAVES * 64) void paged_attn_decode_kernel(AttnA
       den = __builtin_fmaf(l_s[w][g], a, den);
     }
     const int64_t head = (int64_t)b * p.Hq + kvh * G + g;
-    if (!TAIL && p.NS == 1 && p.out != nullptr) {  // out == nullptr: the caller wants the partial results whatever NS is
+    if (p.NS == 1 && p.out != nullptr) {  // out == nullptr: the caller wants the partial results whatever NS is
       const float r = attn_inv_denominator(den);
       store_wt(reinterpret_cast<uint32_t*>(p.out + head * D + d), pack_bf16x2(__fmul_rn(n0, r), __fmul_rn(n1, r)));
     } else {
-      float* part = p.ws + (head * p.NS + (TAIL ? p.slot0 : 0) + split) * PART;
+      float* part = p.ws + (head * p.NS + split) * PART;
       store_wt(reinterpret_cast<uint2*>(part + d), make_uint2(__float_as_uint(n0), __float_as_uint(n1)));
       if (d == 0) store_wt(reinterpret_cast<uint2*>(part + D), make_uint2(__float_as_uint(mm), __float_as_uint(den)));
     }
@@ -650,6 +644,10 @@ __global__ __launch_bounds__(ATT_MAX_D / 2) void attn_merge_kernel(const float* 
 }
 
 inline int64_t attn_slices(int64_t T) { return (T + ATT_KPG - 1) / ATT_KPG; }
+// sized for the larger head dimension, so that the size does not depend on D
+inline int64_t attn_workspace_bytes(int64_t B, int64_t Hq, int64_t ns) {
+  return B * Hq * ns * (ATT_MAX_D + 4) * (int64_t)sizeof(float);
+}
 
 }  // namespace aq
 
@@ -726,68 +724,6 @@ extern "C" int64_t aq_paged_attn_decode_workspace_bytes(int64_t B, int64_t Hq, i
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || total_len <= 0) return 0;
   const int64_t ns = aq::attn_slices(total_len);
   return ns == 1 ? 0 : aq::attn_workspace_bytes(B, Hq, ns);
-}
-
-int64_t aq::attn_tail_slices(int64_t positions) { return attn_slices(positions); }
-
-template <int D, bool WHOLE>
-static void attn_tail_launch(int64_t G, dim3 grid, dim3 block, hipStream_t st, const aq::AttnArgs& a) {
-#define AQ_TAIL_CASE(G_)                                                                                                       \
-  case G_:                                                                                                                     \
-    aq::queue_kernel((aq::paged_attn_decode_kernel<G_, D, WHOLE, false, false, true>), grid, block, 0, st, a);                 \
-    break;
-  switch (G) {
-    AQ_TAIL_CASE(1)
-    AQ_TAIL_CASE(2)
-    AQ_TAIL_CASE(3)
-    AQ_TAIL_CASE(4)
-    AQ_TAIL_CASE(6)
-    AQ_TAIL_CASE(8)
-  }
-#undef AQ_TAIL_CASE
-}
-
-int aq::attn_tail(const AttnTail& t, hipStream_t st) {
-  const int64_t ns = attn_slices(t.T - t.t0);
-  AttnArgs a{};
-  a.q = static_cast<const uint16_t*>(t.q);
-  a.kc = static_cast<const uint16_t*>(t.kc);
-  a.vc = static_cast<const uint16_t*>(t.vc);
-  a.table = t.table;
-  a.lens = t.lens;
-  a.ws = t.ws;
-  a.P = t.P;
-  a.T = t.T;
-  a.t0 = t.t0;
-  a.tail_ns = (int)ns;
-  a.slot0 = t.slot0;
-  a.page = t.page;
-  a.n_pages = t.n_pages;
-  a.scale_log2e = t.scale * 1.44269504088896341f;
-  a.B = (int)t.B;
-  a.Hq = (int)t.Hq;
-  a.Hkv = (int)t.Hkv;
-  a.NS = t.NS;
-  a.lens_at = t.lens ? t.lens : t.table;
-  a.by_hkv = UDiv::of((uint32_t)t.Hkv);
-  a.by_ns = UDiv::of((uint32_t)ns);
-  if (t.T <= ((int64_t)1 << 31) && t.page <= ((int64_t)1 << 31)) a.by_page = UDiv::of((uint32_t)t.page);
-  a.page_shift = 62;
-  for (int sh = 6; sh < 62; ++sh)
-    if (t.page == ((int64_t)1 << sh)) a.page_shift = sh;
-  const dim3 grid((unsigned)(t.B * t.Hkv * ns)), block(ATT_WAVES * 64);
-  const int64_t G = t.Hq / t.Hkv;
-  const bool whole = a.page_shift < 62;
-  if (t.D == 128)
-    (whole ? attn_tail_launch<128, true> : attn_tail_launch<128, false>)(G, grid, block, st, a);
-  else
-    (whole ? attn_tail_launch<64, true> : attn_tail_launch<64, false>)(G, grid, block, st, a);
-  return (int)hipGetLastError();
-}
-
-int aq::attn_merge(const float* ws, void* out, int64_t B, int64_t Hq, int NS, int64_t D, hipStream_t st) {
-  queue_kernel(attn_merge_kernel, dim3((unsigned)(B * Hq)), dim3((unsigned)(D / 2)), 0, st, ws, static_cast<uint16_t*>(out), NS, (int)D);
-  return (int)hipGetLastError();
 }
 
 template <int G, int D, bool WHOLE>

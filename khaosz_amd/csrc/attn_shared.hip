@@ -4,16 +4,17 @@
 // once for the whole batch:
 //
 //   prefix   the G query heads of a KV head of all B sequences are B G rows of one product against the shared keys: scores,
-//            softmax statistics and values per tile of rows and range of positions, left as partial results;
-//   tail     each sequence's own positions, by the decode kernel (attn_tail);
-//   merge    the partial results of a (sequence, query head) are weighed by exp2(maximum - overall maximum) and added up.
+//            softmax statistics and values per tile of rows and slice of positions, left as partial results;
+//   tail     the same for the G rows of one sequence against its own positions;
+//   merge    the partial results of a row are weighed by exp2(maximum - overall maximum) and added up.
 //
 // softmax over two ranges is the softmax over both: with m, l, n the maximum, denominator and numerator of each range,
 // out = (n1 2^(m1 - m) + n2 2^(m2 - m)) / (l1 2^(m1 - m) + l2 2^(m2 - m)), m = max(m1, m2).  All of them are fp32; probabilities
-// are rounded to bf16 (off by 2^-9 of themselves at most) where the matrix core takes them, the denominator sums them unrounded.
+// are rounded to bf16 (off by 2^-8 of themselves at most) where the matrix core takes them, the denominator sums them unrounded.
 //
-// The prefix kernel computes S^T = K Q^T and O^T = V^T P^T as the prefill kernel does (attn_prefill.hip has the layout): a lane
-// has the scores of one row, nothing changes lanes, K and V rows go straight into LDS one block ahead of the products.
+// Prefix and tail are workgroups of one launch, the prefix's first: those multiply while the tails read.  Both compute S^T = K Q^T and
+// O^T = V^T P^T as the prefill kernel does (attn_prefill.hip has the layout): a lane has the scores of one row, nothing changes lanes,
+// K and V rows go straight into LDS ahead of the products.
 #include "aq_attn.h"
 #include "aq_common.h"
 #include "aq_rows.h"
@@ -24,156 +25,77 @@ struct SharedArgs {
   const uint16_t* q;     // [B, Hq, D]
   const uint16_t* kc;    // [n_pages, page, Hkv, D]
   const uint16_t* vc;
-  const int64_t* table;  // the first sequence's row of the page table: the shared pages
+  const int64_t* table;  // [B, P]; row 0 has the shared pages
   const int64_t* lens;   // [B] or null
-  float* ws;             // [B, Hq, NS, D + 4]; slots 0 .. slices - 1 are written
+  float* ws;             // partial results: [slices][Hkv][tiles of 32 rows] of the prefix, then [B][Hkv][tails]
   int64_t page, n_pages, P;
   float scale_log2e;
-  int T, rows, Hq, Hkv, G, NS;
-  int blocks, per_slice, slices, tiles;  // blocks of 64 shared positions, of one slice; slices; tiles of rows
-  int page_shift;                        // log2 of the page size, or -1
-  int table_lds;                         // entries of the page table that a slice may need, kept in LDS (0: read from memory)
-  UDiv by_g, by_page, by_tiles, by_hkv;
+  int T, s0, rows, Hq, Hkv, G;      // positions, of which the prefix takes s0 (a multiple of 64); B G
+  int slice, slices, tiles, tiles32;  // positions of a prefix slice; slices; tiles of rows of a workgroup, of 32
+  int tail, tails;                  // positions of a tail's slice, slices of a sequence
+  int prefix_wgs;                   // the workgroups behind them are tails
+  int page_shift;                   // log2 of the page size, or -1
+  int table_lds;                    // entries of the page table that a workgroup may need, kept in LDS (0: read from memory)
+  UDiv by_g, by_page, by_tiles, by_hkv, by_tails;
 };
 
 constexpr float SHARED_MASKED = -1.0e30f;  // score (exp2 domain) of a position the sequence may not attend to, as in the decode kernel
 
-// QW x KW wavefronts: QW tiles of 32 rows side by side on the same block of 64 positions, KW blocks at a time.
-template <int D, int QW, int KW>
-__global__ __launch_bounds__(QW* KW * 64) __attribute__((amdgpu_waves_per_eu(D == 128 && KW == 2 ? 1 : 2))) void shared_attn_kernel(SharedArgs p) {
-  constexpr int KB = 64, NT = KB / 32, DSTEPS = D / 16, DT = D / 32;
-  constexpr int ROWB = 2 * D;                       // bytes of a K or V row
-  constexpr int RPI = 1024 / ROWB, LPR = 64 / RPI;  // rows of a 1 KiB load, lanes of a row
-  constexpr int TILE = KB * ROWB;                   // bytes of a block's K (or V)
-  constexpr int LOADS = TILE / 1024 / QW;           // 1 KiB loads of K (and of V) per wavefront and block
-  constexpr int BUF = KW * 2 * TILE;
-  static_assert(LOADS >= 1 && TILE % (1024 * QW) == 0, "whole loads per wavefront");
-  static_assert((KW - 1) * QW * (DT * 16 + 2) * 256 <= 2 * BUF, "the wavefronts' sums fit the buffers");
-  __shared__ int seen_s[QW];
-  extern __shared__ __align__(1024) uint8_t sh_lds[];  // 2 buffers of KW [K block | V block]; page table
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int qw = wave % QW, kw = wave / QW;
-  const int col = lane & 31, g = lane >> 5;
-  // Workgroups i and i + 8 run on one XCD: the tiles of a (KV head, slice) follow one another there, so that its L2 has the keys and
-  // values the first one read.
-  const int turn = (int)blockIdx.x >> 3, ty = p.by_tiles(turn), tile = turn - ty * p.tiles, combo = ty * 8 + ((int)blockIdx.x & 7);
-  if (combo >= p.slices * p.Hkv) return;
-  const int slice = p.by_hkv(combo), kvh = combo - slice * p.Hkv;
-  const int j0 = slice * p.per_slice, j1 = j0 + p.per_slice < p.blocks ? j0 + p.per_slice : p.blocks;
-  const int nit = (j1 - j0 + KW - 1) / KW;
+// A partial result of n rows: numerators as 16-byte groups of 4 dimensions, the n rows of a group side by side (what the lanes of a
+// product hold, so that it is stored and read by whole lines), then the n maxima and the n denominators.
+__host__ __device__ constexpr int part_floats(int D, int n) { return (D + 4) * n; }
 
-  const int r0 = (tile * QW + qw) * 32, row = r0 + col < p.rows ? r0 + col : p.rows - 1;  // rows past the end: the last one again
-  const int b = p.by_g(row), head = kvh * p.G + (row - b * p.G);
-  int vis = p.T, seen = p.T;  // positions this lane's row may attend to; that any row of the workgroup looks at
-  int* const table = reinterpret_cast<int*>(sh_lds + 2 * BUF);
-  auto phys_of = [&](int lp) -> int {
-    const int64_t t = lp < p.P ? p.table[lp] : -1;
-    return t >= 0 && t < p.n_pages ? (int)t : -1;
-  };
-  const int lp0 = p.table_lds ? (int)p.by_page((uint32_t)(j0 * KB)) : 0;
-  if (p.table_lds) {
-    for (int i = tid; i < p.table_lds; i += QW * KW * 64) table[i] = phys_of(lp0 + i);
-    if (!p.lens) __syncthreads();
-  }
-  if (p.lens) {
-    const int64_t n = p.lens[b];
-    vis = n <= 0 ? 0 : n < p.T ? (int)n : p.T;
-    int most = vis ? vis : p.T;  // a row without any length weighs every position alike
+// s_waitcnt for n vector-memory operations still in flight (gfx9 encoding), and a barrier that leaves them in flight.
+#define SH_WAIT_VMCNT(n) __builtin_amdgcn_s_waitcnt(0x0f70 | ((n) & 15) | (((n) >> 4) << 14))
+#define SH_WAIT_LGKM() __builtin_amdgcn_s_waitcnt(0xc07f)
+__device__ __forceinline__ void sh_barrier() {
+  asm volatile("" ::: "memory");
+  SH_WAIT_LGKM();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// What a wavefront keeps of its 32 rows: lane = (row col, half g of the positions of a 32 x 32 product).
+template <int D>
+struct SharedRows {
+  uint4 qf[D / 16];    // Q^T operand: dimensions 16 step + 8 g .. + 8
+  pa_f32x16 o[D / 32];  // O^T: register r of tile dt is dimension 32 dt + 8 (r / 4) + 4 g + r % 4
+  float m, l;          // bound of the row's scores; this lane's half of its denominator
+  int vis;             // positions the row may attend to, 0 .. T
+
+  __device__ __forceinline__ void start(const uint16_t* q, int g, int visible) {
 #pragma unroll
-    for (int off = 32; off; off >>= 1) {
-      const int o = __shfl_xor(most, off, 64);
-      most = o > most ? o : most;
-    }
-    if (kw == 0 && lane == 0) seen_s[qw] = most;
-    __syncthreads();
-    seen = seen_s[0];
+    for (int st = 0; st < D / 16; ++st) qf[st] = *reinterpret_cast<const uint4*>(q + g * 8 + st * 16);
 #pragma unroll
-    for (int i = 1; i < QW; ++i) seen = seen_s[i] > seen ? seen_s[i] : seen;
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
+    m = -INFINITY;
+    l = 0.0f;
+    vis = visible;
   }
 
-  const int chunk0 = qw * LOADS;
-  int pc[LOADS];  // this lane's piece of the rows that the wavefront's loads bring: elements into the row
-#pragma unroll
-  for (int c = 0; c < LOADS; ++c) pc[c] = ((lane % LPR) ^ row_key<D>((chunk0 + c) * RPI + lane / LPR)) * 8;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(pa_lds_void*)sh_lds;
-  auto issue = [&](int it, int buf) __attribute__((always_inline)) {
-    const int j = j0 + it * KW + kw;
-    if (j >= j1) return;  // wavefront-uniform
-    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + buf * BUF + kw * 2 * TILE + chunk0 * 1024);
-    const int rows = seen - j * KB;  // rows that no one looks at are zeros, whatever is stored there
-    const uint16_t* const zero = reinterpret_cast<const uint16_t*>(pa_zero_row);
-    if (p.page_shift >= 6) {  // the whole block lies in one page
-      const int lp = __builtin_amdgcn_readfirstlane((j * KB) >> p.page_shift);
-      const int64_t phys = lp < p.P ? p.table[lp] : -1;
-      const bool mapped = phys >= 0 && phys < p.n_pages;
-      const int64_t first = mapped ? (((phys << p.page_shift) + (j * KB - (lp << p.page_shift))) * p.Hkv + kvh) * D : 0;
-      const int step = p.Hkv * D;
-#pragma unroll
-      for (int c = 0; c < LOADS; ++c) {
-        const int r = (chunk0 + c) * RPI + lane / LPR;
-        const bool there = mapped && r < rows;
-        const uint32_t at = (uint32_t)(r * step + pc[c]);
-        load_row_lds(there ? p.kc + first + at : zero + pc[c], dst + c * 1024);
-        load_row_lds(there ? p.vc + first + at : zero + pc[c], dst + TILE + c * 1024);
-      }
-      return;
-    }
-    // every address first, then the loads: a load is a fence to the compiler, and a lookup behind each one would wait for LDS once per row
-    int64_t at[LOADS];
-#pragma unroll
-    for (int c = 0; c < LOADS; ++c) {
-      const int r = (chunk0 + c) * RPI + lane / LPR, key = j * KB + r;
-      const int lp = p.by_page((uint32_t)key), in_page = key - lp * (int)p.page;
-      const int phys = r >= rows ? -1 : p.table_lds ? table[lp - lp0] : phys_of(lp);
-      at[c] = phys < 0 ? -1 : (((int64_t)phys * p.page + in_page) * p.Hkv + kvh) * D;
-    }
-#pragma unroll
-    for (int c = 0; c < LOADS; ++c) {
-      load_row_lds((at[c] < 0 ? zero : p.kc + at[c]) + pc[c], dst + c * 1024);
-      load_row_lds((at[c] < 0 ? zero : p.vc + at[c]) + pc[c], dst + TILE + c * 1024);
-    }
-  };
-  issue(0, 0);
-
-  uint4 qf[DSTEPS];  // Q^T operand: lane = (row col, dimensions 16 step + 8 g .. + 8)
-  {
-    const uint16_t* src = p.q + ((int64_t)b * p.Hq + head) * D + g * 8;
-#pragma unroll
-    for (int st = 0; st < DSTEPS; ++st) qf[st] = *reinterpret_cast<const uint4*>(src + st * 16);
-  }
-  // fragment addresses inside a block: K row `col`, piece 2 step + g; V rows 4 g + i / 4 (and 8 further), i = lane % 16,
-  // dimensions 16 (lane / 16 % 2) + 4 (i % 4) of a 32-dimension tile
-  const int kfr = col * ROWB + ((g ^ row_key<D>(col)) << 4);  // ^ (2 step) << 4
-  const int vrow = 4 * g + (lane & 15) / 4, vpiece = ((lane >> 4) & 1) * 2 + (lane & 3) / 2;
-  const int vfr0 = vrow * ROWB + ((vpiece ^ row_key<D>(vrow)) << 4) + (lane & 1) * 8;  // ^ dt << 6
-  const int vfr1 = (vrow + 8) * ROWB + ((vpiece ^ row_key<D>(vrow + 8)) << 4) + (lane & 1) * 8;
-
-  pa_f32x16 o[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
-  float m = -INFINITY, l = 0.0f;  // bound of this lane's row's scores; this lane's half of its denominator
-  const bool idle = r0 >= p.rows;  // wavefront-uniform: no row here, only loads
-
-  for (int it = 0; it < nit; ++it) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): block `it` has landed
-    __syncthreads();                     // ... everyone's part of it, and everyone is done with the one before
-    if (it + 1 < nit) issue(it + 1, (it + 1) & 1);
-    const int j = j0 + it * KW + kw, kb0 = j * KB;
-    if (idle || j >= j1) continue;  // wavefront-uniform
-    const bool some = p.lens && __builtin_amdgcn_ballot_w64(kb0 + KB > vis) != 0;  // some row may not attend to some position
-    if (some && __builtin_amdgcn_ballot_w64(vis == 0 || kb0 < vis) == 0) continue;  // none to any
-    const uint8_t* ks = sh_lds + (it & 1) * BUF + kw * 2 * TILE;
-    const uint8_t* vs = ks + TILE;
-    // ---- scores; the fragments of K are read two steps ahead of the products that take them
+  // 32 NT positions from kb0 on, K rows at ks and V rows at vs.  masked (wavefront-uniform): some row may not attend to some of them, or
+  // there are only T.
+  // keys_read() is called when the last K row has been read, values_needed() before the first V row is.
+  template <int NT, class FK, class FV>
+  __device__ __forceinline__ void attend(const uint8_t* ks, const uint8_t* vs, int kb0, bool masked, int T, float scale_log2e,
+                                         FK&& keys_read, FV&& values_needed) {
+    constexpr int DSTEPS = D / 16, DT = D / 32, ROWB = 2 * D;
+    const int lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
+    // fragment addresses inside a block: K row `col`, piece 2 step + g; V rows 4 g + i / 4 (and 8 further), i = lane % 16,
+    // dimensions 16 (lane / 16 % 2) + 4 (i % 4) of a 32-dimension tile
+    const int kfr = col * ROWB + ((g ^ row_key<D>(col)) << 4);  // ^ (2 step) << 4
+    const int vrow = 4 * g + (lane & 15) / 4, vpiece = ((lane >> 4) & 1) * 2 + (lane & 3) / 2;
+    const int vfr0 = vrow * ROWB + ((vpiece ^ row_key<D>(vrow)) << 4) + (lane & 1) * 8;  // ^ dt << 6
+    const int vfr1 = (vrow + 8) * ROWB + ((vpiece ^ row_key<D>(vrow + 8)) << 4) + (lane & 1) * 8;
+    // ---- scores; the fragments of K are read two groups of steps ahead of the products that take them
     pa_f32x16 s[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
     {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
       constexpr int GRP = 4 / NT, NG = DSTEPS / GRP;
       uint4 fa[2][GRP][NT];
       auto ldk = [&](int buf, int st0) __attribute__((always_inline)) {
@@ -199,18 +121,25 @@ __global__ __launch_bounds__(QW* KW * 64) __attribute__((amdgpu_waves_per_eu(D =
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    keys_read();
     // ---- softmax of this lane's row; register r of tile kt is position kb0 + 32 kt + 8 (r / 4) + 4 g + r % 4
-    float sc = p.scale_log2e;
-    if (some) {  // the scores are scaled here, so that a masked one has the same value in every slice
+    float sc = scale_log2e;
+    if (masked) {  // the scores are scaled here, so that a masked one has the same value in every slice
 #pragma unroll
       for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = kb0 + kt * 32 + 8 * (r / 4) + 4 * g + (r % 4);
-          s[kt][r] = key < vis ? s[kt][r] * sc : SHARED_MASKED;
+          s[kt][r] = key < vis ? s[kt][r] * sc : key < T ? SHARED_MASKED : -INFINITY;
         }
       sc = 1.0f;
     }
+    softmax_values<NT>(s, vs, vfr0, vfr1, sc, values_needed);
+  }
+
+  template <int NT, class FV>
+  __device__ __forceinline__ void softmax_values(pa_f32x16 (&s)[NT], const uint8_t* vs, int vfr0, int vfr1, float sc, FV&& values_needed) {
+    constexpr int DT = D / 32, ROWB = 2 * D;
     float bm = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt)
@@ -242,6 +171,7 @@ __global__ __launch_bounds__(QW* KW * 64) __attribute__((amdgpu_waves_per_eu(D =
         pf[kt][s2] = make_uint4(pack_bf16x2(pv[8 * s2 + 0], pv[8 * s2 + 1]), pack_bf16x2(pv[8 * s2 + 2], pv[8 * s2 + 3]),
                                 pack_bf16x2(pv[8 * s2 + 4], pv[8 * s2 + 5]), pack_bf16x2(pv[8 * s2 + 6], pv[8 * s2 + 7]));
     }
+    values_needed();
     // ---- O^T += V^T P^T; all fragments of V are read before the products, whose chains alternate
     constexpr int KK = 2 * NT;
     pa_bf16x8 fv[DT][KK];
@@ -263,91 +193,412 @@ __global__ __launch_bounds__(QW* KW * 64) __attribute__((amdgpu_waves_per_eu(D =
         for (int dt = d0; dt < d0 + 2; ++dt)
           o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv[dt][kk], __builtin_bit_cast(pa_bf16x8, pf[kk >> 1][kk & 1]), o[dt], 0, 0, 0);
   }
-  const LanePair l2 = lanes32_pair(l);
-  l = l2.x + l2.y;
-  // ---- the KW wavefronts of a tile of rows add up their sums
-  if constexpr (KW > 1) {
-    constexpr int SUMS = DT * 16 * 64;  // floats
-    float* const to = reinterpret_cast<float*>(sh_lds) + ((kw - 1) * QW + qw) * (SUMS + 128) + lane;
-    __syncthreads();  // everyone is done with the blocks
-    if (kw > 0) {
+
+  // Whether some row may not attend to some of the positions kb0 .. kb0 + n - 1; *none: no row to any.
+  __device__ __forceinline__ bool masked(const int64_t* lens, int kb0, int n, bool* none) const {
+    *none = false;
+    if (!lens || __builtin_amdgcn_ballot_w64(kb0 + n > vis) == 0) return false;
+    *none = __builtin_amdgcn_ballot_w64(vis == 0 || kb0 < vis) == 0;
+    return true;
+  }
+
+  // A partial result of n rows; a row that saw nothing leaves its maximum only.
+  __device__ __forceinline__ void store(float* part, int n) const {
+    const int lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
+    const LanePair l2 = lanes32_pair(l);
+    if (col >= n) return;
+    if (m != -INFINITY) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) to[(dt * 16 + r) * 64] = o[dt][r];
-      to[SUMS] = m;
-      to[SUMS + 64] = l;
+      for (int i = 0; i < D / 8; ++i)
+        *reinterpret_cast<v4f*>(part + ((2 * i + g) * n + col) * 4) = v4f{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2],
+                                                                         o[i / 4][4 * (i % 4) + 3]};
     }
-    __syncthreads();
-    if (kw > 0) return;
+    if (g == 0) part[D * n + col] = m;
+    else part[(D + 1) * n + col] = l2.x + l2.y;
+  }
+
+  // The same of the KW wavefronts that share these rows (as the tile-th of `tiles`), whose sums meet in LDS: each adds up and stores its
+  // share of the dimensions.  lds: 32 D numbers a wavefront that no load is still to arrive in; ml: 128.  (One wavefront that adds up and
+  // stores everything takes 2.0 us of a tail's 8.7, this 1.)
+  template <int KW>
+  __device__ __forceinline__ void join_and_store(v4f* lds, float* ml, int kw, int tile, int tiles, float* part, int n) const {
+    constexpr int GROUPS = D / 8, SHARE = GROUPS / KW;  // groups of 4 sums
+    const int lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5, at = kw * tiles + tile;
+    const LanePair l2 = lanes32_pair(l);
 #pragma unroll
-    for (int k = 1; k < KW; ++k) {
-      const float* from = reinterpret_cast<const float*>(sh_lds) + ((k - 1) * QW + qw) * (SUMS + 128) + lane;
-      const float mk = from[SUMS], lk = from[SUMS + 64], mn = fmaxf(m, mk);
-      const float a0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), a1 = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - mn);
-      m = mn;
-      l = l * a0 + lk * a1;
+    for (int i = 0; i < GROUPS; ++i)
+      lds[(at * GROUPS + i) * 64 + lane] = v4f{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
+    ml[at * 128 + lane] = m;
+    ml[at * 128 + 64 + lane] = l2.x + l2.y;
+    sh_barrier();
+    float w[KW], most = -INFINITY, sum = 0.0f;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+    for (int k = 0; k < KW; ++k) {
+      w[k] = ml[(k * tiles + tile) * 128 + lane];
+      most = fmaxf(most, w[k]);
+    }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] = __builtin_fmaf(from[(dt * 16 + r) * 64], a1, o[dt][r] * a0);
+    for (int k = 0; k < KW; ++k) {
+      w[k] = w[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w[k] - most);
+      sum = __builtin_fmaf(ml[(k * tiles + tile) * 128 + 64 + lane], w[k], sum);
+    }
+    if (col >= n) return;
+    if (most != -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < SHARE; ++i) {
+        const int c = kw * SHARE + i;
+        v4f x = lds[(tile * GROUPS + c) * 64 + lane];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) x[d] *= w[0];
+#pragma unroll
+        for (int k = 1; k < KW; ++k) {
+          const v4f y = lds[((k * tiles + tile) * GROUPS + c) * 64 + lane];
+#pragma unroll
+          for (int d = 0; d < 4; ++d) x[d] = __builtin_fmaf(y[d], w[k], x[d]);
+        }
+        *reinterpret_cast<v4f*>(part + ((2 * c + g) * n + col) * 4) = x;
+      }
+    }
+    if (kw == 0) part[(g == 0 ? D : D + 1) * n + col] = g == 0 ? most : sum;
+  }
+};
+
+// The page table of one sequence.
+struct SharedPages {
+  const int64_t* table;
+  int* lds;  // ids of the pages from lp0 on, or null
+  int lp0;
+
+  __device__ __forceinline__ int phys(const SharedArgs& p, int lp) const {
+    const int64_t t = lp < p.P ? table[lp] : -1;
+    return t >= 0 && t < p.n_pages ? (int)t : -1;
+  }
+  // (a barrier has to follow before load() is called)
+  __device__ __forceinline__ void fetch(const SharedArgs& p, int first, int* place, int threads) {
+    lds = nullptr;
+    lp0 = 0;
+    if (!p.table_lds) return;
+    lds = place;
+    lp0 = (int)p.by_page((uint32_t)first);
+    for (int i = threadIdx.x; i < p.table_lds; i += threads) lds[i] = phys(p, lp0 + i);
+  }
+
+  // N loads of 1 KiB: rows r0, r0 + rows of a load, .. of the block of KB positions at kb0, into LDS from `dst` on, those of keys and (BOTH) of
+  // values `apart` bytes further.  Rows from `seen` on, which no one looks at, are zeros whatever is stored there; so are unmapped pages.
+  template <int D, int KB, int N, bool KEYS, bool VALUES>
+  __device__ __forceinline__ void load(const SharedArgs& p, int kvh, int kb0, int seen, int r0, uint32_t dst, uint32_t apart) const {
+    constexpr int ROWB = 2 * D, RPI = 1024 / ROWB, LPR = 64 / RPI;
+    const int lane = threadIdx.x & 63;
+    const int rows = seen - kb0;
+    const uint16_t* const zero = reinterpret_cast<const uint16_t*>(pa_zero_row);
+    int pc[N];  // this lane's piece of the rows: elements into the row
+#pragma unroll
+    for (int c = 0; c < N; ++c) pc[c] = ((lane % LPR) ^ row_key<D>(r0 + c * RPI + lane / LPR)) * 8;
+    constexpr int SHIFT = KB == 64 ? 6 : 5;
+    if (p.page_shift >= SHIFT) {  // the whole block lies in one page
+      const int lp = __builtin_amdgcn_readfirstlane(kb0 >> p.page_shift);
+      const int64_t id = rows > 0 && lp < p.P ? table[lp] : -1;
+      const bool mapped = id >= 0 && id < p.n_pages;
+      const int64_t first = mapped ? (((id << p.page_shift) + (kb0 - (lp << p.page_shift))) * p.Hkv + kvh) * D : 0;
+      const int step = p.Hkv * D;
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        const int r = r0 + c * RPI + lane / LPR;
+        const bool there = mapped && r < rows;
+        const uint32_t at = (uint32_t)(r * step + pc[c]);
+        if (KEYS) load_row_lds(there ? p.kc + first + at : zero + pc[c], dst + c * 1024);
+        if (VALUES) load_row_lds(there ? p.vc + first + at : zero + pc[c], dst + (KEYS ? apart : 0) + c * 1024);
+      }
+      return;
+    }
+    // every address first, then the loads: a load is a fence to the compiler, and a lookup behind each one would wait for LDS once per row
+    int64_t at[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const int r = r0 + c * RPI + lane / LPR, key = kb0 + r;
+      const int lp = p.by_page((uint32_t)key), in_page = key - lp * (int)p.page;
+      const int id = r >= rows ? -1 : lds ? lds[lp - lp0] : phys(p, lp);
+      at[c] = id < 0 ? -1 : (((int64_t)id * p.page + in_page) * p.Hkv + kvh) * D;
+    }
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      if (KEYS) load_row_lds((at[c] < 0 ? zero : p.kc + at[c]) + pc[c], dst + c * 1024);
+      if (VALUES) load_row_lds((at[c] < 0 ? zero : p.vc + at[c]) + pc[c], dst + (KEYS ? apart : 0) + c * 1024);
     }
   }
-  // ---- register r of tile dt is dimension 32 dt + 8 (r / 4) + 4 g + r % 4 of row col
-  if (r0 + col < p.rows) {
-    float* part = p.ws + (((int64_t)b * p.Hq + head) * p.NS + slice) * (D + 4);
+};
+
+__device__ __forceinline__ int visible(const SharedArgs& p, int b) {
+  if (!p.lens) return p.T;
+  const int64_t n = p.lens[b];
+  return n <= 0 ? 0 : n < p.T ? (int)n : p.T;
+}
+
+// A tile of 32 QW rows of all sequences against a slice of the shared positions.  QW x KW wavefronts: QW tiles of 32 rows side by side on
+// the same block of KB positions, KW blocks at a time, the next KW ahead of the products.  (More buffers gain nothing: 64 x 8192 positions
+// of 32/8 heads of 128 20.0 us with two, 22.2 with four that leave room for one workgroup per compute unit.)
+template <int D, int QW, int KW, int KB>
+__device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds, float* ml, int* table_lds) {
+  constexpr int ROWB = 2 * D, RPI = 1024 / ROWB;    // bytes of a K or V row; rows of a 1 KiB load
+  constexpr int TILE = KB * ROWB;                   // bytes of a block's K (or V)
+  constexpr int LOADS = TILE / 1024 / QW;           // 1 KiB loads of K (and of V) per wavefront and block
+  constexpr int BUF = KW * 2 * TILE;
+  static_assert(LOADS >= 1 && TILE % (1024 * QW) == 0, "whole loads per wavefront");
+  static_assert(KW == 1 || KW * QW * 128 * D <= 2 * BUF, "the wavefronts' sums fit the buffers");
+  __shared__ int seen_s[QW];
+  const int lane = threadIdx.x & 63, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), qw = wave % QW, kw = wave / QW;
+  // Workgroups i and i + 8 run on one XCD: the tiles of a (KV head, slice) follow one another there, so that its L2 has the keys and
+  // values the first one read.
+  const int turn = (int)blockIdx.x >> 3, ty = p.by_tiles(turn), tile = turn - ty * p.tiles, combo = ty * 8 + ((int)blockIdx.x & 7);
+  if (combo >= p.slices * p.Hkv) return;
+  const int slice = p.by_hkv(combo), kvh = combo - slice * p.Hkv;
+  const int k0 = slice * p.slice, k1 = k0 + p.slice < p.s0 ? k0 + p.slice : p.s0;
+  const int nit = (k1 - k0 + KW * KB - 1) / (KW * KB);
+
+  const int t32 = tile * QW + qw, r0 = t32 * 32, row = r0 + col < p.rows ? r0 + col : p.rows - 1;  // rows past the end: the last one again
+  const int b = p.by_g(row), head = kvh * p.G + (row - b * p.G);
+  SharedPages pages{p.table, nullptr, 0};
+  pages.fetch(p, k0, table_lds, QW * KW * 64);
+  const int vis = visible(p, b);
+  int seen = k1;  // positions that any row of the workgroup looks at
+  if (p.lens) {
+    int most = vis ? vis : p.T;  // a row without any length weighs every position alike
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int off = 32; off; off >>= 1) {
+      const int o = __shfl_xor(most, off, 64);
+      most = o > most ? o : most;
+    }
+    if (kw == 0 && lane == 0) seen_s[qw] = most;
+    __syncthreads();
+    most = seen_s[0];
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
-        *reinterpret_cast<float4*>(part + dt * 32 + 8 * a + 4 * g) = make_float4(o[dt][4 * a], o[dt][4 * a + 1], o[dt][4 * a + 2], o[dt][4 * a + 3]);
-    if (g == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
+    for (int i = 1; i < QW; ++i) most = seen_s[i] > most ? seen_s[i] : most;
+    seen = most < k1 ? most : k1;
+  } else if (p.table_lds) {
+    __syncthreads();
+  }
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(pa_lds_void*)lds;
+  auto issue = [&](int it, int buf) __attribute__((always_inline)) {
+    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + buf * BUF + kw * 2 * TILE + qw * LOADS * 1024);
+    pages.template load<D, KB, LOADS, true, true>(p, kvh, k0 + (it * KW + kw) * KB, seen, qw * LOADS * RPI, dst, TILE);
+  };
+  issue(0, 0);
+  SharedRows<D> rows;
+  rows.start(p.q + ((int64_t)b * p.Hq + head) * D, lane >> 5, vis);
+  const bool idle = r0 >= p.rows;  // wavefront-uniform: no row here, only loads
+
+  for (int it = 0; it < nit; ++it) {
+    SH_WAIT_VMCNT(0);  // this wavefront's part of the blocks has landed
+    sh_barrier();      // ... everyone's, and everyone is done with the ones before
+    if (it + 1 < nit) issue(it + 1, (it + 1) & 1);
+    const int kb0 = k0 + (it * KW + kw) * KB;
+    bool none;
+    const bool masked = rows.masked(p.lens, kb0, KB, &none);
+    if (idle || none || kb0 >= k1) continue;  // wavefront-uniform
+    const uint8_t* ks = lds + (it & 1) * BUF + kw * 2 * TILE;
+    rows.template attend<KB / 32>(ks, ks + TILE, kb0, masked, p.T, p.scale_log2e, [] {}, [] {});
+  }
+  const int n = p.rows - r0 < 32 ? p.rows - r0 : 32;  // idle: none
+  float* const part = p.ws + (int64_t)((slice * p.Hkv + kvh) * p.tiles32 + t32) * part_floats(D, 32);
+  if constexpr (KW > 1) {
+    sh_barrier();  // everyone is done with the blocks
+    rows.template join_and_store<KW>(reinterpret_cast<v4f*>(lds), ml, kw, qw, QW, part, n);
+  } else if (!idle) {
+    rows.store(part, n);
   }
 }
 
-// How a call is cut: `blocks` blocks of 64 shared positions (a part of one is left to the tails), per_slice of them to a workgroup.
+// The G rows of one sequence against a slice of its own positions.  KW wavefronts, each by itself: blocks of 32 positions in turn, the
+// next block's keys requested when the last key has been read, its values when the last value has.
+template <int D, int KW>
+__device__ __forceinline__ void shared_tail(const SharedArgs& p, uint8_t* lds, float* ml, int* table_lds) {
+  constexpr int KB = 32, TILE = KB * 2 * D, LOADS = TILE / 1024;
+  static_assert(128 * D <= 2 * TILE, "the wavefronts' sums fit the buffers");
+  const int lane = threadIdx.x & 63, col = lane & 31, kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wg = (int)blockIdx.x - p.prefix_wgs, bh = p.by_tails(wg), slice = wg - bh * p.tails, b = p.by_hkv(bh), kvh = bh - b * p.Hkv;
+  const int k0 = p.s0 + slice * p.tail, k1 = k0 + p.tail < p.T ? k0 + p.tail : p.T;
+  const int vis = visible(p, b), seen = vis && vis < k1 ? vis : k1;  // rows behind the sequence's length: zeros
+  SharedPages pages{p.table + (int64_t)b * p.P, nullptr, 0};
+  pages.fetch(p, k0, table_lds, KW * 64);
+  if (p.table_lds) __syncthreads();
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(pa_lds_void*)lds + kw * 2 * TILE);
+  uint8_t* const ks = lds + kw * 2 * TILE;
+  int kb0 = k0 + kw * KB;
+  SharedRows<D> rows;
+  rows.start(p.q + ((int64_t)b * p.Hq + kvh * p.G + (col < p.G ? col : 0)) * D, lane >> 5, vis);
+  if (kb0 < seen) {  // wavefront-uniform, as all below
+    pages.template load<D, KB, LOADS, true, false>(p, kvh, kb0, seen, 0, at, 0);
+    pages.template load<D, KB, LOADS, false, true>(p, kvh, kb0, seen, 0, at + TILE, 0);
+    // The queries have arrived, as far as the compiler knows too: otherwise it waits for them in every turn, by a count that takes in
+    // the blocks on their way.
+    SH_WAIT_VMCNT(0);
+    for (;;) {
+      const int next = kb0 + KW * KB;
+      const bool more = next < seen;
+      asm volatile("" ::: "memory");
+      rows.template attend<1>(
+          ks, ks + TILE, kb0, kb0 + KB > vis, p.T, p.scale_log2e,
+          [&] {
+            SH_WAIT_LGKM();
+            if (more) pages.template load<D, KB, LOADS, true, false>(p, kvh, next, seen, 0, at, 0);
+          },
+          [&] {
+            if (more) SH_WAIT_VMCNT(LOADS);  // this block's values have landed
+            else SH_WAIT_VMCNT(0);
+            asm volatile("" ::: "memory");
+          });
+      if (!more) break;
+      SH_WAIT_LGKM();
+      pages.template load<D, KB, LOADS, false, true>(p, kvh, next, seen, 0, at + TILE, 0);
+      SH_WAIT_VMCNT(LOADS);  // the next block's keys have
+      kb0 = next;
+    }
+  }
+  // (the sums go where this wavefront's own blocks were)
+  const int64_t prefix = (int64_t)p.slices * p.Hkv * p.tiles32 * part_floats(D, 32);
+  rows.template join_and_store<KW>(reinterpret_cast<v4f*>(lds), ml, kw, 0, 1, p.ws + prefix + (int64_t)wg * part_floats(D, p.G), p.G);
+}
+
+constexpr int SHARED_LDS = 512;  // bytes of the blocks of either kind of workgroup, per dimension
+
+template <int D, int QW, int KW, int KB>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void shared_attn_kernel(SharedArgs p) {
+  static_assert(QW * KW == 4 && 2 * KW * KB * 4 * D == SHARED_LDS * D, "four wavefronts, 128 D bytes each");
+  __shared__ float ml[4 * 128];
+  extern __shared__ __align__(1024) uint8_t sh_lds[];  // blocks; page table
+  int* const table = reinterpret_cast<int*>(sh_lds + SHARED_LDS * D);
+  if ((int)blockIdx.x < p.prefix_wgs) shared_prefix<D, QW, KW, KB>(p, sh_lds, ml, table);
+  else shared_tail<D, 4>(p, sh_lds, ml, table);
+}
+
+// The slices of a row added up: a half wavefront has 4 dimensions of the 32 rows of a tile, so that the prefix's slices are read by whole
+// lines, and every PARTS-th slice, four of them requested before any is used; the parts meet in LDS.
+template <int D, int PARTS>
+__global__ __launch_bounds__(PARTS * 32) void shared_merge_kernel(const float* ws, uint16_t* out, int slices, int tails, int tiles32, int rows, int Hkv, int G) {
+  constexpr int GRP = 4;
+  __shared__ float sums[PARTS][6][32];
+  const int col = threadIdx.x & 31, part = threadIdx.x >> 5, c = blockIdx.y;  // group of 4 dimensions
+  const int kvh = (int)blockIdx.x / tiles32, t32 = (int)blockIdx.x - kvh * tiles32;
+  const int n32 = rows - t32 * 32 < 32 ? rows - t32 * 32 : 32, row = t32 * 32 + (col < n32 ? col : n32 - 1);
+  const int b = row / G, g = row - b * G;
+  const int64_t step = (int64_t)Hkv * tiles32 * part_floats(D, 32);
+  const float* const prefix = ws + (int64_t)blockIdx.x * part_floats(D, 32);
+  const float* const tail = ws + slices * step + ((int64_t)b * Hkv + kvh) * tails * part_floats(D, G);
+  float mm = -INFINITY, den = 0.0f, n[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s0 = part; s0 < slices + tails; s0 += PARTS * GRP) {
+    float m[GRP], l[GRP];
+    v4f v[GRP];
+    float mx = mm;
+#pragma unroll
+    for (int i = 0; i < GRP; ++i) {
+      const int s = s0 + i * PARTS;
+      const bool is_tail = s >= slices;
+      const float* from = is_tail ? tail + (s - slices) * part_floats(D, G) : prefix + s * step;
+      const int k = is_tail ? G : n32, at = is_tail ? g : row - t32 * 32;
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+      v[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      if (s < slices + tails) {
+        m[i] = from[D * k + at];
+        l[i] = from[(D + 1) * k + at];
+        v[i] = *reinterpret_cast<const v4f*>(from + (c * k + at) * 4);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < GRP; ++i) mx = fmaxf(mx, m[i]);
+    const float old = mm == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mm - mx);
+    mm = mx;
+    den *= old;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) n[d] *= old;
+#pragma unroll
+    for (int i = 0; i < GRP; ++i) {
+      const bool some = m[i] != -INFINITY;  // otherwise only the maximum was written
+      const float w = some ? __builtin_amdgcn_exp2f(m[i] - mm) : 0.0f;
+      den = __builtin_fmaf(some ? l[i] : 0.0f, w, den);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) n[d] = __builtin_fmaf(some ? v[i][d] : 0.0f, w, n[d]);
+    }
+  }
+  sums[part][0][col] = mm;
+  sums[part][1][col] = den;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) sums[part][2 + d][col] = n[d];
+  __syncthreads();
+  if (part > 0 || col >= n32) return;
+  float mx = mm;
+#pragma unroll
+  for (int i = 1; i < PARTS; ++i) mx = fmaxf(mx, sums[i][0][col]);
+  den = 0.0f;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) n[d] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const float mi = sums[i][0][col], w = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - mx);
+    den = __builtin_fmaf(sums[i][1][col], w, den);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) n[d] = __builtin_fmaf(sums[i][2 + d][col], w, n[d]);
+  }
+  const float r = attn_inv_denominator(den);
+  *reinterpret_cast<uint2*>(out + (((int64_t)b * Hkv + kvh) * G + g) * D + c * 4) =
+      make_uint2(pack_bf16x2(__fmul_rn(n[0], r), __fmul_rn(n[1], r)), pack_bf16x2(__fmul_rn(n[2], r), __fmul_rn(n[3], r)));
+}
+
+// How a call is cut.
 struct SharedPlan {
-  int64_t s0;  // positions that the prefix kernel takes; 0: none, the decode kernel takes all of them
-  int qw, kw, blocks, per_slice, slices, tail;
+  int64_t s0;  // positions that the prefix takes; 0: none, the decode kernel takes all of them
+  int qw, slice, slices, tail, tails;
+  int64_t bytes;
 };
 
 constexpr int SHARED_TABLE_MAX = 2048;  // page-table entries kept in LDS
 
 static SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t shared) {
   SharedPlan p{};
-  const int64_t rows = B * (Hq / Hkv), s0 = (shared < T ? shared : T) / 64 * 64;
-  if (B < 2 || s0 < 64) {
-    p.tail = (int)attn_tail_slices(T);
-    return p;
-  }
+  const int64_t G = Hq / Hkv, rows = B * G, s0 = (shared < T ? shared : T) / 64 * 64, cus = device_cus();
+  if (B < 2 || s0 < 64) return p;
   p.s0 = s0;
-  p.blocks = (int)(s0 / 64);
-  if (rows <= 64) p.qw = 2, p.kw = 2;
-  else p.qw = 4, p.kw = 1;
-  const int64_t tiles = (rows + 32 * p.qw - 1) / (32 * p.qw), per_cu = p.kw == 1 ? 2 : D == 64 ? 2 : 1;
-  int64_t want = device_cus() * per_cu / (tiles * Hkv);
+  const int64_t tiles64 = (rows + 63) / 64, floor = s0 < 4096 ? 128 : 256;
+  p.qw = rows > 128 && tiles64 * Hkv * (s0 / 256) > 2 * cus ? 4 : 2;
+  const int64_t tiles = (rows + 32 * p.qw - 1) / (32 * p.qw);
+  int64_t want = (B * (T - s0) >= 8 * s0 ? cus / 2 : cus) / (tiles * Hkv);
   if (want < 1) want = 1;
-  int64_t per = (p.blocks + want - 1) / want;
-  per = (per + p.kw - 1) / p.kw * p.kw;
-  p.per_slice = (int)per;
-  p.slices = (int)((p.blocks + per - 1) / per);
-  p.tail = T > s0 ? (int)attn_tail_slices(T - s0) : 0;
+  int64_t slice = ((s0 + want - 1) / want + 63) / 64 * 64;
+  if (slice < floor) slice = floor;
+  p.slice = (int)slice;
+  p.slices = (int)((s0 + slice - 1) / slice);
+  if (T > s0) {
+    int64_t n = 2 * cus / (B * Hkv), most = (T - s0 + 127) / 128;
+    if (n < 1) n = 1;
+    if (n > most) n = most;
+    p.tail = (int)(((T - s0 + n - 1) / n + 127) / 128 * 128);
+    p.tails = (int)((T - s0 + p.tail - 1) / p.tail);
+  }
+  p.bytes = ((int64_t)p.slices * Hkv * ((rows + 31) / 32) * part_floats((int)D, 32) + B * Hkv * p.tails * part_floats((int)D, (int)G)) * (int64_t)sizeof(float);
   return p;
 }
 
-template <int D, int QW, int KW>
-static int launch_shared(SharedArgs& a, hipStream_t st) {
-  constexpr int BUFS = 2 * KW * 2 * 64 * 2 * D;
-  size_t lds = BUFS;
+template <int D, int QW>
+static int launch_shared(SharedArgs& a, int64_t tail_wgs, uint16_t* out, hipStream_t st) {
+  constexpr int KW = 4 / QW, KB = 64 / KW;
+  size_t lds = SHARED_LDS * D;
   a.tiles = (a.rows + 32 * QW - 1) / (32 * QW);
   a.by_tiles = UDiv::of((uint32_t)a.tiles);
-  if (a.page_shift < 6) {
-    const int64_t entries = ((int64_t)a.per_slice * 64 + a.page - 1) / a.page + 1;
+  if (a.page_shift < (KB == 64 ? 6 : 5) || (tail_wgs && a.page_shift < 5)) {
+    const int64_t most = a.slice > a.tail ? a.slice : a.tail, entries = (most + a.page - 1) / a.page + 1;
     a.table_lds = entries <= SHARED_TABLE_MAX ? (int)entries : 0;
     lds += (size_t)a.table_lds * sizeof(int);
   }
-  const int64_t combos = (int64_t)a.slices * a.Hkv;
-  queue_kernel(shared_attn_kernel<D, QW, KW>, dim3((unsigned)((combos + 7) / 8 * 8 * a.tiles)), dim3(QW * KW * 64), lds, st, a);
+  const int64_t combos = (int64_t)a.slices * a.Hkv, prefix_wgs = (combos + 7) / 8 * 8 * a.tiles;
+  if (prefix_wgs + tail_wgs > 0x7fffffff) return AQ_E_RANGE;
+  a.prefix_wgs = (int)prefix_wgs;
+  queue_kernel(shared_attn_kernel<D, QW, KW, KB>, dim3((unsigned)(prefix_wgs + tail_wgs)), dim3(256), lds, st, a);
+  if (const int rc = (int)hipGetLastError()) return rc;
+  const int64_t tiles = (int64_t)a.Hkv * a.tiles32;
+  const bool few = tiles * (D / 4) < 16 * device_cus();
+  queue_kernel(few ? shared_merge_kernel<D, 8> : shared_merge_kernel<D, 4>, dim3((unsigned)tiles, D / 4), dim3(few ? 256 : 128), 0, st, a.ws, out,
+               a.slices, a.tails, a.tiles32, a.rows, a.Hkv, a.G);
   return (int)hipGetLastError();
 }
 
@@ -357,8 +608,7 @@ extern "C" int64_t aq_paged_attn_decode_shared_workspace_bytes(int64_t B, int64_
                                                                int64_t shared_len) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || total_len <= 0 || shared_len < 0 || total_len > (1 << 30) || (D != 64 && D != 128)) return 0;
   const aq::SharedPlan p = aq::shared_plan(B, Hq, Hkv, D, total_len, shared_len);
-  if (!p.s0) return aq_paged_attn_decode_workspace_bytes(B, Hq, Hkv, total_len);
-  return aq::attn_workspace_bytes(B, Hq, p.slices + p.tail);
+  return p.s0 ? p.bytes : aq_paged_attn_decode_workspace_bytes(B, Hq, Hkv, total_len);
 }
 
 extern "C" int aq_paged_attn_decode_shared(const void* q, const void* k_cache, const void* v_cache, const int64_t* page_table,
@@ -378,12 +628,9 @@ extern "C" int aq_paged_attn_decode_shared(const void* q, const void* k_cache, c
   if (!plan.s0)
     return aq_paged_attn_decode(q, k_cache, v_cache, page_table, P, total_len, seq_lens, page_size, n_pages, scale, out, B, Hq, Hkv, D,
                                 workspace, workspace_bytes, stream);
-  const int ns = plan.slices + plan.tail;
-  const int64_t tiles = (B * (Hq / Hkv) + 32 * plan.qw - 1) / (32 * plan.qw);
-  if (((int64_t)plan.slices * Hkv + 8) * tiles > 0x7fffffff || B * Hkv * plan.tail > 0x7fffffff) return AQ_E_RANGE;
   if (!workspace) return AQ_E_NULL;
   if (aq::check_ptr16(workspace)) return AQ_E_ALIGN;
-  if (workspace_bytes < aq::attn_workspace_bytes(B, Hq, ns)) return AQ_E_WORKSPACE;
+  if (workspace_bytes < plan.bytes) return AQ_E_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   aq::SharedArgs a{};
   a.q = static_cast<const uint16_t*>(q);
@@ -397,31 +644,26 @@ extern "C" int aq_paged_attn_decode_shared(const void* q, const void* k_cache, c
   a.P = P;
   a.scale_log2e = scale * 1.44269504088896341f;
   a.T = (int)total_len;
+  a.s0 = (int)plan.s0;
   a.rows = (int)(B * (Hq / Hkv));
   a.Hq = (int)Hq;
   a.Hkv = (int)Hkv;
   a.G = (int)(Hq / Hkv);
-  a.NS = ns;
-  a.blocks = plan.blocks;
-  a.per_slice = plan.per_slice;
+  a.slice = plan.slice;
   a.slices = plan.slices;
+  a.tiles32 = (a.rows + 31) / 32;
+  a.tail = plan.tail;
+  a.tails = plan.tails;
   a.page_shift = -1;
-  for (int sh = 6; sh < 31; ++sh)
+  for (int sh = 5; sh < 31; ++sh)
     if (page_size == ((int64_t)1 << sh)) a.page_shift = sh;
   a.by_g = aq::UDiv::of((uint32_t)a.G);
   a.by_hkv = aq::UDiv::of((uint32_t)a.Hkv);
+  a.by_tails = aq::UDiv::of((uint32_t)(a.tails ? a.tails : 1));
   // (pages above 2^30 hold every position: the quotient is 0 for any divisor as large)
   a.by_page = aq::UDiv::of((uint32_t)(page_size < (1 << 30) ? page_size : 1 << 30));
-  int rc;
-  if (D == 128)
-    rc = plan.kw == 2 ? aq::launch_shared<128, 2, 2>(a, st) : aq::launch_shared<128, 4, 1>(a, st);
-  else
-    rc = plan.kw == 2 ? aq::launch_shared<64, 2, 2>(a, st) : aq::launch_shared<64, 4, 1>(a, st);
-  if (rc) return rc;
-  if (plan.tail) {
-    rc = aq::attn_tail({q, k_cache, v_cache, page_table, seq_lens, a.ws, P, plan.s0, total_len, page_size, n_pages, B, Hq, Hkv, D, scale, ns,
-                        plan.slices}, st);
-    if (rc) return rc;
-  }
-  return aq::attn_merge(a.ws, out, B, Hq, ns, D, st);
+  const int64_t tail_wgs = B * Hkv * plan.tails;
+  uint16_t* const o = static_cast<uint16_t*>(out);
+  if (D == 128) return plan.qw == 2 ? aq::launch_shared<128, 2>(a, tail_wgs, o, st) : aq::launch_shared<128, 4>(a, tail_wgs, o, st);
+  return plan.qw == 2 ? aq::launch_shared<64, 2>(a, tail_wgs, o, st) : aq::launch_shared<64, 4>(a, tail_wgs, o, st);
 }
