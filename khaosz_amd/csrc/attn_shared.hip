@@ -400,7 +400,7 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
     rows.template attend<KB / 32>(ks, ks + TILE, kb0, masked, p.T, p.scale_log2e, [] {}, [] {});
   }
   const int n = p.rows - r0 < 32 ? p.rows - r0 : 32;  // idle: none
-  float* const part = p.ws + (int64_t)((slice * p.Hkv + kvh) * p.tiles32 + t32) * part_floats(D, 32);
+  float* const part = p.ws + (((int64_t)slice * p.Hkv + kvh) * p.tiles32 + t32) * part_floats(D, 32);
   if constexpr (KW > 1) {
     sh_barrier();  // everyone is done with the blocks
     rows.template join_and_store<KW>(reinterpret_cast<v4f*>(lds), ml, kw, qw, QW, part, n);
@@ -554,24 +554,45 @@ struct SharedPlan {
 
 constexpr int SHARED_TABLE_MAX = 2048;  // page-table entries kept in LDS
 
+// Whether reading the first s0 positions once is the faster form: what each form has beside the other.  The decode kernel reads the keys and
+// values of B x T positions (0.1 a megabyte), and past 2048 of them it has two launches with a merge of more slices (4).  Here there is the
+// merge (2, and 2 more where the decode kernel is a single launch), the tails' megabytes, and 0.6 a million products of a row with a
+// position and 128 dimensions.  The weights are fitted to both forms' times from a graph at 11168 random sizes (2 to 128 sequences, 2 to 8 KV heads
+// of 1 to 4 rows, both head dimensions, pages of 16 to 256, 64 to 40000 positions): the rule's choice costs 1.006 times the better form's
+// time in the mean, always sharing 1.100, never 1.62.  us, decode kernel | shared: 2 x 1088 positions of which 1024 shared, 16/4 heads of
+// 128 7.8 | 8.6; 2 x 2112 of 2048 9.5 | 8.7; 8 x 2112 of 2048 12.2 | 8.9; 32 x 576 of 512 10.4 | 9.5; 32 x 1024 of 512 12.0 | 14.4;
+// 32 x 2560 of 2048 23.3 | 16.3; 122 x 152 of 128 8.9 | 15.8.
+static bool sharing_pays(int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t T, int64_t s0) {
+  const double position = 4e-6 * (double)(Hkv * D);  // megabytes
+  const double apart = 0.1 * position * (double)(B * T) + (T > 2048 ? 4.0 : 0.0);
+  const double shared = 2.0 + (T > 256 ? 0.0 : 2.0) + 0.1 * position * (double)(B * (T - s0)) + 0.6e-6 / 128 * (double)(D * Hkv * G) * (double)B * (double)s0;
+  return shared < apart;
+}
+
 static SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t T, int64_t shared) {
   SharedPlan p{};
   const int64_t G = Hq / Hkv, rows = B * G, s0 = (shared < T ? shared : T) / 64 * 64, cus = device_cus();
-  if (B < 2 || s0 < 64) return p;
+  if (B < 2 || s0 < 64 || !sharing_pays(B, Hkv, G, D, T, s0)) return p;
   p.s0 = s0;
-  const int64_t tiles64 = (rows + 63) / 64, floor = s0 < 4096 ? 128 : 256;
-  p.qw = rows > 128 && tiles64 * Hkv * (s0 / 256) > 2 * cus ? 4 : 2;
-  const int64_t tiles = (rows + 32 * p.qw - 1) / (32 * p.qw);
+  // A workgroup has 64 rows, or 128 where there are many: fewer keys and values go into the compute units then (64 x 8448 positions of which
+  // 8192 shared, 32/8 heads of 128 39.2 | 36.3 us), but too few workgroups otherwise (32 x 4300 of 4096, 16/4 heads of 128 14.6 | 16.0).
+  p.qw = rows > 128 && (rows + 63) / 64 * Hkv * (s0 / 256) > 2 * cus ? 4 : 2;
+  // As many slices as fill the compute units once, half as many where the tails are most of the work anyway; but short ones cost the merge
+  // more than they save (16 x 8300 of 8192, 16/4 heads of 128, slices of 64, 128, 256, 512: 24.5, 18.4, 15.4, 17.7; 8 x 2591 of 2048, 64,
+  // 128, 256: 13.7, 11.4, 12.3).
+  const int64_t tiles = (rows + 32 * p.qw - 1) / (32 * p.qw), shortest = s0 < 4096 ? 128 : 256;
   int64_t want = (B * (T - s0) >= 8 * s0 ? cus / 2 : cus) / (tiles * Hkv);
   if (want < 1) want = 1;
   int64_t slice = ((s0 + want - 1) / want + 63) / 64 * 64;
-  if (slice < floor) slice = floor;
+  if (slice < shortest) slice = shortest;
   p.slice = (int)slice;
   p.slices = (int)((s0 + slice - 1) / slice);
   if (T > s0) {
-    int64_t n = 2 * cus / (B * Hkv), most = (T - s0 + 127) / 128;
-    if (n < 1) n = 1;
+    // one workgroup of tails per compute unit, four of half the size at head dimension 64 (32 x 1024 of 512, 16/4 heads of 128, one or two:
+    // 11.0 | 12.7 without the merge; 33 x 1401 of 1008, 24/4 of 64, one, two or four: 10.8, 7.9, 6.9); 128 positions are one block for each wavefront
+    int64_t n = (D == 64 ? 4 : 1) * cus / (B * Hkv), most = (T - s0 + 127) / 128;
     if (n > most) n = most;
+    if (n < 1) n = 1;
     p.tail = (int)(((T - s0 + n - 1) / n + 127) / 128 * 128);
     p.tails = (int)((T - s0 + p.tail - 1) / p.tail);
   }

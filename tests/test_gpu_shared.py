@@ -67,41 +67,65 @@ def _case(B, Hq, Hkv, D, page, shared, T, seed=0, extra=3, gain=1.0):
     return [t.to(DEV) for t in (q, k, v, table)]
 
 
+def _is_shared(q, k, T, shared):
+    """Whether the call reads the shared positions once: it then keeps other partial results than the decode kernel, which takes calls that
+    would gain nothing."""
+    (B, Hq, D), Hkv = q.shape, k.shape[2]
+    return ops.paged_attn_shared_workspace_bytes(B, Hq, Hkv, D, T, shared, DEV) != ops.paged_attn_workspace_bytes(B, Hq, Hkv, T)
+
+
 @pytest.mark.parametrize("B,Hq,Hkv,D,page,shared,T", [
-    (2, 1, 1, 64, 64, 64, 65),          # the smallest shared block
-    (2, 24, 4, 64, 128, 512, 576),
-    (3, 16, 4, 128, 64, 64, 64),        # everything is shared
-    (2, 4, 4, 128, 1, 70, 131),         # pages of one position
-    (9, 6, 2, 128, 16, 160, 161),       # three heads a KV head, one own position
-    (5, 8, 1, 64, 24, 456, 500),        # pages end inside a block
+    (2, 1, 1, 64, 64, 2048, 2049),      # two rows, one own position
+    (2, 24, 4, 64, 128, 2432, 2500),
+    (3, 16, 4, 128, 64, 2112, 2112),    # everything is shared
+    (2, 4, 4, 128, 1, 2070, 2131),      # pages of one position
+    (9, 6, 2, 128, 16, 2160, 2161),     # three heads a KV head, one own position
+    (5, 8, 1, 64, 24, 2088, 2150),      # pages end inside a block
     (33, 24, 4, 64, 16, 1008, 1401),
-    (17, 16, 2, 128, 48, 960, 1300),    # 136 rows a KV head: a tile and a piece of one
-    (70, 4, 2, 128, 256, 1024, 1030),   # 140 rows
-    (128, 2, 2, 64, 64, 320, 333),      # 128 rows, one head each
+    (17, 16, 2, 128, 48, 2064, 2300),   # 136 rows a KV head: two tiles and a piece of one
+    (17, 16, 4, 128, 48, 960, 1300),    # 68 rows
+    (70, 4, 2, 128, 256, 1024, 1030),
+    (128, 2, 2, 64, 64, 640, 660),
     (130, 3, 1, 128, 64, 640, 700),     # 390 rows
+    (66, 16, 8, 128, 64, 4096, 4170),   # 132 rows of many: tiles of 128
+    (34, 32, 8, 64, 32, 8192, 8200),    # the same, pages of half a block
+    (66, 16, 8, 128, 24, 4104, 4110),   # pages of another size
+    (2, 2, 2, 128, 3, 20001, 20300),    # more pages in a slice than are kept in LDS: 20001 positions of one tile
+    (300, 8, 1, 64, 128, 512, 777),
+    (2, 8, 1, 128, 4096, 4096, 9000),   # one page holds all that is shared; long tails
+    (4, 4, 4, 64, 1, 2600, 30000),      # tails with pages of one position
     (8, 16, 4, 128, 64, 2048, 2591),
     (4, 32, 8, 128, 128, 4096, 4100),
-    (3, 2, 1, 64, 4096, 4096, 4200),    # one page holds all that is shared
     (2, 2, 2, 128, 100, 20000, 20001),  # long, pages of an odd size
 ])
 def test_against_64_bits(B, Hq, Hkv, D, page, shared, T):
     _say("shared", B, Hq, Hkv, D, page, shared, T)
     q, k, v, table = _case(B, Hq, Hkv, D, page, shared, T, seed=T + B)
+    assert _is_shared(q, k, T, shared)
     want, tol = _expected(q, k, v, table, T)
     _check(ops.paged_attn_decode_shared(q, k, v, table, T, shared), want, tol)
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("shared", [0, 1, 63, 64, 65, 127, 128, 200, 255, 256, 300, 399, 400, 1 << 40])
+@pytest.mark.parametrize("shared", [0, 1, 63, 64, 65, 900, 1500, 1535, 1536, 1537, 2000, 2239, 2240, 2299, 2300, 1 << 40])
 def test_any_shared_length_means_the_same(D, shared):
     """The promise may cut a page or a block anywhere, or reach past the last position."""
     _say("shared lengths", D, shared)
-    q, k, v, table = _case(5, 8, 2, D, 40, 400, 400)
-    want, tol = _expected(q, k, v, table, 400)
-    got = ops.paged_attn_decode_shared(q, k, v, table, 400, shared)
+    q, k, v, table = _case(5, 8, 2, D, 40, 2300, 2300)
+    want, tol = _expected(q, k, v, table, 2300)
+    got = ops.paged_attn_decode_shared(q, k, v, table, 2300, shared)
     _check(got, want, tol)
+    assert _is_shared(q, k, 2300, shared) == (shared >= 64)
     if shared < 64:
-        assert torch.equal(got, ops.paged_attn_decode(q, k, v, table, 400))
+        assert torch.equal(got, ops.paged_attn_decode(q, k, v, table, 2300))
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,page,shared,T", [(2, 24, 4, 64, 128, 512, 576), (8, 16, 4, 128, 64, 512, 700), (3, 4, 2, 64, 16, 64, 65)])
+def test_calls_that_gain_nothing_by_it_are_the_decode_kernels(B, Hq, Hkv, D, page, shared, T):
+    q, k, v, table = _case(B, Hq, Hkv, D, page, shared, T)
+    lens = torch.randint(0, T + 1, (B,)).to(DEV)
+    assert not _is_shared(q, k, T, shared)
+    assert torch.equal(ops.paged_attn_decode_shared(q, k, v, table, T, shared, seq_lens=lens), ops.paged_attn_decode(q, k, v, table, T, seq_lens=lens))
 
 
 def test_one_sequence_shares_nothing():
@@ -110,39 +134,45 @@ def test_one_sequence_shares_nothing():
 
 
 @pytest.mark.parametrize("B,Hq,Hkv,D,page,shared,T,lens", [
-    (4, 8, 2, 64, 64, 256, 700, [700, 257, 300, 699]),
-    (4, 8, 2, 128, 64, 256, 700, [700, 256, 255, 1]),            # ends at the border, inside, at once
-    (6, 4, 4, 64, 16, 512, 520, [520, 0, 64, 65, 130, 511]),     # one without any length: the average of all positions
-    (3, 4, 2, 128, 64, 128, 512, [0, -5, 100000]),               # cut to 0 .. T
-    (70, 6, 2, 64, 24, 240, 301, None),
-    (150, 4, 4, 128, 64, 320, 330, None),
+    (4, 8, 2, 64, 64, 1792, 2300, [2300, 1793, 1900, 2299]),
+    (4, 8, 2, 128, 64, 1792, 2300, [2300, 1792, 1791, 1]),              # ends at the border, inside, at once
+    (6, 4, 4, 64, 16, 2048, 2056, [2056, 0, 64, 65, 130, 2047]),        # one without any length: the average of all positions
+    (3, 4, 2, 128, 64, 1920, 2212, [0, -5, 100000]),                    # cut to 0 .. T
+    (70, 6, 2, 64, 24, 1032, 1101, None),
+    (150, 4, 4, 128, 64, 640, 677, None),
+    (66, 16, 8, 128, 64, 4096, 4170, None),
+    (66, 16, 8, 64, 20, 8200, 8230, None),
 ])
 def test_sequences_at_different_positions(B, Hq, Hkv, D, page, shared, T, lens):
     _say("shared lens", B, Hq, Hkv, D, page, shared, T)
     q, k, v, table = _case(B, Hq, Hkv, D, page, shared, T, seed=B)
     lens = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(B)) if lens is None else torch.tensor(lens)
+    assert _is_shared(q, k, T, shared)
     want, tol = _expected(q, k, v, table, T, lens)
     _check(ops.paged_attn_decode_shared(q, k, v, table, T, shared, seq_lens=lens.to(DEV)), want, tol)
 
 
 def test_all_sequences_without_any_length():
-    q, k, v, table = _case(3, 4, 2, 64, 16, 320, 400)
+    q, k, v, table = _case(3, 4, 2, 64, 16, 2048, 2101)
     lens = torch.zeros(3, dtype=torch.int64)
-    want, tol = _expected(q, k, v, table, 400, lens)
-    _check(ops.paged_attn_decode_shared(q, k, v, table, 400, 320, seq_lens=lens.to(DEV)), want, tol)
+    assert _is_shared(q, k, 2101, 2048)
+    want, tol = _expected(q, k, v, table, 2101, lens)
+    _check(ops.paged_attn_decode_shared(q, k, v, table, 2101, 2048, seq_lens=lens.to(DEV)), want, tol)
 
 
 @pytest.mark.parametrize("page", [16, 64, 128])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 def test_what_lies_behind_every_length_may_hold_anything(page, value):
     """Shared positions that no sequence sees, and each sequence's own behind its length."""
-    q, k, v, table = _case(4, 8, 2, 128, page, 640, 900, seed=page)
+    T, shared = 2500, 2176
+    q, k, v, table = _case(4, 8, 2, 128, page, shared, T, seed=page)
+    assert _is_shared(q, k, T, shared)
     lens = torch.tensor([300, 500, 20, 499])
-    got = ops.paged_attn_decode_shared(q, k, v, table, 900, 640, seq_lens=lens.to(DEV))
-    own = torch.tensor([900, 700, 641, 800])
-    far = ops.paged_attn_decode_shared(q, k, v, table, 900, 640, seq_lens=own.to(DEV))
+    got = ops.paged_attn_decode_shared(q, k, v, table, T, shared, seq_lens=lens.to(DEV))
+    own = torch.tensor([2500, 2300, 2177, 2400])
+    far = ops.paged_attn_decode_shared(q, k, v, table, T, shared, seq_lens=own.to(DEV))
     k2, v2, k3, v3 = k.clone(), v.clone(), k.clone(), v.clone()
-    pos = torch.arange(900, device=DEV)
+    pos = torch.arange(T, device=DEV)
     for b in range(4):
         behind = pos[500:]
         k2[table[b, behind // page], behind % page] = value
@@ -150,50 +180,54 @@ def test_what_lies_behind_every_length_may_hold_anything(page, value):
         behind = pos[int(own[b]):]
         k3[table[b, behind // page], behind % page] = value
         v3[table[b, behind // page], behind % page] = value
-    assert torch.equal(ops.paged_attn_decode_shared(q, k2, v2, table, 900, 640, seq_lens=lens.to(DEV)), got)
-    assert torch.equal(ops.paged_attn_decode_shared(q, k3, v3, table, 900, 640, seq_lens=own.to(DEV)), far)
+    assert torch.equal(ops.paged_attn_decode_shared(q, k2, v2, table, T, shared, seq_lens=lens.to(DEV)), got)
+    assert torch.equal(ops.paged_attn_decode_shared(q, k3, v3, table, T, shared, seq_lens=own.to(DEV)), far)
 
 
 @pytest.mark.parametrize("page", [16, 64, 200])
 def test_unmapped_pages_are_zero_keys_and_values(page):
-    q, k, v, table = _case(6, 8, 2, 128, page, 600, 1001, seed=page)
+    q, k, v, table = _case(6, 8, 2, 128, page, 1800, 2201, seed=page)
+    assert _is_shared(q, k, 2201, 1800)
     table[:, 1] = -1                          # shared
     table[:, 2] = k.shape[0]                  # a page past the cache
-    table[2, 600 // page + 1] = -7            # one sequence's own
+    table[2, 1800 // page + 1] = -7           # one sequence's own
     table[3, -1] = 1 << 40
-    want, tol = _expected(q, k, v, table, 1001)
-    _check(ops.paged_attn_decode_shared(q, k, v, table, 1001, 600), want, tol)
+    want, tol = _expected(q, k, v, table, 2201)
+    _check(ops.paged_attn_decode_shared(q, k, v, table, 2201, 1800), want, tol)
 
 
 def test_positions_past_the_page_table_are_unmapped():
-    q, k, v, table = _case(3, 4, 2, 64, 64, 256, 300)
-    short = table[:, :3].contiguous()
-    want, tol = _expected(q, k, v, short, 300)
-    _check(ops.paged_attn_decode_shared(q, k, v, short, 300, 256), want, tol)
+    for page in (64, 24):
+        q, k, v, table = _case(3, 4, 2, 64, page, 2112, 2200)
+        short = table[:, :1000 // page].contiguous()
+        assert _is_shared(q, k, 2200, 2112)
+        want, tol = _expected(q, k, v, short, 2200)
+        _check(ops.paged_attn_decode_shared(q, k, v, short, 2200, 2112), want, tol)
 
 
 def test_large_scores_and_a_scale():
     """Scores of some hundreds: the running maximum is raised block by block."""
-    q, k, v, table = _case(7, 4, 2, 128, 64, 768, 800, gain=20.0)
+    q, k, v, table = _case(7, 4, 2, 128, 64, 2048, 2080, gain=20.0)
+    assert _is_shared(q, k, 2080, 2048)
     k[table[0, 5], 3] = k[table[0, 5], 3] * 4
     for scale in (None, 0.02, 1.0):
-        want, tol = _expected(q, k, v, table, 800, scale=scale)
-        _check(ops.paged_attn_decode_shared(q, k, v, table, 800, 768, scale=scale), want, tol)
+        want, tol = _expected(q, k, v, table, 2080, scale=scale)
+        _check(ops.paged_attn_decode_shared(q, k, v, table, 2080, 2048, scale=scale), want, tol)
 
 
 def test_strided_inputs_and_a_workspace():
-    q, k, v, table = _case(5, 8, 2, 64, 32, 448, 500)
-    want = ops.paged_attn_decode_shared(q, k, v, table, 500, 448)
+    q, k, v, table = _case(5, 8, 2, 64, 32, 2240, 2300)
+    want = ops.paged_attn_decode_shared(q, k, v, table, 2300, 2240)
     wide = torch.zeros(5, 8, 100, dtype=torch.bfloat16, device=DEV)
     wide[..., 8:72] = q
-    tall = torch.zeros(5, 40, dtype=torch.int64, device=DEV)
+    tall = torch.zeros(5, 90, dtype=torch.int64, device=DEV)
     tall[:, 3:3 + table.shape[1]] = table
-    assert torch.equal(ops.paged_attn_decode_shared(wide[..., 8:72], k, v, tall[:, 3:3 + table.shape[1]], 500, 448), want)
-    need = ops.paged_attn_shared_workspace_bytes(5, 8, 2, 64, 500, 448, DEV)
+    assert torch.equal(ops.paged_attn_decode_shared(wide[..., 8:72], k, v, tall[:, 3:3 + table.shape[1]], 2300, 2240), want)
+    need = ops.paged_attn_shared_workspace_bytes(5, 8, 2, 64, 2300, 2240, DEV)
     ws = torch.full((need // 4 + 64,), float("nan"), device=DEV)
-    assert torch.equal(ops.paged_attn_decode_shared(q, k, v, table, 500, 448, workspace=ws), want)
+    assert torch.equal(ops.paged_attn_decode_shared(q, k, v, table, 2300, 2240, workspace=ws), want)
     assert bool(ws[need // 4:].isnan().all())
-    assert torch.equal(ops.paged_attn_decode_shared(q, k, v, table, 500, 448, workspace=ws[:16]), want)  # too small: one of its own
+    assert torch.equal(ops.paged_attn_decode_shared(q, k, v, table, 2300, 2240, workspace=ws[:16]), want)  # too small: one of its own
 
 
 def test_the_same_bits_each_time_and_on_another_stream():
@@ -211,34 +245,35 @@ def test_the_same_bits_each_time_and_on_another_stream():
 def test_pages_beyond_32_bits():
     """Offsets of the last pages pass 2^32 elements."""
     page, Hkv, D = 64, 8, 128
-    n_pages = (1 << 32) // (page * Hkv * D) + 40
+    n_pages = (1 << 32) // (page * Hkv * D) + 60
     k, v = (torch.empty(n_pages, page, Hkv, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
     g = torch.Generator(device=DEV).manual_seed(1)
-    k[-40:].normal_(generator=g)
-    v[-40:].normal_(generator=g)
+    k[-60:].normal_(generator=g)
+    v[-60:].normal_(generator=g)
     q = torch.randn(3, 16, D, generator=g, device=DEV).to(torch.bfloat16)
-    table = (n_pages - 40 + torch.cat([torch.arange(8).expand(3, -1), 8 + torch.arange(9).view(3, 3)], 1)).to(DEV)
-    got = ops.paged_attn_decode_shared(q, k, v, table, 700, 512)
-    near = ops.paged_attn_decode_shared(q, k[-40:].clone(), v[-40:].clone(), table - (n_pages - 40), 700, 512)
+    table = (n_pages - 60 + torch.cat([torch.arange(32).expand(3, -1), 32 + torch.arange(9).view(3, 3)], 1)).to(DEV)
+    assert _is_shared(q, k, 2200, 2048)
+    got = ops.paged_attn_decode_shared(q, k, v, table, 2200, 2048)
+    near = ops.paged_attn_decode_shared(q, k[-60:].clone(), v[-60:].clone(), table - (n_pages - 60), 2200, 2048)
     assert torch.equal(got, near)
 
 
 def test_captured_and_replayed():
     """Two graphs and eager calls in turn, on new inputs each time."""
-    cases = [_case(8, 16, 4, 128, 64, 1024, 1200, seed=s) for s in range(3)]
-    lens = torch.randint(1025, 1201, (8,), generator=torch.Generator().manual_seed(0)).to(DEV)
-    want = [ops.paged_attn_decode_shared(*c, 1200, 1024, seq_lens=lens) for c in cases]
+    cases = [_case(8, 16, 4, 128, 64, 2048, 2200, seed=s) for s in range(3)]
+    lens = torch.randint(2049, 2201, (8,), generator=torch.Generator().manual_seed(0)).to(DEV)
+    want = [ops.paged_attn_decode_shared(*c, 2200, 2048, seq_lens=lens) for c in cases]
     held = [t.clone() for t in cases[0]]
     graphs, outs = [], []
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        ops.paged_attn_decode_shared(*held, 1200, 1024, seq_lens=lens)
+        ops.paged_attn_decode_shared(*held, 2200, 2048, seq_lens=lens)
     torch.cuda.current_stream().wait_stream(side)
     for _ in range(2):
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            outs.append(ops.paged_attn_decode_shared(*held, 1200, 1024, seq_lens=lens))
+            outs.append(ops.paged_attn_decode_shared(*held, 2200, 2048, seq_lens=lens))
         graphs.append(g)
     for turn in range(6):
         c = turn % 3
@@ -246,7 +281,7 @@ def test_captured_and_replayed():
             t.copy_(x)
         graphs[turn % 2].replay()
         graphs[1 - turn % 2].replay()
-        other = ops.paged_attn_decode_shared(*cases[(c + 1) % 3], 1200, 1024, seq_lens=lens)
+        other = ops.paged_attn_decode_shared(*cases[(c + 1) % 3], 2200, 2048, seq_lens=lens)
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[c]) and torch.equal(outs[1], want[c]) and torch.equal(other, want[(c + 1) % 3]), turn
 

@@ -11,7 +11,7 @@ P = 1 << 20  # a fake, aligned pointer: refused before any launch
 
 
 def _attn(**change):
-    a = dict(q=P, k=P, v=P, table=P, cols=8, total=100, shared=64, lens=None, page=16, n_pages=9, scale=0.1, out=P, B=2, Hq=4, Hkv=2, D=64,
+    a = dict(q=P, k=P, v=P, table=P, cols=200, total=3000, shared=2990, lens=None, page=16, n_pages=9, scale=0.1, out=P, B=2, Hq=4, Hkv=2, D=64,
              ws=P, ws_bytes=1 << 30, stream=None)
     a.update(change)
     return _abi.load().aq_paged_attn_decode_shared(*a.values())
@@ -71,7 +71,10 @@ def test_sizes_of_workspaces():
     assert lib.aq_compact_pages_workspace_bytes(-1) == 0
     size = lib.aq_paged_attn_decode_shared_workspace_bytes
     assert size(0, 4, 2, 64, 100, 64) == 0 and size(2, 5, 2, 64, 100, 64) == 0 and size(2, 4, 2, 64, 0, 0) == 0
-    assert size(2, 4, 2, 64, 100, 0) == lib.aq_paged_attn_decode_workspace_bytes(2, 4, 2, 100)
+    for total, shared in ((100, 0), (100, 64), (3000, 0), (3000, 63)):  # nothing to gain: the decode kernel's
+        assert size(2, 4, 2, 64, total, shared) == lib.aq_paged_attn_decode_workspace_bytes(2, 4, 2, total)
+    # 256 compute units where there is no device: 23 slices of 128 positions of the first 2944, whole blocks of 64, and a tail a sequence
+    assert size(2, 4, 2, 64, 3000, 2990) == 4 * (23 * 2 * 68 * 32 + 2 * 2 * 68 * 2)
 
 
 def test_cpu_tensors_are_refused():
@@ -104,7 +107,7 @@ def test_a_cache_finds_what_its_rows_share():
 
 def _model(**options):
     torch.manual_seed(0)
-    m = AutoRegressiveLM(LMConfig(vocab_size=97, dim=512, n_layers=2, n_heads=8, n_kv_heads=2, dim_ffn=704, max_len=512, **options)).to("cuda", torch.bfloat16).eval()
+    m = AutoRegressiveLM(LMConfig(vocab_size=97, dim=512, n_layers=2, n_heads=8, n_kv_heads=2, dim_ffn=704, max_len=2304, **options)).to("cuda", torch.bfloat16).eval()
     quantize_model(m)
     fuse_shared_inputs(m, norms=True, decode_attention=True, residuals=True)
     return m
@@ -118,16 +121,18 @@ def test_samples_of_a_prompt(options, mixed, monkeypatch):
     Every attention that the model runs is checked against 64 bits on the tensors it was given.  (The logits are not compared with those of
     unshared sequences: int8 codes that fall the other way grow through the layers.)  What is exact: the first layer's keys and values
     depend on the tokens alone, and samples that were given the same tokens so far have the same logits, bit for bit."""
-    page, prompt = 16, 100
+    page, prompt, full = 16, 2100, 131  # the last of the prompt's 132 pages is begun
     m = _model(**options)
     g = torch.Generator().manual_seed(3)
     ids = torch.randint(0, 97, (1, prompt), generator=g).cuda()
-    cache, plain = m.new_cache(96, page), m.new_cache(96, page)
+    cache, plain = m.new_cache(800, page), m.new_cache(800, page)
     run, calls = ops.paged_attn_decode_shared, []
 
     def checked(q, k, v, table, total, shared, seq_lens=None):
         got = run(q, k, v, table, total, shared, seq_lens=seq_lens)
-        assert shared == 96 and (seq_lens is not None) == mixed
+        assert ops.paged_attn_shared_workspace_bytes(*q.shape[:2], k.shape[2], 64, total, shared, "cuda") != \
+            ops.paged_attn_workspace_bytes(*q.shape[:2], k.shape[2], total)  # read once, not the decode kernel
+        assert shared == full * page and (seq_lens is not None) == mixed
         want, tol = _expected(q, k, v, table, total, None if seq_lens is None else seq_lens.cpu())
         _check(got, want, tol)
         calls.append(total)
@@ -149,21 +154,21 @@ def test_samples_of_a_prompt(options, mixed, monkeypatch):
         return outs[0]
 
     def copied(table, n):  # rows with pages of their own, holding what the shared ones hold
-        own = torch.randperm(96, generator=g)[:table.shape[0] * n].view(-1, n).cuda()
+        own = torch.randperm(800, generator=g)[:table.shape[0] * n].view(-1, n).cuda()
         plain.k_layers[:, own], plain.v_layers[:, own] = cache.k_layers[:, table[:, :n]], cache.v_layers[:, table[:, :n]]
         return own.contiguous()
 
-    table = torch.full((1, 8), -1, dtype=torch.int64, device="cuda")
-    table[0, :7] = torch.randperm(96, generator=g)[:7].cuda()
-    refs = torch.zeros(96, dtype=torch.int32, device="cuda")
-    refs[table[0, :7]] = 1
+    table = torch.full((1, full + 2), -1, dtype=torch.int64, device="cuda")
+    table[0, :full + 1] = torch.randperm(800, generator=g)[:full + 1].cuda()
+    refs = torch.zeros(800, dtype=torch.int32, device="cuda")
+    refs[table[0, :full + 1]] = 1
     with torch.inference_mode():
-        m(ids, paged_cache=cache.bind(table[:, :7].contiguous(), prompt), start_pos=0)
+        m(ids, paged_cache=cache.bind(table[:, :full + 1].contiguous(), prompt), start_pos=0)
     cache.bind(table, prompt)
     forked = cache.fork(refs, torch.zeros(5, dtype=torch.int64, device="cuda"))  # five samples
-    assert forked.missing.item() == 0 and forked.refs.sum().item() == 5 * 7
+    assert forked.missing.item() == 0 and forked.refs.sum().item() == 5 * (full + 1)
     table, refs, total = forked.page_table, forked.refs, prompt
-    alone = copied(table, 7)
+    alone = copied(table, full + 1)
     lens = torch.tensor([prompt] * 5, device="cuda") if mixed else None
     for _ in range(4):
         total += 1
@@ -176,12 +181,12 @@ def test_samples_of_a_prompt(options, mixed, monkeypatch):
     cache.bind(table, total)
     parents = torch.tensor([3, 1, 3, 3], device="cuda")  # two go on, one of them three times
     forked = cache.fork(refs, parents)
-    assert forked.missing.item() == 0 and forked.refs.sum().item() == 4 * 7
+    assert forked.missing.item() == 0 and forked.refs.sum().item() == 4 * (full + 1)
     cache.bind(forked.page_table, total)
     packed = cache.compact(forked.refs)
     table = packed.page_table
-    assert packed.live.item() == 6 + 4 and int(table.max()) == 9
-    alone = copied(table, 7)
+    assert packed.live.item() == full + 4 and int(table.max()) == full + 3
+    alone = copied(table, full + 1)
     lens = lens[parents] if mixed else None
     for _ in range(3):
         total += 1
@@ -191,4 +196,4 @@ def test_samples_of_a_prompt(options, mixed, monkeypatch):
         tokens[3] = tokens[0]
         logits = step(tokens, table, total, lens, alone)
         assert torch.equal(logits[3], logits[0]) and not torch.equal(logits[1], logits[0])
-    assert calls == [t for t in range(101, 108) for _ in range(2)]
+    assert calls == [t for t in range(2101, 2108) for _ in range(2)]
