@@ -479,10 +479,13 @@ int aq_rope_prefill_attn_paged_ahead(const void *q, int64_t q_stride, const floa
  * the others through each sequence's own row.  shared_len may be anything from 0 (nothing is shared: aq_paged_attn_decode) on;
  * what lies past total_len counts for nothing.  A promise that does not hold gives the values of row 0's pages.
  * Results agree with aq_paged_attn_decode within bf16 rounding (probabilities of shared positions are rounded to bf16, sums are
- * fp32 in another order).  seq_lens as there, a sequence may end inside the shared positions; positions that no sequence
- * attends to may hold anything.  total_len at most 2^30, B Hq at most 2^24 (AQ_E_RANGE).
+ * fp32 in another order).  seq_lens as there, a sequence may end inside the shared positions; what lies behind its length may hold anything
+ * and changes nothing of its result.  total_len at most 2^30, B Hq at most 2^24 (AQ_E_RANGE).
+ * aq_paged_attn_decode_shared_positions: how many of the shared positions such a call reads once; 0 where that gains nothing, and
+ * the call is aq_paged_attn_decode's.
  * workspace: 16-byte aligned, aq_paged_attn_decode_shared_workspace_bytes(..) bytes for the same sizes (0: may be NULL); two calls that
  * overlap in time must not share it. */
+int64_t aq_paged_attn_decode_shared_positions(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t total_len, int64_t shared_len);
 int64_t aq_paged_attn_decode_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t total_len,
                                                     int64_t shared_len);
 int aq_paged_attn_decode_shared(const void *q, const void *k_cache, const void *v_cache, const int64_t *page_table,
@@ -499,7 +502,8 @@ int aq_paged_attn_decode_shared(const void *q, const void *k_cache, const void *
  * empty row, all -1).  n = total_len, or seq_lens[parent] (device int64 [B], cut to 0 .. total_len), positions of the parent are
  * written.  Its first child goes on in all of its pages.  Every other child holds the pages that n fills, and gets a page of its own for
  * a page that is partly filled: the written rows of all layers' keys and values are copied there, the rows behind them are left as
- * they were; its later entries are -1.  new_refs = max(refs - entries of the old rows, 0) + entries of the new rows, so rows without a child
+ * they were; its later entries are -1.  (The first child writes on into the parent's partly filled page, whoever else holds it: a holder
+ * that is to keep it as it is comes first, as a row of the table whose first child it is, or holds filled pages only.)  new_refs = max(refs - entries of the old rows, 0) + entries of the new rows, so rows without a child
  * let go of their pages, and the pages that are then free are handed out lowest first, to the rows in order.  missing[0]: rows that
  * found none (their entry is -1).  Sources are held, destinations free: the copies touch no page in use.
  * workspace: aq_fork_pages_workspace_bytes(n_pages, R) bytes.  It and refs are 16-byte aligned.

@@ -19,6 +19,8 @@
 #include "aq_common.h"
 #include "aq_rows.h"
 
+#include <type_traits>
+
 namespace aq {
 
 struct SharedArgs {
@@ -39,7 +41,7 @@ struct SharedArgs {
   UDiv by_g, by_page, by_tiles, by_hkv, by_tails;
 };
 
-constexpr float SHARED_MASKED = -1.0e30f;  // score (exp2 domain) of a position the sequence may not attend to, as in the decode kernel
+constexpr float SHARED_MASKED = -1.0e30f;  // score of every position of a sequence without any length: it weighs them alike, as in the decode kernel
 
 // A partial result of n rows: numerators as 16-byte groups of 4 dimensions, the n rows of a group side by side (what the lanes of a
 // product hold, so that it is stored and read by whole lines), then the n maxima and the n denominators.
@@ -66,19 +68,34 @@ struct SharedRows {
   __device__ __forceinline__ void start(const uint16_t* q, int g, int visible) {
 #pragma unroll
     for (int st = 0; st < D / 16; ++st) qf[st] = *reinterpret_cast<const uint4*>(q + g * 8 + st * 16);
+    vis = visible;
+    clear();
+  }
+
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
     m = -INFINITY;
     l = 0.0f;
-    vis = visible;
+  }
+
+  // Whether some numerator is infinite or NaN; wavefront-uniform.
+  __device__ __forceinline__ bool odd() const {
+    float x = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x = __builtin_fmaf(o[dt][r], 0.0f, x);
+    return __builtin_amdgcn_ballot_w64(x != 0.0f) != 0;  // (0 times either is NaN)
   }
 
   // 32 NT positions from kb0 on, K rows at ks and V rows at vs.  masked (wavefront-uniform): some row may not attend to some of them, or
-  // there are only T.
-  // keys_read() is called when the last K row has been read, values_needed() before the first V row is.
-  template <int NT, class FK, class FV>
+  // (not ALL) there are only T.
+  // keys_read() is called when the last K row has been read, values_needed() before the first V row is.  APART: infinite
+  // values are among V, which 0 does not mask: a row's product leaves out what the row must not see.
+  template <int NT, bool ALL, bool APART, class FK, class FV>
   __device__ __forceinline__ void attend(const uint8_t* ks, const uint8_t* vs, int kb0, bool masked, int T, float scale_log2e,
                                          FK&& keys_read, FV&& values_needed) {
     constexpr int DSTEPS = D / 16, DT = D / 32, ROWB = 2 * D;
@@ -124,21 +141,24 @@ struct SharedRows {
     keys_read();
     // ---- softmax of this lane's row; register r of tile kt is position kb0 + 32 kt + 8 (r / 4) + 4 g + r % 4
     float sc = scale_log2e;
-    if (masked) {  // the scores are scaled here, so that a masked one has the same value in every slice
+    if (masked) {  // the scores are scaled here: those of a sequence without any length have the same value in every slice
+      const float hidden = vis ? -INFINITY : SHARED_MASKED;
+      const int end = vis - kb0 - 4 * g, all = T - kb0 - 4 * g;
 #pragma unroll
       for (int kt = 0; kt < NT; ++kt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = kb0 + kt * 32 + 8 * (r / 4) + 4 * g + (r % 4);
-          s[kt][r] = key < vis ? s[kt][r] * sc : key < T ? SHARED_MASKED : -INFINITY;
+          const int key = kt * 32 + 8 * (r / 4) + r % 4;
+          s[kt][r] = key < end ? s[kt][r] * sc : ALL || key < all ? hidden : -INFINITY;
         }
       sc = 1.0f;
     }
-    softmax_values<NT>(s, vs, vfr0, vfr1, sc, values_needed);
+    softmax_values<NT, APART>(s, vs, vfr0, vfr1, kb0, masked, T, sc, values_needed);
   }
 
-  template <int NT, class FV>
-  __device__ __forceinline__ void softmax_values(pa_f32x16 (&s)[NT], const uint8_t* vs, int vfr0, int vfr1, float sc, FV&& values_needed) {
+  template <int NT, bool APART, class FV>
+  __device__ __forceinline__ void softmax_values(pa_f32x16 (&s)[NT], const uint8_t* vs, int vfr0, int vfr1, int kb0, bool masked, int T, float sc,
+                                                 FV&& values_needed) {
     constexpr int DT = D / 32, ROWB = 2 * D;
     float bm = -INFINITY;
 #pragma unroll
@@ -149,7 +169,7 @@ struct SharedRows {
     bm = fmaxf(b2.x, b2.y) * sc;
     // m only has to bound the exponents: it is raised, and the sums rescaled, when a row of the wavefront would see one above 2^8
     if (__builtin_amdgcn_ballot_w64(bm > m + 8.0f) != 0) {  // wavefront-uniform
-      const float mn = fmaxf(m, bm), alpha = __builtin_amdgcn_exp2f(m - mn);
+      const float mn = fmaxf(m, bm), alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= alpha;
 #pragma unroll
@@ -157,13 +177,14 @@ struct SharedRows {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
     }
+    const float mb = m == -INFINITY ? 0.0f : m;  // (so far every score is -infinity, and weighs nothing, or NaN, and stays that)
     uint4 pf[NT][2];  // P^T operands: tile kt, positions 16 s2 .. + 16
 #pragma unroll
     for (int kt = 0; kt < NT; ++kt) {
       float pv[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        pv[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], sc, -m));
+        pv[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], sc, -mb));
         l += pv[r];
       }
 #pragma unroll
@@ -172,18 +193,44 @@ struct SharedRows {
                                 pack_bf16x2(pv[8 * s2 + 4], pv[8 * s2 + 5]), pack_bf16x2(pv[8 * s2 + 6], pv[8 * s2 + 7]));
     }
     values_needed();
-    // ---- O^T += V^T P^T; all fragments of V are read before the products, whose chains alternate
     constexpr int KK = 2 * NT;
+    auto fragment = [&](int dt, int kk) __attribute__((always_inline)) {  // V^T operand: tile dt, positions 16 kk .. + 16
+      const uint8_t* at = vs + kk * 16 * ROWB;
+      const pa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)(at + (vfr0 ^ (dt << 6))));
+      const pa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)(at + (vfr1 ^ (dt << 6))));
+      return __builtin_bit_cast(pa_bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    if constexpr (APART) {  // a product for each length, of the values that rows of this length see
+      const int g = (threadIdx.x & 63) >> 5, mine = vis ? vis : T;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        uint64_t left = ~0ull;
+        do {
+          const int n = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+          left &= ~__builtin_amdgcn_ballot_w64(mine == n);
+          int end = n - kb0 - 4 * g;
+          asm volatile("" : "+v"(end)::"memory");  // (compared, and the values read, here: nothing of it kept in registers)
+          pa_f32x16 x = o[dt];
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            pa_bf16x8 v = fragment(dt, kk);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (16 * kk + 8 * (j / 4) + j % 4 >= end) v[j] = static_cast<__bf16>(0.0f);
+            x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(pa_bf16x8, pf[kk >> 1][kk & 1]), x, 0, 0, 0);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] = mine == n ? x[r] : o[dt][r];
+        } while (left);
+      }
+      return;
+    }
+    // ---- O^T += V^T P^T; all fragments of V are read before the products, whose chains alternate
     pa_bf16x8 fv[DT][KK];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const uint8_t* at = vs + kk * 16 * ROWB;
-        const pa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)(at + (vfr0 ^ (dt << 6))));
-        const pa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)(at + (vfr1 ^ (dt << 6))));
-        fv[dt][kk] = __builtin_bit_cast(pa_bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-      }
+      for (int kk = 0; kk < KK; ++kk) fv[dt][kk] = fragment(dt, kk);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int d0 = 0; d0 < DT; d0 += 2)
@@ -195,26 +242,27 @@ struct SharedRows {
   }
 
   // Whether some row may not attend to some of the positions kb0 .. kb0 + n - 1; *none: no row to any.
-  __device__ __forceinline__ bool masked(const int64_t* lens, int kb0, int n, bool* none) const {
+  __device__ __forceinline__ bool masked(int kb0, int n, bool* none) const {
     *none = false;
-    if (!lens || __builtin_amdgcn_ballot_w64(kb0 + n > vis) == 0) return false;
+    if (__builtin_amdgcn_ballot_w64(kb0 + n > vis) == 0) return false;
     *none = __builtin_amdgcn_ballot_w64(vis == 0 || kb0 < vis) == 0;
     return true;
   }
 
-  // A partial result of n rows; a row that saw nothing leaves its maximum only.
+  // A partial result of n rows; a row that saw nothing, or scores of -infinity only, leaves its maximum only.  One whose scores are NaN has a NaN
+  // for a maximum, which fmaxf leaves out and the sums take in.
   __device__ __forceinline__ void store(float* part, int n) const {
     const int lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
     const LanePair l2 = lanes32_pair(l);
+    const float sum = l2.x + l2.y, most = sum != sum ? sum : m;
     if (col >= n) return;
-    if (m != -INFINITY) {
+    if (most != -INFINITY) {
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
         *reinterpret_cast<v4f*>(part + ((2 * i + g) * n + col) * 4) = v4f{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2],
                                                                          o[i / 4][4 * (i % 4) + 3]};
     }
-    if (g == 0) part[D * n + col] = m;
-    else part[(D + 1) * n + col] = l2.x + l2.y;
+    part[(g == 0 ? D : D + 1) * n + col] = g == 0 ? most : sum;
   }
 
   // The same of the KW wavefronts that share these rows (as the tile-th of `tiles`), whose sums meet in LDS: each adds up and stores its
@@ -242,6 +290,7 @@ struct SharedRows {
       w[k] = w[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w[k] - most);
       sum = __builtin_fmaf(ml[(k * tiles + tile) * 128 + 64 + lane], w[k], sum);
     }
+    if (sum != sum) most = sum;
     if (col >= n) return;
     if (most != -INFINITY) {
 #pragma unroll
@@ -337,7 +386,7 @@ __device__ __forceinline__ int visible(const SharedArgs& p, int b) {
 // A tile of 32 QW rows of all sequences against a slice of the shared positions.  QW x KW wavefronts: QW tiles of 32 rows side by side on
 // the same block of KB positions, KW blocks at a time, the next KW ahead of the products.  (More buffers gain nothing: 64 x 8192 positions
 // of 32/8 heads of 128 20.0 us with two, 22.2 with four that leave room for one workgroup per compute unit.)
-template <int D, int QW, int KW, int KB>
+template <int D, int QW, int KW, int KB, bool LENS>
 __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds, float* ml, int* table_lds) {
   constexpr int ROWB = 2 * D, RPI = 1024 / ROWB;    // bytes of a K or V row; rows of a 1 KiB load
   constexpr int TILE = KB * ROWB;                   // bytes of a block's K (or V)
@@ -362,7 +411,7 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
   pages.fetch(p, k0, table_lds, QW * KW * 64);
   const int vis = visible(p, b);
   int seen = k1;  // positions that any row of the workgroup looks at
-  if (p.lens) {
+  if constexpr (LENS) {
     int most = vis ? vis : p.T;  // a row without any length weighs every position alike
 #pragma unroll
     for (int off = 32; off; off >>= 1) {
@@ -388,16 +437,47 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
   rows.start(p.q + ((int64_t)b * p.Hq + head) * D, lane >> 5, vis);
   const bool idle = r0 >= p.rows;  // wavefront-uniform: no row here, only loads
 
-  for (int it = 0; it < nit; ++it) {
-    SH_WAIT_VMCNT(0);  // this wavefront's part of the blocks has landed
-    sh_barrier();      // ... everyone's, and everyone is done with the ones before
-    if (it + 1 < nit) issue(it + 1, (it + 1) & 1);
-    const int kb0 = k0 + (it * KW + kw) * KB;
-    bool none;
-    const bool masked = rows.masked(p.lens, kb0, KB, &none);
-    if (idle || none || kb0 >= k1) continue;  // wavefront-uniform
-    const uint8_t* ks = lds + (it & 1) * BUF + kw * 2 * TILE;
-    rows.template attend<KB / 32>(ks, ks + TILE, kb0, masked, p.T, p.scale_log2e, [] {}, [] {});
+  bool hidden = false;  // some row must not see some of the positions
+  auto blocks = [&](auto apart) __attribute__((always_inline)) {
+    constexpr bool APART = decltype(apart)::value;
+    for (int it = 0; it < nit; ++it) {
+      SH_WAIT_VMCNT(0);  // this wavefront's part of the blocks has landed
+      sh_barrier();      // ... everyone's, and everyone is done with the ones before
+      if (it + 1 < nit) issue(it + 1, (it + 1) & 1);
+      const int kb0 = k0 + (it * KW + kw) * KB;
+      const uint8_t* ks = lds + (it & 1) * BUF + kw * 2 * TILE;
+      if (idle || kb0 >= k1) continue;  // wavefront-uniform, as all below
+      bool masked = false, none = false;
+      if constexpr (LENS) {
+        masked = rows.masked(kb0, KB, &none);
+        hidden |= masked;
+      }
+      if (none) continue;
+      if constexpr (APART) {
+#pragma unroll 1
+        for (int at = 0; at < KB; at += 32)
+          rows.template attend<1, true, true>(ks + at * ROWB, ks + TILE + at * ROWB, kb0 + at, masked, p.T, p.scale_log2e, [] {}, [] {});
+      } else {
+        rows.template attend<KB / 32, true, false>(ks, ks + TILE, kb0, masked, p.T, p.scale_log2e, [] {}, [] {});
+      }
+    }
+  };
+  blocks(std::false_type{});
+  if constexpr (LENS) {
+    // 0 masks no infinity and no NaN: where some came out, which other sequences' positions may have brought in, the slice is done again
+    // with every row's own values.  (Looking for them in each block first: 64 x 8448 positions, lengths from 4096 on, 37.2 us instead of 28.2.)
+    __shared__ int odd_s[QW * KW];
+    const bool odd = hidden && rows.odd();
+    if (lane == 0) odd_s[wave] = odd;
+    sh_barrier();
+    int any = 0;
+#pragma unroll
+    for (int i = 0; i < QW * KW; ++i) any |= odd_s[i];
+    if (__builtin_amdgcn_readfirstlane(any)) {  // workgroup-uniform
+      issue(0, 0);
+      rows.clear();
+      blocks(std::true_type{});
+    }
   }
   const int n = p.rows - r0 < 32 ? p.rows - r0 : 32;  // idle: none
   float* const part = p.ws + (((int64_t)slice * p.Hkv + kvh) * p.tiles32 + t32) * part_floats(D, 32);
@@ -437,7 +517,7 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& p, uint8_t* lds, f
       const int next = kb0 + KW * KB;
       const bool more = next < seen;
       asm volatile("" ::: "memory");
-      rows.template attend<1>(
+      rows.template attend<1, false, false>(
           ks, ks + TILE, kb0, kb0 + KB > vis, p.T, p.scale_log2e,
           [&] {
             SH_WAIT_LGKM();
@@ -462,13 +542,13 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& p, uint8_t* lds, f
 
 constexpr int SHARED_LDS = 512;  // bytes of the blocks of either kind of workgroup, per dimension
 
-template <int D, int QW, int KW, int KB>
+template <int D, int QW, int KW, int KB, bool LENS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void shared_attn_kernel(SharedArgs p) {
   static_assert(QW * KW == 4 && 2 * KW * KB * 4 * D == SHARED_LDS * D, "four wavefronts, 128 D bytes each");
   __shared__ float ml[4 * 128];
   extern __shared__ __align__(1024) uint8_t sh_lds[];  // blocks; page table
   int* const table = reinterpret_cast<int*>(sh_lds + SHARED_LDS * D);
-  if ((int)blockIdx.x < p.prefix_wgs) shared_prefix<D, QW, KW, KB>(p, sh_lds, ml, table);
+  if ((int)blockIdx.x < p.prefix_wgs) shared_prefix<D, QW, KW, KB, LENS>(p, sh_lds, ml, table);
   else shared_tail<D, 4>(p, sh_lds, ml, table);
 }
 
@@ -614,7 +694,8 @@ static int launch_shared(SharedArgs& a, int64_t tail_wgs, uint16_t* out, hipStre
   const int64_t combos = (int64_t)a.slices * a.Hkv, prefix_wgs = (combos + 7) / 8 * 8 * a.tiles;
   if (prefix_wgs + tail_wgs > 0x7fffffff) return AQ_E_RANGE;
   a.prefix_wgs = (int)prefix_wgs;
-  queue_kernel(shared_attn_kernel<D, QW, KW, KB>, dim3((unsigned)(prefix_wgs + tail_wgs)), dim3(256), lds, st, a);
+  // (a form of its own where sequences may end anywhere: its masks cost the others 3 to 7 % of their time)
+  queue_kernel(a.lens ? shared_attn_kernel<D, QW, KW, KB, true> : shared_attn_kernel<D, QW, KW, KB, false>, dim3((unsigned)(prefix_wgs + tail_wgs)), dim3(256), lds, st, a);
   if (const int rc = (int)hipGetLastError()) return rc;
   const int64_t tiles = (int64_t)a.Hkv * a.tiles32;
   const bool few = tiles * (D / 4) < 16 * device_cus();
@@ -624,6 +705,11 @@ static int launch_shared(SharedArgs& a, int64_t tail_wgs, uint16_t* out, hipStre
 }
 
 }  // namespace aq
+
+extern "C" int64_t aq_paged_attn_decode_shared_positions(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t total_len, int64_t shared_len) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || total_len <= 0 || shared_len < 0 || total_len > (1 << 30) || (D != 64 && D != 128)) return 0;
+  return aq::shared_plan(B, Hq, Hkv, D, total_len, shared_len).s0;
+}
 
 extern "C" int64_t aq_paged_attn_decode_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t total_len,
                                                                int64_t shared_len) {

@@ -784,7 +784,7 @@ def paged_attn_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     """``paged_attn_decode`` for sequences that begin with the same pages: the entries of ``page_table`` for the first
     ``shared_len`` positions are the same in every row (the caller's promise; row 0's pages are read).  Those positions
     are read once and multiplied with all sequences' queries at once.  The results agree with ``paged_attn_decode`` within bf16
-    rounding; ``seq_lens`` as there.  ``workspace``: a contiguous device tensor to reuse across calls, of
+    rounding; ``seq_lens`` as there.  Sizes that gain nothing by it (``paged_attn_shared_positions``) run as ``paged_attn_decode``.  ``workspace``: a contiguous device tensor to reuse across calls, of
     ``paged_attn_shared_workspace_bytes`` bytes; allocated per call when omitted or too small."""
     if workspace is None:
         y = (_host or _native()).paged_attn_decode_shared(q, k_cache, v_cache, page_table, total_len, shared_len, scale, seq_lens)
@@ -815,6 +815,12 @@ def paged_attn_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
                                                          B, Hq, Hkv, D, ws_ptr, ws_bytes, _stream(q))
         _abi.check(rc, "aq_paged_attn_decode_shared")
     return out
+
+
+def paged_attn_shared_positions(B: int, n_heads: int, n_kv_heads: int, head_dim: int, total_len: int, shared_len: int) -> int:
+    """How many of the shared positions ``paged_attn_decode_shared`` reads once at these sizes; 0: nothing is gained by it, and the call is
+    ``paged_attn_decode``'s."""
+    return int(_abi.load().aq_paged_attn_decode_shared_positions(B, n_heads, n_kv_heads, head_dim, int(total_len), int(shared_len)))
 
 
 def paged_attn_shared_workspace_bytes(B: int, n_heads: int, n_kv_heads: int, head_dim: int, total_len: int, shared_len: int, device) -> int:
@@ -870,7 +876,8 @@ def fork_pages(page_table: torch.Tensor, refs: torch.Tensor, parents: torch.Tens
     """New rows of a page table, each a fork of an old one: row i of the result goes on from row ``parents[i]`` (int64 ``[R]``;
     outside ``0 .. B - 1``: an empty row).  Whole pages are held together; the first child of a row goes on in its pages, the others
     get a free page with a copy of what is written of a page that is not full (``total_len`` positions are written, or
-    ``seq_lens`` int64 ``[B]`` of them, in all layers' caches).  Old rows without a child let go of their pages: dropping beams, ending
+    ``seq_lens`` int64 ``[B]`` of them, in all layers' caches).  A row to be kept as it is (a cached prompt whose last page is not full) is forked
+    into itself first: ``parents = [keeper, keeper, ...]``.  Old rows without a child let go of their pages: dropping beams, ending
     sequences and sampling several continuations are one call, and no call waits for the device.  ``refs`` int32
     ``[n_pages]`` counts who holds each page.  The table and the counts given are left as they are; the caches (any type, of 16-byte
     rows) are written in place, free pages only."""

@@ -43,7 +43,8 @@ def _expected(q, kc, vc, table, T, lens=None, scale=None):
             p = torch.exp(s - s.max())
             p = p / p.sum()
             out[b, h] = p @ vh
-            size = float((scale * (kh.abs() @ qh.abs())).max()) if n else 0.0
+            size = scale * (kh.abs() @ qh.abs())
+            size = float(size[size.isfinite()].max()) if n and bool(size.isfinite().any()) else 0.0
             near = 2.0 ** -8 + 2 * size * (D + 4) * 2.0 ** -24 + 2 * T * 2.0 ** -24 + 24 * 2.0 ** -24
             tol[b, h] = 2.0 ** -8 * out[b, h].abs() * (1 + near) + near * (p @ vh.abs())
     return out, tol
@@ -182,6 +183,57 @@ def test_what_lies_behind_every_length_may_hold_anything(page, value):
         v3[table[b, behind // page], behind % page] = value
     assert torch.equal(ops.paged_attn_decode_shared(q, k2, v2, table, T, shared, seq_lens=lens.to(DEV)), got)
     assert torch.equal(ops.paged_attn_decode_shared(q, k3, v3, table, T, shared, seq_lens=own.to(DEV)), far)
+
+
+def _check_odd(got, want, tol):
+    """The same where some of it is infinite or NaN: infinite or NaN there, near everywhere else."""
+    got = got.cpu().double()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    ok = want.isfinite()
+    assert bool((got[want.isinf()] == want[want.isinf()]).all())
+    _check(got[ok], want[ok], tol[ok])
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,page,shared,T", [
+    (4, 8, 2, 128, 16, 2176, 2500), (4, 8, 2, 64, 64, 2176, 2500), (66, 16, 8, 128, 64, 4096, 4140), (66, 16, 8, 64, 24, 4104, 4140)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("where", ["keys", "values"])
+def test_what_lies_behind_a_length_changes_nothing_of_its_result(B, Hq, Hkv, D, page, shared, T, value, where):
+    """... though other sequences see it and have it in theirs: one element of shared position 450, one of a sequence's own."""
+    _say("odd", B, Hq, Hkv, D, page, shared, T, value, where)
+    q, k, v, table = _case(B, Hq, Hkv, D, page, shared, T, seed=page + B)
+    assert _is_shared(q, k, T, shared)
+    lens = torch.randint(200, T + 1, (B,), generator=torch.Generator().manual_seed(B))
+    lens[:4] = torch.tensor([300, 450, 451, T])
+    if B > 4:
+        lens[9] = 0
+    c = k if where == "keys" else v
+    c[table[0, 450 // page], 450 % page, 1, 5] = value
+    c[table[3, (T - 1) // page], (T - 1) % page, 0, D - 1] = value
+    want, tol = _expected(q, k, v, table, T, lens)
+    assert bool(want[:2].isfinite().all()) and (where == "keys" or not bool(want[2:4].isfinite().all()))
+    _check_odd(ops.paged_attn_decode_shared(q, k, v, table, T, shared, seq_lens=lens.to(DEV)), want, tol)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_scores_without_a_bound(D):
+    """Queries that are infinite or NaN, and whole blocks of keys whose scores are -infinity, first ones of a slice among them."""
+    q, k, v, table = _case(5, 8, 2, D, 64, 2176, 2400)
+    assert _is_shared(q, k, 2400, 2176)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    for first in (0, 512, 1111, 2304):
+        for pos in range(first, first + 96):
+            k[table[1, pos // 64], pos % 64, 0, 0] = -float("inf")
+    lens = torch.tensor([2400, 2400, 64, 2399, 30])  # two of them see nothing else: NaN, with the heads of KV head 0
+    for n in (None, lens):
+        want, tol = _expected(q, k, v, table, 2400, n)
+        assert n is None or bool(want[2, 0].isnan().all()) and bool(want[2, 7].isfinite().all())
+        _check_odd(ops.paged_attn_decode_shared(q, k, v, table, 2400, 2176, seq_lens=None if n is None else n.to(DEV)), want, tol)
+    q[1, 2, 7] = float("nan")
+    q[3, 5, 1] = float("inf")  # scores of both infinities
+    want, tol = _expected(q, k, v, table, 2400)
+    assert bool(want[1, 2].isnan().all()) and bool(want[3, 5].isnan().all()) and bool(want[0].isfinite().all())
+    _check_odd(ops.paged_attn_decode_shared(q, k, v, table, 2400, 2176), want, tol)
 
 
 @pytest.mark.parametrize("page", [16, 64, 200])
