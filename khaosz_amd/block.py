@@ -92,8 +92,8 @@ class PagedKV:
     in a single-token step whose sequences sit at different positions; the attention kernels apply it as
     the reference's position mask (transformer.py:40-46).
     ``bind(share_prefix=True)``: the leading pages that all rows of the table have in common (found on the host copy) are
-    read once per single-token step for all sequences, by the paged-cache kernels; results within bf16 rounding of reading them per
-    sequence.  It holds until the next ``bind``."""
+    read once per single-token step for all sequences, by the paged-cache kernels, at sizes that gain by it; results within bf16
+    rounding of reading them per sequence.  It holds until the next ``bind``."""
 
     def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device, dtype,
                  n_layers: int = 1):
@@ -310,7 +310,9 @@ class GQA(nn.Module):
         if (self._decode_attention and S == 1 and attn_mask is None and isinstance(cache, PagedKV) and x.is_cuda
                 and x.dtype == torch.bfloat16):
             qkv = self._project_qkv(x, codes, norm)
-            if cache.shared_len > 0:  # the first positions of all sequences are the same pages: read once
+            if cache.shared_len > 0 and ops.paged_attn_shared_positions(B, self.n_heads, self.n_kv_heads, self.head_dim, cache.total_len,
+                                                                        cache.shared_len) > 0:
+                # the first positions of all sequences are the same pages: read once
                 kc, vc = cache.k_layers[self.layer_id], cache.v_layers[self.layer_id]
                 q = ops.rope_kv_write(qkv.view(B, -1), rotary_emb.reshape(B, -1), cache.page_table, cache.total_len - 1,
                                       kc, vc, self.n_heads, self.n_kv_heads, qk_norm=self._qk_norm())
@@ -464,8 +466,7 @@ class DecoderBlock(nn.Module):
 
     def forward(self, x: Tensor, rotary_emb: Tensor, attention_mask: Optional[Tensor] = None,
                 cache=None) -> Tensor:
-        if (self._norm_quant and self._residual_adds and attention_mask is None and cache is not None
-                and not getattr(cache, "shared_len", 0)):
+        if self._norm_quant and self._residual_adds and attention_mask is None and cache is not None:
             # everything fused, over a paged cache: the same launches, queued by native code in one call
             y = (_host or _native())(self, x, rotary_emb, cache)
             if y is not None:
@@ -489,7 +490,7 @@ class DecoderBlock(nn.Module):
 # trace calls), blocks go operator by operator, through its replacement.
 _OPERATORS = {name: getattr(ops, name) for name in (
     "quant_rowwise_i8", "rmsnorm_quant_rowwise_i8", "swiglu_quant_rowwise_i8", "linear_w8a8", "gemv_w8a8_decode", "gemv_swiglu_ok",
-    "gemv_w8a8_decode_swiglu", "gemv_w8a8_codes", "rope_kv_write", "attn_gemv_fusable", "rope_paged_attn_decode", "gemv_w8a8_attn",
+    "gemv_w8a8_decode_swiglu", "gemv_w8a8_codes", "rope_kv_write", "attn_gemv_fusable", "rope_paged_attn_decode", "paged_attn_decode_shared", "gemv_w8a8_attn",
     "prefill_attn_causal", "prefill_attn_paged", "RMSNORM_QUANT_MAX_K", "SWIGLU_QUANT_MAX_F", "GEMV_ATTN_MAX_ROWS", "GEMV_ATTN_MAX_K",
     "GEMV_ATTN_MAX_SLICES", "GEMV_ATTN_SLICE", "GEMV_ATTN_MAX_WORK")}
 _CLASSES = as_defined(GQA, MLP, PagedKV)

@@ -72,6 +72,7 @@ namespace {
   X(aq_prefill_attn_paged_ahead)                                                                                 \
   X(aq_rope_prefill_attn_causal_ahead)                                                                           \
   X(aq_rope_prefill_attn_paged_ahead)                                                                            \
+  X(aq_paged_attn_decode_shared_positions)                                                                       \
   X(aq_paged_attn_decode_shared_workspace_bytes)                                                                 \
   X(aq_paged_attn_decode_shared)                                                                                 \
   X(aq_fork_pages_workspace_bytes)                                                                               \
@@ -561,7 +562,7 @@ PyObject* compact_pages(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyObject *k_modules, *k_buffers, *k_parameters, *k_qweight, *k_w_scale, *k_bias, *k_weight, *k_norm_eps, *k_forward, *k_fwd_hooks,
     *k_fwd_pre_hooks, *k_compiled, *k_attention, *k_mlp, *k_input_norm, *k_post_norm, *k_qkv, *k_upgate, *k_o_proj, *k_down, *k_q_norm,
     *k_k_norm, *k_decode_attention, *k_use_qk_norm, *k_use_gate, *k_n_heads, *k_n_kv_heads, *k_head_dim, *k_layer_id, *k_swiglu_quant,
-    *k_norm_quant, *k_residual_adds, *k_k_layers, *k_v_layers, *k_page_table, *k_total_len, *k_seq_lens, *k_invalid, *k_page_size,
+    *k_norm_quant, *k_residual_adds, *k_k_layers, *k_v_layers, *k_page_table, *k_total_len, *k_seq_lens, *k_invalid, *k_page_size, *k_shared_len,
     *k_shared, *k_residual, *k_norm, *k_call, *k_decode_rows, *k_forward_codes, *k_forward_attn;
 
 PyObject* dict_of(PyObject* o) {  // borrowed; null if it has none
@@ -925,6 +926,7 @@ int64_t limit_of(PyObject* by_type) {
 struct Block {
   Call c;
   int64_t B, S, M, dim, Hq, Hkv, D, F, total, P, page, n_pages, fr_stride, swiglu_gemv;
+  int64_t shared = 0;  // positions that a step's sequences have in common, where it gains by reading them once
   const float* fr;
   const int64_t* table;
   const int64_t* lens = nullptr;
@@ -953,7 +955,7 @@ struct Block {
   //     -> 184.3; with qk-norm 3.1 99.8 -> 101.1, 6.3 146.3 -> 146.6, 7.9 168.5 -> 167.6, 11.8 222.0 -> 219.4.
   // (48 + 52 sizes, on an empty cache and on top of tokens; on this side of the line 0.2 to 1.5 % faster, one in ten level or 0.4 % slower.)
   bool rotates() const { return !step() && M * Hq * D >= (int64_t(qk_norm ? 4 : 2) << 20); }
-  bool merge() const { return step() && merge_in_projection(B, Hq * D, total); }
+  bool merge() const { return step() && !shared && merge_in_projection(B, Hq * D, total); }
   int queue(const void* in, void* out, char* base, const char** what) const;  // allocates nothing: runs without the interpreter lock
 };
 
@@ -998,6 +1000,8 @@ bool Block::read(PyObject* block, PyObject* px, PyObject* protary, PyObject* cac
   if (!plain(*t, ScalarType::Long, c.dev) || t->dim() != 2 || t->size(0) != B) return false;
   P = t->size(1);
   if (total < S || total > P * page) return false;
+  if (step() && integer(cd, k_shared_len, &shared) && (shared < 0 || !lib.aq_paged_attn_decode_shared_positions(B, Hq, Hkv, D, total, shared)))
+    shared = 0;
   const int64_t layer_bytes = 2 * n_pages * page * Hkv * D;
   kc = static_cast<char*>(k->mutable_data_ptr()) + layer * layer_bytes;
   vc = static_cast<char*>(v->mutable_data_ptr()) + layer * layer_bytes;
@@ -1038,8 +1042,9 @@ void Block::lay_out() {
   // attention
   qkv_rows = m.take(2 * M * qkv.N), att = m.take(2 * M * A);
   codes = m.take(few() ? lib.aq_gemv_w8a8_workspace_bytes(M, longest) : static_cast<size_t>(M * longest));
-  q = step() || rotates() ? 0 : m.take(2 * M * A), k = step() || !direct ? 0 : m.take(2 * M * KV);
+  q = (step() && !shared) || rotates() ? 0 : m.take(2 * M * A), k = step() || !direct ? 0 : m.take(2 * M * KV);
   parts_bytes = !step()   ? 0
+                : shared  ? lib.aq_paged_attn_decode_shared_workspace_bytes(B, Hq, Hkv, D, total, shared)
                 : merge() ? lib.aq_paged_attn_decode_partials_bytes(B, Hq, total)
                           : lib.aq_paged_attn_decode_workspace_bytes(B, Hq, Hkv, total);
   parts = m.take(static_cast<size_t>(parts_bytes));
@@ -1100,7 +1105,19 @@ int Block::queue(const void* in, void* out, char* base, const char** what) const
   char *q = base + qkv_rows, *att = base + this->att, *parts = base + this->parts;
   int rc = normed(qkv, n1, in, q, codes);
   if (rc) return rc;
-  if (step()) {
+  if (shared) {
+    char* qr = base + this->q;
+    *what = "aq_rope_kv_write";
+    rc = qk_norm ? lib.aq_rope_kv_write_qknorm(q, fr, fr_stride, table, P, total - 1, 1, page, kc, vc, n_pages, qr, nullptr, B, Hq, Hkv, D, qn.p,
+                                               kn.p, qn.eps, c.stream)
+                 : lib.aq_rope_kv_write(q, fr, fr_stride, table, P, total - 1, 1, page, kc, vc, n_pages, qr, nullptr, B, Hq, Hkv, D, c.stream);
+    if (rc) return rc;
+    *what = "aq_paged_attn_decode_shared";
+    rc = lib.aq_paged_attn_decode_shared(qr, kc, vc, table, P, total, shared, lens, page, n_pages, scale, att, B, Hq, Hkv, D, parts, parts_bytes,
+                                         c.stream);
+    if (rc) return rc;
+    rc = projected(o, att, in, x1, codes);
+  } else if (step()) {
     *what = "aq_rope_paged_attn_decode";
     if (merge()) {
       rc = qk_norm ? lib.aq_rope_paged_attn_decode_partials_qknorm(q, fr, fr_stride, table, P, total, lens, page, kc, vc, n_pages, scale, B,
@@ -1254,6 +1271,7 @@ PyMODINIT_FUNC PyInit__host() {
               {&k_norm_quant, "_norm_quant"}, {&k_residual_adds, "_residual_adds"}, {&k_k_layers, "k_layers"},
               {&k_v_layers, "v_layers"},      {&k_page_table, "page_table"},    {&k_total_len, "total_len"},
               {&k_seq_lens, "seq_lens"},      {&k_invalid, "_invalid"},         {&k_page_size, "page_size"},
+              {&k_shared_len, "shared_len"},
               {&k_shared, "_shared"},         {&k_residual, "residual"},        {&k_norm, "norm"},
               {&k_call, "__call__"},          {&k_decode_rows, "DECODE_MAX_ROWS"},
               {&k_forward_codes, "forward_codes"}, {&k_forward_attn, "forward_attn"}};

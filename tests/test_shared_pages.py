@@ -77,6 +77,14 @@ def test_sizes_of_workspaces():
     assert size(2, 4, 2, 64, 3000, 2990) == 4 * (23 * 2 * 68 * 32 + 2 * 2 * 68 * 2)
 
 
+def test_positions_that_are_read_once():
+    f = _abi.load().aq_paged_attn_decode_shared_positions
+    assert f(0, 4, 2, 64, 3000, 2990) == 0 and f(2, 5, 2, 64, 3000, 2990) == 0 and f(2, 4, 2, 96, 3000, 2990) == 0 and f(2, 4, 2, 64, 3000, -1) == 0
+    assert f(2, 4, 2, 64, 3000, 2990) == 2944 and f(2, 4, 2, 64, 3000, 1 << 40) == 2944 and f(1, 4, 2, 64, 3000, 2990) == 0
+    assert f(2, 4, 2, 64, 100, 64) == 0 and f(2, 4, 2, 64, 3000, 63) == 0
+    assert ops.paged_attn_shared_positions(2, 4, 2, 64, 3000, 2990) == 2944
+
+
 def test_cpu_tensors_are_refused():
     cache = PagedKV(8, 16, 2, 64, "cpu", torch.bfloat16).bind(torch.arange(8).view(2, 4), 40)
     with pytest.raises(RuntimeError, match="GPU only"):
@@ -197,3 +205,52 @@ def test_samples_of_a_prompt(options, mixed, monkeypatch):
         logits = step(tokens, table, total, lens, alone)
         assert torch.equal(logits[3], logits[0]) and not torch.equal(logits[1], logits[0])
     assert calls == [t for t in range(2101, 2108) for _ in range(2)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("options", [{}, {"use_qk_norm": True}])
+@pytest.mark.parametrize("mixed", [False, True])
+@pytest.mark.parametrize("batch", [3, 40])
+def test_native_blocks_share_too(options, mixed, batch, monkeypatch):
+    """A step with the blocks queued natively, and operator by operator: the same bits, in the logits and in the cache."""
+    m = _model(**options)
+    g = torch.Generator().manual_seed(5)
+    cache = m.new_cache(140 + batch, 16)
+    for c in (cache.k_layers, cache.v_layers):
+        c.copy_(torch.randn(c.shape, generator=g))
+    table = torch.cat([torch.arange(131).expand(batch, -1), 131 + torch.arange(batch)[:, None]], 1).cuda()
+    total = 2101
+    lens = torch.randint(1500, total + 1, (batch,), generator=g).cuda() if mixed else None
+    where = dict(start_pos=total - 1) if lens is None else dict(position_ids=(lens - 1).view(-1, 1))
+    tokens = torch.randint(0, 97, (batch, 1), generator=g).cuda()
+    run, calls, outs, held = ops.paged_attn_decode_shared, [], [], []
+    assert ops.paged_attn_shared_positions(batch, 8, 2, 64, total, 2096) == 2048
+    for alone in (False, True):
+        if alone:
+            monkeypatch.setattr(ops, "paged_attn_decode_shared", lambda *a, **k: (calls.append(a[5]), run(*a, **k))[1])
+        cache.bind(table, total, share_prefix=True)
+        assert cache.shared_len == 2096
+        with torch.inference_mode():
+            outs.append(m(tokens, paged_cache=cache, **where)["logits"])
+        held.append((cache.k_layers.clone(), cache.v_layers.clone()))
+    assert calls == [2096, 2096]
+    assert torch.equal(outs[0], outs[1])
+    assert torch.equal(held[0][0], held[1][0]) and torch.equal(held[0][1], held[1][1])
+
+
+@pytest.mark.gpu
+def test_a_prefix_that_gains_nothing_is_read_as_ever():
+    m = _model()
+    g = torch.Generator().manual_seed(6)
+    cache = m.new_cache(40, 16)
+    for c in (cache.k_layers, cache.v_layers):
+        c.copy_(torch.randn(c.shape, generator=g))
+    table = torch.cat([torch.arange(10).expand(2, -1), 10 + torch.arange(2)[:, None]], 1).cuda()
+    assert ops.paged_attn_shared_positions(2, 8, 2, 64, 165, 160) == 0
+    outs = []
+    for share in (False, True):
+        cache.bind(table, 165, share_prefix=share)
+        assert cache.shared_len == (160 if share else 0)
+        with torch.inference_mode():
+            outs.append(m(torch.tensor([[3], [5]]).cuda(), paged_cache=cache, start_pos=164)["logits"])
+    assert torch.equal(outs[0], outs[1])
