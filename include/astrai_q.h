@@ -506,7 +506,7 @@ int aq_paged_attn_decode_shared(const void *q, const void *k_cache, const void *
  * that is to keep it as it is comes first, as a row of the table whose first child it is, or holds filled pages only.)  new_refs = max(refs - entries of the old rows, 0) + entries of the new rows, so rows without a child
  * let go of their pages, and the pages that are then free are handed out lowest first, to the rows in order.  missing[0]: rows that
  * found none (their entry is -1).  Sources are held, destinations free: the copies touch no page in use.
- * workspace: aq_fork_pages_workspace_bytes(n_pages, R) bytes.  It and refs are 16-byte aligned.
+ * R at most 65536 (AQ_E_RANGE).  workspace: aq_fork_pages_workspace_bytes(n_pages, R) bytes.  It and refs are 16-byte aligned.
  *
  * aq_compact_pages: live[0] = number of pages with refs > 0; the held pages past place live[0] - 1 are moved into the free ones in front of
  * it, the last one held into the first hole, and so on.  where[x] (int64 [n_pages]): where held page x is now, -1 if it is free;

@@ -10,6 +10,14 @@ namespace aq {
 
 constexpr int PG_THREADS = 1024, PG_PAGES = 4 * PG_THREADS;  // of a workgroup that numbers pages: 4 to a thread
 constexpr int PG_COPY = 256, PG_UNIT = 8 * 1024;              // a copying workgroup, and the bytes of its turn: 2 x 16 to a thread
+constexpr int PG_TURN = 4 * PG_COPY, PG_SEGMENTS = 1024;      // where pages are counted in segments: pages of a turn, at most so many segments
+
+// Turns of a segment; as many segments as the pages take.
+static int64_t segment_turns(int64_t n_pages) { return (n_pages + PG_TURN * PG_SEGMENTS - 1) / (PG_TURN * PG_SEGMENTS); }
+static int64_t segments(int64_t n_pages) {
+  const int64_t size = segment_turns(n_pages) * PG_TURN;
+  return (n_pages + size - 1) / size;
+}
 
 // A copy that a row needs: the page, its written positions, the row, and the entry of the row that gets the new page.
 struct ForkCopy {
@@ -28,15 +36,18 @@ struct ForkArgs {
   ForkCopy* copies;        // [R] the same, the rows that need one only
   int32_t* fresh;          // [R] the pages they get, ascending
   int32_t* got;            // [1] rows that get one
+  int32_t* need;           // [1] rows that need one
+  int32_t* free_pages;     // [segments] free pages of each segment, these rows not yet served
   int32_t* gone;           // [n_pages] entries of the old rows that name the page
   int32_t* come;           // [n_pages] entries of the new rows that name it
   uint8_t *k, *v;          // [layers][n_pages][page][row_bytes]
   int64_t layer_bytes, row_bytes, page_bytes, T, n_pages;
-  int B, R, P, layers, page;
+  int B, R, P, layers, page, turns;
   UDiv by_p;  // (one-workgroup form)
 };
 
 // Sum over the threads before this one; *all: over all of them.
+template <int THREADS>
 __device__ __forceinline__ int wg_before(int v, int* s, int* all) {
   const int tid = threadIdx.x, lane = tid & 63;
   int x = v;
@@ -50,7 +61,7 @@ __device__ __forceinline__ int wg_before(int v, int* s, int* all) {
   __syncthreads();
   int base = 0, sum = 0;
 #pragma unroll
-  for (int w = 0; w < PG_THREADS / 64; ++w) {
+  for (int w = 0; w < THREADS / 64; ++w) {
     if (w < tid >> 6) base += s[w];
     sum += s[w];
   }
@@ -58,14 +69,14 @@ __device__ __forceinline__ int wg_before(int v, int* s, int* all) {
   return base + x - v;
 }
 
-// f(x, count of the pages x .. x + 3 that are there) summed over the workgroup, x = 4 i for i in [i0, i1); several loads in flight.
-template <class F>
+// f(i) summed over the workgroup, i in [i0, i1); several loads in flight.
+template <int THREADS, class F>
 __device__ __forceinline__ int wg_count(int64_t i0, int64_t i1, int* s, F&& f) {
   int n = 0;
 #pragma unroll 8
-  for (int64_t i = i0 + threadIdx.x; i < i1; i += PG_THREADS) n += f(i);
+  for (int64_t i = i0 + threadIdx.x; i < i1; i += THREADS) n += f(i);
   int all;
-  wg_before(n, s, &all);
+  wg_before<THREADS>(n, s, &all);
   return all;
 }
 
@@ -107,9 +118,10 @@ __global__ __launch_bounds__(PG_THREADS) void fork_clear_kernel(v4i* p, int64_t 
 
 // ROWS rows of the new table, or (the workgroups behind those) of the old one, whose pages are let go; a thread has a column, so that
 // neighbouring rows with the same page (what sequences share) are one atomic.  (256 old and 300 new rows of 129 columns, 63 of them
-// alike: 9.5 us with one row to a workgroup, most of it 556 atomics on each shared page in turn.)  Counts are whole numbers: the order
+// alike: 9.5 us with one row to a workgroup, most of it 556 atomics on each shared page in turn; 6.9 with two, 5.7 with four, 7.0 with eight,
+// 12.8 with 16, which are 35 workgroups.)  Counts are whole numbers: the order
 // of the atomics changes nothing.
-constexpr int FORK_ROWS = 16;
+constexpr int FORK_ROWS = 4;
 __global__ __launch_bounds__(PG_COPY) void fork_rows_kernel(ForkArgs a, int new_wgs, int chunks) {
   __shared__ int parent_s[FORK_ROWS], whole_s[FORK_ROWS], rest_s[FORK_ROWS], later_s[FORK_ROWS];
   const int tid = threadIdx.x;
@@ -166,39 +178,67 @@ __global__ __launch_bounds__(PG_COPY) void fork_rows_kernel(ForkArgs a, int new_
 }
 
 // The rows that need a page, numbered: returns how many.
-__device__ __forceinline__ int fork_number(const ForkArgs& a, int* s, bool write) {
+template <int THREADS>
+__device__ __forceinline__ int fork_number(const ForkArgs& a, int* s) {
   int done = 0;
-  for (int i0 = 0; i0 < a.R; i0 += PG_THREADS) {
+  for (int i0 = 0; i0 < a.R; i0 += THREADS) {
     const int i = i0 + (int)threadIdx.x;
     ForkCopy w = {-1, 0, 0, 0};
     if (i < a.R) w = a.wants[i];
     int all;
-    const int at = done + wg_before(w.source >= 0, s, &all);
-    if (write && w.source >= 0) a.copies[at] = w;
+    const int at = done + wg_before<THREADS>(w.source >= 0, s, &all);
+    if (w.source >= 0) a.copies[at] = w;
     done += all;
   }
   return done;
 }
 
-// The new counts, and the free pages for the rows that need one: the k-th free page to the k-th row.  Every workgroup counts the rows, and
-// the free pages in front of its own, by itself (40000 pages: 53 us with a load of each count at a time by 256 threads).
-__global__ __launch_bounds__(PG_THREADS) void fork_refs_kernel(ForkArgs a) {
-  __shared__ int s[PG_THREADS / 64];
-  const int64_t i0 = (int64_t)blockIdx.x * PG_THREADS, i = i0 + threadIdx.x, x = 4 * i;
-  int base = wg_count(0, i0, s, [&](int64_t i) {
+// New counts of the pages x .. x + 3, of those that are there (others: 1).
+__device__ __forceinline__ void fork_counts(const ForkArgs& a, int64_t x, int (&c)[4]) {
+  if (x + 4 <= a.n_pages) {
+    const int64_t i = x / 4;
     const v4i r = reinterpret_cast<const v4i*>(a.refs)[i], g = reinterpret_cast<const v4i*>(a.gone)[i], n = reinterpret_cast<const v4i*>(a.come)[i];
-    return (fork_count(r.x, g.x, n.x) == 0) + (fork_count(r.y, g.y, n.y) == 0) + (fork_count(r.z, g.z, n.z) == 0) + (fork_count(r.w, g.w, n.w) == 0);
-  });
-  const int need = fork_number(a, s, blockIdx.x == 0);
-  int c[4] = {1, 1, 1, 1};
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (x + u < a.n_pages) c[u] = fork_count(a.refs[x + u], a.gone[x + u], a.come[x + u]);
-  int all;
-  const int at = base + wg_before((c[0] == 0) + (c[1] == 0) + (c[2] == 0) + (c[3] == 0), s, &all);
-  fork_hand_out(a, x, c, at, need);
-  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+    for (int u = 0; u < 4; ++u) c[u] = fork_count(r[u], g[u], n[u]);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) c[u] = x + u < a.n_pages ? fork_count(a.refs[x + u], a.gone[x + u], a.come[x + u]) : 1;
+}
+
+// The free pages of each segment; the last workgroup numbers the rows.  (Every workgroup counting what lies in front of its own pages
+// instead, in one launch: 40000 pages 12 us, this and the next kernel 4.0 and 3.3.)
+__global__ __launch_bounds__(PG_COPY) void fork_free_kernel(ForkArgs a) {
+  __shared__ int s[PG_COPY / 64];
+  if (blockIdx.x == gridDim.x - 1) {
+    const int need = fork_number<PG_COPY>(a, s);
+    if (threadIdx.x == 0) a.need[0] = need;
+    return;
+  }
+  const int64_t x0 = (int64_t)blockIdx.x * a.turns * PG_TURN;
+  const int n = wg_count<PG_COPY>(0, (int64_t)a.turns * PG_COPY, s, [&](int64_t i) {
+    const int64_t x = x0 + 4 * i;
+    int c[4] = {1, 1, 1, 1};
+    if (x < a.n_pages) fork_counts(a, x, c);
+    return (c[0] == 0) + (c[1] == 0) + (c[2] == 0) + (c[3] == 0);
+  });
+  if (threadIdx.x == 0) a.free_pages[blockIdx.x] = n;
+}
+
+// The new counts, and the free pages for the rows that need one: the k-th free page to the k-th row.
+__global__ __launch_bounds__(PG_COPY) void fork_refs_kernel(ForkArgs a) {
+  __shared__ int s[PG_COPY / 64];
+  const int need = a.need[0];
+  int base = wg_count<PG_COPY>(0, blockIdx.x, s, [&](int64_t i) { return a.free_pages[i]; });
+  for (int turn = 0; turn < a.turns; ++turn) {
+    const int64_t x = (((int64_t)blockIdx.x * a.turns + turn) * PG_COPY + threadIdx.x) * 4;
+    int c[4] = {1, 1, 1, 1}, all;
+    if (x < a.n_pages) fork_counts(a, x, c);
+    const int at = base + wg_before<PG_COPY>((c[0] == 0) + (c[1] == 0) + (c[2] == 0) + (c[3] == 0), s, &all);
+    fork_hand_out(a, x, c, at, need);
     base += all;
+  }
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
     a.got[0] = need < base ? need : base;
     a.missing[0] = need > base ? need - base : 0;
   }
@@ -241,7 +281,7 @@ __global__ __launch_bounds__(PG_THREADS) void fork_one_kernel(ForkArgs a) {
     if (l == 0 && whole >= a.P) a.wants[i] = {-1, 0, i, 0};
   }
   __syncthreads();
-  const int need = fork_number(a, s, true);
+  const int need = fork_number<PG_THREADS>(a, s);
   int base = 0;
   for (int x0 = 0; x0 < pages; x0 += PG_PAGES) {
     const int x = x0 + 4 * tid;
@@ -250,7 +290,7 @@ __global__ __launch_bounds__(PG_THREADS) void fork_one_kernel(ForkArgs a) {
     for (int u = 0; u < 4; ++u)
       if (x + u < (int)a.n_pages) c[u] = fork_count(a.refs[x + u], gone[x + u], come[x + u]);
     int all;
-    const int at = base + wg_before((c[0] == 0) + (c[1] == 0) + (c[2] == 0) + (c[3] == 0), s, &all);
+    const int at = base + wg_before<PG_THREADS>((c[0] == 0) + (c[1] == 0) + (c[2] == 0) + (c[3] == 0), s, &all);
     fork_hand_out(a, x, c, at, need);
     base += all;
   }
@@ -327,48 +367,79 @@ struct CompactArgs {
   int32_t* hole;    // [n_pages] the k-th free one from the bottom
   int32_t* move;    // [n_pages] of a held page past the last place: which move is its own
   int32_t* moves;   // [1]
+  int32_t* held;    // [segments] held pages of each segment
   uint8_t *k, *v;
   int64_t layer_bytes, page_bytes, n_pages, entries;
-  int layers, copy_wgs;
+  int layers, copy_wgs, turns;
 };
 
-// Numbers the pages: live of them are held, places 0 .. live - 1 are to hold them.  Every workgroup counts what lies in front of its own
-// pages, and all, by itself (60000 pages: 96 us with a load at a time by 256 threads).
-__global__ __launch_bounds__(PG_THREADS) void compact_rank_kernel(CompactArgs a) {
-  __shared__ int s[PG_THREADS / 64];
-  const int64_t i0 = (int64_t)blockIdx.x * PG_THREADS, i = i0 + threadIdx.x, x = 4 * i, whole = a.n_pages / 4;
-  auto held4 = [&](int64_t i) {
-    const v4i r = reinterpret_cast<const v4i*>(a.refs)[i];
-    return (r.x > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0);
-  };
-  int r[4] = {0, 0, 0, 0};
+__device__ __forceinline__ void compact_refs(const CompactArgs& a, int64_t x, int (&r)[4]) {  // of the pages x .. x + 3 that are there (others: 0)
+  if (x + 4 <= a.n_pages) {
+    const v4i y = reinterpret_cast<const v4i*>(a.refs)[x / 4];
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (x + u < a.n_pages) r[u] = a.refs[x + u];
-  const int before = wg_count(0, i0, s, held4);
-  int rest = wg_count(i0 + PG_THREADS, whole, s, held4), mine;
-  int at = before + wg_before((r[0] > 0) + (r[1] > 0) + (r[2] > 0) + (r[3] > 0), s, &mine);  // held pages in front of x
-  if (i0 + PG_THREADS <= whole)  // the pages behind the last whole four
-    for (int64_t y = 4 * whole; y < a.n_pages; ++y) rest += a.refs[y] > 0;
-  const int live = before + mine + rest;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int64_t y = x + u;
-    if (y >= a.n_pages) break;
-    const bool held = r[u] > 0;
-    a.where[y] = held && y < live ? y : -1;  // moved pages: their move says
-    a.new_refs[y] = held && y < live ? r[u] : 0;
-    if (held && y >= live) {
-      a.source[live - 1 - at] = (int)y;
-      a.move[y] = live - 1 - at;
-    }
-    if (!held && y < live) a.hole[y - at] = (int)y;
-    at += held;
-    if (y == live - 1) a.moves[0] = live - at;  // free pages among the first live
+    for (int u = 0; u < 4; ++u) r[u] = y[u];
+    return;
   }
-  if (x == 0) {
-    a.live[0] = live;
-    if (live == 0) a.moves[0] = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) r[u] = x + u < a.n_pages ? a.refs[x + u] : 0;
+}
+
+__device__ __forceinline__ int compact_held(const CompactArgs& a, int64_t x) {
+  int r[4] = {0, 0, 0, 0};
+  if (x < a.n_pages) compact_refs(a, x, r);
+  return (r[0] > 0) + (r[1] > 0) + (r[2] > 0) + (r[3] > 0);
+}
+
+__global__ __launch_bounds__(PG_COPY) void compact_count_kernel(CompactArgs a) {
+  __shared__ int s[PG_COPY / 64];
+  const int64_t i0 = (int64_t)blockIdx.x * a.turns * PG_COPY;
+  const int n = wg_count<PG_COPY>(i0, i0 + (int64_t)a.turns * PG_COPY, s, [&](int64_t i) { return compact_held(a, 4 * i); });
+  if (threadIdx.x == 0) a.held[blockIdx.x] = n;
+}
+
+// Numbers the pages: live of them are held, places 0 .. live - 1 are to hold them.  THREADS x 4 pages a turn.  Up to 16384 pages every
+// workgroup counts what lies in front of its own turn, and all, by itself (COUNT): a launch less.  (60000 pages: 12.3 us; counted in
+// segments first, 4.6 and 4.8.)
+constexpr int COMPACT_COUNT = 16384;
+template <int THREADS, bool COUNT>
+__global__ __launch_bounds__(THREADS) void compact_rank_kernel(CompactArgs a) {
+  __shared__ int s[THREADS / 64];
+  const int64_t turns = COUNT ? 1 : a.turns, i0 = (int64_t)blockIdx.x * turns * THREADS;
+  int before, live;
+  if constexpr (COUNT) {
+    auto held = [&](int64_t i) { return compact_held(a, 4 * i); };
+    before = wg_count<THREADS>(0, i0, s, held);
+    live = before + wg_count<THREADS>(i0, (a.n_pages + 3) / 4, s, held);
+  } else {
+    auto held = [&](int64_t i) { return a.held[i]; };
+    before = wg_count<THREADS>(0, blockIdx.x, s, held);
+    live = before + wg_count<THREADS>(blockIdx.x, gridDim.x, s, held);
+  }
+  for (int64_t turn = 0; turn < turns; ++turn) {
+    const int64_t x = 4 * (i0 + turn * THREADS + threadIdx.x);
+    int r[4] = {0, 0, 0, 0}, mine;
+    if (x < a.n_pages) compact_refs(a, x, r);
+    int at = before + wg_before<THREADS>((r[0] > 0) + (r[1] > 0) + (r[2] > 0) + (r[3] > 0), s, &mine);  // held pages in front of x
+    before += mine;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t y = x + u;
+      if (y >= a.n_pages) break;
+      const bool held = r[u] > 0;
+      a.where[y] = held && y < live ? y : -1;  // moved pages: their move says
+      a.new_refs[y] = held && y < live ? r[u] : 0;
+      if (held && y >= live) {
+        a.source[live - 1 - at] = (int)y;
+        a.move[y] = live - 1 - at;
+      }
+      if (!held && y < live) a.hole[y - at] = (int)y;
+      at += held;
+      if (y == live - 1) a.moves[0] = live - at;  // free pages among the first live
+    }
+    if (x == 0) {
+      a.live[0] = live;
+      if (live == 0) a.moves[0] = 0;
+    }
   }
 }
 
@@ -424,7 +495,7 @@ static int check_caches(const void* k, const void* v, int64_t layers, int64_t la
 }
 
 // Workspace of a fork: the list of copies, then the counts.
-static int64_t fork_words(int64_t n_pages, int64_t R) { return 8 * R + (R + 4) / 4 * 4 + 2 * ((n_pages + 3) / 4 * 4); }
+static int64_t fork_words(int64_t n_pages, int64_t R) { return 8 * R + (R + 4 + segments(n_pages) + 1) / 4 * 4 + 2 * ((n_pages + 3) / 4 * 4); }
 
 }  // namespace aq
 
@@ -438,7 +509,7 @@ extern "C" int aq_fork_pages(const int64_t* page_table, int64_t B, int64_t P, co
                              int32_t* new_refs, int32_t* missing, void* workspace, int64_t workspace_bytes, void* stream) {
   if (B < 0 || R < 0 || P <= 0 || total_len < 0) return AQ_E_SHAPE;
   if (const int rc = aq::check_caches(k_layers, v_layers, layers, layer_bytes, n_pages, page_size, row_bytes)) return rc;
-  if (B > (1 << 24) || R > (1 << 24) || P > 0x7fffffff) return AQ_E_RANGE;
+  if (B > (1 << 24) || R > (1 << 16) || P > 0x7fffffff) return AQ_E_RANGE;  // (every row looks for earlier siblings)
   if (total_len > P * page_size) return AQ_E_SHAPE;  // positions the page table does not cover
   if ((B > 0 && !page_table) || (R > 0 && (!parents || !new_table)) || !refs || !new_refs || !missing || !workspace) return AQ_E_NULL;
   if (aq::check_ptr(page_table, 8) || aq::check_ptr(parents, 8) || aq::check_ptr(seq_lens, 8) || aq::check_ptr(new_table, 8) ||
@@ -457,7 +528,9 @@ extern "C" int aq_fork_pages(const int64_t* page_table, int64_t B, int64_t P, co
   a.copies = a.wants + R;
   a.fresh = reinterpret_cast<int32_t*>(a.copies + R);
   a.got = a.fresh + R;
-  a.gone = a.fresh + (R + 4) / 4 * 4;
+  a.need = a.got + 1;
+  a.free_pages = a.need + 1;
+  a.gone = a.fresh + (R + 4 + aq::segments(n_pages) + 1) / 4 * 4;
   a.come = a.gone + (n_pages + 3) / 4 * 4;
   a.k = static_cast<uint8_t*>(k_layers);
   a.v = static_cast<uint8_t*>(v_layers);
@@ -477,14 +550,16 @@ extern "C" int aq_fork_pages(const int64_t* page_table, int64_t B, int64_t P, co
     a.by_p = aq::UDiv::of((uint32_t)P);
     aq::queue_kernel(aq::fork_one_kernel, dim3(1), one, (size_t)(2 * ((n_pages + 3) / 4 * 4) + B) * sizeof(int), st, a);
   } else {
-    const int64_t quads = (n_pages + 3) / 4 * 2, groups = (n_pages + aq::PG_PAGES - 1) / aq::PG_PAGES;
+    const int64_t quads = (n_pages + 3) / 4 * 2, groups = aq::segments(n_pages);
+    a.turns = (int)aq::segment_turns(n_pages);
     aq::queue_kernel(aq::fork_clear_kernel, dim3((unsigned)((quads + aq::PG_THREADS - 1) / aq::PG_THREADS)), one, 0, st,
                      reinterpret_cast<v4i*>(a.gone), quads);
     const int64_t chunks = (P + aq::PG_COPY - 1) / aq::PG_COPY, new_wgs = (R + aq::FORK_ROWS - 1) / aq::FORK_ROWS * chunks;
     const int64_t wgs = new_wgs + (B + aq::FORK_ROWS - 1) / aq::FORK_ROWS * chunks;
     if (wgs > 0x7fffffff) return AQ_E_RANGE;
     if (wgs > 0) aq::queue_kernel(aq::fork_rows_kernel, dim3((unsigned)wgs), dim3(aq::PG_COPY), 0, st, a, (int)new_wgs, (int)chunks);
-    aq::queue_kernel(aq::fork_refs_kernel, dim3((unsigned)groups), one, 0, st, a);
+    aq::queue_kernel(aq::fork_free_kernel, dim3((unsigned)groups + 1), dim3(aq::PG_COPY), 0, st, a);
+    aq::queue_kernel(aq::fork_refs_kernel, dim3((unsigned)groups), dim3(aq::PG_COPY), 0, st, a);
   }
   if (R > 1) {  // (a single row is its parent's first child)
     aq::CopyPlan plan;
@@ -494,7 +569,9 @@ extern "C" int aq_fork_pages(const int64_t* page_table, int64_t B, int64_t P, co
   return (int)hipGetLastError();
 }
 
-extern "C" int64_t aq_compact_pages_workspace_bytes(int64_t n_pages) { return n_pages <= 0 ? 0 : (3 * n_pages + 1) * (int64_t)sizeof(int32_t); }
+extern "C" int64_t aq_compact_pages_workspace_bytes(int64_t n_pages) {
+  return n_pages <= 0 ? 0 : (3 * n_pages + 1 + aq::segments(n_pages)) * (int64_t)sizeof(int32_t);
+}
 
 extern "C" int aq_compact_pages(const int64_t* page_table, int64_t entries, const int32_t* refs, void* k_layers, void* v_layers,
                                 int64_t layers, int64_t layer_bytes, int64_t n_pages, int64_t page_size, int64_t row_bytes,
@@ -518,6 +595,8 @@ extern "C" int aq_compact_pages(const int64_t* page_table, int64_t entries, cons
   a.hole = a.source + n_pages;
   a.move = a.hole + n_pages;
   a.moves = a.move + n_pages;
+  a.held = a.moves + 1;
+  a.turns = (int)aq::segment_turns(n_pages);
   a.k = static_cast<uint8_t*>(k_layers);
   a.v = static_cast<uint8_t*>(v_layers);
   a.layer_bytes = layer_bytes;
@@ -526,7 +605,13 @@ extern "C" int aq_compact_pages(const int64_t* page_table, int64_t entries, cons
   a.entries = entries;
   a.layers = (int)layers;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  aq::queue_kernel(aq::compact_rank_kernel, dim3((unsigned)((n_pages + aq::PG_PAGES - 1) / aq::PG_PAGES)), dim3(aq::PG_THREADS), 0, st, a);
+  if (n_pages <= aq::COMPACT_COUNT) {
+    aq::queue_kernel(aq::compact_rank_kernel<aq::PG_THREADS, true>, dim3((unsigned)((n_pages + aq::PG_PAGES - 1) / aq::PG_PAGES)), dim3(aq::PG_THREADS), 0, st, a);
+  } else {
+    const dim3 groups((unsigned)aq::segments(n_pages)), threads(aq::PG_COPY);
+    aq::queue_kernel(aq::compact_count_kernel, groups, threads, 0, st, a);
+    aq::queue_kernel(aq::compact_rank_kernel<aq::PG_COPY, false>, groups, threads, 0, st, a);
+  }
   aq::CopyPlan plan;
   a.copy_wgs = (int)aq::copy_plan(plan, n_pages / 2, layers, a.page_bytes);
   const int64_t work = entries > n_pages / 2 ? entries : n_pages / 2, rest = (work + aq::PG_COPY - 1) / aq::PG_COPY;

@@ -114,7 +114,8 @@ def test_fork_small(page, total, parents):
 @pytest.mark.parametrize("B,R,P,page,n_pages,layers,seed", [(64, 64, 23, 16, 2000, 2, 0), (1, 300, 5, 64, 400, 1, 1), (200, 40, 30, 4, 6100, 1, 2),
                                                            (256, 300, 17, 16, 9000, 3, 3), (2, 2, 2049, 2, 4200, 1, 4),
                                                            (70, 90, 200, 4, 14500, 1, 5), (4, 9, 3, 16, 8193, 1, 6), (300, 5000, 2, 4, 5700, 1, 7),
-                                                           (5, 7, 4, 16, 8190, 1, 8), (64, 2100, 3, 4, 4097, 2, 9)])
+                                                           (5, 7, 4, 16, 8190, 1, 8), (64, 2100, 3, 4, 4097, 2, 9),
+                                                           (300, 700, 3600, 2, 1100003, 1, 10)])
 def test_fork_rows_at_lengths_of_their_own(B, R, P, page, n_pages, layers, seed):
     _say("fork lens", B, R, P, page, n_pages)
     table, refs, k, v = _state(B, P, n_pages, page, layers=layers, seed=seed, common=min(3, P - 1), heads=1)
@@ -169,7 +170,7 @@ def test_fork_and_compact_one_layer_of_any_type(dtype):
     _equal(got, want, kd.unsqueeze(0), vd.unsqueeze(0))
 
 
-@pytest.mark.parametrize("n_pages,live", [(1, 0), (1, 1), (8, 3), (100, 0), (100, 100), (4096, 2000), (4097, 4096), (5000, 1), (20000, 11111), (70001, 35000)])
+@pytest.mark.parametrize("n_pages,live", [(1, 0), (1, 1), (8, 3), (100, 0), (100, 100), (4096, 2000), (4097, 4096), (5000, 1), (16384, 9000), (16385, 16000), (20000, 11111), (70001, 35000), (1100003, 600001)])
 def test_compact(n_pages, live):
     _say("compact", n_pages, live)
     g = torch.Generator().manual_seed(n_pages + live)

@@ -42,7 +42,7 @@ def _fork(**change):
     (dict(table=None), -1), (dict(refs=None), -1), (dict(parents=None), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(new_table=None), -1),
     (dict(new_refs=None), -1), (dict(missing=None), -1), (dict(ws=None), -1), (dict(k=P + 8), -4), (dict(v=P + 4), -4), (dict(table=P + 4), -4),
     (dict(parents=P + 4), -4), (dict(lens=P + 4), -4), (dict(refs=P + 2), -4), (dict(new_refs=P + 2), -4), (dict(new_table=P + 4), -4),
-    (dict(ws=P + 8), -4), (dict(refs=P + 8), -4), (dict(total=49), -2), (dict(ws_bytes=100), -5), (dict(n_pages=0x7fffffff, layer_bytes=1 << 62), -6), (dict(R=1 << 25), -6), (dict(B=1 << 25), -6),
+    (dict(ws=P + 8), -4), (dict(refs=P + 8), -4), (dict(total=49), -2), (dict(ws_bytes=100), -5), (dict(n_pages=0x7fffffff, layer_bytes=1 << 62), -6), (dict(R=1 << 25), -6), (dict(R=(1 << 16) + 1), -6), (dict(B=1 << 25), -6),
 ])
 def test_forks_are_refused_before_any_launch(change, code):
     assert _fork(**change) == code
