@@ -244,19 +244,43 @@ __global__ __launch_bounds__(PG_COPY) void fork_refs_kernel(ForkArgs a) {
   }
 }
 
-// All of the above by one workgroup, its counts in LDS, for small tables and caches: one launch instead of three.
+// All of the above by one workgroup, its counts and rows in LDS, for small tables and caches: one launch instead of four.  What it waits for is
+// a chain of reads, so that the counts are requested first and each row's parent and length looked up once (1 row into 8, 64 pages, and
+// 64 into 64, 2048 pages: 4.7 and 6.4 us with every entry looking them up and the list of copies read back from memory, 4.5 and 5.8).
 constexpr int FORK_ONE_PAGES = 8192, FORK_ONE_ROWS = 4096, FORK_ONE_ENTRIES = 32768;
+struct ForkRow {
+  int parent, whole, rest, source;  // row of the table or -1, pages that are full, rows of the next one, and its page if it is copied, or -1
+};
+static size_t fork_one_lds(int64_t n_pages, int64_t B, int64_t R) { return (n_pages + 3) / 4 * 8 * sizeof(int) + (B + 3) / 4 * 4 * sizeof(int) + R * sizeof(ForkRow); }
+
 __global__ __launch_bounds__(PG_THREADS) void fork_one_kernel(ForkArgs a) {
   __shared__ int s[PG_THREADS / 64];
   extern __shared__ __align__(16) int pg_lds[];
   const int tid = threadIdx.x, pages = ((int)a.n_pages + 3) & ~3;
   int *const gone = pg_lds, *const come = gone + pages, *const first_of = come + pages;
+  ForkRow* const rows = reinterpret_cast<ForkRow*>(first_of + ((a.B + 3) & ~3));
+  int refs[FORK_ONE_PAGES / PG_PAGES][4];
+#pragma unroll
+  for (int t = 0; t < FORK_ONE_PAGES / PG_PAGES; ++t)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int x = t * PG_PAGES + 4 * tid + u;
+      refs[t][u] = x < (int)a.n_pages ? a.refs[x] : 1;
+    }
   for (int x = tid; x < 2 * pages; x += PG_THREADS) gone[x] = 0;
   for (int p = tid; p < a.B; p += PG_THREADS) first_of[p] = a.R;
   __syncthreads();
   for (int i = tid; i < a.R; i += PG_THREADS) {
     const int64_t p = a.parents[i];
-    if (p >= 0 && p < a.B) atomicMin(first_of + p, i);
+    ForkRow r = {-1, 0, 0, -1};
+    if (p >= 0 && p < a.B) {
+      const int64_t n = fork_length(a, (int)p);
+      r.parent = (int)p;
+      r.whole = (int)(n / a.page);
+      r.rest = (int)(n - (int64_t)r.whole * a.page);
+      atomicMin(first_of + p, i);
+    }
+    rows[i] = r;
   }
 #pragma unroll 2
   for (int x = tid; x < a.B * a.P; x += PG_THREADS) {
@@ -267,29 +291,33 @@ __global__ __launch_bounds__(PG_THREADS) void fork_one_kernel(ForkArgs a) {
 #pragma unroll 2
   for (int x = tid; x < a.R * a.P; x += PG_THREADS) {
     const int i = a.by_p((uint32_t)x), l = x - i * a.P;
-    const int64_t parent = a.parents[i];
-    const bool known = parent >= 0 && parent < a.B;
-    const int p = known ? (int)parent : 0;
-    const int64_t n = known ? fork_length(a, p) : 0;
-    const int whole = (int)(n / a.page), mine = known ? fork_entry(a, p, l) : -1;
-    const bool first = known && first_of[p] == i;
-    const int e = first || l < whole ? mine : -1;
+    const ForkRow r = rows[i];
+    const int mine = r.parent >= 0 ? fork_entry(a, r.parent, l) : -1;
+    const bool first = r.parent >= 0 && first_of[r.parent] == i;
+    const int e = first || l < r.whole ? mine : -1;
     a.new_table[x] = e;
     if (e >= 0) atomicAdd(come + e, 1);
-    const int rest = (int)(n - (int64_t)whole * a.page);
-    if (l == whole) a.wants[i] = {!first && rest > 0 ? mine : -1, rest, i, whole};
-    if (l == 0 && whole >= a.P) a.wants[i] = {-1, 0, i, 0};
+    if (l == r.whole && !first && r.rest > 0) rows[i].source = mine;
   }
   __syncthreads();
-  const int need = fork_number<PG_THREADS>(a, s);
-  int base = 0;
-  for (int x0 = 0; x0 < pages; x0 += PG_PAGES) {
-    const int x = x0 + 4 * tid;
-    int c[4] = {1, 1, 1, 1};
+  int need = 0, base = 0;
+  for (int i0 = 0; i0 < a.R; i0 += PG_THREADS) {
+    const int i = i0 + tid;
+    ForkRow r = {-1, 0, 0, -1};
+    if (i < a.R) r = rows[i];
+    int all;
+    const int at = need + wg_before<PG_THREADS>(r.source >= 0, s, &all);
+    if (r.source >= 0) a.copies[at] = {r.source, r.rest, i, r.whole};
+    need += all;
+  }
+#pragma unroll
+  for (int t = 0; t < FORK_ONE_PAGES / PG_PAGES; ++t) {
+    if (t * PG_PAGES >= pages) break;
+    const int x = t * PG_PAGES + 4 * tid;
+    int c[4] = {1, 1, 1, 1}, all;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (x + u < (int)a.n_pages) c[u] = fork_count(a.refs[x + u], gone[x + u], come[x + u]);
-    int all;
+      if (x + u < (int)a.n_pages) c[u] = fork_count(refs[t][u], gone[x + u], come[x + u]);
     const int at = base + wg_before<PG_THREADS>((c[0] == 0) + (c[1] == 0) + (c[2] == 0) + (c[3] == 0), s, &all);
     fork_hand_out(a, x, c, at, need);
     base += all;
@@ -471,9 +499,9 @@ __global__ __launch_bounds__(PG_COPY) void compact_move_kernel(CompactArgs a, Co
   });
 }
 
-// At most `most` pages are copied; 8 workgroups fill a compute unit.  Returns the workgroups.
-static unsigned copy_plan(CopyPlan& p, int64_t most, int64_t layers, int64_t page_bytes) {
-  const int64_t chunks = (page_bytes + PG_UNIT - 1) / PG_UNIT, units = 2 * layers * chunks, room = (int64_t)device_cus() * 8;
+// At most `most` pages are copied, at most `bytes` of each; 8 workgroups fill a compute unit.  Returns the workgroups.
+static unsigned copy_plan(CopyPlan& p, int64_t most, int64_t layers, int64_t bytes) {
+  const int64_t chunks = (bytes + PG_UNIT - 1) / PG_UNIT, units = 2 * layers * chunks, room = (int64_t)device_cus() * 8;
   const int64_t wgs = most < 1 ? 1 : most < room / units + 1 && most * units < room ? most * units : room;
   p.units = (int)units;
   p.chunks = (int)chunks;
@@ -548,7 +576,7 @@ extern "C" int aq_fork_pages(const int64_t* page_table, int64_t B, int64_t P, co
   const dim3 one(aq::PG_THREADS);
   if (n_pages <= aq::FORK_ONE_PAGES && B <= aq::FORK_ONE_ROWS && R <= aq::FORK_ONE_ROWS && (B + R) * P <= aq::FORK_ONE_ENTRIES) {
     a.by_p = aq::UDiv::of((uint32_t)P);
-    aq::queue_kernel(aq::fork_one_kernel, dim3(1), one, (size_t)(2 * ((n_pages + 3) / 4 * 4) + B) * sizeof(int), st, a);
+    aq::queue_kernel(aq::fork_one_kernel, dim3(1), one, aq::fork_one_lds(n_pages, B, R), st, a);
   } else {
     const int64_t quads = (n_pages + 3) / 4 * 2, groups = aq::segments(n_pages);
     a.turns = (int)aq::segment_turns(n_pages);
@@ -561,9 +589,11 @@ extern "C" int aq_fork_pages(const int64_t* page_table, int64_t B, int64_t P, co
     aq::queue_kernel(aq::fork_free_kernel, dim3((unsigned)groups + 1), dim3(aq::PG_COPY), 0, st, a);
     aq::queue_kernel(aq::fork_refs_kernel, dim3((unsigned)groups), dim3(aq::PG_COPY), 0, st, a);
   }
-  if (R > 1) {  // (a single row is its parent's first child)
+  // Written rows of a page that is partly filled: one number for all, or anything where sequences have lengths of their own.
+  const int64_t written = !seq_lens ? total_len % page_size : total_len < page_size ? total_len : page_size - 1;
+  if (R > 1 && written > 0) {  // (a single row is its parent's first child)
     aq::CopyPlan plan;
-    const unsigned wgs = aq::copy_plan(plan, R - 1, layers, a.page_bytes);
+    const unsigned wgs = aq::copy_plan(plan, R - 1, layers, written * row_bytes);
     aq::queue_kernel(aq::fork_copy_kernel, dim3(wgs), dim3(aq::PG_COPY), 0, st, a, plan);
   }
   return (int)hipGetLastError();
