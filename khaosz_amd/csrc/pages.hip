@@ -499,6 +499,69 @@ __global__ __launch_bounds__(PG_COPY) void compact_move_kernel(CompactArgs a, Co
   });
 }
 
+// Both of the above in one launch for small caches: every workgroup numbers all pages by itself, 4 to a thread, and keeps the moves in LDS.
+// us in two launches | one, half the pages held: 128 pages of 64 KB 7.9 | 6.1, 128 of 256 KB 12.1 | 9.4, 512 of them (128 MB of keys) 29.7 | 28.4,
+// but 1000 of them 49.5 | 51.1 and in two layers 105 | 114.  (16 pages to a thread, 4096 pages: 9.1 | 14.4.)
+constexpr int COMPACT_SMALL = 4 * PG_COPY;
+constexpr int64_t COMPACT_SMALL_BYTES = (int64_t)1 << 27;  // of all keys
+__global__ __launch_bounds__(PG_COPY) void compact_small_kernel(CompactArgs a, CopyPlan plan) {
+  __shared__ int s[PG_COPY / 64], moves_s, source[COMPACT_SMALL / 2], hole[COMPACT_SMALL / 2];
+  const int x = (int)threadIdx.x * 4, n_pages = (int)a.n_pages;
+  int r[4] = {0, 0, 0, 0}, live;
+  if (x < n_pages) compact_refs(a, x, r);
+  if (threadIdx.x == 0) moves_s = 0;
+  const int at0 = wg_before<PG_COPY>((r[0] > 0) + (r[1] > 0) + (r[2] > 0) + (r[3] > 0), s, &live);
+  int at = at0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int y = x + u;
+    const bool held = r[u] > 0;
+    if (held && y >= live) source[live - 1 - at] = y;
+    if (!held && y < live) hole[y - at] = y;
+    at += held;
+    if (y == live - 1) moves_s = live - at;  // free pages among the first live
+  }
+  __syncthreads();
+  const int moves = moves_s;
+  if ((int)blockIdx.x < a.copy_wgs) {
+    each_unit(plan, copy_first(plan), moves, [&](int c, int64_t layer, int values, int64_t at) {
+      const int64_t left = a.page_bytes - at;
+      uint8_t* const base = (values ? a.v : a.k) + layer * a.layer_bytes + at;
+      const int from = __builtin_amdgcn_readfirstlane(source[c]), to = __builtin_amdgcn_readfirstlane(hole[c]);
+      copy_unit(base + from * a.page_bytes, base + to * a.page_bytes, (int)(left < PG_UNIT ? left : PG_UNIT));
+    });
+    return;
+  }
+  const int64_t stride = (int64_t)(gridDim.x - a.copy_wgs) * PG_COPY, me = (int64_t)((int)blockIdx.x - a.copy_wgs) * PG_COPY + threadIdx.x;
+  for (int64_t i = me; i < a.entries; i += stride) {
+    const int64_t e = a.table[i];
+    int64_t to = -1;
+    if (e >= 0 && e < n_pages && a.refs[e] > 0) {
+      to = e;
+      if (e >= live) {  // source[] falls
+        int lo = 0;
+        for (int step = COMPACT_SMALL / 4; step; step >>= 1)
+          if (lo + step < moves && source[lo + step] >= (int)e) lo += step;
+        to = hole[lo];
+      }
+    }
+    a.new_table[i] = to;
+  }
+  if ((int)blockIdx.x != a.copy_wgs) return;
+  at = at0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int y = x + u;
+    const bool held = r[u] > 0;
+    if (y < n_pages) {
+      a.where[y] = !held ? -1 : y < live ? y : hole[live - 1 - at];
+      a.new_refs[y] = y >= live ? 0 : held ? r[u] : a.refs[source[y - at]];
+    }
+    at += held;
+  }
+  if (threadIdx.x == 0) a.live[0] = live;
+}
+
 // At most `most` pages are copied, at most `bytes` of each; 8 workgroups fill a compute unit.  Returns the workgroups.
 static unsigned copy_plan(CopyPlan& p, int64_t most, int64_t layers, int64_t bytes) {
   const int64_t chunks = (bytes + PG_UNIT - 1) / PG_UNIT, units = 2 * layers * chunks, room = (int64_t)device_cus() * 8;
@@ -635,16 +698,21 @@ extern "C" int aq_compact_pages(const int64_t* page_table, int64_t entries, cons
   a.entries = entries;
   a.layers = (int)layers;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (n_pages <= aq::COMPACT_COUNT) {
-    aq::queue_kernel(aq::compact_rank_kernel<aq::PG_THREADS, true>, dim3((unsigned)((n_pages + aq::PG_PAGES - 1) / aq::PG_PAGES)), dim3(aq::PG_THREADS), 0, st, a);
-  } else {
-    const dim3 groups((unsigned)aq::segments(n_pages)), threads(aq::PG_COPY);
-    aq::queue_kernel(aq::compact_count_kernel, groups, threads, 0, st, a);
-    aq::queue_kernel(aq::compact_rank_kernel<aq::PG_COPY, false>, groups, threads, 0, st, a);
-  }
   aq::CopyPlan plan;
   a.copy_wgs = (int)aq::copy_plan(plan, n_pages / 2, layers, a.page_bytes);
   const int64_t work = entries > n_pages / 2 ? entries : n_pages / 2, rest = (work + aq::PG_COPY - 1) / aq::PG_COPY;
-  aq::queue_kernel(aq::compact_move_kernel, dim3((unsigned)(a.copy_wgs + (rest < 1 ? 1 : rest < 256 ? rest : 256))), dim3(aq::PG_COPY), 0, st, a, plan);
+  const dim3 wgs((unsigned)(a.copy_wgs + (rest < 1 ? 1 : rest < 256 ? rest : 256))), threads(aq::PG_COPY);
+  if (n_pages <= aq::COMPACT_SMALL && layers * n_pages * a.page_bytes <= aq::COMPACT_SMALL_BYTES) {
+    aq::queue_kernel(aq::compact_small_kernel, wgs, threads, 0, st, a, plan);
+    return (int)hipGetLastError();
+  }
+  if (n_pages <= aq::COMPACT_COUNT) {
+    aq::queue_kernel(aq::compact_rank_kernel<aq::PG_THREADS, true>, dim3((unsigned)((n_pages + aq::PG_PAGES - 1) / aq::PG_PAGES)), dim3(aq::PG_THREADS), 0, st, a);
+  } else {
+    const dim3 groups((unsigned)aq::segments(n_pages));
+    aq::queue_kernel(aq::compact_count_kernel, groups, threads, 0, st, a);
+    aq::queue_kernel(aq::compact_rank_kernel<aq::PG_COPY, false>, groups, threads, 0, st, a);
+  }
+  aq::queue_kernel(aq::compact_move_kernel, wgs, threads, 0, st, a, plan);
   return (int)hipGetLastError();
 }

@@ -171,7 +171,7 @@ def test_fork_and_compact_one_layer_of_any_type(dtype):
     _equal(got, want, kd.unsqueeze(0), vd.unsqueeze(0))
 
 
-@pytest.mark.parametrize("n_pages,live", [(1, 0), (1, 1), (8, 3), (100, 0), (100, 100), (4096, 2000), (4097, 4096), (5000, 1), (16384, 9000), (16385, 16000), (20000, 11111), (70001, 35000), (1100003, 600001)])
+@pytest.mark.parametrize("n_pages,live", [(1, 0), (1, 1), (8, 3), (100, 0), (100, 100), (1000, 1), (1023, 500), (1024, 512), (1025, 1024), (4095, 2047), (4096, 4096), (4096, 2000), (4097, 4096), (5000, 1), (16384, 9000), (16385, 16000), (20000, 11111), (70001, 35000), (1100003, 600001)])
 def test_compact(n_pages, live):
     _say("compact", n_pages, live)
     g = torch.Generator().manual_seed(n_pages + live)
