@@ -384,6 +384,100 @@ __global__ __launch_bounds__(PG_COPY) void fork_copy_kernel(ForkArgs a, CopyPlan
   });
 }
 
+// Numbering and copies in one launch for small tables and caches: every workgroup numbers the rows by itself, a thread to a row and to four
+// pages, and the last one writes table and counts.  (us in two launches | one: 1 row into 8 over 64 pages, a layer 7.5 | 4.8, 24 layers 9.4 | 7.2; 16 rows
+// into 16 of 13 columns 7.9 | 5.7; 64 into 64 of 8 8.0 | 6.1; but 200 into 250 of 4 8.2 | 9.2.)
+constexpr int FORK_SMALL_PAGES = 4 * PG_COPY, FORK_SMALL_ROWS = PG_COPY, FORK_SMALL_ENTRIES = 1024;
+constexpr int64_t FORK_SMALL_BYTES = (int64_t)1 << 27;  // copied at most
+__global__ __launch_bounds__(PG_COPY) void fork_small_kernel(ForkArgs a, CopyPlan plan, int copy_wgs) {
+  __shared__ int s[PG_COPY / 64], gone[FORK_SMALL_PAGES], come[FORK_SMALL_PAGES], first_of[FORK_SMALL_ROWS], slot[FORK_SMALL_ROWS], order[FORK_SMALL_ROWS],
+      fresh[FORK_SMALL_ROWS];
+  __shared__ ForkRow rows[FORK_SMALL_ROWS];
+  const int tid = threadIdx.x, x0 = 4 * tid;
+  const int64_t parent = tid < a.R ? a.parents[tid] : -1;
+  int c[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    c[u] = x0 + u < (int)a.n_pages ? a.refs[x0 + u] : 1;
+    gone[x0 + u] = come[x0 + u] = 0;
+  }
+  first_of[tid] = a.R;
+  __syncthreads();
+  ForkRow mine = {-1, 0, 0, -1};
+  if (parent >= 0 && parent < a.B) {
+    const int64_t n = fork_length(a, (int)parent);
+    mine.parent = (int)parent;
+    mine.whole = (int)(n / a.page);
+    mine.rest = (int)(n - (int64_t)mine.whole * a.page);
+    atomicMin(first_of + parent, tid);
+  }
+  rows[tid] = mine;
+#pragma unroll 4
+  for (int x = tid; x < a.B * a.P; x += PG_COPY) {
+    const int64_t e = a.table[x];
+    if (e >= 0 && e < a.n_pages) atomicAdd(gone + e, 1);
+  }
+  __syncthreads();
+  // entry x of the new table, but that of a copy
+  auto entry = [&](int x, int* row, int* copied) __attribute__((always_inline)) {
+    const int i = a.by_p((uint32_t)x), l = x - i * a.P;
+    const ForkRow r = rows[i];
+    const int e = r.parent >= 0 ? fork_entry(a, r.parent, l) : -1;
+    const bool first = r.parent >= 0 && first_of[r.parent] == i;
+    *row = i;
+    *copied = l == r.whole && !first && r.rest > 0 ? e : -1;
+    return first || l < r.whole ? e : -1;
+  };
+#pragma unroll 4
+  for (int x = tid; x < a.R * a.P; x += PG_COPY) {
+    int i, copied;
+    const int e = entry(x, &i, &copied);
+    if (e >= 0) atomicAdd(come + e, 1);
+    if (copied >= 0) rows[i].source = copied;
+  }
+  __syncthreads();
+  int need, base;
+  const bool wants = tid < a.R && rows[tid].source >= 0;
+  const int mine_at = wg_before<PG_COPY>(wants, s, &need);
+  slot[tid] = mine_at;
+  if (wants) order[mine_at] = tid;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) c[u] = x0 + u < (int)a.n_pages ? fork_count(c[u], gone[x0 + u], come[x0 + u]) : 1;
+  int at = wg_before<PG_COPY>((c[0] == 0) + (c[1] == 0) + (c[2] == 0) + (c[3] == 0), s, &base);
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (c[u] == 0) {
+      if (at < need) {
+        fresh[at] = x0 + u;
+        c[u] = 1;
+      }
+      ++at;
+    }
+  __syncthreads();
+  const int got = need < base ? need : base;
+  if ((int)blockIdx.x < copy_wgs) {
+    each_unit(plan, copy_first(plan), got, [&](int k, int64_t layer, int values, int64_t from) {
+      const int i = order[k];
+      const int rest = __builtin_amdgcn_readfirstlane(rows[i].rest), source = __builtin_amdgcn_readfirstlane(rows[i].source);
+      const int to = __builtin_amdgcn_readfirstlane(fresh[k]);
+      const int64_t bytes = rest * a.row_bytes - from;
+      if (bytes <= 0) return;
+      uint8_t* const base = (values ? a.v : a.k) + layer * a.layer_bytes + from;
+      copy_unit(base + source * a.page_bytes, base + to * a.page_bytes, (int)(bytes < PG_UNIT ? bytes : PG_UNIT));
+    });
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (x0 + u < (int)a.n_pages) a.new_refs[x0 + u] = c[u];
+  for (int x = tid; x < a.R * a.P; x += PG_COPY) {
+    int i, copied;
+    const int e = entry(x, &i, &copied);
+    a.new_table[x] = copied < 0 ? e : slot[i] < got ? fresh[slot[i]] : -1;
+  }
+  if (tid == 0) a.missing[0] = need - got;
+}
+
 struct CompactArgs {
   const int64_t* table;  // entries in all
   const int32_t* refs;
@@ -636,29 +730,33 @@ extern "C" int aq_fork_pages(const int64_t* page_table, int64_t B, int64_t P, co
   a.P = (int)P;
   a.layers = (int)layers;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 one(aq::PG_THREADS);
+  const dim3 one(aq::PG_THREADS), threads(aq::PG_COPY);
+  // Written rows of a page that is partly filled: one number for all, or anything where sequences have lengths of their own.
+  const int64_t written = !seq_lens ? total_len % page_size : total_len < page_size ? total_len : page_size - 1;
+  aq::CopyPlan plan{};
+  unsigned copy_wgs = 0;  // (a single row is its parent's first child)
+  if (R > 1 && written > 0) copy_wgs = aq::copy_plan(plan, R - 1, layers, written * row_bytes);
+  if (P <= aq::FORK_ONE_ENTRIES) a.by_p = aq::UDiv::of((uint32_t)P);
+  if (n_pages <= aq::FORK_SMALL_PAGES && B <= aq::FORK_SMALL_ROWS && R <= aq::FORK_SMALL_ROWS && (B + R) * P <= aq::FORK_SMALL_ENTRIES &&
+      2 * layers * R * written * row_bytes <= aq::FORK_SMALL_BYTES) {
+    aq::queue_kernel(aq::fork_small_kernel, dim3(copy_wgs + 1), threads, 0, st, a, plan, (int)copy_wgs);
+    return (int)hipGetLastError();
+  }
   if (n_pages <= aq::FORK_ONE_PAGES && B <= aq::FORK_ONE_ROWS && R <= aq::FORK_ONE_ROWS && (B + R) * P <= aq::FORK_ONE_ENTRIES) {
-    a.by_p = aq::UDiv::of((uint32_t)P);
     aq::queue_kernel(aq::fork_one_kernel, dim3(1), one, aq::fork_one_lds(n_pages, B, R), st, a);
   } else {
     const int64_t quads = (n_pages + 3) / 4 * 2, groups = aq::segments(n_pages);
     a.turns = (int)aq::segment_turns(n_pages);
-    aq::queue_kernel(aq::fork_clear_kernel, dim3((unsigned)((quads + aq::PG_THREADS - 1) / aq::PG_THREADS)), one, 0, st,
-                     reinterpret_cast<v4i*>(a.gone), quads);
     const int64_t chunks = (P + aq::PG_COPY - 1) / aq::PG_COPY, new_wgs = (R + aq::FORK_ROWS - 1) / aq::FORK_ROWS * chunks;
     const int64_t wgs = new_wgs + (B + aq::FORK_ROWS - 1) / aq::FORK_ROWS * chunks;
     if (wgs > 0x7fffffff) return AQ_E_RANGE;
-    if (wgs > 0) aq::queue_kernel(aq::fork_rows_kernel, dim3((unsigned)wgs), dim3(aq::PG_COPY), 0, st, a, (int)new_wgs, (int)chunks);
-    aq::queue_kernel(aq::fork_free_kernel, dim3((unsigned)groups + 1), dim3(aq::PG_COPY), 0, st, a);
-    aq::queue_kernel(aq::fork_refs_kernel, dim3((unsigned)groups), dim3(aq::PG_COPY), 0, st, a);
+    aq::queue_kernel(aq::fork_clear_kernel, dim3((unsigned)((quads + aq::PG_THREADS - 1) / aq::PG_THREADS)), one, 0, st,
+                     reinterpret_cast<v4i*>(a.gone), quads);
+    if (wgs > 0) aq::queue_kernel(aq::fork_rows_kernel, dim3((unsigned)wgs), threads, 0, st, a, (int)new_wgs, (int)chunks);
+    aq::queue_kernel(aq::fork_free_kernel, dim3((unsigned)groups + 1), threads, 0, st, a);
+    aq::queue_kernel(aq::fork_refs_kernel, dim3((unsigned)groups), threads, 0, st, a);
   }
-  // Written rows of a page that is partly filled: one number for all, or anything where sequences have lengths of their own.
-  const int64_t written = !seq_lens ? total_len % page_size : total_len < page_size ? total_len : page_size - 1;
-  if (R > 1 && written > 0) {  // (a single row is its parent's first child)
-    aq::CopyPlan plan;
-    const unsigned wgs = aq::copy_plan(plan, R - 1, layers, written * row_bytes);
-    aq::queue_kernel(aq::fork_copy_kernel, dim3(wgs), dim3(aq::PG_COPY), 0, st, a, plan);
-  }
+  if (copy_wgs) aq::queue_kernel(aq::fork_copy_kernel, dim3(copy_wgs), threads, 0, st, a, plan);
   return (int)hipGetLastError();
 }
 

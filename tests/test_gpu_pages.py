@@ -116,7 +116,8 @@ def test_fork_small(page, total, parents):
                                                            (70, 90, 200, 4, 14500, 1, 5), (4, 9, 3, 16, 8193, 1, 6), (300, 5000, 2, 4, 5700, 1, 7),
                                                            (5, 7, 4, 16, 8190, 1, 8), (64, 2100, 3, 4, 4097, 2, 9),
                                                            (300, 700, 3600, 2, 1100003, 1, 10), (4000, 4090, 4, 4, 8190, 1, 11),
-                                                           (4096, 4095, 4, 4, 4110, 1, 12)])
+                                                           (4096, 4095, 4, 4, 4110, 1, 12), (256, 256, 2, 4, 1024, 2, 13),
+                                                           (100, 1, 8, 16, 1021, 1, 14), (3, 253, 4, 16, 1024, 3, 15), (256, 256, 2, 4, 1025, 1, 16)])
 def test_fork_rows_at_lengths_of_their_own(B, R, P, page, n_pages, layers, seed):
     _say("fork lens", B, R, P, page, n_pages)
     table, refs, k, v = _state(B, P, n_pages, page, layers=layers, seed=seed, common=min(3, P - 1), heads=1)
