@@ -332,10 +332,18 @@ struct SharedPages {
     for (int i = threadIdx.x; i < p.table_lds; i += threads) lds[i] = phys(p, lp0 + i);
   }
 
+  // The page of the block at kb0, where a block lies in one page; requested a block ahead, so that no load waits for it.
+  template <int KB>
+  __device__ __forceinline__ int64_t page_of(const SharedArgs& p, int kb0) const {
+    if (p.page_shift < (KB == 64 ? 6 : 5)) return -1;
+    const int lp = __builtin_amdgcn_readfirstlane(kb0 >> p.page_shift);
+    return kb0 < p.T && lp < p.P ? table[lp] : -1;
+  }
+
   // N loads of 1 KiB: rows r0, r0 + rows of a load, .. of the block of KB positions at kb0, into LDS from `dst` on, those of keys and (BOTH) of
   // values `apart` bytes further.  Rows from `seen` on, which no one looks at, are zeros whatever is stored there; so are unmapped pages.
   template <int D, int KB, int N, bool KEYS, bool VALUES>
-  __device__ __forceinline__ void load(const SharedArgs& p, int kvh, int kb0, int seen, int r0, uint32_t dst, uint32_t apart) const {
+  __device__ __forceinline__ void load(const SharedArgs& p, int kvh, int kb0, int64_t id, int seen, int r0, uint32_t dst, uint32_t apart) const {
     constexpr int ROWB = 2 * D, RPI = 1024 / ROWB, LPR = 64 / RPI;
     const int lane = threadIdx.x & 63;
     const int rows = seen - kb0;
@@ -346,7 +354,6 @@ struct SharedPages {
     constexpr int SHIFT = KB == 64 ? 6 : 5;
     if (p.page_shift >= SHIFT) {  // the whole block lies in one page
       const int lp = __builtin_amdgcn_readfirstlane(kb0 >> p.page_shift);
-      const int64_t id = rows > 0 && lp < p.P ? table[lp] : -1;
       const bool mapped = id >= 0 && id < p.n_pages;
       const int64_t first = mapped ? (((id << p.page_shift) + (kb0 - (lp << p.page_shift))) * p.Hkv + kvh) * D : 0;
       const int step = p.Hkv * D;
@@ -428,9 +435,12 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
     __syncthreads();
   }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(pa_lds_void*)lds;
+  int64_t page = pages.template page_of<KB>(p, k0 + kw * KB);
   auto issue = [&](int it, int buf) __attribute__((always_inline)) {
     const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + buf * BUF + kw * 2 * TILE + qw * LOADS * 1024);
-    pages.template load<D, KB, LOADS, true, true>(p, kvh, k0 + (it * KW + kw) * KB, seen, qw * LOADS * RPI, dst, TILE);
+    const int kb0 = k0 + (it * KW + kw) * KB;
+    pages.template load<D, KB, LOADS, true, true>(p, kvh, kb0, page, seen, qw * LOADS * RPI, dst, TILE);
+    page = pages.template page_of<KB>(p, kb0 + KW * KB);
   };
   issue(0, 0);
   SharedRows<D> rows;
@@ -474,6 +484,7 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
 #pragma unroll
     for (int i = 0; i < QW * KW; ++i) any |= odd_s[i];
     if (__builtin_amdgcn_readfirstlane(any)) {  // workgroup-uniform
+      page = pages.template page_of<KB>(p, k0 + kw * KB);
       issue(0, 0);
       rows.clear();
       blocks(std::true_type{});
@@ -508,8 +519,10 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& p, uint8_t* lds, f
   SharedRows<D> rows;
   rows.start(p.q + ((int64_t)b * p.Hq + kvh * p.G + (col < p.G ? col : 0)) * D, lane >> 5, vis);
   if (kb0 < seen) {  // wavefront-uniform, as all below
-    pages.template load<D, KB, LOADS, true, false>(p, kvh, kb0, seen, 0, at, 0);
-    pages.template load<D, KB, LOADS, false, true>(p, kvh, kb0, seen, 0, at + TILE, 0);
+    int64_t page = pages.template page_of<KB>(p, kb0);
+    pages.template load<D, KB, LOADS, true, false>(p, kvh, kb0, page, seen, 0, at, 0);
+    pages.template load<D, KB, LOADS, false, true>(p, kvh, kb0, page, seen, 0, at + TILE, 0);
+    page = pages.template page_of<KB>(p, kb0 + KW * KB);
     // The queries have arrived, as far as the compiler knows too: otherwise it waits for them in every turn, by a count that takes in
     // the blocks on their way.
     SH_WAIT_VMCNT(0);
@@ -521,7 +534,7 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& p, uint8_t* lds, f
           ks, ks + TILE, kb0, kb0 + KB > vis, p.T, p.scale_log2e,
           [&] {
             SH_WAIT_LGKM();
-            if (more) pages.template load<D, KB, LOADS, true, false>(p, kvh, next, seen, 0, at, 0);
+            if (more) pages.template load<D, KB, LOADS, true, false>(p, kvh, next, page, seen, 0, at, 0);
           },
           [&] {
             if (more) SH_WAIT_VMCNT(LOADS);  // this block's values have landed
@@ -530,7 +543,8 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& p, uint8_t* lds, f
           });
       if (!more) break;
       SH_WAIT_LGKM();
-      pages.template load<D, KB, LOADS, false, true>(p, kvh, next, seen, 0, at + TILE, 0);
+      pages.template load<D, KB, LOADS, false, true>(p, kvh, next, page, seen, 0, at + TILE, 0);
+      page = pages.template page_of<KB>(p, next + KW * KB);
       SH_WAIT_VMCNT(LOADS);  // the next block's keys have
       kb0 = next;
     }
