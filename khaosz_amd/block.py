@@ -106,7 +106,7 @@ class PagedKV:
         self._safe = None        # device table with -1 replaced by 0
         self._invalid = None     # device bool [B, P * page_size] or None when everything is mapped
         self._host = None        # host copy of the table
-        self._common = None      # leading columns that are the same in all of its rows, once asked for
+        self._common = None      # leading columns with one page in all of its rows, once asked for
         self.total_len = 0
         self.shared_len = 0      # leading positions that a single-token step reads once for all sequences
         self.seq_lens: Optional[Tensor] = None
@@ -130,7 +130,7 @@ class PagedKV:
         self.shared_len = 0
         if share_prefix and self._host.shape[0] > 1:
             if self._common is None:
-                self._common = int((self._host == self._host[:1]).all(0).long().cumprod(0).sum())
+                self._common = int(((self._host == self._host[:1]).all(0) & (self._host[0] >= 0)).long().cumprod(0).sum())
             self.shared_len = max(0, min(self._common * self.page_size, total_len - 1))  # the new token's page is its own
         return self
 

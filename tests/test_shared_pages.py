@@ -110,7 +110,11 @@ def test_a_cache_finds_what_its_rows_share():
     table[1, 0] = 4
     assert cache.bind(table, 60, share_prefix=True, refresh=True).shared_len == 0
     assert cache.bind(table[:1], 60, share_prefix=True).shared_len == 0  # one sequence
-    assert cache.bind(torch.full((2, 3), -1), 40, share_prefix=True).shared_len == 39  # unmapped alike
+    assert cache.bind(torch.full((2, 3), -1), 40, share_prefix=True).shared_len == 0
+    table = torch.tensor([[5, -1, -1], [5, -1, -1]])  # pages that are still to come are not shared
+    assert cache.bind(table, 40, share_prefix=True).shared_len == 16
+    table[0, 1], table[1, 1] = 7, 8
+    assert cache.bind(table, 40, share_prefix=True).shared_len == 16
 
 
 def _model(**options):
