@@ -15,6 +15,13 @@
 // Prefix and tail are workgroups of one launch, the prefix's first: those multiply while the tails read.  Both compute S^T = K Q^T and
 // O^T = V^T P^T as the prefill kernel does (attn_prefill.hip has the layout): a lane has the scores of one row, nothing changes lanes,
 // K and V rows go straight into LDS ahead of the products.
+//
+// us a call; what its bytes take at the 5.2 TB/s of a large copy; the decode kernel, which reads the prefix for every sequence; what bounds the call:
+//   8 x 2591 positions of which 2048 shared, 16/4 heads of 128     9.6   2.5   13.8  the latency of two launches
+//   33 x 1401 of 1008, own lengths, 24/4 of 64, pages of 16        10.3  1.5   12.9  the same, and a lookup of the page per row
+//   64 x 8448 of 8192, 32/8 of 128                                 33.4  19.6   208  a wavefront's chain in the prefix beside the tails' loads
+//   16 x 65600 of 65536, 16/4 of 128                               37.4  26.3   333  HBM: 6.5 TB/s inside the loop, 2.3 us before it; the merge 4.7
+//   256 x 4500 of 4096, own lengths, 16/4 of 128                   43.9  22.5   221  tails of 200 positions, mostly beginning and end; the merge 5.3
 #include "aq_attn.h"
 #include "aq_common.h"
 #include "aq_rows.h"
@@ -393,6 +400,8 @@ __device__ __forceinline__ int visible(const SharedArgs& p, int b) {
 // A tile of 32 QW rows of all sequences against a slice of the shared positions.  QW x KW wavefronts: QW tiles of 32 rows side by side on
 // the same block of KB positions, KW blocks at a time, the next KW ahead of the products.  (More buffers gain nothing: 64 x 8192 positions
 // of 32/8 heads of 128 20.0 us with two, 22.2 with four that leave room for one workgroup per compute unit.)
+// Few rows: bound by HBM (16 x 65536 positions, 16/4 heads of 128: 20.6 us for 134 MB in the loop).  Many: 64 x 8192 positions take 12.0 us in the
+// loop, 6.9 without the products, 10 without the loads; the matrix core is busy for 3.9, and the store of the partial results adds 1.4.
 template <int D, int QW, int KW, int KB, bool LENS>
 __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds, float* ml, int* table_lds) {
   constexpr int ROWB = 2 * D, RPI = 1024 / ROWB;    // bytes of a K or V row; rows of a 1 KiB load
@@ -500,7 +509,8 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
   }
 }
 
-// The G rows of one sequence against a slice of its own positions.  KW wavefronts, each by itself: blocks of 32 positions in turn, the
+// The G rows of one sequence against a slice of its own positions.  Bound by HBM and by what a workgroup waits for before its first and after
+// its last block (64 sequences of 256 positions, 32/8 heads of 128: 67 MB in 15.5 us; 256 of 404, 16/4: 212 MB in 46).  KW wavefronts, each by itself: blocks of 32 positions in turn, the
 // next block's keys requested when the last key has been read, its values when the last value has.
 template <int D, int KW>
 __device__ __forceinline__ void shared_tail(const SharedArgs& p, uint8_t* lds, float* ml, int* table_lds) {
@@ -567,7 +577,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
 }
 
 // The slices of a row added up: a half wavefront has 4 dimensions of the 32 rows of a tile, so that the prefix's slices are read by whole
-// lines, and every PARTS-th slice, four of them requested before any is used; the parts meet in LDS.
+// lines, and every PARTS-th slice, four of them requested before any is used; the parts meet in LDS.  (64 x 8448 positions: 17 MB in 5.4 us; 16 parts
+// 36.6 us for the call instead of 33.8, eight slices requested at once 35.4; 8 x 2591 with four parts 10.0 instead of 9.6.)
 template <int D, int PARTS>
 __global__ __launch_bounds__(PARTS * 32) void shared_merge_kernel(const float* ws, uint16_t* out, int slices, int tails, int tiles32, int rows, int Hkv, int G) {
   constexpr int GRP = 4;
