@@ -19,6 +19,12 @@ __device__ __forceinline__ void load_row_lds(const uint16_t* src, uint32_t at) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(at) : "memory");  // m0 needs a wait state
 }
 
+// The same, the address a wavefront-uniform base and an offset in bytes.  A memory instruction that reads a scalar register which a vector
+// instruction (v_readfirstlane, or v_readlane of a spilled register) has written needs 5 wait states; the compiler cannot see that this is one.
+__device__ __forceinline__ void load_row_lds(const uint16_t* base, uint32_t offset, uint32_t at) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "{m0}"(at) : "memory");
+}
+
 // The 16-byte piece of row r that sits in slot s of the row is s ^ row_key(r): the low bits of r, reversed.  16 rows
 // reading the same piece (K) fall on all slots of the bank lines; the 8 neighbouring rows x 64 bytes of a transposing
 // read (V) are told apart by their lowest bits, which reversed move a row's pieces by 64 bytes and more.

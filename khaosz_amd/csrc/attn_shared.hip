@@ -319,6 +319,12 @@ struct SharedRows {
   }
 };
 
+__device__ __forceinline__ const uint16_t* uniform(const uint16_t* p) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<const uint16_t*>((uint64_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32 |
+                                           (uint32_t)__builtin_amdgcn_readfirstlane((int)a));
+}
+
 // The page table of one sequence.
 struct SharedPages {
   const int64_t* table;
@@ -339,12 +345,16 @@ struct SharedPages {
     for (int i = threadIdx.x; i < p.table_lds; i += threads) lds[i] = phys(p, lp0 + i);
   }
 
-  // The page of the block at kb0, where a block lies in one page; requested a block ahead, so that no load waits for it.
-  template <int KB>
-  __device__ __forceinline__ int64_t page_of(const SharedArgs& p, int kb0) const {
+  // The page of the block at kb0 (before `end`), where a block lies in one page; requested a block ahead, so that no load waits for it.
+  // SCALAR: a vector load would count among the rows on their way.
+  template <int KB, bool SCALAR = true>
+  __device__ __forceinline__ int64_t page_of(const SharedArgs& p, int kb0, int end) const {
     if (p.page_shift < (KB == 64 ? 6 : 5)) return -1;
     const int lp = __builtin_amdgcn_readfirstlane(kb0 >> p.page_shift);
-    return kb0 < p.T && lp < p.P ? table[lp] : -1;
+    typedef const __attribute__((address_space(4))) int64_t* constant;
+    if (kb0 >= end || lp >= p.P) return -1;
+    if constexpr (SCALAR) return ((constant)(uintptr_t)table)[lp];
+    else return table[lp];
   }
 
   // N loads of 1 KiB: rows r0, r0 + rows of a load, .. of the block of KB positions at kb0, into LDS from `dst` on, those of keys and (BOTH) of
@@ -364,6 +374,16 @@ struct SharedPages {
       const bool mapped = id >= 0 && id < p.n_pages;
       const int64_t first = mapped ? (((id << p.page_shift) + (kb0 - (lp << p.page_shift))) * p.Hkv + kvh) * D : 0;
       const int step = p.Hkv * D;
+      if (mapped && rows >= KB) {  // (wavefront-uniform) the whole block is there: only the base changes from block to block
+        const uint16_t *const kc = uniform(p.kc + first), *const vc = uniform(p.vc + first);
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const uint32_t at = 2 * (uint32_t)((r0 + c * RPI + lane / LPR) * step + pc[c]);
+          if (KEYS) load_row_lds(kc, at, dst + c * 1024);
+          if (VALUES) load_row_lds(vc, at, dst + (KEYS ? apart : 0) + c * 1024);
+        }
+        return;
+      }
 #pragma unroll
       for (int c = 0; c < N; ++c) {
         const int r = r0 + c * RPI + lane / LPR;
@@ -444,12 +464,12 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
     __syncthreads();
   }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(pa_lds_void*)lds;
-  int64_t page = pages.template page_of<KB>(p, k0 + kw * KB);
+  int64_t page = pages.template page_of<KB>(p, k0 + kw * KB, seen);
   auto issue = [&](int it, int buf) __attribute__((always_inline)) {
     const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + buf * BUF + kw * 2 * TILE + qw * LOADS * 1024);
     const int kb0 = k0 + (it * KW + kw) * KB;
     pages.template load<D, KB, LOADS, true, true>(p, kvh, kb0, page, seen, qw * LOADS * RPI, dst, TILE);
-    page = pages.template page_of<KB>(p, kb0 + KW * KB);
+    page = pages.template page_of<KB>(p, kb0 + KW * KB, seen);
   };
   issue(0, 0);
   SharedRows<D> rows;
@@ -493,7 +513,7 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
 #pragma unroll
     for (int i = 0; i < QW * KW; ++i) any |= odd_s[i];
     if (__builtin_amdgcn_readfirstlane(any)) {  // workgroup-uniform
-      page = pages.template page_of<KB>(p, k0 + kw * KB);
+      page = pages.template page_of<KB>(p, k0 + kw * KB, seen);
       issue(0, 0);
       rows.clear();
       blocks(std::true_type{});
@@ -512,7 +532,7 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
 // The G rows of one sequence against a slice of its own positions.  Bound by HBM and by what a workgroup waits for before its first and after
 // its last block (64 sequences of 256 positions, 32/8 heads of 128: 67 MB in 15.5 us; 256 of 404, 16/4: 212 MB in 46).  KW wavefronts, each by itself: blocks of 32 positions in turn, the
 // next block's keys requested when the last key has been read, its values when the last value has.
-template <int D, int KW>
+template <int D, int KW, bool LENS>
 __device__ __forceinline__ void shared_tail(const SharedArgs& p, uint8_t* lds, float* ml, int* table_lds) {
   constexpr int KB = 32, TILE = KB * 2 * D, LOADS = TILE / 1024;
   static_assert(128 * D <= 2 * TILE, "the wavefronts' sums fit the buffers");
@@ -529,10 +549,11 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& p, uint8_t* lds, f
   SharedRows<D> rows;
   rows.start(p.q + ((int64_t)b * p.Hq + kvh * p.G + (col < p.G ? col : 0)) * D, lane >> 5, vis);
   if (kb0 < seen) {  // wavefront-uniform, as all below
-    int64_t page = pages.template page_of<KB>(p, kb0);
+    // (us with a vector and a scalar load here: 8 x 2591 positions of which 2048 shared 9.7 | 10.0, 256 x 4500 of 4096 with lengths 40.6 | 38.8)
+    int64_t page = pages.template page_of<KB, LENS>(p, kb0, seen);
     pages.template load<D, KB, LOADS, true, false>(p, kvh, kb0, page, seen, 0, at, 0);
     pages.template load<D, KB, LOADS, false, true>(p, kvh, kb0, page, seen, 0, at + TILE, 0);
-    page = pages.template page_of<KB>(p, kb0 + KW * KB);
+    page = pages.template page_of<KB>(p, kb0 + KW * KB, seen);
     // The queries have arrived, as far as the compiler knows too: otherwise it waits for them in every turn, by a count that takes in
     // the blocks on their way.
     SH_WAIT_VMCNT(0);
@@ -554,7 +575,7 @@ __device__ __forceinline__ void shared_tail(const SharedArgs& p, uint8_t* lds, f
       if (!more) break;
       SH_WAIT_LGKM();
       pages.template load<D, KB, LOADS, false, true>(p, kvh, next, page, seen, 0, at + TILE, 0);
-      page = pages.template page_of<KB>(p, next + KW * KB);
+      page = pages.template page_of<KB>(p, next + KW * KB, seen);
       SH_WAIT_VMCNT(LOADS);  // the next block's keys have
       kb0 = next;
     }
@@ -573,7 +594,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
   extern __shared__ __align__(1024) uint8_t sh_lds[];  // blocks; page table
   int* const table = reinterpret_cast<int*>(sh_lds + SHARED_LDS * D);
   if ((int)blockIdx.x < p.prefix_wgs) shared_prefix<D, QW, KW, KB, LENS>(p, sh_lds, ml, table);
-  else shared_tail<D, 4>(p, sh_lds, ml, table);
+  else shared_tail<D, 4, LENS>(p, sh_lds, ml, table);
 }
 
 // The slices of a row added up: a half wavefront has 4 dimensions of the 32 rows of a tile, so that the prefix's slices are read by whole
