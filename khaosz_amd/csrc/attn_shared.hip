@@ -44,6 +44,7 @@ struct SharedArgs {
   int tail, tails;                  // positions of a tail's slice, slices of a sequence
   int prefix_wgs;                   // the workgroups behind them are tails
   int page_shift;                   // log2 of the page size, or -1
+  int page_rows;                    // pages hold whole loads of 1 KiB of one head's rows: 512 / D of them
   int table_lds;                    // entries of the page table that a workgroup may need, kept in LDS (0: read from memory)
   UDiv by_g, by_page, by_tiles, by_hkv, by_tails;
 };
@@ -393,6 +394,29 @@ struct SharedPages {
         if (VALUES) load_row_lds(there ? p.vc + first + at : zero + pc[c], dst + (KEYS ? apart : 0) + c * 1024);
       }
       return;
+    }
+    if (p.page_rows && lds && rows >= KB) {  // the rows of a load lie in one page: a lookup and a base per load
+      int id[N];
+      bool mapped = true;
+#pragma unroll
+      for (int c = 0; c < N; ++c) id[c] = lds[p.by_page((uint32_t)(kb0 + r0 + c * RPI)) - lp0];
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        id[c] = __builtin_amdgcn_readfirstlane(id[c]);
+        mapped = mapped && id[c] >= 0;
+      }
+      if (mapped) {
+        const int step = p.Hkv * D, row = (lane / LPR) * step;
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const int key = __builtin_amdgcn_readfirstlane(kb0 + r0 + c * RPI), in_page = key - (int)p.by_page((uint32_t)key) * (int)p.page;
+          const int64_t first = (((int64_t)id[c] * p.page + in_page) * p.Hkv + kvh) * D;
+          const uint32_t at = 2 * (uint32_t)(row + pc[c]);
+          if (KEYS) load_row_lds(uniform(p.kc + first), at, dst + c * 1024);
+          if (VALUES) load_row_lds(uniform(p.vc + first), at, dst + (KEYS ? apart : 0) + c * 1024);
+        }
+        return;
+      }
     }
     // every address first, then the loads: a load is a fence to the compiler, and a lookup behind each one would wait for LDS once per row
     int64_t at[N];
@@ -813,6 +837,7 @@ extern "C" int aq_paged_attn_decode_shared(const void* q, const void* k_cache, c
   a.by_g = aq::UDiv::of((uint32_t)a.G);
   a.by_hkv = aq::UDiv::of((uint32_t)a.Hkv);
   a.by_tails = aq::UDiv::of((uint32_t)(a.tails ? a.tails : 1));
+  a.page_rows = page_size % (512 / D) == 0;
   // (pages above 2^30 hold every position: the quotient is 0 for any divisor as large)
   a.by_page = aq::UDiv::of((uint32_t)(page_size < (1 << 30) ? page_size : 1 << 30));
   const int64_t tail_wgs = B * Hkv * plan.tails;
