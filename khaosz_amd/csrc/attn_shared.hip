@@ -708,8 +708,8 @@ constexpr int SHARED_TABLE_MAX = 2048;  // page-table entries kept in LDS
 // values of B x T positions (0.1 a megabyte), and past 2048 of them it has two launches with a merge of more slices (4).  Here there is the
 // merge (2, and 2 more where the decode kernel is a single launch), the tails' megabytes, and 0.6 a million products of a row with a
 // position and 128 dimensions.  The weights are fitted to both forms' times from a graph at 11168 random sizes (2 to 128 sequences, 2 to 8 KV heads
-// of 1 to 4 rows, both head dimensions, pages of 16 to 256, 64 to 40000 positions): the rule's choice costs 1.006 times the better form's
-// time in the mean, always sharing 1.100, never 1.62.  us, decode kernel | shared: 2 x 1088 positions of which 1024 shared, 16/4 heads of
+// of 1 to 8 rows, both head dimensions, pages of 16 to 256, 64 to 10000 positions): at 15385 others the rule's choice costs 1.008 times the
+// better form's time in the mean, always sharing 1.098, never 1.63.  us, decode kernel | shared: 2 x 1088 positions of which 1024 shared, 16/4 heads of
 // 128 7.8 | 8.6; 2 x 2112 of 2048 9.5 | 8.7; 8 x 2112 of 2048 12.2 | 8.9; 32 x 576 of 512 10.4 | 9.5; 32 x 1024 of 512 12.0 | 14.4;
 // 32 x 2560 of 2048 23.3 | 16.3; 122 x 152 of 128 8.9 | 15.8.
 static bool sharing_pays(int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t T, int64_t s0) {
@@ -777,7 +777,9 @@ static int launch_shared(SharedArgs& a, int64_t tail_wgs, uint16_t* out, hipStre
 }  // namespace aq
 
 extern "C" int64_t aq_paged_attn_decode_shared_positions(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t total_len, int64_t shared_len) {
-  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || total_len <= 0 || shared_len < 0 || total_len > (1 << 30) || (D != 64 && D != 128)) return 0;
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || total_len <= 0 || shared_len < 0 || total_len > (1 << 30) || (D != 64 && D != 128) ||
+      !aq::attn_group_ok(Hq / Hkv))
+    return 0;
   return aq::shared_plan(B, Hq, Hkv, D, total_len, shared_len).s0;
 }
 

@@ -79,7 +79,7 @@ def test_sizes_of_workspaces():
 
 def test_positions_that_are_read_once():
     f = _abi.load().aq_paged_attn_decode_shared_positions
-    assert f(0, 4, 2, 64, 3000, 2990) == 0 and f(2, 5, 2, 64, 3000, 2990) == 0 and f(2, 4, 2, 96, 3000, 2990) == 0 and f(2, 4, 2, 64, 3000, -1) == 0
+    assert f(0, 4, 2, 64, 3000, 2990) == 0 and f(2, 5, 2, 64, 3000, 2990) == 0 and f(2, 10, 2, 64, 3000, 2990) == 0 and f(2, 4, 2, 96, 3000, 2990) == 0 and f(2, 4, 2, 64, 3000, -1) == 0
     assert f(2, 4, 2, 64, 3000, 2990) == 2944 and f(2, 4, 2, 64, 3000, 1 << 40) == 2944 and f(1, 4, 2, 64, 3000, 2990) == 0
     assert f(2, 4, 2, 64, 100, 64) == 0 and f(2, 4, 2, 64, 3000, 63) == 0
     assert ops.paged_attn_shared_positions(2, 4, 2, 64, 3000, 2990) == 2944
