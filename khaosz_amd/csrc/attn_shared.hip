@@ -463,7 +463,6 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
   if (combo >= p.slices * p.Hkv) return;
   const int slice = p.by_hkv(combo), kvh = combo - slice * p.Hkv;
   const int k0 = slice * p.slice, k1 = k0 + p.slice < p.s0 ? k0 + p.slice : p.s0;
-  const int nit = (k1 - k0 + KW * KB - 1) / (KW * KB);
 
   const int t32 = tile * QW + qw, r0 = t32 * 32, row = r0 + col < p.rows ? r0 + col : p.rows - 1;  // rows past the end: the last one again
   const int b = p.by_g(row), head = kvh * p.G + (row - b * p.G);
@@ -487,6 +486,7 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
   } else if (p.table_lds) {
     __syncthreads();
   }
+  const int nit = __builtin_amdgcn_readfirstlane(seen > k0 ? (seen - k0 + KW * KB - 1) / (KW * KB) : 0);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(pa_lds_void*)lds;
   int64_t page = pages.template page_of<KB>(p, k0 + kw * KB, seen);
   auto issue = [&](int it, int buf) __attribute__((always_inline)) {
@@ -495,7 +495,7 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
     pages.template load<D, KB, LOADS, true, true>(p, kvh, kb0, page, seen, qw * LOADS * RPI, dst, TILE);
     page = pages.template page_of<KB>(p, kb0 + KW * KB, seen);
   };
-  issue(0, 0);
+  if (nit) issue(0, 0);
   SharedRows<D> rows;
   rows.start(p.q + ((int64_t)b * p.Hq + head) * D, lane >> 5, vis);
   const bool idle = r0 >= p.rows;  // wavefront-uniform: no row here, only loads
