@@ -258,3 +258,47 @@ def test_a_prefix_that_gains_nothing_is_read_as_ever():
         with torch.inference_mode():
             outs.append(m(torch.tensor([[3], [5]]).cuda(), paged_cache=cache, start_pos=164)["logits"])
     assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.gpu
+def test_a_captured_step():
+    """A step of the model over a shared prefix in a graph, replayed on new tokens and new pages, with eager steps between."""
+    m = _model()
+    g = torch.Generator().manual_seed(7)
+    cache = m.new_cache(160, 16)
+    table = torch.cat([torch.arange(131).expand(6, -1), 131 + torch.arange(6)[:, None]], 1).cuda()
+    cache.bind(table, 2101, share_prefix=True)
+    assert ops.paged_attn_shared_positions(6, 8, 2, 64, 2101, cache.shared_len) == 2048
+    fills = [torch.randn(cache.k_layers.shape, generator=g) for _ in range(3)]
+    tokens = [torch.randint(0, 97, (6, 1), generator=g).cuda() for _ in range(3)]
+    held = tokens[0].clone()
+
+    def fill(i):
+        cache.k_layers.copy_(fills[i])
+        cache.v_layers.copy_(fills[(i + 1) % 3])
+
+    def step(t):
+        with torch.inference_mode():
+            return m(t, paged_cache=cache, start_pos=2100)["logits"]
+
+    want = []
+    for i in range(3):
+        fill(i)
+        want.append(step(tokens[i]).clone())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(held)
+    for turn in range(5):
+        i = turn % 3
+        fill(i)
+        held.copy_(tokens[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i]), turn
+        fill((i + 1) % 3)
+        assert torch.equal(step(tokens[(i + 1) % 3]), want[(i + 1) % 3]), turn
