@@ -727,11 +727,12 @@ static SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int
   // A workgroup has 64 rows, or 128 where there are many: fewer keys and values go into the compute units then (64 x 8448 positions of which
   // 8192 shared, 32/8 heads of 128 39.2 | 36.3 us), but too few workgroups otherwise (32 x 4300 of 4096, 16/4 heads of 128 14.6 | 16.0).
   p.qw = rows > 128 && (rows + 63) / 64 * Hkv * (s0 / 256) > 2 * cus ? 4 : 2;
-  // As many slices as fill the compute units once, half as many where the tails are most of the work anyway; but short ones cost the merge
-  // more than they save (16 x 8300 of 8192, 16/4 heads of 128, slices of 64, 128, 256, 512: 24.5, 18.4, 15.4, 17.7; 8 x 2591 of 2048, 64,
+  // As many slices as fill the compute units once, half (three quarters) as many where the tails are most of the work anyway (with lengths, 256 x 4500
+  // positions of which 4096 shared, 16/4 heads of 128, half, three quarters, all: 38.1, 39.9, 41.6; 256 x 2400 of 2048, 24/4 of 64: 27.9, 21.8, 22.9); but
+  // short ones cost the merge more than they save (16 x 8300 of 8192, 16/4 heads of 128, slices of 64, 128, 256, 512: 24.5, 18.4, 15.4, 17.7; 8 x 2591 of 2048, 64,
   // 128, 256: 13.7, 11.4, 12.3).
   const int64_t tiles = (rows + 32 * p.qw - 1) / (32 * p.qw), shortest = s0 < 4096 ? 128 : 256;
-  int64_t want = (B * (T - s0) >= 8 * s0 ? cus / 2 : cus) / (tiles * Hkv);
+  int64_t want = (B * (T - s0) < 8 * s0 ? cus : D == 64 ? cus * 3 / 4 : cus / 2) / (tiles * Hkv);
   if (want < 1) want = 1;
   int64_t slice = ((s0 + want - 1) / want + 63) / 64 * 64;
   if (slice < shortest) slice = shortest;
