@@ -554,8 +554,9 @@ __device__ __forceinline__ void shared_prefix(const SharedArgs& p, uint8_t* lds,
 }
 
 // The G rows of one sequence against a slice of its own positions.  Bound by HBM and by what a workgroup waits for before its first and after
-// its last block (64 sequences of 256 positions, 32/8 heads of 128: 67 MB in 15.5 us; 256 of 404, 16/4: 212 MB in 46).  KW wavefronts, each by itself: blocks of 32 positions in turn, the
-// next block's keys requested when the last key has been read, its values when the last value has.
+// its last block (64 sequences of 256 positions, 32/8 heads of 128: 67 MB in 15.5 us; 256 of 404, 16/4: 212 MB in 46).  KW wavefronts, each
+// by itself: blocks of 32 positions in turn, the next block's keys requested when the last key has been read, its values when the last
+// value has.
 template <int D, int KW, bool LENS>
 __device__ __forceinline__ void shared_tail(const SharedArgs& p, uint8_t* lds, float* ml, int* table_lds) {
   constexpr int KB = 32, TILE = KB * 2 * D, LOADS = TILE / 1024;
@@ -766,7 +767,8 @@ static int launch_shared(SharedArgs& a, int64_t tail_wgs, uint16_t* out, hipStre
   if (prefix_wgs + tail_wgs > 0x7fffffff) return AQ_E_RANGE;
   a.prefix_wgs = (int)prefix_wgs;
   // (a form of its own where sequences may end anywhere: its masks cost the others 3 to 7 % of their time)
-  queue_kernel(a.lens ? shared_attn_kernel<D, QW, KW, KB, true> : shared_attn_kernel<D, QW, KW, KB, false>, dim3((unsigned)(prefix_wgs + tail_wgs)), dim3(256), lds, st, a);
+  queue_kernel(a.lens ? shared_attn_kernel<D, QW, KW, KB, true> : shared_attn_kernel<D, QW, KW, KB, false>,
+               dim3((unsigned)(prefix_wgs + tail_wgs)), dim3(256), lds, st, a);
   if (const int rc = (int)hipGetLastError()) return rc;
   const int64_t tiles = (int64_t)a.Hkv * a.tiles32;
   const bool few = tiles * (D / 4) < 16 * device_cus();
