@@ -60,7 +60,8 @@ def _build_host(force: bool) -> None:
     t = os.path.dirname(torch.__file__)
     inc = [os.path.join(t, "include"), os.path.join(t, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], "/opt/rocm/include"]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-Werror=shadow", "-fPIC", "-shared",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            *(x for d in inc for x in ("-isystem", d)), src, "-o", HOST_EXT, "-L" + os.path.join(t, "lib"), "-ltorch_python", "-ltorch_cpu",
            "-ltorch_hip", "-lc10", "-lc10_hip"]
     r = subprocess.run(cmd, capture_output=True, text=True)

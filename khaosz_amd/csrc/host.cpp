@@ -938,7 +938,10 @@ struct Block {
   Gain n1, n2, qn, kn;
 
   // the intermediate results' places in the scratch memory, `most` bytes
-  size_t x1, sx, qkv_rows, att, codes, q, k, parts, up_gate, h_codes, most;
+  struct Places {
+    size_t x1, sx, qkv_rows, att, codes, q, k, parts, up_gate, h_codes;
+  } place;
+  size_t most;
   int64_t parts_bytes;
 
   bool read(PyObject* block, PyObject* x, PyObject* rotary, PyObject* cache);
@@ -969,9 +972,9 @@ bool Block::read(PyObject* block, PyObject* px, PyObject* protary, PyObject* cac
   // the modules
   PyObject* d = dict_of(block);
   if (!d || !truth(d, k_norm_quant) || !truth(d, k_residual_adds)) return false;
-  PyObject *att = nested(d, k_modules, k_attention), *mlp = nested(d, k_modules, k_mlp);
-  if (!ordinary(att, types.gqa) || !ordinary(mlp, types.mlp)) return false;
-  PyObject *ad = dict_of(att), *md = dict_of(mlp);
+  PyObject *attn = nested(d, k_modules, k_attention), *mlp = nested(d, k_modules, k_mlp);
+  if (!ordinary(attn, types.gqa) || !ordinary(mlp, types.mlp)) return false;
+  PyObject *ad = dict_of(attn), *md = dict_of(mlp);
   int64_t layer;
   if (!truth(ad, k_decode_attention) || !truth(md, k_swiglu_quant) || get(ad, k_use_gate) != Py_False || !integer(ad, k_n_heads, &Hq) ||
       !integer(ad, k_n_kv_heads, &Hkv) || !integer(ad, k_head_dim, &D) || !integer(ad, k_layer_id, &layer))
@@ -1037,21 +1040,21 @@ bool Block::read(PyObject* block, PyObject* px, PyObject* protary, PyObject* cac
 void Block::lay_out() {
   const int64_t A = Hq * D, KV = Hkv * D, longest = dim > A ? dim : A, widest = F > dim ? F : dim;
   Scratch m;
-  x1 = m.take(2 * M * dim), sx = m.take(4 * M);
-  const size_t shared = m.used;
+  place.x1 = m.take(2 * M * dim), place.sx = m.take(4 * M);
+  const size_t behind_x1 = m.used;
   // attention
-  qkv_rows = m.take(2 * M * qkv.N), att = m.take(2 * M * A);
-  codes = m.take(few() ? lib.aq_gemv_w8a8_workspace_bytes(M, longest) : static_cast<size_t>(M * longest));
-  q = (step() && !shared) || rotates() ? 0 : m.take(2 * M * A), k = step() || !direct ? 0 : m.take(2 * M * KV);
+  place.qkv_rows = m.take(2 * M * qkv.N), place.att = m.take(2 * M * A);
+  place.codes = m.take(few() ? lib.aq_gemv_w8a8_workspace_bytes(M, longest) : static_cast<size_t>(M * longest));
+  place.q = (step() && !shared) || rotates() ? 0 : m.take(2 * M * A), place.k = step() || !direct ? 0 : m.take(2 * M * KV);
   parts_bytes = !step()   ? 0
                 : shared  ? lib.aq_paged_attn_decode_shared_workspace_bytes(B, Hq, Hkv, D, total, shared)
                 : merge() ? lib.aq_paged_attn_decode_partials_bytes(B, Hq, total)
                           : lib.aq_paged_attn_decode_workspace_bytes(B, Hq, Hkv, total);
-  parts = m.take(static_cast<size_t>(parts_bytes));
+  place.parts = m.take(static_cast<size_t>(parts_bytes));
   // the MLP, over the attention's results
-  m.used = shared;
-  up_gate = m.take(2 * M * (swiglu_gemv ? F : 2 * F));
-  h_codes = m.take(few() ? lib.aq_gemv_w8a8_workspace_bytes(M, widest) : static_cast<size_t>(M * widest));
+  m.used = behind_x1;
+  place.up_gate = m.take(2 * M * (swiglu_gemv ? F : 2 * F));
+  place.h_codes = m.take(few() ? lib.aq_gemv_w8a8_workspace_bytes(M, widest) : static_cast<size_t>(M * widest));
   most = m.most;
 }
 
@@ -1061,8 +1064,8 @@ void Block::lay_out() {
 int Block::queue(const void* in, void* out, char* base, const char** what) const {
   const bool few = this->few();
   const int64_t W = qkv.N, A = Hq * D, KV = Hkv * D;
-  void* x1 = base + this->x1;
-  float* sx = reinterpret_cast<float*>(base + this->sx);
+  void* x1 = base + place.x1;
+  float* sx = reinterpret_cast<float*>(base + place.sx);
 
   // y = projection of normalised tokens / of tokens as they are (+ residual); codes: room for M rows of the projection's K
   auto normed = [&](const Proj& p, const Gain& g, const void* x, void* y, size_t at) {
@@ -1102,11 +1105,11 @@ int Block::queue(const void* in, void* out, char* base, const char** what) const
                                        c.stream);
   };
 
-  char *q = base + qkv_rows, *att = base + this->att, *parts = base + this->parts;
-  int rc = normed(qkv, n1, in, q, codes);
+  char *q = base + place.qkv_rows, *att = base + place.att, *parts = base + place.parts;
+  int rc = normed(qkv, n1, in, q, place.codes);
   if (rc) return rc;
   if (shared) {
-    char* qr = base + this->q;
+    char* qr = base + place.q;
     *what = "aq_rope_kv_write";
     rc = qk_norm ? lib.aq_rope_kv_write_qknorm(q, fr, fr_stride, table, P, total - 1, 1, page, kc, vc, n_pages, qr, nullptr, B, Hq, Hkv, D, qn.p,
                                                kn.p, qn.eps, c.stream)
@@ -1116,7 +1119,7 @@ int Block::queue(const void* in, void* out, char* base, const char** what) const
     rc = lib.aq_paged_attn_decode_shared(qr, kc, vc, table, P, total, shared, lens, page, n_pages, scale, att, B, Hq, Hkv, D, parts, parts_bytes,
                                          c.stream);
     if (rc) return rc;
-    rc = projected(o, att, in, x1, codes);
+    rc = projected(o, att, in, x1, place.codes);
   } else if (step()) {
     *what = "aq_rope_paged_attn_decode";
     if (merge()) {
@@ -1135,10 +1138,10 @@ int Block::queue(const void* in, void* out, char* base, const char** what) const
                    : lib.aq_rope_paged_attn_decode(q, fr, fr_stride, table, P, total, lens, page, kc, vc, n_pages, scale, att, B, Hq, Hkv,
                                                    D, ws, parts_bytes, c.stream);
       if (rc) return rc;
-      rc = projected(o, att, in, x1, codes);
+      rc = projected(o, att, in, x1, place.codes);
     }
   } else {
-    char *qr = base + this->q, *kr = direct ? base + k : nullptr;
+    char *qr = base + place.q, *kr = direct ? base + place.k : nullptr;
     const void *qg = qk_norm ? qn.p : nullptr, *kg = qk_norm ? kn.p : nullptr;
     const bool late = rotates();
     *what = "aq_rope_kv_write";
@@ -1164,17 +1167,17 @@ int Block::queue(const void* in, void* out, char* base, const char** what) const
                                                   c.stream);
     }
     if (rc) return rc;
-    rc = projected(o, att, in, x1, codes);
+    rc = projected(o, att, in, x1, place.codes);
   }
   if (rc) return rc;
 
-  char *h = base + up_gate, *hq = base + h_codes;
+  char *h = base + place.up_gate, *hq = base + place.h_codes;
   if (swiglu_gemv) {
     *what = "aq_gemv_w8a8_decode_swiglu";
     rc = lib.aq_gemv_w8a8_decode_swiglu(x1, AQ_BF16, n2.p, n2.eps, ug.w, ug.s, ug.b.p, ug.b.code, h, AQ_BF16, M, F, dim, c.stream);
-    return rc ? rc : projected(down, h, x1, out, h_codes);
+    return rc ? rc : projected(down, h, x1, out, place.h_codes);
   }
-  rc = normed(ug, n2, x1, h, h_codes);
+  rc = normed(ug, n2, x1, h, place.h_codes);
   if (rc) return rc;
   *what = "aq_swiglu_quant_rowwise_i8";
   rc = lib.aq_swiglu_quant_rowwise_i8(h, AQ_BF16, M, F, 2 * F, reinterpret_cast<int8_t*>(hq), sx, c.stream);

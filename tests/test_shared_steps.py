@@ -1,0 +1,87 @@
+"""Decode steps of a fused block on long contexts, with and without a shared prefix: queued natively in one call, a block has to give the bits
+of the step-by-step path, whose operators get scratch memory of their own (GPU)."""
+import sys
+
+import pytest
+import torch
+
+from khaosz_amd import block, fuse_shared_inputs, ops, quantize_model
+from khaosz_amd.block import DecoderBlock, PagedKV, rotary_table
+
+DEV, DT = "cuda:0", torch.bfloat16
+
+
+def _block(heads, kv_heads, dim, **options):
+    torch.manual_seed(11)
+    b = DecoderBlock(heads * dim, heads, 704, kv_heads, **options)
+    b.reset_parameters()
+    b = b.to(DEV).to(DT)
+    quantize_model(b)
+    fuse_shared_inputs(b, norms=True, decode_attention=True, residuals=True)
+    return b
+
+
+def _step(batch, heads, kv_heads, dim, page, total, shared=0, mixed=False):
+    """Tokens, angles, and a cache bound for a step whose rows share their first `shared` positions (whole pages)."""
+    g = torch.Generator(device=DEV).manual_seed(total + batch)
+    common = shared // page
+    mine = -(-total // page) - common
+    n_pages = common + batch * mine
+    ids = torch.randperm(n_pages, generator=g, device=DEV)
+    table = torch.cat([ids[:common].expand(batch, -1), ids[common:].view(batch, mine)], 1).contiguous()
+    cache = PagedKV(n_pages, page, kv_heads, dim, DEV, DT)
+    cache.k_layers.normal_(generator=g)
+    cache.v_layers.normal_(generator=g)
+    lens = torch.randint(total // 2, total + 1, (batch,), generator=g, device=DEV) if mixed else None
+    angles = rotary_table(dim, total, device=DEV)[total - 1:].unsqueeze(0).expand(batch, -1, -1)
+    x = torch.randn(batch, 1, heads * dim, generator=g, device=DEV).to(DT)
+    return x, angles, cache.bind(table, total, seq_lens=lens, share_prefix=shared > 0)
+
+
+def _counted(monkeypatch, name):
+    calls, real = [], getattr(ops, name)
+    monkeypatch.setattr(ops, name, lambda *a, **k: (calls.append(1), real(*a, **k))[1])
+    return calls
+
+
+def _native_and_step_by_step(monkeypatch, b, x, angles, cache, operator):
+    k0, v0 = cache.k_layers.clone(), cache.v_layers.clone()
+    with torch.inference_mode():
+        got = block._native()(b, x, angles, cache)
+        assert got is not None  # queued natively
+        held = cache.k_layers.clone(), cache.v_layers.clone()
+        cache.k_layers.copy_(k0)
+        cache.v_layers.copy_(v0)
+        calls = _counted(monkeypatch, operator)
+        want = b(x, angles, None, cache)
+    assert len(calls) == 1
+    assert bool(want.isfinite().all()) and torch.equal(got, want)
+    assert torch.equal(held[0], cache.k_layers) and torch.equal(held[1], cache.v_layers)
+    assert not torch.equal(held[0], k0)  # the step's own key
+
+
+# contexts on which reading all positions once, were they shared, would take less scratch memory than the decode kernel does, and some where not
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,page,total", [
+    (8, 24, 4, 64, 128, 4096), (8, 24, 4, 64, 16, 4097), (32, 24, 4, 64, 64, 769), (32, 24, 4, 64, 24, 800), (16, 24, 4, 64, 64, 1601),
+    (64, 32, 8, 128, 64, 2113), (64, 16, 4, 128, 64, 4161), (8, 16, 4, 128, 64, 700), (1, 16, 4, 128, 64, 9000)])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_steps_without_a_shared_prefix(monkeypatch, batch, heads, kv_heads, dim, page, total, mixed):
+    print("step", batch, heads, kv_heads, dim, page, total, mixed, file=sys.stderr, flush=True)
+    b = _block(heads, kv_heads, dim)
+    x, angles, cache = _step(batch, heads, kv_heads, dim, page, total, mixed=mixed)
+    assert cache.shared_len == 0
+    _native_and_step_by_step(monkeypatch, b, x, angles, cache, "rope_paged_attn_decode")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,page,total,shared", [
+    (64, 32, 8, 128, 64, 8448, 8192), (16, 16, 4, 128, 128, 65600, 65536), (17, 8, 2, 64, 64, 4200, 2048), (70, 6, 2, 64, 24, 4500, 4104),
+    (8, 16, 4, 128, 64, 2591, 2048), (33, 24, 4, 64, 16, 1401, 1008)])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_steps_over_a_shared_prefix(monkeypatch, batch, heads, kv_heads, dim, page, total, shared, mixed):
+    print("shared step", batch, heads, kv_heads, dim, page, total, shared, mixed, file=sys.stderr, flush=True)
+    b = _block(heads, kv_heads, dim)
+    x, angles, cache = _step(batch, heads, kv_heads, dim, page, total, shared, mixed)
+    assert cache.shared_len == shared
+    _native_and_step_by_step(monkeypatch, b, x, angles, cache, "paged_attn_decode_shared")
