@@ -490,7 +490,8 @@ class DecoderBlock(nn.Module):
 # trace calls), blocks go operator by operator, through its replacement.
 _OPERATORS = {name: getattr(ops, name) for name in (
     "quant_rowwise_i8", "rmsnorm_quant_rowwise_i8", "swiglu_quant_rowwise_i8", "linear_w8a8", "gemv_w8a8_decode", "gemv_swiglu_ok",
-    "gemv_w8a8_decode_swiglu", "gemv_w8a8_codes", "rope_kv_write", "attn_gemv_fusable", "rope_paged_attn_decode", "paged_attn_decode_shared", "gemv_w8a8_attn",
+    "gemv_w8a8_decode_swiglu", "gemv_w8a8_codes", "rope_kv_write", "attn_gemv_fusable", "rope_paged_attn_decode",
+    "paged_attn_shared_positions", "paged_attn_decode_shared", "gemv_w8a8_attn",
     "prefill_attn_causal", "prefill_attn_paged", "RMSNORM_QUANT_MAX_K", "SWIGLU_QUANT_MAX_F", "GEMV_ATTN_MAX_ROWS", "GEMV_ATTN_MAX_K",
     "GEMV_ATTN_MAX_SLICES", "GEMV_ATTN_SLICE", "GEMV_ATTN_MAX_WORK")}
 _CLASSES = as_defined(GQA, MLP, PagedKV)

@@ -85,3 +85,22 @@ def test_steps_over_a_shared_prefix(monkeypatch, batch, heads, kv_heads, dim, pa
     x, angles, cache = _step(batch, heads, kv_heads, dim, page, total, shared, mixed)
     assert cache.shared_len == shared
     _native_and_step_by_step(monkeypatch, b, x, angles, cache, "paged_attn_decode_shared")
+
+
+@pytest.mark.gpu
+def test_a_replaced_rule_of_sharing_is_asked_by_fused_blocks(monkeypatch):
+    """A program that replaces the rule has its blocks read the prefix once, or not, as its own rule says."""
+    b = _block(8, 2, 64)
+    x, angles, cache = _step(40, 8, 2, 64, 16, 2101, 2096)
+    table = cache.page_table
+    with torch.inference_mode():
+        shared = b(x, angles, None, cache)
+        apart = b(x, angles, None, cache.bind(table, 2101))
+        assert not torch.equal(shared, apart)  # (probabilities are rounded in one of them)
+        cache.bind(table, 2101, share_prefix=True)
+        asked, rule = [], ops.paged_attn_shared_positions
+        monkeypatch.setattr(ops, "paged_attn_shared_positions", lambda *a: (asked.append(a), 0)[1])
+        assert torch.equal(b(x, angles, None, cache), apart)
+        assert asked == [(40, 8, 2, 64, 2101, 2096)]
+        monkeypatch.setattr(ops, "paged_attn_shared_positions", lambda *a: (asked.append(a), rule(*a))[1])
+        assert torch.equal(b(x, angles, None, cache), shared) and len(asked) == 2
