@@ -483,9 +483,12 @@ int aq_rope_prefill_attn_paged_ahead(const void *q, int64_t q_stride, const floa
  * and changes nothing of its result.  total_len at most 2^30, B Hq at most 2^24 (AQ_E_RANGE).
  * aq_paged_attn_decode_shared_positions: how many of the shared positions such a call reads once; 0 where that gains nothing, and
  * the call is aq_paged_attn_decode's.
+ * aq_paged_attn_decode_shared_step_positions: the same of a model's step, which otherwise takes aq_rope_paged_attn_decode: to read a prefix
+ * once costs it a launch of aq_rope_kv_write more.  0, or what the function above gives.
  * workspace: 16-byte aligned, aq_paged_attn_decode_shared_workspace_bytes(..) bytes for the same sizes (0: may be NULL); two calls that
  * overlap in time must not share it. */
 int64_t aq_paged_attn_decode_shared_positions(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t total_len, int64_t shared_len);
+int64_t aq_paged_attn_decode_shared_step_positions(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t total_len, int64_t shared_len);
 int64_t aq_paged_attn_decode_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t total_len,
                                                     int64_t shared_len);
 int aq_paged_attn_decode_shared(const void *q, const void *k_cache, const void *v_cache, const int64_t *page_table,

@@ -91,6 +91,7 @@ SYMBOLS = {
     "aq_rope_prefill_attn_paged_ahead": (_int, [_vp, _i64, _vp, _i64, _vp, ctypes.c_float, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp,
                                                 ctypes.c_float, _i64, _i64, _i64, _i64, _i64, _vp, _int, _vp]),
     "aq_paged_attn_decode_shared_positions": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "aq_paged_attn_decode_shared_step_positions": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "aq_paged_attn_decode_shared_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "aq_paged_attn_decode_shared": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64, ctypes.c_float, _vp, _i64, _i64,
                                            _i64, _i64, _vp, _i64, _vp]),

@@ -92,8 +92,9 @@ class PagedKV:
     in a single-token step whose sequences sit at different positions; the attention kernels apply it as
     the reference's position mask (transformer.py:40-46).
     ``bind(share_prefix=True)``: the leading pages that all rows of the table have in common (found on the host copy) are
-    read once per single-token step for all sequences, by the paged-cache kernels, at sizes that gain by it; results within bf16
-    rounding of reading them per sequence.  It holds until the next ``bind``."""
+    read once per single-token step for all sequences, by the paged-cache kernels, at sizes where a fitted rule
+    (``ops.paged_attn_shared_positions`` with ``step``) finds that a step is not slower for it; results within bf16 rounding of reading them
+    per sequence.  It holds until the next ``bind``."""
 
     def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device, dtype,
                  n_layers: int = 1):
@@ -311,7 +312,7 @@ class GQA(nn.Module):
                 and x.dtype == torch.bfloat16):
             qkv = self._project_qkv(x, codes, norm)
             if cache.shared_len > 0 and ops.paged_attn_shared_positions(B, self.n_heads, self.n_kv_heads, self.head_dim, cache.total_len,
-                                                                        cache.shared_len) > 0:
+                                                                        cache.shared_len, step=True) > 0:
                 # the first positions of all sequences are the same pages: read once
                 kc, vc = cache.k_layers[self.layer_id], cache.v_layers[self.layer_id]
                 q = ops.rope_kv_write(qkv.view(B, -1), rotary_emb.reshape(B, -1), cache.page_table, cache.total_len - 1,

@@ -72,7 +72,7 @@ namespace {
   X(aq_prefill_attn_paged_ahead)                                                                                 \
   X(aq_rope_prefill_attn_causal_ahead)                                                                           \
   X(aq_rope_prefill_attn_paged_ahead)                                                                            \
-  X(aq_paged_attn_decode_shared_positions)                                                                       \
+  X(aq_paged_attn_decode_shared_step_positions)                                                                  \
   X(aq_paged_attn_decode_shared_workspace_bytes)                                                                 \
   X(aq_paged_attn_decode_shared)                                                                                 \
   X(aq_fork_pages_workspace_bytes)                                                                               \
@@ -1003,7 +1003,7 @@ bool Block::read(PyObject* block, PyObject* px, PyObject* protary, PyObject* cac
   if (!plain(*t, ScalarType::Long, c.dev) || t->dim() != 2 || t->size(0) != B) return false;
   P = t->size(1);
   if (total < S || total > P * page) return false;
-  if (step() && integer(cd, k_shared_len, &shared) && (shared < 0 || !lib.aq_paged_attn_decode_shared_positions(B, Hq, Hkv, D, total, shared)))
+  if (step() && integer(cd, k_shared_len, &shared) && (shared < 0 || !lib.aq_paged_attn_decode_shared_step_positions(B, Hq, Hkv, D, total, shared)))
     shared = 0;
   const int64_t layer_bytes = 2 * n_pages * page * Hkv * D;
   kc = static_cast<char*>(k->mutable_data_ptr()) + layer * layer_bytes;

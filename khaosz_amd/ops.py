@@ -818,10 +818,14 @@ def paged_attn_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     return out
 
 
-def paged_attn_shared_positions(B: int, n_heads: int, n_kv_heads: int, head_dim: int, total_len: int, shared_len: int) -> int:
+def paged_attn_shared_positions(B: int, n_heads: int, n_kv_heads: int, head_dim: int, total_len: int, shared_len: int,
+                                step: bool = False) -> int:
     """How many of the shared positions ``paged_attn_decode_shared`` reads once at these sizes; 0: nothing is gained by it, and the call is
-    ``paged_attn_decode``'s."""
-    return int(_abi.load().aq_paged_attn_decode_shared_positions(B, n_heads, n_kv_heads, head_dim, int(total_len), int(shared_len)))
+    ``paged_attn_decode``'s.  ``step``: how many a model's step does, whose other form is ``rope_paged_attn_decode`` and which
+    needs ``rope_kv_write`` in front of ``paged_attn_decode_shared``."""
+    lib = _abi.load()
+    rule = lib.aq_paged_attn_decode_shared_step_positions if step else lib.aq_paged_attn_decode_shared_positions
+    return int(rule(B, n_heads, n_kv_heads, head_dim, int(total_len), int(shared_len)))
 
 
 def paged_attn_shared_workspace_bytes(B: int, n_heads: int, n_kv_heads: int, head_dim: int, total_len: int, shared_len: int, device) -> int:

@@ -76,8 +76,8 @@ def test_steps_without_a_shared_prefix(monkeypatch, batch, heads, kv_heads, dim,
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("batch,heads,kv_heads,dim,page,total,shared", [
-    (64, 32, 8, 128, 64, 8448, 8192), (16, 16, 4, 128, 128, 65600, 65536), (17, 8, 2, 64, 64, 4200, 2048), (70, 6, 2, 64, 24, 4500, 4104),
-    (8, 16, 4, 128, 64, 2591, 2048), (33, 24, 4, 64, 16, 1401, 1008)])
+    (64, 32, 8, 128, 64, 8448, 8192), (16, 16, 4, 128, 128, 65600, 65536), (40, 8, 2, 64, 64, 4200, 2048), (70, 6, 2, 64, 24, 4500, 4104),
+    (8, 16, 4, 128, 64, 2591, 2048), (33, 24, 4, 64, 16, 1401, 1296)])
 @pytest.mark.parametrize("mixed", [False, True])
 def test_steps_over_a_shared_prefix(monkeypatch, batch, heads, kv_heads, dim, page, total, shared, mixed):
     print("shared step", batch, heads, kv_heads, dim, page, total, shared, mixed, file=sys.stderr, flush=True)
@@ -99,8 +99,34 @@ def test_a_replaced_rule_of_sharing_is_asked_by_fused_blocks(monkeypatch):
         assert not torch.equal(shared, apart)  # (probabilities are rounded in one of them)
         cache.bind(table, 2101, share_prefix=True)
         asked, rule = [], ops.paged_attn_shared_positions
-        monkeypatch.setattr(ops, "paged_attn_shared_positions", lambda *a: (asked.append(a), 0)[1])
+        monkeypatch.setattr(ops, "paged_attn_shared_positions", lambda *a, **k: (asked.append((a, k)), 0)[1])
         assert torch.equal(b(x, angles, None, cache), apart)
-        assert asked == [(40, 8, 2, 64, 2101, 2096)]
-        monkeypatch.setattr(ops, "paged_attn_shared_positions", lambda *a: (asked.append(a), rule(*a))[1])
+        assert asked == [((40, 8, 2, 64, 2101, 2096), {"step": True})]
+        monkeypatch.setattr(ops, "paged_attn_shared_positions", lambda *a, **k: (asked.append((a, k)), rule(*a, **k))[1])
         assert torch.equal(b(x, angles, None, cache), shared) and len(asked) == 2
+
+
+def test_sizes_whose_steps_share():
+    """A step shares no more than the operator does, and less often: it has a launch more then."""
+    rule = ops.paged_attn_shared_positions
+    for sizes in ((40, 8, 2, 64, 2101, 2096), (3, 8, 2, 64, 2101, 2096), (64, 32, 8, 128, 8448, 8192), (2, 16, 4, 128, 65600, 65536)):
+        assert rule(*sizes, step=True) == rule(*sizes) == sizes[5] // 64 * 64
+    for sizes in ((57, 32, 8, 128, 217, 208), (16, 32, 8, 128, 861, 576), (3, 32, 8, 128, 2097, 592), (9, 16, 4, 128, 2889, 1408)):
+        assert rule(*sizes) == sizes[5] // 64 * 64 and rule(*sizes, step=True) == 0
+    for sizes in ((0, 4, 2, 64, 3000, 2990), (2, 5, 2, 64, 3000, 2990), (2, 4, 2, 96, 3000, 2990), (2, 4, 2, 64, 3000, -1), (2, 4, 2, 64, 0, 0),
+                  (1, 4, 2, 64, 3000, 2990), (2, 4, 2, 64, 3000, 63)):
+        assert rule(*sizes, step=True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,page,total,shared", [(57, 32, 8, 128, 16, 217, 208), (16, 32, 8, 128, 64, 861, 576)])
+def test_steps_that_gain_nothing_by_sharing_are_as_ever(monkeypatch, batch, heads, kv_heads, dim, page, total, shared):
+    """Sizes at which the operator alone gains by reading the prefix once and a step does not (in a graph 9 and 5 us of 100 a block lost)."""
+    assert ops.paged_attn_shared_positions(batch, heads, kv_heads, dim, total, shared) > 0
+    b = _block(heads, kv_heads, dim)
+    x, angles, cache = _step(batch, heads, kv_heads, dim, page, total, shared)
+    assert cache.shared_len == shared
+    _native_and_step_by_step(monkeypatch, b, x, angles, cache, "rope_paged_attn_decode")
+    with torch.inference_mode():
+        got = b(x, angles, None, cache)
+        assert torch.equal(got, b(x, angles, None, cache.bind(cache.page_table, total)))
