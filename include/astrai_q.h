@@ -478,8 +478,8 @@ int aq_rope_prefill_attn_paged_ahead(const void *q, int64_t q_stride, const floa
  * every row.  Those positions are read once, through row 0, and multiplied with the queries of all sequences at once on the matrix core;
  * the others through each sequence's own row.  shared_len may be anything from 0 (nothing is shared: aq_paged_attn_decode) on;
  * what lies past total_len counts for nothing.  A promise that does not hold gives the values of row 0's pages.
- * Results agree with aq_paged_attn_decode within bf16 rounding (probabilities of shared positions are rounded to bf16, sums are
- * fp32 in another order).  seq_lens as there, a sequence may end inside the shared positions; what lies behind its length may hold anything
+ * Results agree with aq_paged_attn_decode within bf16 rounding (where shared positions are read once, the probabilities of all positions, each
+ * sequence's own among them, are rounded to bf16 for the matrix core, which that kernel keeps in fp32; sums are fp32 in another order).  seq_lens as there, a sequence may end inside the shared positions; what lies behind its length may hold anything
  * and changes nothing of its result.  total_len at most 2^30, B Hq at most 2^24 (AQ_E_RANGE).
  * aq_paged_attn_decode_shared_positions: how many of the shared positions such a call reads once; 0 where that gains nothing, and
  * the call is aq_paged_attn_decode's.

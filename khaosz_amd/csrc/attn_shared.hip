@@ -10,7 +10,8 @@
 //
 // softmax over two ranges is the softmax over both: with m, l, n the maximum, denominator and numerator of each range,
 // out = (n1 2^(m1 - m) + n2 2^(m2 - m)) / (l1 2^(m1 - m) + l2 2^(m2 - m)), m = max(m1, m2).  All of them are fp32; probabilities
-// are rounded to bf16 (off by 2^-8 of themselves at most) where the matrix core takes them, the denominator sums them unrounded.
+// are rounded to bf16 (off by 2^-8 of themselves at most) where the matrix core takes them, in the prefix and in the tails alike, the denominator
+// sums them unrounded.
 //
 // Prefix and tail are workgroups of one launch, the prefix's first: those multiply while the tails read.  Both compute S^T = K Q^T and
 // O^T = V^T P^T as the prefill kernel does (attn_prefill.hip has the layout): a lane has the scores of one row, nothing changes lanes,
@@ -724,7 +725,7 @@ static bool sharing_pays(int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t T
 // for the first two.  Weights fitted to blocks' times in a graph at 1550 random sizes that the rule above shares (7 head layouts), of
 // which a third lost by it; the merge that sharing saves past 2048 positions counts by how much of them is shared, and by more than the fit
 // gives it (1.6), so that few sequences, level within 1 us there, share.  At 840 other sizes, a third of them with lengths: 25 lose more than
-// 1 us by this rule (5.1 of 128 at most), 122 by the operator's (9.1 of 105 at most); 0.75 % above the better form's time in the mean.  us a block, apart | shared:
+// 1 us by this rule (5.1 of 128 at most), 122 by the operator's (9.1 of 59 at most); 0.75 % above the better form's time in the mean.  us a block, apart | shared:
 // not shared  57 x 217 positions of which 208 shared, 32/8 heads of 128 105.9 | 115.9; 16 x 861 of 576 97.0 | 101.7; 3 x 2097 of 592 81.5 | 85.0;
 // shared      16 x 2101 of 2096, 24/4 heads of 64 41.5 | 39.5; 40 x 4096 of 4000 63.8 | 47.0; 16 x 8200 of 8000, 16/4 of 128 73.2 | 49.5;
 //             8 x 2101 of 2096 37.6 | 35.7; 2 x 2101 of 2096 31.6 | 32.7.

@@ -784,7 +784,7 @@ def paged_attn_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     """``paged_attn_decode`` for sequences that begin with the same pages: the entries of ``page_table`` for the first
     ``shared_len`` positions are the same in every row (the caller's promise; row 0's pages are read).  Those positions
     are read once and multiplied with all sequences' queries at once.  The results agree with ``paged_attn_decode`` within bf16
-    rounding; ``seq_lens`` as there.  Sizes that gain nothing by it (``paged_attn_shared_positions``) run as ``paged_attn_decode``.
+    rounding (the probabilities of all positions are rounded to bf16 on the way); ``seq_lens`` as there.  Sizes that gain nothing by it (``paged_attn_shared_positions``) run as ``paged_attn_decode``.
     ``workspace``: a contiguous device tensor to reuse across calls, of ``paged_attn_shared_workspace_bytes`` bytes; allocated per call when
     omitted or too small."""
     if workspace is None:

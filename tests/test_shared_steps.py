@@ -130,3 +130,34 @@ def test_steps_that_gain_nothing_by_sharing_are_as_ever(monkeypatch, batch, head
     with torch.inference_mode():
         got = b(x, angles, None, cache)
         assert torch.equal(got, b(x, angles, None, cache.bind(cache.page_table, total)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_probabilities_of_own_positions_are_rounded_too(dim):
+    """The probabilities of each sequence's own positions are rounded to bf16 (by half a step, 2^-8 of themselves at most), as those of the
+    shared ones are, and the denominator sums them unrounded.  Weights are taken relative to the largest of a range: where all scores
+    are 0 they are 1, nothing is rounded, and the sums of small whole numbers are exact.  Where every second own position has the score 1/2, own
+    weights are 1 and 2^-1/2: the own positions may move the result by that rounding, the shared ones, whose weights are 1, not at all."""
+    batch, page, shared, total = 6, 64, 2048, 2560
+    g = torch.Generator().manual_seed(dim)
+    common, mine = shared // page, (total - shared) // page
+    n_pages = common + batch * mine
+    table = torch.cat([torch.arange(common).expand(batch, -1), common + torch.arange(batch * mine).view(batch, mine)], 1).cuda()
+    v = torch.randint(-3, 4, (n_pages, page, 2, dim), generator=g).to(DT).cuda()
+    k = torch.zeros_like(v)
+    k[common:, ::2, :, 0] = 1.0  # every second of the sequences' own positions
+    q = torch.zeros(batch, 8, dim, dtype=DT, device=DEV)
+    for weight in (0.0, 0.5):
+        q[:, :, 0] = weight  # scores 0 and weight in the exp2 domain: a scale of ln 2
+        got = ops.paged_attn_decode_shared(q, k, v, table, total, shared, scale=0.6931471805599453)
+        assert ops.paged_attn_shared_positions(batch, 8, 2, dim, total, shared) == shared
+        for b in range(batch):
+            values = v[table[b]].flatten(0, 1).double()  # [total, heads, dim]
+            p = torch.where(k[table[b]].flatten(0, 1)[:, :1, :1] > 0, 2.0 ** weight, 1.0).double()
+            want = (p * values).sum(0) / p.sum()
+            moved = (2.0 ** -8 if weight else 0.0) * (p * values.abs())[shared:].sum(0) / p.sum()
+            # fp32: T terms in each sum, the exponential and the division 8 steps of 2^-24 each; then the result's own half step
+            near = moved + (2 * total + 16) * 2.0 ** -24 * (p * values.abs()).sum(0) / p.sum()
+            tol = (near + 2.0 ** -8 * (want.abs() + near)).repeat_interleave(4, 0)
+            assert bool(((got[b].double() - want.repeat_interleave(4, 0)).abs() <= tol).all())
