@@ -505,10 +505,12 @@ int aq_paged_attn_decode_shared(const void *q, const void *k_cache, const void *
  * empty row, all -1).  n = total_len, or seq_lens[parent] (device int64 [B], cut to 0 .. total_len), positions of the parent are
  * written.  Its first child goes on in all of its pages.  Every other child holds the pages that n fills, and gets a page of its own for
  * a page that is partly filled: the written rows of all layers' keys and values are copied there, the rows behind them are left as
- * they were; its later entries are -1.  (The first child writes on into the parent's partly filled page, whoever else holds it: a holder
- * that is to keep it as it is comes first, as a row of the table whose first child it is, or holds filled pages only.)  new_refs = max(refs - entries of the old rows, 0) + entries of the new rows, so rows without a child
- * let go of their pages, and the pages that are then free are handed out lowest first, to the rows in order.  missing[0]: rows that
- * found none (their entry is -1).  Sources are held, destinations free: the copies touch no page in use.
+ * they were; its later entries are -1.
+ * The first child goes on in that page itself WHOEVER ELSE HOLDS IT: refs is not asked.  A row whose n ends inside a page that another row or
+ * holder still reads (a sequence rolled back behind a fork, a cached prompt whose last page is not full) must not write on there: name it
+ * twice, leave the first child to those who read the page (or drop it in the next fork) and go on with the second, which has a copy.
+ * new_refs = max(refs - entries of the old rows, 0) + entries of the new rows, so rows without a child let go of their pages, and the
+ * pages that are then free are handed out lowest first, to the rows in order.  missing[0]: rows that found none (their entry is -1).  Sources are held, destinations free: the copies touch no page in use.
  * R at most 65536 (AQ_E_RANGE).  workspace: aq_fork_pages_workspace_bytes(n_pages, R) bytes.  It and refs are 16-byte aligned.
  *
  * aq_compact_pages: live[0] = number of pages with refs > 0; the held pages past place live[0] - 1 are moved into the free ones in front of

@@ -137,7 +137,8 @@ class PagedKV:
 
     def fork(self, refs: Tensor, parents: Tensor, seq_lens: Optional[Tensor] = None) -> "ops.ForkedPages":
         """Rows for the next step, forks of the bound table's (``ops.fork_pages``): row i goes on from row ``parents[i]``,
-        whose first ``total_len`` (or ``seq_lens``) positions are written.  Bind the table it returns."""
+        whose first ``total_len`` (or ``seq_lens``) positions are written.  Bind the table it returns.  A row that ends inside a page which
+        others still read is named twice and goes on as its second child: the first writes on in that page itself."""
         if self.page_table is None:
             raise ValueError("fork() needs a bound page table")
         return ops.fork_pages(self.page_table, refs, parents, self.k_layers, self.v_layers, self.total_len, seq_lens)

@@ -881,8 +881,10 @@ def fork_pages(page_table: torch.Tensor, refs: torch.Tensor, parents: torch.Tens
     """New rows of a page table, each a fork of an old one: row i of the result goes on from row ``parents[i]`` (int64 ``[R]``;
     outside ``0 .. B - 1``: an empty row).  Whole pages are held together; the first child of a row goes on in its pages, the others
     get a free page with a copy of what is written of a page that is not full (``total_len`` positions are written, or
-    ``seq_lens`` int64 ``[B]`` of them, in all layers' caches).  A row to be kept as it is (a cached prompt whose last page is not full) is forked
-    into itself first: ``parents = [keeper, keeper, ...]``.  Old rows without a child let go of their pages: dropping beams, ending
+    ``seq_lens`` int64 ``[B]`` of them, in all layers' caches).  The first child writes on in the partly filled page whoever else holds it, as
+    ``refs`` is not asked: a row that ends inside a page which another row, or another holder, still reads (a cached prompt whose last page is not
+    full; with ``seq_lens``, a sequence rolled back into pages that it shares) is named twice, ``parents = [.., row, row]``, and goes on
+    as its second child, which has a copy; the first is kept for those readers, or dropped in the next fork.  Old rows without a child let go of their pages: dropping beams, ending
     sequences and sampling several continuations are one call, and no call waits for the device.  ``refs`` int32
     ``[n_pages]`` counts who holds each page.  The table and the counts given are left as they are; the caches (any type, of 16-byte
     rows) are written in place, free pages only."""

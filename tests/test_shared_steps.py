@@ -161,3 +161,31 @@ def test_probabilities_of_own_positions_are_rounded_too(dim):
             near = moved + (2 * total + 16) * 2.0 ** -24 * (p * values.abs()).sum(0) / p.sum()
             tol = (near + 2.0 ** -8 * (want.abs() + near)).repeat_interleave(4, 0)
             assert bool(((got[b].double() - want.repeat_interleave(4, 0)).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+def test_a_row_rolled_back_into_a_page_that_others_read():
+    """Such a row is named twice: its second child has a copy of what is written, and what it writes reaches no other row.  Its first child is
+    dropped in the next fork, which leaves the counts as if it had not been."""
+    page, n_pages = 16, 12
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(2, n_pages, page, 2, 64, generator=g).to(DT).cuda() for _ in range(2))
+    table = torch.tensor([[3, 5, 7, -1], [3, 5, 2, -1]], device=DEV)  # both hold page 5 as a full one ..
+    refs = torch.zeros(n_pages, dtype=torch.int32, device=DEV)
+    refs[table[0, :2]], refs[table[:, 2]] = 2, 1
+    lens = torch.tensor([40, 21], device=DEV)  # .. and the second is set back to its 5th position in it
+    k0, v0 = k.clone(), v.clone()
+    one = ops.fork_pages(table, refs, torch.tensor([0, 1, 1], device=DEV), k, v, 48, seq_lens=lens)
+    assert one.page_table.tolist() == [[3, 5, 7, -1], [3, 5, 2, -1], [3, 0, -1, -1]] and one.missing.item() == 0
+    assert torch.equal(k[:, 0, :5], k0[:, 5, :5]) and torch.equal(v[:, 0, :5], v0[:, 5, :5])
+    lens = torch.tensor([40, 21, 21], device=DEV)
+    two = ops.fork_pages(one.page_table, one.refs, torch.tensor([0, 2], device=DEV), k, v, 48, seq_lens=lens)
+    assert two.page_table.tolist() == [[3, 5, 7, -1], [3, 0, -1, -1]]
+    want = torch.zeros(n_pages, dtype=torch.int32)
+    want[3], want[5], want[7], want[0] = 2, 1, 1, 1
+    assert torch.equal(two.refs.cpu(), want)
+    qkv = torch.randn(2, (2 + 2 * 2) * 64, generator=g).to(DT).cuda()  # a token at position 21 of the row that was set back
+    ops.rope_kv_write(qkv[1:], rotary_table(64, 22, device=DEV)[21:], two.page_table[1:], 21, k[0], v[0], 2, 2)
+    assert not torch.equal(k[0, 0, 5], k0[0, 0, 5])
+    others = [x for x in range(n_pages) if x != 0]
+    assert torch.equal(k[:, others], k0[:, others]) and torch.equal(v[:, others], v0[:, others])
