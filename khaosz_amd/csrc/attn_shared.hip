@@ -745,9 +745,10 @@ static SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int
   // 8192 shared, 32/8 heads of 128 39.2 | 36.3 us), but too few workgroups otherwise (32 x 4300 of 4096, 16/4 heads of 128 14.6 | 16.0).
   p.qw = rows > 128 && (rows + 63) / 64 * Hkv * (s0 / 256) > 2 * cus ? 4 : 2;
   // As many slices as fill the compute units once, half (three quarters) as many where the tails are most of the work anyway (with lengths, 256 x 4500
-  // positions of which 4096 shared, 16/4 heads of 128, half, three quarters, all: 38.1, 39.9, 41.6; 256 x 2400 of 2048, 24/4 of 64: 27.9, 21.8, 22.9); but
-  // short ones cost the merge more than they save (16 x 8300 of 8192, 16/4 heads of 128, slices of 64, 128, 256, 512: 24.5, 18.4, 15.4, 17.7; 8 x 2591 of 2048, 64,
-  // 128, 256: 13.7, 11.4, 12.3).
+  // positions of which 4096 shared, 16/4 heads of 128, half, three quarters, all: 38.1, 39.9, 41.6; 256 x 2400 of 2048, 24/4 of 64: 27.9, 21.8, 22.9; over
+  // the best of the three in the mean of random sizes of 8 head layouts 1.009, 1.011, 1.020 at 218 such of 128, 1.019, 1.012, 1.019 at 328 of 64, and
+  // 1.038, 1.012, 1.011 at 654 with shorter tails); but short ones cost the merge more than they save (16 x 8300 of 8192, 16/4 heads of 128,
+  // slices of 64, 128, 256, 512: 24.5, 18.4, 15.4, 17.7; 8 x 2591 of 2048, 64, 128, 256: 13.7, 11.4, 12.3).
   const int64_t tiles = (rows + 32 * p.qw - 1) / (32 * p.qw), shortest = s0 < 4096 ? 128 : 256;
   int64_t want = (B * (T - s0) < 8 * s0 ? cus : D == 64 ? cus * 3 / 4 : cus / 2) / (tiles * Hkv);
   if (want < 1) want = 1;
@@ -756,9 +757,10 @@ static SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int
   p.slice = (int)slice;
   p.slices = (int)((s0 + slice - 1) / slice);
   if (T > s0) {
-    // one workgroup of tails per compute unit, four of half the size at head dimension 64 (32 x 1024 of 512, 16/4 heads of 128, one or two:
-    // 11.0 | 12.7 without the merge; 33 x 1401 of 1008, 24/4 of 64, one, two or four: 10.8, 7.9, 6.9); 128 positions are one block for each wavefront
-    int64_t n = (D == 64 ? 4 : 1) * cus / (B * Hkv), most = (T - s0 + 127) / 128;
+    // one workgroup of tails per compute unit, two of half the size at head dimension 64; 128 positions are one block for each wavefront.  (One, two
+    // or four, over the best of them in the mean of random sizes: 1.019, 1.015, 1.029 at 750 of head dimension 64, 1.014, 1.022, 1.043 at 450 of 128; us
+    // 100 x 900 of 768, 24/4 of 64, with lengths 12.2, 12.2, 14.5; 33 x 1401 of 1008 12.3, 10.7, 10.6; 64 x 1000 of 512, 16/4 of 128 19.5, 21.1, 23.6.)
+    int64_t n = (D == 64 ? 2 : 1) * cus / (B * Hkv), most = (T - s0 + 127) / 128;
     if (n > most) n = most;
     if (n < 1) n = 1;
     p.tail = (int)(((T - s0 + n - 1) / n + 127) / 128 * 128);
