@@ -18,11 +18,11 @@
 // K and V rows go straight into LDS ahead of the products.
 //
 // us a call; what its bytes take at the 5.2 TB/s of a large copy; the decode kernel, which reads the prefix for every sequence; what bounds the call:
-//   8 x 2591 positions of which 2048 shared, 16/4 heads of 128     9.7   2.5   13.8  the latency of two launches
-//   33 x 1401 of 1008, own lengths, 24/4 of 64, pages of 16        10.4  1.5   12.6  the same
-//   64 x 8448 of 8192, 32/8 of 128                                 33.9  19.6   208  a wavefront's chain in the prefix beside the tails' loads
-//   16 x 65600 of 65536, 16/4 of 128                               37.7  26.3   350  HBM: 6.5 TB/s inside the loop, 2.3 us before it; the merge 4.8
-//   256 x 4500 of 4096, own lengths, 16/4 of 128                   39.0  22.5   222  tails of 200 positions, mostly beginning and end; the merge 5.3
+//   8 x 2591 positions of which 2048 shared, 16/4 heads of 128     9.3   2.5   13.8  the latency of two launches
+//   33 x 1401 of 1008, own lengths, 24/4 of 64, pages of 16        10.8  1.5   12.6  the same
+//   64 x 8448 of 8192, 32/8 of 128                                 34.8  19.6   208  a wavefront's chain in the prefix beside the tails' loads
+//   16 x 65600 of 65536, 16/4 of 128                               36.0  26.3   350  HBM: 6.5 TB/s inside the loop, 20.6 of the launch's 32.3; the merge 4.8
+//   256 x 4500 of 4096, own lengths, 16/4 of 128                   39.4  22.5   222  tails of 200 positions, mostly beginning and end; the merge 5.3
 #include "aq_attn.h"
 #include "aq_common.h"
 #include "aq_rows.h"

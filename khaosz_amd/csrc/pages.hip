@@ -4,8 +4,8 @@
 // so that a step of a search can be captured with the decode steps around it.
 //
 // What bounds them: pages that move, HBM (500 of 1024 pages, 24 layers, 1.6 GB: 300 to 340 us by the card, 5.2 TB/s; 64 beams of which 24 go on, 220 MB:
-// 46.1); else launches and the chain of reads in each: table, counts, free pages, copies (1 row into 8, 24 layers, 22 MB: 6.5; 40 of 128 pages: 6.5;
-// 256 rows into 300 over 40000 pages, five launches: 19.7).
+// 46.3); else launches and the chain of reads in each: table, counts, free pages, copies (from a graph 1 row into 8, 24 layers, 22 MB: 6.7; 40 of 128
+// pages: 4.7; 256 rows into 300 over 40000 pages, five launches: 16.8; queued one by one 6.8, 6.8 and 19.6, what the host takes for them).
 //
 // refs[page] counts who holds a page: rows of the table, and whoever else (a cache of prompts).  0: free.
 #include "aq_common.h"
