@@ -93,7 +93,7 @@ class PagedKV:
     the reference's position mask (transformer.py:40-46).
     ``bind(share_prefix=True)``: the leading pages that all rows of the table have in common (found on the host copy) are
     read once per single-token step for all sequences, by the paged-cache kernels, at sizes where a fitted rule
-    (``ops.paged_attn_shared_positions`` with ``step``) finds that a step is not slower for it; results within bf16 rounding of reading them
+    (``ops.paged_attn_shared_positions`` with ``step``) finds that a step gains or is level; results within bf16 rounding of reading them
     per sequence.  It holds until the next ``bind``."""
 
     def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device, dtype,

@@ -724,15 +724,17 @@ static bool sharing_pays(int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t T
 // The same for a model's step.  Its other form rotates, writes the pages and attends in one launch (and a merge); sharing has a launch in front
 // for the first two.  Weights fitted to blocks' times in a graph at 1550 random sizes that the rule above shares (7 head layouts), of
 // which a third lost by it; the merge that sharing saves past 2048 positions counts by how much of them is shared, and by more than the fit
-// gives it (1.6), so that few sequences, level within 1 us there, share.  At 840 other sizes, a third of them with lengths: 25 lose more than
-// 1 us by this rule (5.1 of 128 at most), 122 by the operator's (9.1 of 59 at most); 0.75 % above the better form's time in the mean.  us a block, apart | shared:
-// not shared  57 x 217 positions of which 208 shared, 32/8 heads of 128 105.9 | 115.9; 16 x 861 of 576 97.0 | 101.7; 3 x 2097 of 592 81.5 | 85.0;
+// gives it (1.6), so that few sequences, level within 1 us there, share.  At 840 sizes it was not fitted to, a third of them with lengths: 28 lose
+// more than 1 us by this rule (8 of 129 at most), 123 by the operator's (8 of 129 at most), 94 us and 333 in all; 91 us of the 1441 that sharing can gain are
+// left; 0.5 % above the better form's time in the mean, 1.0 % by the operator's rule.  us a block, apart | shared:
+// not shared  57 x 217 positions of which 208 shared, 32/8 heads of 128 105.9 | 115.9; 49 x 1162 of 400, 8/8 of 64 47.0 | 51.3; 3 x 2097 of 592,
+//             32/8 of 128 81.5 | 85.0;
 // shared      16 x 2101 of 2096, 24/4 heads of 64 41.5 | 39.5; 40 x 4096 of 4000 63.8 | 47.0; 16 x 8200 of 8000, 16/4 of 128 73.2 | 49.5;
 //             8 x 2101 of 2096 37.6 | 35.7; 2 x 2101 of 2096 31.6 | 32.7.
-static bool step_sharing_pays(int64_t B, int64_t Hkv, int64_t D, int64_t T, int64_t s0) {
+static bool step_sharing_pays(int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t T, int64_t s0) {
   const double position = 4e-6 * (double)(Hkv * D);  // megabytes
-  const double apart = 0.08 * position * (double)(B * T) + (T > 2048 ? 2.9 * (double)s0 / (double)T : 0.0);
-  const double shared = 3.0 + (T > 256 ? 0.0 : 3.0) + 0.1 * position * (double)(B * (T - s0));
+  const double apart = (0.05 + 0.006 * (double)G) * position * (double)(B * T) + (T > 2048 ? 2.1 * (double)s0 / (double)T : 0.0);
+  const double shared = 2.2 + (T > 256 ? 0.0 : 3.0) + 0.09 * position * (double)(B * (T - s0));
   return shared < apart;
 }
 
@@ -806,7 +808,7 @@ extern "C" int64_t aq_paged_attn_decode_shared_positions(int64_t B, int64_t Hq, 
 
 extern "C" int64_t aq_paged_attn_decode_shared_step_positions(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t total_len, int64_t shared_len) {
   const int64_t s0 = aq_paged_attn_decode_shared_positions(B, Hq, Hkv, D, total_len, shared_len);
-  return s0 && aq::step_sharing_pays(B, Hkv, D, total_len, s0) ? s0 : 0;
+  return s0 && aq::step_sharing_pays(B, Hkv, Hq / Hkv, D, total_len, s0) ? s0 : 0;
 }
 
 extern "C" int64_t aq_paged_attn_decode_shared_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t total_len,

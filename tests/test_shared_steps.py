@@ -111,7 +111,7 @@ def test_sizes_whose_steps_share():
     rule = ops.paged_attn_shared_positions
     for sizes in ((40, 8, 2, 64, 2101, 2096), (3, 8, 2, 64, 2101, 2096), (64, 32, 8, 128, 8448, 8192), (2, 16, 4, 128, 65600, 65536)):
         assert rule(*sizes, step=True) == rule(*sizes) == sizes[5] // 64 * 64
-    for sizes in ((57, 32, 8, 128, 217, 208), (16, 32, 8, 128, 861, 576), (3, 32, 8, 128, 2097, 592), (9, 16, 4, 128, 2889, 1408)):
+    for sizes in ((57, 32, 8, 128, 217, 208), (49, 8, 8, 64, 1162, 400), (3, 32, 8, 128, 2097, 592), (120, 16, 4, 128, 254, 208)):
         assert rule(*sizes) == sizes[5] // 64 * 64 and rule(*sizes, step=True) == 0
     for sizes in ((0, 4, 2, 64, 3000, 2990), (2, 5, 2, 64, 3000, 2990), (2, 4, 2, 96, 3000, 2990), (2, 4, 2, 64, 3000, -1), (2, 4, 2, 64, 0, 0),
                   (1, 4, 2, 64, 3000, 2990), (2, 4, 2, 64, 3000, 63)):
@@ -119,9 +119,9 @@ def test_sizes_whose_steps_share():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("batch,heads,kv_heads,dim,page,total,shared", [(57, 32, 8, 128, 16, 217, 208), (16, 32, 8, 128, 64, 861, 576)])
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,page,total,shared", [(57, 32, 8, 128, 16, 217, 208), (49, 8, 8, 64, 16, 1162, 400)])
 def test_steps_that_gain_nothing_by_sharing_are_as_ever(monkeypatch, batch, heads, kv_heads, dim, page, total, shared):
-    """Sizes at which the operator alone gains by reading the prefix once and a step does not (in a graph 9 and 5 us of 100 a block lost)."""
+    """Sizes at which the operator alone gains by reading the prefix once and a step does not (in a graph a block of 106 us loses 10, one of 47 loses 4)."""
     assert ops.paged_attn_shared_positions(batch, heads, kv_heads, dim, total, shared) > 0
     b = _block(heads, kv_heads, dim)
     x, angles, cache = _step(batch, heads, kv_heads, dim, page, total, shared)
