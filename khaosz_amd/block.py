@@ -313,7 +313,7 @@ class GQA(nn.Module):
                 and x.dtype == torch.bfloat16):
             qkv = self._project_qkv(x, codes, norm)
             if cache.shared_len > 0 and ops.paged_attn_shared_positions(B, self.n_heads, self.n_kv_heads, self.head_dim, cache.total_len,
-                                                                        cache.shared_len, step=True) > 0:
+                                                                        cache.shared_len, True) > 0:
                 # the first positions of all sequences are the same pages: read once
                 kc, vc = cache.k_layers[self.layer_id], cache.v_layers[self.layer_id]
                 q = ops.rope_kv_write(qkv.view(B, -1), rotary_emb.reshape(B, -1), cache.page_table, cache.total_len - 1,

@@ -99,10 +99,10 @@ def test_a_replaced_rule_of_sharing_is_asked_by_fused_blocks(monkeypatch):
         assert not torch.equal(shared, apart)  # (probabilities are rounded in one of them)
         cache.bind(table, 2101, share_prefix=True)
         asked, rule = [], ops.paged_attn_shared_positions
-        monkeypatch.setattr(ops, "paged_attn_shared_positions", lambda *a, **k: (asked.append((a, k)), 0)[1])
+        monkeypatch.setattr(ops, "paged_attn_shared_positions", lambda *a: (asked.append(a), 0)[1])
         assert torch.equal(b(x, angles, None, cache), apart)
-        assert asked == [((40, 8, 2, 64, 2101, 2096), {"step": True})]
-        monkeypatch.setattr(ops, "paged_attn_shared_positions", lambda *a, **k: (asked.append((a, k)), rule(*a, **k))[1])
+        assert asked == [(40, 8, 2, 64, 2101, 2096, True)]
+        monkeypatch.setattr(ops, "paged_attn_shared_positions", lambda *a: (asked.append(a), rule(*a))[1])
         assert torch.equal(b(x, angles, None, cache), shared) and len(asked) == 2
 
 
