@@ -528,6 +528,49 @@ int aq_compact_pages(const int64_t *page_table, int64_t entries, const int32_t *
                      int64_t *new_table, int32_t *new_refs, int64_t *where, int32_t *live, void *workspace,
                      int64_t workspace_bytes, void *stream);
 
+/* ---- routed experts (DeepSeekMoE, astrai/model/components/mlp.py:31-93, whose forward runs the experts one after the other): from the
+ * router's logits to the layer's output without the host learning how many tokens an expert got.
+ *
+ * aq_route_topk: logits [T, E] of `dtype` (ld elements between tokens).  A token's choices are its k largest logits, the largest first, equal
+ * ones the lowest expert first; -inf and NaN are never chosen, a token with fewer than k others has -1 in the places left (a
+ * padded token: a row of -inf).  experts [T, k] int32; weights [T, k] fp32, exp(x - max) over the sum of the chosen ones (renormalize != 0) or of all E (softmax), 0 in places without an
+ * expert.  The choices in the experts' order, by token inside an expert: expert e has rows offsets[e] .. offsets[e + 1] - 1 (offsets int32 [E + 1]),
+ * rows [T, k] int32 the row of each choice (-1: none), tokens [T k] int32 the token of each row (-1 past offsets[E]).
+ * E at most 512, k at most 16, T at most 2^24 (AQ_E_RANGE).  workspace: aq_route_topk_workspace_bytes(T, E) bytes (0: may be NULL), 4-byte aligned; calls
+ * that overlap in time must not share it. */
+int64_t aq_route_topk_workspace_bytes(int64_t T, int64_t E);
+int aq_route_topk(const void *logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t k, int renormalize,
+                  float *weights, int32_t *experts, int32_t *rows, int32_t *tokens, int32_t *offsets, void *workspace,
+                  int64_t workspace_bytes, void *stream);
+
+/* aq_linear_w8a8 of E experts at once: row r of y [R, N], offsets[e] <= r < offsets[e + 1], is expert e's Linear (wq [E, N, K], sw [E, N], bias
+ * [E, N] or NULL) on row tokens[r] of xq [x_rows, K], sx [x_rows]; tokens NULL: on row r itself, and x_rows = R.  Groups may be empty.  Rows of
+ * y past offsets[E] are left as they are.  A token outside 0 .. x_rows - 1 counts as a row of zeros; offsets outside 0 .. R count as the nearest bound, offsets must not fall.
+ * E at most 512; N K and x_rows K at most 2^31 - 17 (AQ_E_RANGE).
+ * aq_swiglu_w8a8_grouped: wq [E, 2 F, K] is every expert's up on top of its gate (sw [E, 2 F]); h [R, F] = up * silu(gate), both as the
+ * Linear above would have stored them in h's type.  F a multiple of 16. */
+int aq_linear_w8a8_grouped(const int8_t *xq, const float *sx, int64_t x_rows, const int8_t *wq, const float *sw,
+                           const void *bias, int bias_dtype, const int32_t *offsets, int64_t E,
+                           const int32_t *tokens, int64_t R, void *y, int y_dtype, int64_t N, int64_t K, void *stream);
+int aq_swiglu_w8a8_grouped(const int8_t *xq, const float *sx, int64_t x_rows, const int8_t *wq, const float *sw,
+                           const int32_t *offsets, int64_t E, const int32_t *tokens, int64_t R, void *h, int h_dtype,
+                           int64_t F, int64_t K, void *stream);
+
+/* out[t] = sum_j weights[t, j] y[rows[t, j]] (+ residual[t]) in fp32 in the order of j, the residual last, rounded once to `dtype`, the type of
+ * y [R, N], residual [T, N] (or NULL) and out [T, N].  rows outside 0 .. R - 1 count for nothing.  out may be residual, and must not overlap y.  k at most 64. */
+int aq_combine_rows(const void *y, int dtype, int64_t R, int64_t N, const int32_t *rows, const float *weights,
+                    int64_t T, int64_t k, const void *residual, void *out, void *stream);
+
+/* The experts' whole MLP on x [T, dim]: quantised per token, up, gate and SwiGLU (up_gate [E, 2 F, dim]), h quantised per row, down ([E, dim, F]),
+ * the weighted sum of each token's rows (+ residual): the results of the functions above one after the other, the experts' outputs in x's type in
+ * between.  offsets, tokens, rows, weights as aq_route_topk leaves them.  workspace: aq_experts_w8a8_workspace_bytes(..) bytes, 16-byte aligned; calls that
+ * overlap in time must not share it. */
+int64_t aq_experts_w8a8_workspace_bytes(int x_dtype, int64_t T, int64_t k, int64_t dim, int64_t F);
+int aq_experts_w8a8(const void *x, int x_dtype, int64_t T, int64_t dim, const int32_t *offsets, int64_t E,
+                    const int32_t *tokens, const int32_t *rows, const float *weights, int64_t k, const int8_t *up_gate,
+                    const float *up_gate_scale, const int8_t *down, const float *down_scale, int64_t F,
+                    const void *residual, void *out, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

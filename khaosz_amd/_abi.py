@@ -100,6 +100,13 @@ SYMBOLS = {
                              _i64, _vp]),
     "aq_compact_pages_workspace_bytes": (_i64, [_i64]),
     "aq_compact_pages": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "aq_route_topk_workspace_bytes": (_i64, [_i64, _i64]),
+    "aq_route_topk": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "aq_linear_w8a8_grouped": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _int, _vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _vp]),
+    "aq_swiglu_w8a8_grouped": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _vp]),
+    "aq_combine_rows": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp]),
+    "aq_experts_w8a8_workspace_bytes": (_i64, [_int, _i64, _i64, _i64, _i64]),
+    "aq_experts_w8a8": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp]),
 }
 
 # csrc/aq_lab.h: the lab library's additions (measurement probes, the tile-forcing test hook)

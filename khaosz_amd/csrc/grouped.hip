@@ -1,0 +1,268 @@
+// One Linear per expert on the rows of that expert, any number of rows each: y[r] = (float(sum_k xq[t, k] wq[e, n, k]) sx[t]) sw[e, n] (+ bias[e, n])
+// for the rows offsets[e] <= r < offsets[e + 1] of expert e, t = tokens[r] or r itself: the arithmetic of the single Linear, three rounded
+// operations and one cast.  SwiGLU: the weights are up and gate stacked, both rounded to the output's type, h = up silu(gate).
+//
+// The groups' sizes are known on the device alone.  A launch has workgroups for the most tiles of rows that any split of R rows over
+// E experts can need; each finds its own by a scan over the offsets, and those past the last one end.
+#include "aq_gemm.h"
+
+namespace aq {
+
+constexpr int GP_MAX_E = 512;
+
+struct GroupedArgs {
+  const uint8_t* x;
+  const float* sx;
+  const uint8_t* w;
+  const float* sw;
+  const void* bias;
+  int bias_dtype;
+  const int32_t* offsets;
+  const int32_t* tokens;
+  void* y;
+  int64_t w_bytes;  // of one expert
+  int x_rows, R, E;
+  int N;            // weight rows of an expert (SwiGLU: up and gate)
+  int K;
+};
+
+struct RowTile {
+  int e, first, end;  // rows first .. end - 1; end of the expert's rows
+};
+
+// Tile `idx` of the list that has ceil(rows / BM) tiles of every expert: every lane looks at a run of experts.  false: there is none.
+// Offsets outside 0 .. R, or that fall, count as the nearest that do not: nothing is read or written outside the R rows.
+template <int BM, int PER>
+__device__ __forceinline__ bool find_tile(const GroupedArgs& p, int idx, int lane, RowTile& t) {
+  int o[PER + 1], n = 0, mine[PER];
+#pragma unroll
+  for (int i = 0; i <= PER; ++i) {
+    const int e = lane * PER + i;
+    o[i] = p.offsets[e < p.E ? e : p.E];
+  }
+#pragma unroll
+  for (int i = 0; i <= PER; ++i) o[i] = o[i] < 0 ? 0 : o[i] > p.R ? p.R : o[i];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int rows = o[i + 1] - o[i];
+    mine[i] = rows > 0 ? (rows + BM - 1) / BM : 0;
+    n += mine[i];
+  }
+  int upto = n;
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x142, 0xa, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x143, 0xc, 0xf, false);
+  const unsigned long long past = __ballot(upto > idx);
+  if (!past) return false;
+  const int at = __builtin_ctzll(past);
+  int before = upto - n, e = lane * PER, first = o[0], end = o[1];
+#pragma unroll
+  for (int i = 1; i < PER; ++i)
+    if (before + mine[i - 1] <= idx) before += mine[i - 1], e = lane * PER + i, first = o[i], end = o[i + 1];
+    else break;
+  t.e = __builtin_amdgcn_readlane(e, at);
+  t.first = __builtin_amdgcn_readlane(first, at) + (idx - __builtin_amdgcn_readlane(before, at)) * BM;
+  t.end = __builtin_amdgcn_readlane(end, at);
+  return true;
+}
+template <int BM>
+__device__ __forceinline__ bool find_tile(const GroupedArgs& p, int idx, int lane, RowTile& t) {
+  return p.E <= 64 ? find_tile<BM, 1>(p, idx, lane, t) : find_tile<BM, GP_MAX_E / 64>(p, idx, lane, t);
+}
+
+// The most tiles of BM rows that R rows over E experts can need.
+static int64_t most_tiles(int64_t R, int64_t E, int64_t BM) {
+  const int64_t used = R < E ? R : E;
+  return used + (R - used) / BM;
+}
+
+__device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
+  return p.bias_dtype == AQ_BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(p.bias)[i]) : static_cast<const float*>(p.bias)[i];
+}
+template <int OUT>
+__device__ __forceinline__ void store_out(void* y, int64_t i, float v) {
+  if constexpr (OUT == OUT_BF16) static_cast<uint16_t*>(y)[i] = (uint16_t)f32_to_bf16_bits(v);
+  else static_cast<float*>(y)[i] = v;
+}
+template <int OUT>
+__device__ __forceinline__ float as_stored(float v) {
+  return OUT == OUT_BF16 ? bf16_bits_to_f32(f32_to_bf16_bits(v)) : v;
+}
+
+// Tiles of 16 rows x 32 weight rows: four wavefronts take every fourth 128-byte line of K, operands straight from memory into registers, the
+// sums meet in LDS.
+constexpr int GF_ROWS = 16, GF_COLS = 32, GF_WAVES = 4;
+template <int OUT, bool SWI>
+__global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs p) {
+  __shared__ int part[GF_WAVES][2][GF_ROWS][17];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  RowTile t;
+  if (!find_tile<GF_ROWS>(p, blockIdx.y, lane, t)) return;
+  const int K = p.K, FH = SWI ? p.N / 2 : p.N;
+  const int n0 = (int)blockIdx.x * (SWI ? 16 : GF_COLS);
+  const uint8_t* const w = p.w + t.e * p.w_bytes;
+  const __amdgpu_buffer_rsrc_t Wr = make_rsrc(w, (uint32_t)p.w_bytes), Xr = make_rsrc(p.x, (uint32_t)p.x_rows * (uint32_t)K);
+  const int r16 = lane & 15, q16 = (lane >> 4) * 16;
+  const int row = t.first + r16;
+  int tok = -1;
+  if (row < t.end) tok = p.tokens ? p.tokens[row] : row;
+  const bool live = tok >= 0 && tok < p.x_rows;
+  const uint32_t xo = (uint32_t)tok * (uint32_t)K + q16;
+  const int na = n0 + r16, nb = SWI ? FH + na : na + 16;
+  const bool ina = na < FH, inb = SWI ? ina : nb < FH;
+  const uint32_t ao = (uint32_t)na * (uint32_t)K + q16, bo = (uint32_t)nb * (uint32_t)K + q16;
+  v4i acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  const int lines = (K + 127) / 128;
+  constexpr int DEEP = 4;
+  for (int l0 = wave; l0 < lines; l0 += GF_WAVES * DEEP) {
+    v4i xv[2 * DEEP], av[2 * DEEP], bv[2 * DEEP];
+#pragma unroll
+    for (int i = 0; i < 2 * DEEP; ++i) {
+      const int k = (l0 + i / 2 * GF_WAVES) * 128 + i % 2 * 64;
+      const bool in = k + q16 < K;
+      av[i] = __builtin_amdgcn_raw_buffer_load_b128(Wr, in && ina ? ao + k : OOB_OFFSET, 0, 2);
+      bv[i] = __builtin_amdgcn_raw_buffer_load_b128(Wr, in && inb ? bo + k : OOB_OFFSET, 0, 2);
+      xv[i] = __builtin_amdgcn_raw_buffer_load_b128(Xr, in && live ? xo + k : OOB_OFFSET, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * DEEP; ++i) {
+      acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv[i], av[i], acc[0], 0, 0, 0);
+      acc[1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv[i], bv[i], acc[1], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[wave][g][(lane >> 4) * 4 + i][r16] = acc[g][i];
+  __syncthreads();
+  const int m = tid >> 4, c = tid & 15, out_row = t.first + m;
+  if (out_row >= t.end) return;
+  const int otok = p.tokens ? p.tokens[out_row] : out_row;
+  const float sx = otok >= 0 && otok < p.x_rows ? p.sx[otok] : 0.0f;
+  float y[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    int s = 0;
+#pragma unroll
+    for (int v = 0; v < GF_WAVES; ++v) s += part[v][g][m][c];
+    const int n = SWI ? g * FH + n0 + c : n0 + g * 16 + c;
+    if (n >= p.N) continue;
+    const int64_t at = (int64_t)t.e * p.N + n;
+    y[g] = __fmul_rn(__fmul_rn((float)s, sx), p.sw[at]);
+    if (p.bias) y[g] = __fadd_rn(y[g], load_bias(p, at));
+    if constexpr (!SWI) store_out<OUT>(p.y, (int64_t)out_row * p.N + n, y[g]);
+  }
+  if constexpr (SWI)
+    if (n0 + c < FH) store_out<OUT>(p.y, (int64_t)out_row * FH + n0 + c, swiglu_repro(as_stored<OUT>(y[0]), as_stored<OUT>(y[1])));
+}
+
+template <int OUT, bool SWI>
+static int launch_grouped(const GroupedArgs& a, hipStream_t st) {
+  const int64_t tiles = most_tiles(a.R, a.E, GF_ROWS), cols = (a.N + GF_COLS - 1) / GF_COLS;
+  if (tiles > 65535 || cols > 0x7fffffff) return AQ_E_RANGE;
+  queue_kernel((grouped_few_kernel<OUT, SWI>), dim3((unsigned)cols, (unsigned)tiles), dim3(GF_WAVES * 64), 0, st, a);
+  return (int)hipGetLastError();
+}
+
+static int grouped(const int8_t* xq, const float* sx, int64_t x_rows, const int8_t* wq, const float* sw, const void* bias, int bias_dtype,
+                   const int32_t* offsets, int64_t E, const int32_t* tokens, int64_t R, void* y, int y_dtype, int64_t N, int64_t K, bool swiglu,
+                   void* stream) {
+  if (y_dtype != AQ_F32 && y_dtype != AQ_BF16) return AQ_E_DTYPE;
+  if (bias && bias_dtype != AQ_F32 && bias_dtype != AQ_BF16) return AQ_E_DTYPE;
+  if (x_rows < 0 || E <= 0 || R < 0 || N <= 0 || K <= 0 || K % 16 || (!tokens && x_rows != R)) return AQ_E_SHAPE;
+  if (E > GP_MAX_E || R > 0x7fffffff || N > 0x7fffffff || N * K > (int64_t)OOB_OFFSET || x_rows * K > (int64_t)OOB_OFFSET) return AQ_E_RANGE;
+  if (R == 0) return AQ_OK;
+  if (!offsets || !wq || !sw || !y || (x_rows > 0 && (!xq || !sx))) return AQ_E_NULL;
+  if (check_ptr16(xq) || check_ptr16(wq) || check_ptr16(y) || check_ptr(sx, 4) || check_ptr(sw, 4) || check_ptr(offsets, 4) || check_ptr(tokens, 4) ||
+      check_ptr(bias, bias_dtype == AQ_BF16 ? 2 : 4))
+    return AQ_E_ALIGN;
+  GroupedArgs a{};
+  a.x = reinterpret_cast<const uint8_t*>(xq);
+  a.sx = sx;
+  a.w = reinterpret_cast<const uint8_t*>(wq);
+  a.sw = sw;
+  a.bias = bias;
+  a.bias_dtype = bias_dtype;
+  a.offsets = offsets;
+  a.tokens = tokens;
+  a.y = y;
+  a.w_bytes = N * K;
+  a.x_rows = (int)x_rows;
+  a.R = (int)R;
+  a.E = (int)E;
+  a.N = (int)N;
+  a.K = (int)K;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (swiglu) return y_dtype == AQ_BF16 ? launch_grouped<OUT_BF16, true>(a, st) : launch_grouped<OUT_F32, true>(a, st);
+  return y_dtype == AQ_BF16 ? launch_grouped<OUT_BF16, false>(a, st) : launch_grouped<OUT_F32, false>(a, st);
+}
+
+// Scratch of a whole layer: codes and scales of x, h (later the experts' outputs), codes and scales of h.
+struct ExpertsScratch {
+  int64_t xq, sx, h, hq, sh, bytes;
+  ExpertsScratch(int64_t T, int64_t R, int64_t dim, int64_t F, int size) {
+    auto take = [&](int64_t n) {
+      const int64_t at = bytes;
+      bytes += (n + 255) / 256 * 256;
+      return at;
+    };
+    bytes = 0;
+    xq = take(T * dim);
+    sx = take(T * 4);
+    h = take(R * (F > dim ? F : dim) * size);
+    hq = take(R * F);
+    sh = take(R * 4);
+  }
+};
+
+}  // namespace aq
+
+extern "C" int aq_linear_w8a8_grouped(const int8_t* xq, const float* sx, int64_t x_rows, const int8_t* wq, const float* sw, const void* bias,
+                                      int bias_dtype, const int32_t* offsets, int64_t E, const int32_t* tokens, int64_t R, void* y, int y_dtype,
+                                      int64_t N, int64_t K, void* stream) {
+  return aq::grouped(xq, sx, x_rows, wq, sw, bias, bias_dtype, offsets, E, tokens, R, y, y_dtype, N, K, false, stream);
+}
+
+extern "C" int aq_swiglu_w8a8_grouped(const int8_t* xq, const float* sx, int64_t x_rows, const int8_t* wq, const float* sw, const int32_t* offsets,
+                                      int64_t E, const int32_t* tokens, int64_t R, void* h, int h_dtype, int64_t F, int64_t K, void* stream) {
+  if (F <= 0 || F % 16) return AQ_E_SHAPE;
+  return aq::grouped(xq, sx, x_rows, wq, sw, nullptr, AQ_F32, offsets, E, tokens, R, h, h_dtype, 2 * F, K, true, stream);
+}
+
+extern "C" int64_t aq_experts_w8a8_workspace_bytes(int x_dtype, int64_t T, int64_t k, int64_t dim, int64_t F) {
+  if (T <= 0 || k <= 0 || dim <= 0 || F <= 0 || T > (int64_t)1 << 24 || k > 64 || dim > (1 << 24) || F > (1 << 24)) return 0;
+  return aq::ExpertsScratch(T, T * k, dim, F, x_dtype == AQ_BF16 ? 2 : 4).bytes;
+}
+
+extern "C" int aq_experts_w8a8(const void* x, int x_dtype, int64_t T, int64_t dim, const int32_t* offsets, int64_t E, const int32_t* tokens,
+                               const int32_t* rows, const float* weights, int64_t k, const int8_t* up_gate, const float* up_gate_scale,
+                               const int8_t* down, const float* down_scale, int64_t F, const void* residual, void* out, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+  if (x_dtype != AQ_F32 && x_dtype != AQ_BF16) return AQ_E_DTYPE;
+  if (T < 0 || dim <= 0 || dim % 16 || E <= 0 || k <= 0 || F <= 0 || F % 16) return AQ_E_SHAPE;
+  if (E > aq::GP_MAX_E || k > 64 || T > (int64_t)1 << 24 || dim > (1 << 24) || F > (1 << 24) || T * k * F > (int64_t)aq::OOB_OFFSET ||
+      T * dim > (int64_t)aq::OOB_OFFSET || 2 * F * dim > (int64_t)aq::OOB_OFFSET)
+    return AQ_E_RANGE;
+  if (T == 0) return AQ_OK;
+  if (!x || !offsets || !tokens || !rows || !weights || !up_gate || !up_gate_scale || !down || !down_scale || !out || !workspace) return AQ_E_NULL;
+  if (aq::check_ptr16(x) || aq::check_ptr16(up_gate) || aq::check_ptr16(down) || aq::check_ptr16(out) || aq::check_ptr16(workspace) ||
+      aq::check_ptr(up_gate_scale, 4) || aq::check_ptr(down_scale, 4) || aq::check_ptr(offsets, 4) ||
+      aq::check_ptr(tokens, 4) || aq::check_ptr(rows, 4) || aq::check_ptr(weights, 4))
+    return AQ_E_ALIGN;
+  if (workspace_bytes < aq_experts_w8a8_workspace_bytes(x_dtype, T, k, dim, F)) return AQ_E_WORKSPACE;
+  const int64_t R = T * k;
+  const aq::ExpertsScratch s(T, R, dim, F, x_dtype == AQ_BF16 ? 2 : 4);
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  int8_t *const xq = reinterpret_cast<int8_t*>(ws + s.xq), *const hq = reinterpret_cast<int8_t*>(ws + s.hq);
+  float *const sx = reinterpret_cast<float*>(ws + s.sx), *const sh = reinterpret_cast<float*>(ws + s.sh);
+  void* const h = ws + s.h;
+  int rc = aq_quant_rowwise_i8(x, x_dtype, T, dim, dim, xq, sx, stream);
+  if (rc == AQ_OK) rc = aq_swiglu_w8a8_grouped(xq, sx, T, up_gate, up_gate_scale, offsets, E, tokens, R, h, x_dtype, F, dim, stream);
+  if (rc == AQ_OK) rc = aq_quant_rowwise_i8(h, x_dtype, R, F, F, hq, sh, stream);
+  if (rc == AQ_OK) rc = aq_linear_w8a8_grouped(hq, sh, R, down, down_scale, nullptr, AQ_F32, offsets, E, nullptr, R, h, x_dtype, dim, F, stream);
+  if (rc == AQ_OK) rc = aq_combine_rows(h, x_dtype, R, dim, rows, weights, T, k, residual, out, stream);
+  return rc;
+}

@@ -78,7 +78,14 @@ namespace {
   X(aq_fork_pages_workspace_bytes)                                                                               \
   X(aq_fork_pages)                                                                                               \
   X(aq_compact_pages_workspace_bytes)                                                                            \
-  X(aq_compact_pages)
+  X(aq_compact_pages)                                                                                            \
+  X(aq_route_topk_workspace_bytes)                                                                               \
+  X(aq_route_topk)                                                                                               \
+  X(aq_linear_w8a8_grouped)                                                                                      \
+  X(aq_swiglu_w8a8_grouped)                                                                                      \
+  X(aq_combine_rows)                                                                                             \
+  X(aq_experts_w8a8_workspace_bytes)                                                                             \
+  X(aq_experts_w8a8)
 
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -553,6 +560,138 @@ PyObject* compact_pages(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                                 where.mutable_data_ptr<int64_t>(), live.mutable_data_ptr<int32_t>(), ws.mutable_data_ptr(), need, c.stream);
   });
   return rc ? fail(rc, "aq_compact_pages") : tuple_of({&table, &refs, &where, &live});
+  END_HANDLE_TH_ERRORS
+}
+
+// route_topk(logits, k, renormalize) -> (weights, experts, rows, tokens, offsets)
+PyObject* route_topk(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS AQ_ARGS(3);
+  const Tensor* x = unpack(args[0]);
+  Call c;
+  int64_t k;
+  if (!x || !c.at(*x) || act_code(x->scalar_type()) < 0 || !x->is_contiguous() || x->dim() != 2 || !whole(args[1], &k) || !PyBool_Check(args[2]))
+    return none();
+  const int64_t T = x->size(0), E = x->size(1);
+  if (k < 1 || k > E) return none();
+  c.current_stream();
+  const int64_t need = lib.aq_route_topk_workspace_bytes(T, E);
+  Tensor weights = c.empty({T, k}, ScalarType::Float), experts = c.empty({T, k}, ScalarType::Int), rows = c.empty({T, k}, ScalarType::Int),
+         tokens = c.empty({T * k}, ScalarType::Int), offsets = c.empty({E + 1}, ScalarType::Int), ws;
+  if (need) ws = c.empty({need}, ScalarType::Byte);
+  const int rc = queued([&] {
+    return lib.aq_route_topk(x->const_data_ptr(), act_code(x->scalar_type()), T, E, E, k, args[2] == Py_True, weights.mutable_data_ptr<float>(),
+                             experts.mutable_data_ptr<int32_t>(), rows.mutable_data_ptr<int32_t>(), tokens.mutable_data_ptr<int32_t>(),
+                             offsets.mutable_data_ptr<int32_t>(), need ? ws.mutable_data_ptr() : nullptr, need, c.stream);
+  });
+  return rc ? fail(rc, "aq_route_topk") : tuple_of({&weights, &experts, &rows, &tokens, &offsets});
+  END_HANDLE_TH_ERRORS
+}
+
+// stacked weight codes [E, N, K] of several experts and their scales [E, N]
+bool experts_of(PyObject* wq, PyObject* sw, int dev, const Tensor** w, const Tensor** s) {
+  *w = unpack(wq);
+  *s = unpack(sw);
+  return *w && *s && plain(**w, ScalarType::Char, dev) && plain(**s, ScalarType::Float, dev) && (*w)->dim() == 3 && (*s)->dim() == 2 &&
+         (*s)->size(0) == (*w)->size(0) && (*s)->size(1) == (*w)->size(1) && aligned16((*w)->const_data_ptr());
+}
+bool int32s(const Tensor* t, int64_t n, int dev) { return t && plain(*t, ScalarType::Int, dev) && t->numel() == n; }
+
+// linear_w8a8_grouped(xq, sx, wq, sw, offsets, tokens or None, bias or None, out_dtype) -> y, and (.., tokens or None, out_dtype) -> h
+PyObject* grouped(PyObject* const* args, bool swiglu) {
+  const Tensor *xq = unpack(args[0]), *sx = unpack(args[1]), *w, *s, *offsets = unpack(args[4]), *tokens = nullptr;
+  Call c;
+  ScalarType type;
+  if (!xq || !sx || !c.at(*xq) || !plain(*xq, ScalarType::Char, c.dev) || xq->dim() != 2 || !aligned16(xq->const_data_ptr()) ||
+      !plain(*sx, ScalarType::Float, c.dev) || sx->numel() != xq->size(0) || !experts_of(args[2], args[3], c.dev, &w, &s) ||
+      w->size(2) != xq->size(1) || !int32s(offsets, w->size(0) + 1, c.dev) || offsets->dim() != 1 || args[swiglu ? 6 : 7] == Py_None ||
+      !out_type(args[swiglu ? 6 : 7], ScalarType::Float, &type))
+    return none();
+  if (args[5] != Py_None) {
+    tokens = unpack(args[5]);
+    if (!tokens || !int32s(tokens, tokens->numel(), c.dev) || tokens->dim() != 1) return none();
+  }
+  const int64_t E = w->size(0), N = w->size(1), K = w->size(2), R = tokens ? tokens->numel() : xq->size(0);
+  if (K < 16 || K % 16 || N < 1 || (swiglu && N % 32)) return none();
+  const Tensor* bias = nullptr;
+  if (!swiglu && args[6] != Py_None) {
+    bias = unpack(args[6]);
+    if (!bias || act_code(bias->scalar_type()) < 0 || !plain(*bias, bias->scalar_type(), c.dev) || bias->dim() != 2 || bias->size(0) != E || bias->size(1) != N)
+      return none();
+  }
+  c.current_stream();
+  Tensor y = c.empty({R, swiglu ? N / 2 : N}, type);
+  const int rc = queued([&] {
+    const auto *xp = static_cast<const int8_t*>(xq->const_data_ptr()), *wp = static_cast<const int8_t*>(w->const_data_ptr());
+    const auto *sp = static_cast<const float*>(sx->const_data_ptr()), *vp = static_cast<const float*>(s->const_data_ptr());
+    const int32_t *op = offsets->const_data_ptr<int32_t>(), *tp = tokens ? tokens->const_data_ptr<int32_t>() : nullptr;
+    return swiglu ? lib.aq_swiglu_w8a8_grouped(xp, sp, xq->size(0), wp, vp, op, E, tp, R, y.mutable_data_ptr(), act_code(type), N / 2, K, c.stream)
+                  : lib.aq_linear_w8a8_grouped(xp, sp, xq->size(0), wp, vp, bias ? bias->const_data_ptr() : nullptr,
+                                               bias ? act_code(bias->scalar_type()) : AQ_F32, op, E, tp, R, y.mutable_data_ptr(), act_code(type), N, K,
+                                               c.stream);
+  });
+  return rc ? fail(rc, swiglu ? "aq_swiglu_w8a8_grouped" : "aq_linear_w8a8_grouped") : THPVariable_Wrap(y);
+}
+PyObject* linear_w8a8_grouped(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS AQ_ARGS(8);
+  return grouped(args, false);
+  END_HANDLE_TH_ERRORS
+}
+PyObject* swiglu_w8a8_grouped(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS AQ_ARGS(7);
+  return grouped(args, true);
+  END_HANDLE_TH_ERRORS
+}
+
+// combine_rows(y, rows, weights, residual or None) -> out
+PyObject* combine_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS AQ_ARGS(4);
+  const Tensor *y = unpack(args[0]), *rows = unpack(args[1]), *weights = unpack(args[2]);
+  Call c;
+  const void* res;
+  if (!y || !rows || !weights || !c.at(*y) || act_code(y->scalar_type()) < 0 || !plain(*y, y->scalar_type(), c.dev) || y->dim() != 2 ||
+      rows->dim() != 2 || !int32s(rows, rows->numel(), c.dev) || !plain(*weights, ScalarType::Float, c.dev) || weights->sizes() != rows->sizes())
+    return none();
+  const int64_t T = rows->size(0), k = rows->size(1), R = y->size(0), N = y->size(1);
+  if (N < 1 || !residual_of(args[3], T, N, y->scalar_type(), c.dev, &res)) return none();
+  c.current_stream();
+  Tensor out = c.empty({T, N}, y->scalar_type());
+  const int rc = queued([&] {
+    return lib.aq_combine_rows(y->const_data_ptr(), act_code(y->scalar_type()), R, N, rows->const_data_ptr<int32_t>(),
+                               weights->const_data_ptr<float>(), T, k, res, out.mutable_data_ptr(), c.stream);
+  });
+  return rc ? fail(rc, "aq_combine_rows") : THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// experts_w8a8(x, routing, up_gate, up_gate_scale, down, down_scale, residual or None) -> out
+PyObject* experts_w8a8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS AQ_ARGS(7);
+  const Tensor *x = unpack(args[0]), *ug, *us, *dw, *ds;
+  Call c;
+  const void* res;
+  if (!x || !c.at(*x) || act_code(x->scalar_type()) < 0 || !plain(*x, x->scalar_type(), c.dev) || x->dim() != 2 || !aligned16(x->const_data_ptr()) ||
+      !PyTuple_Check(args[1]) || PyTuple_GET_SIZE(args[1]) != 5 || !experts_of(args[2], args[3], c.dev, &ug, &us) ||
+      !experts_of(args[4], args[5], c.dev, &dw, &ds))
+    return none();
+  const int64_t T = x->size(0), dim = x->size(1), E = ug->size(0), F = dw->size(2);
+  const Tensor *weights = unpack(PyTuple_GET_ITEM(args[1], 0)), *rows = unpack(PyTuple_GET_ITEM(args[1], 2)),
+               *tokens = unpack(PyTuple_GET_ITEM(args[1], 3)), *offsets = unpack(PyTuple_GET_ITEM(args[1], 4));
+  if (T < 1 || dim < 16 || dim % 16 || F < 16 || F % 16 || ug->size(1) != 2 * F || ug->size(2) != dim || dw->size(0) != E || dw->size(1) != dim ||
+      !rows || rows->dim() != 2 || rows->size(0) != T || !int32s(rows, rows->numel(), c.dev) || !weights ||
+      !plain(*weights, ScalarType::Float, c.dev) || weights->sizes() != rows->sizes() || !int32s(tokens, rows->numel(), c.dev) ||
+      tokens->dim() != 1 || !int32s(offsets, E + 1, c.dev) || offsets->dim() != 1 || !residual_of(args[6], T, dim, x->scalar_type(), c.dev, &res))
+    return none();
+  c.current_stream();
+  const int64_t k = rows->size(1), need = lib.aq_experts_w8a8_workspace_bytes(act_code(x->scalar_type()), T, k, dim, F);
+  Tensor out = c.empty({T, dim}, x->scalar_type()), ws = c.empty({need}, ScalarType::Byte);
+  const int rc = queued([&] {
+    return lib.aq_experts_w8a8(x->const_data_ptr(), act_code(x->scalar_type()), T, dim, offsets->const_data_ptr<int32_t>(), E,
+                               tokens->const_data_ptr<int32_t>(), rows->const_data_ptr<int32_t>(), weights->const_data_ptr<float>(), k,
+                               static_cast<const int8_t*>(ug->const_data_ptr()), static_cast<const float*>(us->const_data_ptr()),
+                               static_cast<const int8_t*>(dw->const_data_ptr()), static_cast<const float*>(ds->const_data_ptr()), F, res,
+                               out.mutable_data_ptr(), ws.mutable_data_ptr(), need, c.stream);
+  });
+  return rc ? fail(rc, "aq_experts_w8a8") : THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
 
@@ -1250,6 +1389,11 @@ PyMethodDef methods[] = {
     AQ_METHOD(paged_attn_decode_shared),
     AQ_METHOD(fork_pages),
     AQ_METHOD(compact_pages),
+    AQ_METHOD(route_topk),
+    AQ_METHOD(linear_w8a8_grouped),
+    AQ_METHOD(swiglu_w8a8_grouped),
+    AQ_METHOD(combine_rows),
+    AQ_METHOD(experts_w8a8),
     AQ_METHOD(block_forward),
     {nullptr, nullptr, 0, nullptr},
 };

@@ -936,6 +936,190 @@ def compact_pages(page_table: torch.Tensor, refs: torch.Tensor, k_layers: torch.
     return CompactedPages(table, counts, where, live)
 
 
+class Routing(NamedTuple):
+    """What ``route_topk`` gives for ``T`` tokens and ``k`` choices each: the weights (float32 ``[T, k]``) and the experts (int32 ``[T, k]``, -1: none),
+    and the choices in the experts' order: expert e has rows ``offsets[e] .. offsets[e + 1] - 1`` (int32 ``[E + 1]``), ``rows`` (int32 ``[T, k]``) is the row of
+    each choice (-1: none) and ``tokens`` (int32 ``[T k]``) the token of each row (-1 past the last one in use)."""
+    weights: torch.Tensor
+    experts: torch.Tensor
+    rows: torch.Tensor
+    tokens: torch.Tensor
+    offsets: torch.Tensor
+
+
+def _int32(t: torch.Tensor, shape, what: str) -> torch.Tensor:
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    return t.contiguous()
+
+
+def route_topk(logits: torch.Tensor, k: int, renormalize: bool = True) -> Routing:
+    """Experts of each token from the router's logits ``[T, E]`` (float32 or bfloat16): the ``k`` largest, the largest first, equal ones the lowest
+    expert first.  Weights are the softmax over the chosen logits, or over all ``E`` with ``renormalize=False``.  -inf and NaN are never
+    chosen: a token with fewer than ``k`` other logits (a padded one: all -inf) has -1 and weight 0 in the places left.  The choices are sorted by
+    expert on the device (by token inside an expert), so that no call waits to learn how many each got.  ``E`` at most 512, ``k`` at most 16.
+    (DeepSeekMoE.forward, mlp.py:72-82, takes the top k of the probabilities rounded to the activations' type, whose ties have no order.)"""
+    r = (_host or _native()).route_topk(logits, k, renormalize)
+    if r is not None:
+        return Routing(*r)
+    _need_gpu(logits)
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [T, E], got {list(logits.shape)}")
+    code, (T, E), k, dev = _dt(logits, "logits"), logits.shape, int(k), logits.device
+    if E > 1 and logits.stride(1) != 1 or T > 1 and logits.stride(0) < E:
+        logits = logits.contiguous()
+    if not 0 < k <= E:
+        raise ValueError(f"k must be 1 .. {E}, got {k}")
+    weights = torch.empty((T, k), dtype=torch.float32, device=dev)
+    experts, rows = (torch.empty((T, k), dtype=torch.int32, device=dev) for _ in range(2))
+    tokens = torch.empty((T * k,), dtype=torch.int32, device=dev)
+    offsets = torch.empty((E + 1,), dtype=torch.int32, device=dev)
+    lib = _abi.load()
+    ws = torch.empty((lib.aq_route_topk_workspace_bytes(T, E),), dtype=torch.uint8, device=dev)
+    with _OnDevice(dev):
+        rc = lib.aq_route_topk(logits.data_ptr(), code, T, E, logits.stride(0) if T > 1 else E, k, int(bool(renormalize)), weights.data_ptr(),
+                               experts.data_ptr(), rows.data_ptr(), tokens.data_ptr(), offsets.data_ptr(), ws.data_ptr(), ws.numel(), _stream(logits))
+    _abi.check(rc, "aq_route_topk")
+    return Routing(weights, experts, rows, tokens, offsets)
+
+
+def _grouped_args(xq, sx, wq, sw, offsets, tokens, what):
+    """Checked operands of a grouped product -> (xq, sx, wq, sw, offsets, tokens, rows)."""
+    _need_gpu(xq, sx, wq, sw, offsets, tokens)
+    if xq.dtype != torch.int8 or xq.dim() != 2 or wq.dtype != torch.int8 or wq.dim() != 3 or wq.shape[2] != xq.shape[1]:
+        raise ValueError(f"{what}: xq must be int8 [rows, K] and wq int8 [E, N, K]")
+    _check_k(xq.shape[1])
+    if sx.dtype != torch.float32 or sx.numel() != xq.shape[0] or sw.dtype != torch.float32 or tuple(sw.shape) != tuple(wq.shape[:2]):
+        raise ValueError(f"{what}: scales must be float32, a number per row of xq and per row of each expert's weight")
+    offsets = _int32(offsets, (wq.shape[0] + 1,), f"{what}: offsets")
+    if tokens is not None:
+        if tokens.dim() != 1:
+            raise ValueError(f"{what}: tokens must be int32 [R]")
+        tokens = _int32(tokens, tokens.shape, f"{what}: tokens")
+    return (xq.contiguous(), sx.contiguous(), wq.contiguous(), sw.contiguous(), offsets, tokens,
+            xq.shape[0] if tokens is None else tokens.numel())
+
+
+def linear_w8a8_grouped(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, offsets: torch.Tensor,
+                        tokens: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                        out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``linear_w8a8`` of several experts at once, ``wq`` int8 ``[E, N, K]``, ``sw`` ``[E, N]``, ``bias`` ``[E, N]``: rows ``offsets[e] .. offsets[e + 1] - 1``
+    (int32 ``[E + 1]``, on the device; a group may be empty) of the result ``[R, N]`` are expert e's Linear on rows ``tokens[r]`` (int32 ``[R]``) of ``xq`` ``[T, K]``, or,
+    without ``tokens``, on the same rows of ``xq`` ``[R, K]``: the bits of the single calls.  Rows past ``offsets[E]`` are not written.  A token
+    outside ``0 .. T - 1`` counts as a row of zeros.  ``E`` at most 512."""
+    y = (_host or _native()).linear_w8a8_grouped(xq, sx, wq, sw, offsets, tokens, bias, out_dtype)
+    if y is not None:
+        return y
+    xq, sx, wq, sw, offsets, tokens, R = _grouped_args(xq, sx, wq, sw, offsets, tokens, "linear_w8a8_grouped")
+    E, N, K = wq.shape
+    if out_dtype not in _DT:
+        raise ValueError(f"out_dtype {out_dtype} is not supported (float32 or bfloat16)")
+    bias_ptr, bias_dt = None, _abi.AQ_F32
+    if bias is not None:
+        _need_gpu(xq, bias)
+        if tuple(bias.shape) != (E, N):
+            raise ValueError(f"bias must be [{E}, {N}], got {list(bias.shape)}")
+        bias = bias.contiguous()
+        bias_ptr, bias_dt = bias.data_ptr(), _dt(bias, "bias")
+    y = torch.empty((R, N), dtype=out_dtype, device=xq.device)
+    with _OnDevice(xq.device):
+        rc = _abi.load().aq_linear_w8a8_grouped(xq.data_ptr(), sx.data_ptr(), xq.shape[0], wq.data_ptr(), sw.data_ptr(), bias_ptr, bias_dt,
+                                                offsets.data_ptr(), E, None if tokens is None else tokens.data_ptr(), R, y.data_ptr(),
+                                                _DT[out_dtype], N, K, _stream(xq))
+    _abi.check(rc, "aq_linear_w8a8_grouped")
+    return y
+
+
+def swiglu_w8a8_grouped(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, offsets: torch.Tensor,
+                        tokens: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``h = up * silu(gate)`` of several experts at once: ``wq`` int8 ``[E, 2F, K]`` is each expert's up on top of its gate, the rest as in
+    ``linear_w8a8_grouped``; up and gate are rounded to ``out_dtype`` first, as two Linears would have stored them (``gemv_w8a8_decode_swiglu``
+    does the same for one MLP).  Returns ``[R, F]``; ``F`` a multiple of 16."""
+    h = (_host or _native()).swiglu_w8a8_grouped(xq, sx, wq, sw, offsets, tokens, out_dtype)
+    if h is not None:
+        return h
+    xq, sx, wq, sw, offsets, tokens, R = _grouped_args(xq, sx, wq, sw, offsets, tokens, "swiglu_w8a8_grouped")
+    E, N, K = wq.shape
+    if N % 32:
+        raise ValueError(f"wq holds up and gate one on top of the other, of a multiple of 16 rows each: got {N} rows")
+    if out_dtype not in _DT:
+        raise ValueError(f"out_dtype {out_dtype} is not supported (float32 or bfloat16)")
+    h = torch.empty((R, N // 2), dtype=out_dtype, device=xq.device)
+    with _OnDevice(xq.device):
+        rc = _abi.load().aq_swiglu_w8a8_grouped(xq.data_ptr(), sx.data_ptr(), xq.shape[0], wq.data_ptr(), sw.data_ptr(), offsets.data_ptr(), E,
+                                                None if tokens is None else tokens.data_ptr(), R, h.data_ptr(), _DT[out_dtype], N // 2, K,
+                                                _stream(xq))
+    _abi.check(rc, "aq_swiglu_w8a8_grouped")
+    return h
+
+
+def combine_rows(y: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The experts' outputs back in the tokens' order: ``out[t] = sum_j weights[t, j] * y[rows[t, j]]`` (``y`` ``[R, N]``, ``rows`` int32 and ``weights``
+    float32 ``[T, k]``), plus ``residual[t]`` (what shared experts gave, or the residual stream), summed in fp32 in the order of j and rounded once.  Rows
+    outside ``0 .. R - 1`` (-1: no expert) count for nothing.  ``k`` at most 64."""
+    out = (_host or _native()).combine_rows(y, rows, weights, residual)
+    if out is not None:
+        return out
+    _need_gpu(y, rows, weights, residual)
+    if y.dim() != 2 or rows.dim() != 2:
+        raise ValueError("y must be [R, N] and rows [T, k]")
+    code, (R, N), (T, k) = _dt(y, "y"), y.shape, rows.shape
+    rows = _int32(rows, rows.shape, "rows")
+    if weights.dtype != torch.float32 or weights.shape != rows.shape:
+        raise ValueError(f"weights must be float32 [{T}, {k}]")
+    res = _residual_arg(residual, T, N, y.dtype, y.device)
+    y, weights = y.contiguous(), weights.contiguous()
+    out = torch.empty((T, N), dtype=y.dtype, device=y.device)
+    with _OnDevice(y.device):
+        rc = _abi.load().aq_combine_rows(y.data_ptr(), code, R, N, rows.data_ptr(), weights.data_ptr(), T, k,
+                                         None if res is None else res.data_ptr(), out.data_ptr(), _stream(y))
+    _abi.check(rc, "aq_combine_rows")
+    return out
+
+
+def experts_w8a8(x: torch.Tensor, routing: Routing, up_gate: torch.Tensor, up_gate_scale: torch.Tensor, down: torch.Tensor, down_scale: torch.Tensor,
+                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The routed experts' MLP on ``x`` ``[T, dim]``: each token's rows through its experts' up, gate, SwiGLU and down, weighted and summed
+    (``residual`` ``[T, dim]`` added).  ``up_gate`` int8 ``[E, 2F, dim]`` with scales ``[E, 2F]``, ``down`` int8 ``[E, dim, F]`` with scales ``[E, dim]``.  The bits of
+    ``quant_rowwise_i8``, ``swiglu_w8a8_grouped``, ``quant_rowwise_i8``, ``linear_w8a8_grouped`` and ``combine_rows`` one after the other (what
+    DeepSeekMoE.forward, mlp.py:83-91, does expert by expert), in one call that waits for nothing."""
+    out = (_host or _native()).experts_w8a8(x, routing, up_gate, up_gate_scale, down, down_scale, residual)
+    if out is not None:
+        return out
+    weights, _, rows, tokens, offsets = routing
+    _need_gpu(x, weights, rows, tokens, offsets, up_gate, up_gate_scale, down, down_scale, residual)
+    if x.dim() != 2:
+        raise ValueError(f"x must be [T, dim], got {list(x.shape)}")
+    code, (T, dim) = _dt(x, "x"), x.shape
+    _check_k(dim)
+    for w, what in ((up_gate, "up_gate"), (down, "down")):
+        if w.dtype != torch.int8 or w.dim() != 3:
+            raise ValueError(f"{what} must be int8 [E, out, in]")
+    E, F = up_gate.shape[0], down.shape[2]
+    if tuple(up_gate.shape) != (E, 2 * F, dim) or tuple(down.shape) != (E, dim, F) or F % 16:
+        raise ValueError(f"up_gate must be [E, 2F, {dim}] and down [E, {dim}, F] with F a multiple of 16, got {list(up_gate.shape)} and {list(down.shape)}")
+    for s, w, what in ((up_gate_scale, up_gate, "up_gate_scale"), (down_scale, down, "down_scale")):
+        if s.dtype != torch.float32 or tuple(s.shape) != tuple(w.shape[:2]):
+            raise ValueError(f"{what} must be float32 {list(w.shape[:2])}")
+    if rows.dim() != 2 or rows.shape[0] != T:
+        raise ValueError(f"the routing is not of {T} tokens")
+    k = rows.shape[1]
+    rows, tokens, offsets = _int32(rows, (T, k), "rows"), _int32(tokens, (T * k,), "tokens"), _int32(offsets, (E + 1,), "offsets")
+    if weights.dtype != torch.float32 or tuple(weights.shape) != (T, k):
+        raise ValueError(f"weights must be float32 [{T}, {k}]")
+    res = _residual_arg(residual, T, dim, x.dtype, x.device)
+    x, weights, up_gate, up_gate_scale, down, down_scale = (t.contiguous() for t in (x, weights, up_gate, up_gate_scale, down, down_scale))
+    out = torch.empty_like(x)
+    lib = _abi.load()
+    ws = torch.empty((lib.aq_experts_w8a8_workspace_bytes(code, T, k, dim, F),), dtype=torch.uint8, device=x.device)
+    with _OnDevice(x.device):
+        rc = lib.aq_experts_w8a8(x.data_ptr(), code, T, dim, offsets.data_ptr(), E, tokens.data_ptr(), rows.data_ptr(), weights.data_ptr(), k,
+                                 up_gate.data_ptr(), up_gate_scale.data_ptr(), down.data_ptr(), down_scale.data_ptr(), F,
+                                 None if res is None else res.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(x))
+    _abi.check(rc, "aq_experts_w8a8")
+    return out
+
+
 def linear_fp8(xq, sx, wq, sw, bias=None, out_dtype=torch.bfloat16, residual=None) -> torch.Tensor:
     """FP8 e4m3fn GEMM with fp32 accumulation: y = (acc * sx[0]) * sw[0] (+ bias), cast, (+ residual)."""
     y = (_host or _native()).linear_fp8(xq, sx, wq, sw, bias, out_dtype, residual)
