@@ -113,6 +113,7 @@ SYMBOLS = {
 LAB_LIB_PATH = os.path.join(_HERE, "lib", "libastrai_q_lab.so")
 LAB_SYMBOLS = {
     "aq_lab_set_gemm_tile": (_int, [_int]),
+    "aq_lab_set_grouped_kernel": (_int, [_int]),
     "aq_lab_choose_gemm_tile": (_int, [_i64, _i64, _i64, _int, _int, _int, _int]),
     "aq_lab_probe_mfma": (_int, [_int, _int, _int, _int, _vp, _vp, _vp]),
     "aq_lab_probe_copy": (_int, [_vp, _vp, _i64, _int, _vp]),
@@ -195,6 +196,7 @@ class lab_library:
     def __exit__(self, *exc):
         global _lib
         _lib.aq_lab_set_gemm_tile(0)
+        _lib.aq_lab_set_grouped_kernel(0)
         _lib = self._saved
         host().bind(_lib._handle)
         return False

@@ -1,0 +1,64 @@
+// What the grouped products (one Linear per expert, ragged rows) share.
+#ifndef AQ_GROUPED_H
+#define AQ_GROUPED_H
+
+#include "aq_gemm.h"
+
+namespace aq {
+
+constexpr int GP_MAX_E = 512;
+constexpr int64_t GP_MAX_R = 1 << 25;  // counts of tiles fit 31 bits, whatever the offsets say
+
+struct GroupedArgs {
+  const uint8_t* x;
+  const float* sx;
+  const uint8_t* w;
+  const float* sw;
+  const void* bias;
+  int bias_dtype;
+  const int32_t* offsets;
+  const int32_t* tokens;
+  void* y;
+  int64_t w_bytes;  // of one expert
+  int x_rows, R, E;
+  int N;            // weight rows of an expert (SwiGLU: up and gate)
+  int K;
+};
+
+// Inclusive sum over the 64 lanes
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1 and so on
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+}
+
+// The most tiles of BM rows that R rows over E experts can need.
+inline int64_t grouped_most_tiles(int64_t R, int64_t E, int64_t BM) {
+  const int64_t used = R < E ? R : E;
+  return used + (R - used) / BM;
+}
+
+// up silu(gate) of fp32 projections, which are rounded to the output's type first.  fp32: the layer's frozen arithmetic.  bf16: the hardware's
+// exponential and reciprocal, 1 step of fp32 each, for a result that is rounded to 2^-8; the difference is below 2^-16 and the exponential's
+// argument its largest part.  (The frozen form takes 35 operations, and the epilogue of a tile of K = 2048 then half as long as its products.)
+template <int OUT>
+__device__ __forceinline__ float grouped_swiglu(float up, float gate) {
+  if constexpr (OUT == OUT_F32) {
+    return swiglu_repro(up, gate);
+  } else {
+    const uint32_t pair = pack_bf16x2(up, gate);
+    const float u = __uint_as_float(pair << 16), g = __uint_as_float(pair & 0xffff0000u);
+    return u * (g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896341f)));
+  }
+}
+
+// grouped_walk.hip
+template <int OUT, bool SWI>
+int grouped_walk_launch(const GroupedArgs& a, hipStream_t st);
+
+}  // namespace aq
+
+#endif  // AQ_GROUPED_H

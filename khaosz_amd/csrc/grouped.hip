@@ -4,27 +4,11 @@
 //
 // The groups' sizes are known on the device alone.  A launch has workgroups for the most tiles of rows that any split of R rows over
 // E experts can need; each finds its own by a scan over the offsets, and those past the last one end.
-#include "aq_gemm.h"
+#include <cmath>
+
+#include "aq_grouped.h"
 
 namespace aq {
-
-constexpr int GP_MAX_E = 512;
-
-struct GroupedArgs {
-  const uint8_t* x;
-  const float* sx;
-  const uint8_t* w;
-  const float* sw;
-  const void* bias;
-  int bias_dtype;
-  const int32_t* offsets;
-  const int32_t* tokens;
-  void* y;
-  int64_t w_bytes;  // of one expert
-  int x_rows, R, E;
-  int N;            // weight rows of an expert (SwiGLU: up and gate)
-  int K;
-};
 
 struct RowTile {
   int e, first, end;  // rows first .. end - 1; end of the expert's rows
@@ -48,13 +32,7 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs& p, int idx, int lan
     mine[i] = rows > 0 ? (rows + BM - 1) / BM : 0;
     n += mine[i];
   }
-  int upto = n;
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xf, 0xf, false);
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xf, 0xf, false);
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xf, 0xf, false);
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xf, 0xf, false);
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x142, 0xa, 0xf, false);
-  upto += __builtin_amdgcn_update_dpp(0, upto, 0x143, 0xc, 0xf, false);
+  const int upto = wave_scan(n);
   const unsigned long long past = __ballot(upto > idx);
   if (!past) return false;
   const int at = __builtin_ctzll(past);
@@ -73,12 +51,6 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs& p, int idx, int lan
   return p.E <= 64 ? find_tile<BM, 1>(p, idx, lane, t) : find_tile<BM, GP_MAX_E / 64>(p, idx, lane, t);
 }
 
-// The most tiles of BM rows that R rows over E experts can need.
-static int64_t most_tiles(int64_t R, int64_t E, int64_t BM) {
-  const int64_t used = R < E ? R : E;
-  return used + (R - used) / BM;
-}
-
 __device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
   return p.bias_dtype == AQ_BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(p.bias)[i]) : static_cast<const float*>(p.bias)[i];
 }
@@ -87,11 +59,6 @@ __device__ __forceinline__ void store_out(void* y, int64_t i, float v) {
   if constexpr (OUT == OUT_BF16) static_cast<uint16_t*>(y)[i] = (uint16_t)f32_to_bf16_bits(v);
   else static_cast<float*>(y)[i] = v;
 }
-template <int OUT>
-__device__ __forceinline__ float as_stored(float v) {
-  return OUT == OUT_BF16 ? bf16_bits_to_f32(f32_to_bf16_bits(v)) : v;
-}
-
 // Tiles of 16 rows x 32 weight rows: four wavefronts take every fourth 128-byte line of K, operands straight from memory into registers, the
 // sums meet in LDS.
 constexpr int GF_ROWS = 16, GF_COLS = 32, GF_WAVES = 4;
@@ -156,12 +123,29 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
     if constexpr (!SWI) store_out<OUT>(p.y, (int64_t)out_row * p.N + n, y[g]);
   }
   if constexpr (SWI)
-    if (n0 + c < FH) store_out<OUT>(p.y, (int64_t)out_row * FH + n0 + c, swiglu_repro(as_stored<OUT>(y[0]), as_stored<OUT>(y[1])));
+    if (n0 + c < FH) store_out<OUT>(p.y, (int64_t)out_row * FH + n0 + c, grouped_swiglu<OUT>(y[0], y[1]));
+}
+
+#ifdef AQ_LAB
+static int g_forced_grouped = 0;  // lab build only: 0 = by size
+#endif
+
+// Which kernel: walked tiles where they are at least 7 to 4 compute units (R rows dealt out evenly reach E (1 - e^(-R / E)) experts), or where experts
+// have more rows than the tile of 16.
+enum { GROUPED_FEW = 1, GROUPED_WALK = 2 };
+static int choose_grouped(const GroupedArgs& a) {
+  if (a.N > (1 << 20)) return GROUPED_FEW;  // (a tile's rows by 32-bit offsets)
+#ifdef AQ_LAB
+  if (g_forced_grouped) return g_forced_grouped;
+#endif
+  const double used = a.E * (1.0 - std::exp(-(double)a.R / a.E));
+  return used * ((a.N + 255) / 256) >= 1.75 * device_cus() || a.R > 24 * a.E ? GROUPED_WALK : GROUPED_FEW;
 }
 
 template <int OUT, bool SWI>
 static int launch_grouped(const GroupedArgs& a, hipStream_t st) {
-  const int64_t tiles = most_tiles(a.R, a.E, GF_ROWS), cols = (a.N + GF_COLS - 1) / GF_COLS;
+  if (choose_grouped(a) == GROUPED_WALK) return grouped_walk_launch<OUT, SWI>(a, st);
+  const int64_t tiles = grouped_most_tiles(a.R, a.E, GF_ROWS), cols = (a.N + GF_COLS - 1) / GF_COLS;
   if (tiles > 65535 || cols > 0x7fffffff) return AQ_E_RANGE;
   queue_kernel((grouped_few_kernel<OUT, SWI>), dim3((unsigned)cols, (unsigned)tiles), dim3(GF_WAVES * 64), 0, st, a);
   return (int)hipGetLastError();
@@ -173,7 +157,7 @@ static int grouped(const int8_t* xq, const float* sx, int64_t x_rows, const int8
   if (y_dtype != AQ_F32 && y_dtype != AQ_BF16) return AQ_E_DTYPE;
   if (bias && bias_dtype != AQ_F32 && bias_dtype != AQ_BF16) return AQ_E_DTYPE;
   if (x_rows < 0 || E <= 0 || R < 0 || N <= 0 || K <= 0 || K % 16 || (!tokens && x_rows != R)) return AQ_E_SHAPE;
-  if (E > GP_MAX_E || R > 0x7fffffff || N > 0x7fffffff || N * K > (int64_t)OOB_OFFSET || x_rows * K > (int64_t)OOB_OFFSET) return AQ_E_RANGE;
+  if (E > GP_MAX_E || R > GP_MAX_R || N > 0x7fffffff || N * K > (int64_t)OOB_OFFSET || x_rows * K > (int64_t)OOB_OFFSET) return AQ_E_RANGE;
   if (R == 0) return AQ_OK;
   if (!offsets || !wq || !sw || !y || (x_rows > 0 && (!xq || !sx))) return AQ_E_NULL;
   if (check_ptr16(xq) || check_ptr16(wq) || check_ptr16(y) || check_ptr(sx, 4) || check_ptr(sw, 4) || check_ptr(offsets, 4) || check_ptr(tokens, 4) ||
@@ -243,7 +227,7 @@ extern "C" int aq_experts_w8a8(const void* x, int x_dtype, int64_t T, int64_t di
                                int64_t workspace_bytes, void* stream) {
   if (x_dtype != AQ_F32 && x_dtype != AQ_BF16) return AQ_E_DTYPE;
   if (T < 0 || dim <= 0 || dim % 16 || E <= 0 || k <= 0 || F <= 0 || F % 16) return AQ_E_SHAPE;
-  if (E > aq::GP_MAX_E || k > 64 || T > (int64_t)1 << 24 || dim > (1 << 24) || F > (1 << 24) || T * k * F > (int64_t)aq::OOB_OFFSET ||
+  if (E > aq::GP_MAX_E || k > 64 || T > (int64_t)1 << 24 || dim > (1 << 24) || F > (1 << 24) || T * k > aq::GP_MAX_R || T * k * F > (int64_t)aq::OOB_OFFSET ||
       T * dim > (int64_t)aq::OOB_OFFSET || 2 * F * dim > (int64_t)aq::OOB_OFFSET)
     return AQ_E_RANGE;
   if (T == 0) return AQ_OK;
@@ -266,3 +250,11 @@ extern "C" int aq_experts_w8a8(const void* x, int x_dtype, int64_t T, int64_t di
   if (rc == AQ_OK) rc = aq_combine_rows(h, x_dtype, R, dim, rows, weights, T, k, residual, out, stream);
   return rc;
 }
+
+#ifdef AQ_LAB
+extern "C" int aq_lab_set_grouped_kernel(int kind) {
+  if (kind < 0 || kind > aq::GROUPED_WALK) return AQ_E_SHAPE;
+  aq::g_forced_grouped = kind;
+  return AQ_OK;
+}
+#endif

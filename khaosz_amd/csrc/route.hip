@@ -7,7 +7,7 @@
 // a workgroup's 64 tokens leave a bit each in a 64-bit word per expert (an OR: any order gives the same word), and the number of
 // bits below a token's own is its place among them.  No atomic whose order shows.
 // What bounds it: launches and chains of latencies; the bytes (10.5 MB for 16384 tokens of 256 experts) would take 2 us.
-#include "aq_common.h"
+#include "aq_grouped.h"
 
 namespace aq {
 
@@ -122,17 +122,6 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int t, int l, float* w
   const float chosen = row_sum(e);
   *weight = mine ? e / (a.renormalize ? chosen : total) : 0.0f;
   return mine ? K::expert(mine) : -1;
-}
-
-// Inclusive sum over the 64 lanes
-__device__ __forceinline__ int wave_scan(int v) {
-  auto add = [](int x, int y) { return x + y; };
-  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));  // row_shr:1 and so on
-  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
-  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
-  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
-  v = add(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // row_bcast:15
-  return add(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
 }
 
 // first[e] = total of the experts before e, for e <= E, by one wavefront

@@ -164,6 +164,18 @@ def _on(*ts):
     return tuple(None if t is None else t.to(DEV) for t in ts)
 
 
+@pytest.fixture(params=["by size", "rows of 16", "walked tiles"])
+def kernel(request):
+    """The kernel that the library takes for the sizes, and each of them whatever the sizes."""
+    from khaosz_amd import _abi
+    if request.param == "by size":
+        yield request.param
+        return
+    with _abi.lab_library() as lab:
+        assert lab.aq_lab_set_grouped_kernel({"rows of 16": 1, "walked tiles": 2}[request.param]) == 0
+        yield request.param
+
+
 GROUPS = {
     "one row": [1],
     "one expert": [37],
@@ -179,8 +191,8 @@ GROUPS = {
 
 @pytest.mark.parametrize("K,N", [(16, 1), (48, 33), (128, 64), (208, 100), (1408, 31), (512, 200), (1040, 257)])
 @pytest.mark.parametrize("groups", list(GROUPS))
-def test_grouped_linear_bits(groups, K, N):
-    _say("grouped linear", groups, K, N)
+def test_grouped_linear_bits(kernel, groups, K, N):
+    _say("grouped linear", kernel, groups, K, N)
     counts = GROUPS[groups]
     for tokens, dtype, bias in ((None, torch.bfloat16, None), (50, torch.float32, torch.float32), (3, torch.bfloat16, torch.bfloat16)):
         xq, sx, wq, sw, offsets, tok, b = _operands(counts, K, N, K + N, tokens, bias=bias)
@@ -192,9 +204,9 @@ def test_grouped_linear_bits(groups, K, N):
 
 
 @pytest.mark.parametrize("K,N", [(2048, 272), (4096, 96), (528, 514)])
-def test_grouped_linear_bits_many_rows(K, N):
+def test_grouped_linear_bits_many_rows(kernel, K, N):
     """Enough rows an expert for whole tiles of any kernel."""
-    _say("grouped linear, many rows", K, N)
+    _say("grouped linear, many rows", kernel, K, N)
     counts = [700, 0, 513, 260, 1, 256, 255, 1000]
     for tokens, dtype in ((None, torch.bfloat16), (777, torch.float32)):
         xq, sx, wq, sw, offsets, tok, b = _operands(counts, K, N, K, tokens, bias=torch.float32)
@@ -214,7 +226,7 @@ def test_grouped_linear_is_the_single_linear():
             assert torch.equal(got[lo:hi], ops.linear_w8a8(xq[at], sx[at], wq[e], sw[e], b[e]))
 
 
-def test_grouped_linear_largest_sums():
+def test_grouped_linear_largest_sums(kernel):
     """Codes of one sign throughout: sums of 4096 * 127^2, past what fp32 holds exactly."""
     xq, sx, wq, sw, offsets, tok, b = _operands([3, 20, 140], 4096, 40, 1, loud=True)
     want = _projections(xq, sx, wq, sw, offsets, tok, b).to(torch.float32)
@@ -222,7 +234,7 @@ def test_grouped_linear_largest_sums():
 
 
 @pytest.mark.parametrize("counts", [[2, 1, 0], [30, 200, 0]])
-def test_grouped_rows_behind_the_last_are_left_and_odd_tokens_are_zeros(counts):
+def test_grouped_rows_behind_the_last_are_left_and_odd_tokens_are_zeros(kernel, counts):
     from khaosz_amd import _abi
     R, live, K, N = sum(counts) + 37, sum(counts), 64, 48
     xq, sx, wq, sw, offsets, _, _ = _operands(counts, K, N, 9, 50)
@@ -249,7 +261,7 @@ def test_grouped_rows_behind_the_last_are_left_and_odd_tokens_are_zeros(counts):
             assert torch.equal(out.cpu()[keep], want[keep])
 
 
-def test_grouped_offsets_out_of_bounds_touch_nothing_else():
+def test_grouped_offsets_out_of_bounds_touch_nothing_else(kernel):
     """Offsets below 0, past R or falling are the caller's mistake: other rows and other memory stay as they are."""
     from khaosz_amd import _abi
     R, K, N = 40, 32, 16
@@ -265,10 +277,10 @@ def test_grouped_offsets_out_of_bounds_touch_nothing_else():
 
 @pytest.mark.parametrize("K,F", [(16, 16), (64, 48), (208, 112), (1536, 96), (1040, 272)])
 @pytest.mark.parametrize("groups", ["one row", "empty ends", "tile edges", "a large one", "200 experts"])
-def test_grouped_swiglu(groups, K, F):
+def test_grouped_swiglu(kernel, groups, K, F):
     """h is up silu(gate) of the projections as stored: off by the exponential's two steps, a sum, a quotient, a product (7 half steps of fp32; a
     bf16 result by a faster exponential, within 2^-16), and the rounding to the output's type."""
-    _say("grouped swiglu", groups, K, F)
+    _say("grouped swiglu", kernel, groups, K, F)
     for tokens, dtype in ((None, torch.bfloat16), (29, torch.float32)):
         xq, sx, wq, sw, offsets, tok, _ = _operands(GROUPS[groups], K, 2 * F, K + F, tokens)
         sw *= 30.0 / math.sqrt(K)  # gates from -50 to 50
