@@ -55,9 +55,9 @@ __device__ __forceinline__ float grouped_swiglu(float up, float gate) {
   }
 }
 
-// grouped_walk.hip
+// grouped_walk.hip: tiles of 128 rows and 256, 128 or 64 (not SwiGLU: 128) weight rows
 template <int OUT, bool SWI>
-int grouped_walk_launch(const GroupedArgs& a, hipStream_t st);
+int grouped_walk_launch(const GroupedArgs& a, int width, hipStream_t st);
 
 }  // namespace aq
 

@@ -21,8 +21,8 @@ extern "C" {
  * Process-wide and unsynchronised -- which is why it does not exist in the product library. */
 int aq_lab_set_gemm_tile(int rows);
 
-/* Forces the kernel of every later grouped product through the lab library: 1 (tiles of 16 rows), 2 (walked tiles of 128 x 256), 0 = by
- * size.  As above. */
+/* Forces the kernel of every later grouped product through the lab library: 1 (tiles of 16 rows), 2, 3, 4 (walked tiles of
+ * 128 rows x 256, 128, 64 weight rows), 0 = by size.  As above. */
 int aq_lab_set_grouped_kernel(int kind);
 
 /* The tile with which the library multiplies M x K by N x K codes (y_dtype AQ_F32, AQ_BF16, or -1 for int32 sums; residual: whether

@@ -132,19 +132,20 @@ static int g_forced_grouped = 0;  // lab build only: 0 = by size
 
 // Which kernel: walked tiles where they are at least 7 to 4 compute units (R rows dealt out evenly reach E (1 - e^(-R / E)) experts), or where experts
 // have more rows than the tile of 16.
-enum { GROUPED_FEW = 1, GROUPED_WALK = 2 };
+enum { GROUPED_FEW = 1, GROUPED_WALK_256 = 2, GROUPED_WALK_128 = 3, GROUPED_WALK_64 = 4 };
 static int choose_grouped(const GroupedArgs& a) {
   if (a.N > (1 << 20)) return GROUPED_FEW;  // (a tile's rows by 32-bit offsets)
 #ifdef AQ_LAB
   if (g_forced_grouped) return g_forced_grouped;
 #endif
   const double used = a.E * (1.0 - std::exp(-(double)a.R / a.E));
-  return used * ((a.N + 255) / 256) >= 1.75 * device_cus() || a.R > 24 * a.E ? GROUPED_WALK : GROUPED_FEW;
+  return used * ((a.N + 255) / 256) >= 1.75 * device_cus() || a.R > 24 * a.E ? GROUPED_WALK_256 : GROUPED_FEW;
 }
 
 template <int OUT, bool SWI>
 static int launch_grouped(const GroupedArgs& a, hipStream_t st) {
-  if (choose_grouped(a) == GROUPED_WALK) return grouped_walk_launch<OUT, SWI>(a, st);
+  const int kind = choose_grouped(a);
+  if (kind != GROUPED_FEW) return grouped_walk_launch<OUT, SWI>(a, kind == GROUPED_WALK_256 ? 256 : kind == GROUPED_WALK_128 ? 128 : 64, st);
   const int64_t tiles = grouped_most_tiles(a.R, a.E, GF_ROWS), cols = (a.N + GF_COLS - 1) / GF_COLS;
   if (tiles > 65535 || cols > 0x7fffffff) return AQ_E_RANGE;
   queue_kernel((grouped_few_kernel<OUT, SWI>), dim3((unsigned)cols, (unsigned)tiles), dim3(GF_WAVES * 64), 0, st, a);
@@ -253,7 +254,7 @@ extern "C" int aq_experts_w8a8(const void* x, int x_dtype, int64_t T, int64_t di
 
 #ifdef AQ_LAB
 extern "C" int aq_lab_set_grouped_kernel(int kind) {
-  if (kind < 0 || kind > aq::GROUPED_WALK) return AQ_E_SHAPE;
+  if (kind < 0 || kind > aq::GROUPED_WALK_64) return AQ_E_SHAPE;
   aq::g_forced_grouped = kind;
   return AQ_OK;
 }

@@ -164,7 +164,7 @@ def _on(*ts):
     return tuple(None if t is None else t.to(DEV) for t in ts)
 
 
-@pytest.fixture(params=["by size", "rows of 16", "walked tiles"])
+@pytest.fixture(params=["by size", "rows of 16", "walked 256", "walked 128", "walked 64"])
 def kernel(request):
     """The kernel that the library takes for the sizes, and each of them whatever the sizes."""
     from khaosz_amd import _abi
@@ -172,7 +172,7 @@ def kernel(request):
         yield request.param
         return
     with _abi.lab_library() as lab:
-        assert lab.aq_lab_set_grouped_kernel({"rows of 16": 1, "walked tiles": 2}[request.param]) == 0
+        assert lab.aq_lab_set_grouped_kernel({"rows of 16": 1, "walked 256": 2, "walked 128": 3, "walked 64": 4}[request.param]) == 0
         yield request.param
 
 
