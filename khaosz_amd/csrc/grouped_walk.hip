@@ -3,23 +3,24 @@
 //
 // Every workgroup takes the offsets into LDS, and a wavefront's lanes hold the running count of tiles, so that a tile's expert is two ballots
 // away.  Inside an expert tiles go in groups of 8 by rows, then by columns: the 32 tiles that an XCD works on at a time share 2 MB of rows and 2 MB of
-// weights.  The rows' tokens of the next tile are fetched into LDS under this tile's first step, for its first two stages are requested in the
-// last two.
+// weights.  The rows' tokens of the next tile are fetched into LDS under this tile's first step, for its first stages are requested in the
+// last steps.
 #include "aq_grouped.h"
 
 namespace aq {
 
 typedef int v2i_t __attribute__((ext_vector_type(2)));
 
-constexpr int GW_BM = 128, GW_BK = 128, GW_STAGES = 3, GW_THREADS = 512, GW_GROUP = 8;
+constexpr int GW_BM = 128, GW_BK = 128, GW_THREADS = 512, GW_GROUP = 8;
 
-// WM x WN wavefronts, each 32 TM rows by 32 TN weight rows of a tile of 128 x BN.
-template <int WM_, int TN_>
+// WM x WN wavefronts, each 32 TM rows by 32 TN weight rows of a tile of 128 x BN, K steps through NST stages.
+template <int WM_, int TN_, int NST_>
 struct GroupedShape {
-  static constexpr int WM = WM_, WN = 8 / WM_, TM = 4 / WM_, TN = TN_, BN = 32 * TN * WN;
+  static constexpr int WM = WM_, WN = 8 / WM_, TM = 4 / WM_, TN = TN_, BN = 32 * TN * WN, NST = NST_;
   static constexpr int STAGE = (GW_BM + BN) * GW_BK;
-  static constexpr int SX = GW_STAGES * STAGE, TOK = SX + 8 * 64 * 4, OFF = TOK + GW_BM * 4, LDS = OFF + (GP_MAX_E + 1) * 4;
+  static constexpr int SX = NST * STAGE, TOK = SX + 8 * 64 * 4, OFF = TOK + GW_BM * 4, LDS = OFF + (GP_MAX_E + 1) * 4;
   static_assert(LDS <= 160 * 1024, "LDS of one compute unit");
+  static_assert(NST >= 3, "a stage in use, one that lands, one on its way");
 };
 
 __device__ __forceinline__ void fetch_dword_to_lds(__amdgpu_buffer_rsrc_t r, void* to, uint32_t at) {
@@ -49,13 +50,15 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass drops a kernel in whose generic lambdas it finds the device's operations)
   __shared__ __attribute__((aligned(1024))) uint8_t smem[S::LDS];
   constexpr int BK = GW_BK, BN = S::BN, TM = S::TM, TN = S::TN, A_LOADS = GW_BM / 64, B_LOADS = BN / 64, NLOADS = A_LOADS + B_LOADS, NKS = 4;
+  constexpr int NST = S::NST, AHEAD = NST - 1;     // a step requests the stage that many steps on
+  constexpr int BEHIND = (NST - 2) * NLOADS;       // loads behind the next stage's when a step ends
   static_assert(!SWI || TN == 2, "up and gate in one lane");
   constexpr int V = SWI || TN == 1 ? 1 : 2;  // neighbouring outputs of a lane
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wave_m = wave / S::WN, wave_n = wave % S::WN;
   const int K = p.K, N = p.N, FH = SWI ? N / 2 : N;
-  const int steps = (K + BK - 1) / BK, nk = steps < 4 ? 4 : steps;  // (steps past K are of zeros)
+  const int steps = (K + BK - 1) / BK, nk = steps < 2 * AHEAD ? 2 * AHEAD : steps;  // (steps past K are of zeros)
   const int col = lane & 31, rq = (lane >> 5) * 4;
   float* const sx_lds = reinterpret_cast<float*>(smem + S::SX) + wave * 64;
   int32_t* const tok_lds = reinterpret_cast<int32_t*>(smem + S::TOK);
@@ -180,10 +183,10 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
   using l2 = std::integral_constant<int, NLOADS * 2 / 3>;
   using all = std::integral_constant<int, NLOADS>;
   int b_cur = 0;  // buffer of the current stage
-  // A K step of a tile with TMV accumulator rows: its first fragments are in af[0].  Requests the stage two steps on into the buffer that the
+  // A K step of a tile with TMV accumulator rows: its first fragments are in af[0].  Requests the stage AHEAD steps on into the buffer that the
   // step before left, and waits for the next one: `behind` says how.
   auto step = [&](auto tm_c, int k_ld, auto&& behind) {
-    const int b_next = b_cur == GW_STAGES - 1 ? 0 : b_cur + 1, b_prev = b_cur == 0 ? GW_STAGES - 1 : b_cur - 1;
+    const int b_next = b_cur == NST - 1 ? 0 : b_cur + 1, b_prev = b_cur == 0 ? NST - 1 : b_cur - 1;
     const uint8_t *st = smem + b_cur * S::STAGE, *st_next = smem + b_next * S::STAGE;
     slot(tm_c, c0{}, st, 1, k_ld, b_prev, c0{}, l1{});
     slot(tm_c, c1{}, st, 2, k_ld, b_prev, l1{}, l2{});
@@ -195,7 +198,7 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
     b_cur = b_next;
   };
   static_assert(NKS == 4, "four sub-steps");
-  auto landed = [&]() { AQ_WAIT_VMCNT(NLOADS); };  // nothing behind the next stage's loads but this step's own
+  auto landed = [&]() { AQ_WAIT_VMCNT(BEHIND); };  // nothing behind the next stage's loads but the later stages'
 
   WalkTile now = locate(id);
   if (gather) {
@@ -206,11 +209,11 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
   fr_a = fragments_of(now);
   int my_tok = token(now, first_row(now) + (lane & (32 * TM - 1)));  // of the row whose scale this lane fetches
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int s = 0; s < AHEAD; ++s)
 #pragma unroll
     for (int q = 0; q < NLOADS; ++q) issue_load(s * BK, s, q);
   __builtin_amdgcn_s_waitcnt(0xc07f);  // the tokens are read: the next tile's may come
-  AQ_WAIT_VMCNT(NLOADS);               // stage 0 has landed
+  AQ_WAIT_VMCNT(BEHIND);               // stage 0 has landed
   AQ_BARRIER();
 #pragma unroll
   for (int f = 0; f < TM + TN; ++f) load_frag(smem, 0, f, af[0], bf[0]);
@@ -231,17 +234,19 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
     const bool last = id >= count;
     WalkTile next = now;
     if (!last) next = locate(id);
-    // its tokens, 16 rows to a wavefront (one operation of each, counted below); they are there two steps on
+    // its tokens, 16 rows to a wavefront (one operation of each, counted below); they are there before step AHEAD
     if (lane < 16)
       fetch_dword_to_lds(Tr, tok_lds + wave * 16, (uint32_t)(next.first + wave * 16 + lane) * 4u);
-    int k0 = 2 * BK;
-    step(tm_c, k0, [&]() {  // behind the next stage's loads: the stores of the tile before, the tokens
-      if (stores == 2) AQ_WAIT_VMCNT(NLOADS + 1 + 2 * ROW_STORES);
-      else if (stores == 1) AQ_WAIT_VMCNT(NLOADS + 1 + ROW_STORES);
-      else AQ_WAIT_VMCNT(NLOADS + 1);
-    });
-    for (int s = 1; s < nk - 2; ++s) step(tm_c, k0 += BK, landed);
-    // the epilogue's operands, then the next tile's first two stages
+    int k0 = AHEAD * BK;
+#pragma unroll
+    for (int s = 0; s < NST - 2; ++s, k0 += BK)
+      step(tm_c, k0, [&]() {  // behind the next stage's loads: the stores of the tile before and the tokens, too
+        if (stores == 2) AQ_WAIT_VMCNT(BEHIND + 1 + 2 * ROW_STORES);
+        else if (stores == 1) AQ_WAIT_VMCNT(BEHIND + 1 + ROW_STORES);
+        else AQ_WAIT_VMCNT(BEHIND + 1);
+      });
+    for (int s = NST - 2; s < nk - AHEAD; ++s, k0 += BK) step(tm_c, k0, landed);
+    // the epilogue's operands, then the next tile's first stages
     const int mw = now.first + first_row(now), nt = now.n0, end = now.end;
     const int64_t scales = (int64_t)now.e * N;
     auto my_column = [&](int j) { return nt + (V == 2 ? wave_n * 64 + 2 * col + j : wave_n * 32 + col); };  // of h or y
@@ -274,8 +279,9 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
 #pragma unroll
       for (int i = 0; i < NLOADS; ++i) vo[i] = OOB_OFFSET;
     }
-    step(tm_c, 0, landed);
-    step(tm_c, BK, [&]() {
+#pragma unroll
+    for (int s = 0; s < AHEAD - 1; ++s) step(tm_c, s * BK, landed);
+    step(tm_c, (AHEAD - 1) * BK, [&]() {
       landed();
       fr_a = next_fr_a;  // (the fragments read behind this step's barrier are the next tile's)
     });
@@ -364,17 +370,17 @@ static int walk_launch(const GroupedArgs& a, hipStream_t st) {
   const int tiles_n = (a.N + S::BN - 1) / S::BN;
   const int64_t most = grouped_most_tiles(a.R, a.E, GW_BM) * tiles_n;
   if (most > 0x7fffffff) return AQ_E_RANGE;
-  const int64_t room = (int64_t)device_cus() * (S::LDS <= 80 * 1024 ? 2 : 1);
-  queue_kernel(grouped_walk_kernel<S, OUT, SWI>, dim3((unsigned)(most < room ? most : room)), dim3(GW_THREADS), 0, st, a, tiles_n,
+  const int cus = device_cus();
+  queue_kernel(grouped_walk_kernel<S, OUT, SWI>, dim3((unsigned)(most < cus ? most : cus)), dim3(GW_THREADS), 0, st, a, tiles_n,
                UDiv::of((uint32_t)tiles_n));
   return (int)hipGetLastError();
 }
 template <int OUT, bool SWI>
 int grouped_walk_launch(const GroupedArgs& a, int width, hipStream_t st) {
-  if (width == 256) return walk_launch<GroupedShape<2, 2>, OUT, SWI>(a, st);
+  if (width == 256) return walk_launch<GroupedShape<2, 2, 3>, OUT, SWI>(a, st);
   if constexpr (!SWI)
-    if (width == 64) return walk_launch<GroupedShape<4, 1>, OUT, SWI>(a, st);
-  return walk_launch<GroupedShape<4, 2>, OUT, SWI>(a, st);
+    if (width == 64) return walk_launch<GroupedShape<4, 1, 6>, OUT, SWI>(a, st);
+  return walk_launch<GroupedShape<4, 2, 4>, OUT, SWI>(a, st);
 }
 template int grouped_walk_launch<OUT_BF16, false>(const GroupedArgs&, int, hipStream_t);
 template int grouped_walk_launch<OUT_F32, false>(const GroupedArgs&, int, hipStream_t);
