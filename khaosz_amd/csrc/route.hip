@@ -7,24 +7,30 @@
 // a workgroup's 64 tokens leave a bit each in a 64-bit word per expert (an OR: any order gives the same word), and the number of
 // bits below a token's own is its place among them.  No atomic whose order shows.
 // What bounds it: launches and chains of latencies; the bytes (10.5 MB for 16384 tokens of 256 experts) would take 2 us.
+#include <type_traits>
+
 #include "aq_grouped.h"
 
 namespace aq {
 
-constexpr int RT_THREADS = 1024;
-constexpr int RT_TOKENS = RT_THREADS / 16;  // tokens of a pass: 16 lanes each, 64 of them
-constexpr int RT_ONE_PASSES = 4;            // passes of the kernel that does it all in one workgroup
+constexpr int RT_THREADS = 1024, RT_TOKENS = RT_THREADS / 16;  // a workgroup's tokens: 16 lanes each
+constexpr int RT_ONE_PASSES = 2;  // of the kernel that does it all in one workgroup (64 experts, 6 choices: 128 tokens 6.1 us, by two launches 6.7; 256 10.0 and 6.7)
+constexpr int RT_FEW_THREADS = 256, RT_FEW_TOKENS = RT_FEW_THREADS / 16, RT_FEW_T = 2048;  // up to RT_FEW_T tokens: more, smaller workgroups
 constexpr int RT_MAX_E = 512, RT_MAX_K = 16;
 constexpr int RT_MOST_CHUNKS = 512;  // larger batches: more passes to a chunk
-constexpr int RT_GROUP = 4;          // chunks of a workgroup that hands out rows
+constexpr int RT_GROUP = RT_TOKENS / RT_FEW_TOKENS;  // chunks of a workgroup that hands out rows, at most
 
 struct RouteArgs {
   const void* logits;
   int64_t ld;  // logits between tokens
   float* weights;
   int32_t *experts, *rows, *tokens, *offsets;
-  uint16_t* counts;  // [chunks][E]
+  uint16_t* counts;  // [chunks][pitch]
   int T, E, k, renormalize, passes, chunks;
+  int chunk;  // tokens of a chunk
+  int group;  // chunks of a workgroup that hands out rows
+  int pitch;  // of counts
+  int whole;  // lanes' runs of logits are whole, aligned vectors
 };
 
 typedef unsigned long long u64;
@@ -62,7 +68,21 @@ struct Key;
 template <>
 struct Key<true> {
   using type = uint32_t;
-  static __device__ __forceinline__ uint32_t load(const void* p, int64_t i) { return (uint32_t)static_cast<const uint16_t*>(p)[i] << 16; }
+  // logits l V .. l V + V - 1 of token t, as the bits of fp32; -inf behind the last
+  template <int V>
+  static __device__ __forceinline__ void load(const RouteArgs& a, int t, int l, uint32_t (&bits)[V]) {
+    const uint16_t* const p = static_cast<const uint16_t*>(a.logits) + (int64_t)t * a.ld + l * V;
+    if (a.whole && t < a.T) {
+#pragma unroll
+      for (int v = 0; v < V; v += 4) {
+        const uint2 q = *reinterpret_cast<const uint2*>(p + v);
+        bits[v] = q.x << 16, bits[v + 1] = q.x & 0xffff0000u, bits[v + 2] = q.y << 16, bits[v + 3] = q.y & 0xffff0000u;
+      }
+      return;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) bits[v] = t < a.T && l * V + v < a.E ? (uint32_t)p[v] << 16 : 0xff800000u;
+  }
   static __device__ __forceinline__ type make(uint32_t ordered, int e) { return (ordered & 0xffff0000u) | (0xffffu - (uint32_t)e); }
   static __device__ __forceinline__ int expert(type k) { return (int)(0xffffu - (k & 0xffffu)); }
   static __device__ __forceinline__ float value(type k) { return __uint_as_float((k >> 31 ? k ^ 0x80000000u : ~k) & 0xffff0000u); }
@@ -70,7 +90,20 @@ struct Key<true> {
 template <>
 struct Key<false> {
   using type = u64;
-  static __device__ __forceinline__ uint32_t load(const void* p, int64_t i) { return static_cast<const uint32_t*>(p)[i]; }
+  template <int V>
+  static __device__ __forceinline__ void load(const RouteArgs& a, int t, int l, uint32_t (&bits)[V]) {
+    const uint32_t* const p = static_cast<const uint32_t*>(a.logits) + (int64_t)t * a.ld + l * V;
+    if (a.whole && t < a.T) {
+#pragma unroll
+      for (int v = 0; v < V; v += 4) {
+        const uint4 q = *reinterpret_cast<const uint4*>(p + v);
+        bits[v] = q.x, bits[v + 1] = q.y, bits[v + 2] = q.z, bits[v + 3] = q.w;
+      }
+      return;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) bits[v] = t < a.T && l * V + v < a.E ? p[v] : 0xff800000u;
+  }
   static __device__ __forceinline__ type make(uint32_t ordered, int e) { return (u64)ordered << 32 | (0xffffu - (uint32_t)e); }
   static __device__ __forceinline__ int expert(type k) { return (int)(0xffffu - ((uint32_t)k & 0xffffu)); }
   static __device__ __forceinline__ float value(type k) {
@@ -79,30 +112,34 @@ struct Key<false> {
   }
 };
 
-// exp(x - most), most the largest of them: 1 for it, infinite or not
-__device__ __forceinline__ float exp_below(float x, float most) { return x == most ? 1.0f : expf(x - most); }
+// exp(x - most), most the largest of them: 1 for it, infinite or not.  2^(t log2 e), the product's rounding taken back to first order, by the hardware's
+// exponential (one step).
+__device__ __forceinline__ float exp_below(float x, float most) {
+  const float t = fmaxf(x - most, -150.0f);  // (2^-216 is 0)
+  const float y = t * 1.44269502e0f;
+  const float rest = __builtin_fmaf(t, 1.92596303e-8f, __builtin_fmaf(t, 1.44269502e0f, -y));
+  const float e = __builtin_amdgcn_exp2f(y);
+  return x == most ? 1.0f : __builtin_fmaf(e * 0.693147182f, rest, e);
+}
 
 // The choices of token t by the 16 lanes that hold it: lane j has choice j < k (expert -1: there is none) and its weight.
 template <bool BF16, int V>
 __device__ __forceinline__ int choose(const RouteArgs& a, int t, int l, float* weight) {
   using K = Key<BF16>;
-  typename K::type key[V];
+  using key_t = typename K::type;
+  key_t key[V];
+  uint32_t bits[V];
+  K::template load<V>(a, t, l, bits);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int e = v * 16 + l;
-    uint32_t bits = 0xff800000u;  // -inf
-    if (t < a.T && e < a.E) bits = K::load(a.logits, (int64_t)t * a.ld + e);
-    const float x = __uint_as_float(bits) + 0.0f;  // (-0 counts as 0)
+    const float x = __uint_as_float(bits[v]) + 0.0f;  // (-0 counts as 0)
     const uint32_t u = __float_as_uint(x);
-    key[v] = x > -__builtin_inff() ? K::make(u >> 31 ? ~u : u | 0x80000000u, e) : 0;
+    key[v] = x > -__builtin_inff() ? K::make(u >> 31 ? ~u : u | 0x80000000u, l * V + v) : 0;
   }
-  auto best = [&]() {
-    auto b = key[0];
+  key_t b = key[0], mine = 0;
 #pragma unroll
-    for (int v = 1; v < V; ++v) b = larger(b, key[v]);
-    return row_max(b);
-  };
-  typename K::type mine = 0, b = best();
+  for (int v = 1; v < V; ++v) b = larger(b, key[v]);
+  b = row_max(b);
   const float most = K::value(b);
   float total = 0.0f;
   if (!a.renormalize && b) {
@@ -111,12 +148,14 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int t, int l, float* w
       if (key[v]) total += exp_below(K::value(key[v]), most);
     total = row_sum(total);
   }
-  for (int j = 0; j < a.k; ++j) {
-    if (j) b = best();
+  for (int j = 0;;) {
     if (l == j) mine = b;
+    if (++j == a.k) break;
+    // the largest key below b: those that are not wrap around in the difference and come last
+    key_t d = key[0] - b;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (key[v] == b) key[v] = 0;
+    for (int v = 1; v < V; ++v) d = larger(d, key[v] - b);
+    b = b ? row_max(d) + b : 0;
   }
   const float e = mine ? exp_below(K::value(mine), most) : 0.0f;
   const float chosen = row_sum(e);
@@ -146,15 +185,16 @@ __device__ __forceinline__ void experts_scan(const uint32_t* counts, uint32_t* f
 
 // ONE: all tokens in one workgroup's passes, rows handed out at the end.  Otherwise a chunk of `passes` passes: the choices, each with its
 // place among the chunk's choices of its expert (in `rows` until the next launch), and the chunk's counts.
-template <bool BF16, int V, bool ONE>
-__global__ __launch_bounds__(RT_THREADS) void route_choose_kernel(RouteArgs a) {
+template <bool BF16, int V, int THREADS, bool ONE>
+__global__ __launch_bounds__(THREADS) void route_choose_kernel(RouteArgs a) {
+  constexpr int TOKENS = THREADS / 16;
   __shared__ u64 asked[RT_MAX_E];
   __shared__ uint32_t count[RT_MAX_E], first[RT_MAX_E + 1];
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, place = tid >> 4;
-  for (int e = tid; e < a.E; e += RT_THREADS) count[e] = 0;
+  for (int e = tid; e < a.E; e += THREADS) count[e] = 0;
   int chose[ONE ? RT_ONE_PASSES : 1], rank[ONE ? RT_ONE_PASSES : 1];
-  auto pass = [&](int i, int t, int& ce, int& cr) {
-    for (int e = tid; e < a.E; e += RT_THREADS) asked[e] = 0;
+  auto pass = [&](int t, int& ce, int& cr) {
+    for (int e = tid; e < a.E; e += THREADS) asked[e] = 0;
     float w;
     ce = choose<BF16, V>(a, t, l, &w);
     __syncthreads();
@@ -168,65 +208,77 @@ __global__ __launch_bounds__(RT_THREADS) void route_choose_kernel(RouteArgs a) {
       if constexpr (!ONE) a.rows[at] = cr;
     }
     __syncthreads();
-    for (int e = tid; e < a.E; e += RT_THREADS) count[e] += (uint32_t)__popcll(asked[e]);
+    for (int e = tid; e < a.E; e += THREADS) count[e] += (uint32_t)__popcll(asked[e]);
   };
   if constexpr (ONE) {
 #pragma unroll
     for (int i = 0; i < RT_ONE_PASSES; ++i) {
       chose[i] = rank[i] = -1;
-      if (i * RT_TOKENS < a.T) pass(i, i * RT_TOKENS + place, chose[i], rank[i]);
+      if (i * TOKENS < a.T) pass(i * TOKENS + place, chose[i], rank[i]);
     }
     __syncthreads();
     if (tid < 64) experts_scan(count, first, a.E, lane);
     __syncthreads();
-    for (int e = tid; e <= a.E; e += RT_THREADS) a.offsets[e] = (int32_t)first[e];
+    for (int e = tid; e <= a.E; e += THREADS) a.offsets[e] = (int32_t)first[e];
 #pragma unroll
     for (int i = 0; i < RT_ONE_PASSES; ++i) {
-      const int t = i * RT_TOKENS + place;
+      const int t = i * TOKENS + place;
       if (t < a.T && l < a.k) {
         const int r = chose[i] >= 0 ? (int)first[chose[i]] + rank[i] : -1;
         a.rows[t * a.k + l] = r;
         if (r >= 0) a.tokens[r] = t;
       }
     }
-    for (int r = (int)first[a.E] + tid; r < a.T * a.k; r += RT_THREADS) a.tokens[r] = -1;
+    for (int r = (int)first[a.E] + tid; r < a.T * a.k; r += THREADS) a.tokens[r] = -1;
   } else {
-    for (int i = 0; i < a.passes; ++i) pass(i, ((int)blockIdx.x * a.passes + i) * RT_TOKENS + place, chose[0], rank[0]);
+    for (int i = 0; i < a.passes; ++i) pass(((int)blockIdx.x * a.passes + i) * TOKENS + place, chose[0], rank[0]);
     __syncthreads();
-    for (int e = tid; e < a.E; e += RT_THREADS) a.counts[(int64_t)blockIdx.x * a.E + e] = (uint16_t)count[e];
+    for (int e = tid; e < a.E; e += THREADS) a.counts[(int64_t)blockIdx.x * a.pitch + e] = (uint16_t)count[e];
   }
 }
 
-// Rows for the choices of RT_GROUP chunks: the experts' first rows, the choices of the chunks before, the place among the chunk's.  Every
-// workgroup adds up all chunks' counts by itself.
+// Rows for the choices of a group of chunks: the experts' first rows, the choices of the chunks before, the place among the chunk's.  Every
+// workgroup adds up all chunks' counts by itself; its first choices (of 64 tokens: all there are) are on their way meanwhile.
 __global__ __launch_bounds__(RT_THREADS) void route_rows_kernel(RouteArgs a) {
   __shared__ uint32_t total[RT_MAX_E], before[RT_MAX_E], first[RT_MAX_E + 1], base[RT_GROUP][RT_MAX_E];
   const int tid = threadIdx.x, E = a.E;
-  const int c0 = (int)blockIdx.x * RT_GROUP;
+  const int c0 = (int)blockIdx.x * a.group;
+  const int64_t all = (int64_t)a.T * a.k, from = (int64_t)c0 * a.chunk * a.k;
+  const int64_t room = (int64_t)a.group * a.chunk * a.k, to = from + room < all ? from + room : all;
+  int64_t s = from + tid;
+  int expert = -1, place = 0;
+  if (s < to) expert = a.experts[s], place = a.rows[s];
   for (int e = tid; e < E; e += RT_THREADS) total[e] = before[e] = 0;
   __syncthreads();
-  int width = 64;  // threads to a run of experts
-  while (width < E) width *= 2;
-  const int e = tid & (width - 1), turns = RT_THREADS / width;
+  int width = 32;  // threads to a chunk's counts, two experts each
+  while (2 * width < E) width *= 2;
+  const int e = 2 * (tid & (width - 1)), turns = RT_THREADS / width;
   if (e < E) {
-    uint32_t all = 0, early = 0;
-#pragma unroll 8
+    uint32_t sum[2] = {0, 0}, early[2] = {0, 0};
+#pragma unroll 16
     for (int c = tid / width; c < a.chunks; c += turns) {
-      const uint32_t n = a.counts[(int64_t)c * E + e];
-      all += n;
-      early += c < c0 ? n : 0;
-      if (c >= c0 && c < c0 + RT_GROUP) base[c - c0][e] = n;
+      const uint32_t two = *reinterpret_cast<const uint32_t*>(a.counts + (int64_t)c * a.pitch + e);
+      const uint32_t n[2] = {two & 0xffffu, two >> 16};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sum[i] += n[i];
+        early[i] += c < c0 ? n[i] : 0;
+        if (c >= c0 && c < c0 + a.group && e + i < E) base[c - c0][e + i] = n[i];
+      }
     }
-    atomicAdd(&total[e], all);  // whole numbers: any order
-    atomicAdd(&before[e], early);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (e + i < E) {
+        atomicAdd(&total[e + i], sum[i]);  // whole numbers: any order
+        atomicAdd(&before[e + i], early[i]);
+      }
   }
   __syncthreads();
   if (tid < 64) experts_scan(total, first, E, tid);
   __syncthreads();
   for (int i = tid; i < E; i += RT_THREADS) {
     uint32_t at = first[i] + before[i];
-#pragma unroll
-    for (int c = 0; c < RT_GROUP; ++c) {
+    for (int c = 0; c < a.group; ++c) {
       const uint32_t n = base[c][i];
       base[c][i] = at;
       at += n;
@@ -235,17 +287,14 @@ __global__ __launch_bounds__(RT_THREADS) void route_rows_kernel(RouteArgs a) {
   __syncthreads();
   if (blockIdx.x == 0)
     for (int i = tid; i <= E; i += RT_THREADS) a.offsets[i] = (int32_t)first[i];
-  const int chunk = a.passes * RT_TOKENS, k = a.k;
-  const int64_t all = (int64_t)a.T * k;
-  for (int c = 0; c < RT_GROUP; ++c) {
-    const int64_t from = (int64_t)(c0 + c) * chunk * k, to = from + (int64_t)chunk * k < all ? from + (int64_t)chunk * k : all;
-    for (int64_t s = from + tid; s < to; s += RT_THREADS) {
-      const int ex = a.experts[s];
-      if (ex < 0) continue;
-      const int r = (int)base[c][ex] + a.rows[s];
+  while (s < to) {
+    if (expert >= 0) {
+      const int t = (int)((uint32_t)s / (uint32_t)a.k), r = (int)base[a.group == 1 ? 0 : (t - c0 * a.chunk) / a.chunk][expert] + place;
       a.rows[s] = r;
-      a.tokens[r] = (int)((uint32_t)s / (uint32_t)k);
+      a.tokens[r] = t;
     }
+    s += RT_THREADS;
+    if (s < to) expert = a.experts[s], place = a.rows[s];
   }
   for (int64_t r = (int64_t)first[E] + (int64_t)blockIdx.x * RT_THREADS + tid; r < all; r += (int64_t)gridDim.x * RT_THREADS) a.tokens[r] = -1;
 }
@@ -254,19 +303,20 @@ static int route_passes(int64_t T) {
   const int64_t n = (T + RT_TOKENS - 1) / RT_TOKENS;
   return (int)((n + RT_MOST_CHUNKS - 1) / RT_MOST_CHUNKS);
 }
-static int64_t route_chunks(int64_t T) {
-  const int64_t chunk = (int64_t)route_passes(T) * RT_TOKENS;
-  return (T + chunk - 1) / chunk;
-}
+static int64_t route_chunk(int64_t T) { return T <= RT_FEW_T ? RT_FEW_TOKENS : (int64_t)route_passes(T) * RT_TOKENS; }
+static int64_t route_chunks(int64_t T) { return (T + route_chunk(T) - 1) / route_chunk(T); }
 
 template <bool BF16, int V>
 static void launch_route(const RouteArgs& a, hipStream_t st) {
   if (a.T <= RT_ONE_PASSES * RT_TOKENS) {
-    queue_kernel((route_choose_kernel<BF16, V, true>), dim3(1), dim3(RT_THREADS), 0, st, a);
-  } else {
-    queue_kernel((route_choose_kernel<BF16, V, false>), dim3((unsigned)a.chunks), dim3(RT_THREADS), 0, st, a);
-    queue_kernel(route_rows_kernel, dim3((unsigned)((a.chunks + RT_GROUP - 1) / RT_GROUP)), dim3(RT_THREADS), 0, st, a);
+    queue_kernel((route_choose_kernel<BF16, V, RT_THREADS, true>), dim3(1), dim3(RT_THREADS), 0, st, a);
+    return;
   }
+  if (a.T <= RT_FEW_T)
+    queue_kernel((route_choose_kernel<BF16, V, RT_FEW_THREADS, false>), dim3((unsigned)a.chunks), dim3(RT_FEW_THREADS), 0, st, a);
+  else
+    queue_kernel((route_choose_kernel<BF16, V, RT_THREADS, false>), dim3((unsigned)a.chunks), dim3(RT_THREADS), 0, st, a);
+  queue_kernel(route_rows_kernel, dim3((unsigned)((a.chunks + a.group - 1) / a.group)), dim3(RT_THREADS), 0, st, a);
 }
 template <bool BF16>
 static void launch_route(const RouteArgs& a, hipStream_t st) {
@@ -277,90 +327,80 @@ static void launch_route(const RouteArgs& a, hipStream_t st) {
 }
 
 // ---- the experts' outputs back to the tokens ------------------------------------------------------------------------
-// out[t] = sum_j weights[t, j] y[rows[t, j]] (+ residual[t]), in fp32 in the order of j, the residual last, rounded once.  A thread has 16 bytes of a
-// token's row (VEC; single values where rows are not whole vectors) and asks for up to 8 choices' before it adds.
-// What bounds it: HBM.
+// out[t] = sum_j weights[t, j] y[rows[t, j]] (+ residual[t]), in fp32 in the order of j, the residual last, rounded once.  A wavefront has 64
+// units of 16 bytes of a token's row (VEC; single values where rows are not whole units): its rows and weights are scalar loads, and it asks for up
+// to 8 rows before it adds the first.  What bounds it: HBM.
 struct CombineArgs {
   const void *y, *res;
   void* out;
   const int32_t* rows;
   const float* weights;
-  int64_t units;  // of 16 bytes (values), in all
-  int64_t R;
-  int k, per;     // units of a token
+  int64_t waves, R;
+  int k, per;  // units of a token
+  UDiv chunks; // wavefronts of a token
+  int n_chunks;
 };
 
 template <bool BF16, bool VEC>
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
   constexpr int N = VEC ? (BF16 ? 8 : 4) : 1, AHEAD = 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.units) return;
-  const int64_t t = a.per == 256 ? (int64_t)blockIdx.x : i / a.per;
-  const int u = (int)(i - t * a.per);
-  auto load = [&](const void* p, int64_t row, float* v) {
-    if constexpr (VEC) {
-      const uint4 q = static_cast<const uint4*>(p)[row * a.per + u];
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if constexpr (BF16) {
-          v[2 * c] = __uint_as_float(w[c] << 16);
-          v[2 * c + 1] = __uint_as_float(w[c] & 0xffff0000u);
-        } else {
-          v[c] = __uint_as_float(w[c]);
-        }
-      }
-    } else {
-      v[0] = BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(p)[row * a.per + u]) : static_cast<const float*>(p)[row * a.per + u];
+  using unit = std::conditional_t<VEC, uint4, std::conditional_t<BF16, uint16_t, uint32_t>>;
+  const int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (w >= a.waves) return;
+  const int t = (int)a.chunks((uint32_t)w), u = ((int)w - t * a.n_chunks) * 64 + (int)(threadIdx.x & 63);
+  const bool in = u < a.per;
+  auto at = [&](const void* p, int64_t row) { return static_cast<const unit*>(p) + row * a.per + u; };
+  auto value = [](const unit& q, int c) {
+    if constexpr (!VEC) return BF16 ? bf16_bits_to_f32(q) : __uint_as_float(q);
+    else {
+      const uint32_t* const d = &q.x;
+      if constexpr (!BF16) return __uint_as_float(d[c]);
+      else return __uint_as_float(c & 1 ? d[c / 2] & 0xffff0000u : d[c / 2] << 16);
     }
   };
+  const int32_t* const rows = a.rows + (int64_t)t * a.k;
+  const float* const weights = a.weights + (int64_t)t * a.k;
   float sum[N];
 #pragma unroll
   for (int c = 0; c < N; ++c) sum[c] = 0.0f;
+  unit r{};
+  if (a.res && in) r = *at(a.res, t);
   for (int j0 = 0; j0 < a.k; j0 += AHEAD) {
     int row[AHEAD];
-    float w[AHEAD], v[AHEAD][N];
+    unit q[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      row[j] = -1;
-      if (j0 + j < a.k) {
-        row[j] = a.rows[t * a.k + j0 + j];
-        w[j] = a.weights[t * a.k + j0 + j];
-        if (row[j] >= a.R) row[j] = -1;
-      }
+      row[j] = j0 + j < a.k ? rows[j0 + j] : -1;
+      if (row[j] >= a.R) row[j] = -1;
     }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j)
-      if (row[j] >= 0) load(a.y, row[j], v[j]);
+      if (row[j] >= 0 && in) q[j] = *at(a.y, row[j]);
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j)
       if (row[j] >= 0) {
+        const float x = weights[j0 + j];
 #pragma unroll
-        for (int c = 0; c < N; ++c) sum[c] += w[j] * v[j][c];
+        for (int c = 0; c < N; ++c) sum[c] += x * value(q[j], c);
       }
   }
   if (a.res) {
-    float v[N];
-    load(a.res, t, v);
 #pragma unroll
-    for (int c = 0; c < N; ++c) sum[c] += v[c];
+    for (int c = 0; c < N; ++c) sum[c] += value(r, c);
   }
-  if constexpr (VEC && BF16) {
-    static_cast<uint4*>(a.out)[i] = make_uint4(pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]), pack_bf16x2(sum[4], sum[5]), pack_bf16x2(sum[6], sum[7]));
-  } else if constexpr (VEC) {
-    static_cast<float4*>(a.out)[i] = make_float4(sum[0], sum[1], sum[2], sum[3]);
-  } else if constexpr (BF16) {
-    static_cast<uint16_t*>(a.out)[i] = (uint16_t)f32_to_bf16_bits(sum[0]);
-  } else {
-    static_cast<float*>(a.out)[i] = sum[0];
-  }
+  if (!in) return;
+  unit* const out = static_cast<unit*>(a.out) + (int64_t)t * a.per + u;
+  if constexpr (VEC && BF16) *out = make_uint4(pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3]), pack_bf16x2(sum[4], sum[5]), pack_bf16x2(sum[6], sum[7]));
+  else if constexpr (VEC) *out = make_uint4(__float_as_uint(sum[0]), __float_as_uint(sum[1]), __float_as_uint(sum[2]), __float_as_uint(sum[3]));
+  else if constexpr (BF16) *out = (uint16_t)f32_to_bf16_bits(sum[0]);
+  else *out = __float_as_uint(sum[0]);
 }
 
 }  // namespace aq
 
 extern "C" int64_t aq_route_topk_workspace_bytes(int64_t T, int64_t E) {
   if (T <= aq::RT_ONE_PASSES * aq::RT_TOKENS || T > (int64_t)1 << 24 || E <= 0) return 0;
-  return aq::route_chunks(T) * E * (int64_t)sizeof(uint16_t);
+  return aq::route_chunks(T) * ((E + 1) / 2 * 2) * (int64_t)sizeof(uint16_t);
 }
 
 extern "C" int aq_route_topk(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t k, int renormalize, float* weights,
@@ -390,8 +430,13 @@ extern "C" int aq_route_topk(const void* logits, int dtype, int64_t T, int64_t E
   a.E = (int)E;
   a.k = (int)k;
   a.renormalize = renormalize != 0;
-  a.passes = aq::route_passes(T);
+  a.passes = T <= aq::RT_FEW_T ? 1 : aq::route_passes(T);
+  a.chunk = T > 0 ? (int)aq::route_chunk(T) : 0;
+  a.group = T <= aq::RT_FEW_T ? aq::RT_GROUP : 1;
   a.chunks = T > 0 ? (int)aq::route_chunks(T) : 0;
+  a.pitch = (int)((E + 1) / 2 * 2);
+  const int run = E <= 64 ? 4 : E <= 128 ? 8 : E <= 256 ? 16 : 32, unit = dtype == AQ_BF16 ? 8 : 16;  // a lane's logits; bytes of four
+  a.whole = E == 16 * run && !aq::check_ptr(logits, unit) && (T <= 1 || ld * (unit / 4) % unit == 0);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == AQ_BF16) aq::launch_route<true>(a, st);
   else aq::launch_route<false>(a, st);
@@ -418,9 +463,11 @@ extern "C" int aq_combine_rows(const void* y, int dtype, int64_t R, int64_t N, c
   a.R = R;
   a.k = (int)k;
   a.per = (int)(vec ? N * size / 16 : N);
-  a.units = T * a.per;
-  const int64_t wgs = (a.units + 255) / 256;
-  if (wgs > 0x7fffffff) return AQ_E_RANGE;
+  a.n_chunks = (a.per + 63) / 64;
+  a.chunks = aq::UDiv::of((uint32_t)a.n_chunks);
+  a.waves = T * a.n_chunks;
+  if (a.waves > 0x7fffffff) return AQ_E_RANGE;
+  const int64_t wgs = (a.waves + 3) / 4;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 g((unsigned)wgs), b(256);
   if (dtype == AQ_BF16) {
