@@ -536,7 +536,7 @@ int aq_compact_pages(const int64_t *page_table, int64_t entries, const int32_t *
  * padded token: a row of -inf).  experts [T, k] int32; weights [T, k] fp32, exp(x - max) over the sum of the chosen ones (renormalize != 0) or of all E (softmax), 0 in places without an
  * expert.  The choices in the experts' order, by token inside an expert: expert e has rows offsets[e] .. offsets[e + 1] - 1 (offsets int32 [E + 1]),
  * rows [T, k] int32 the row of each choice (-1: none), tokens [T k] int32 the token of each row (-1 past offsets[E]).
- * E at most 512, k at most 16, T at most 2^24 (AQ_E_RANGE).  workspace: aq_route_topk_workspace_bytes(T, E) bytes (0: may be NULL), 4-byte aligned; calls
+ * E at most 512, k at most 16, T at most 2^24 (AQ_E_RANGE).  workspace: aq_route_topk_workspace_bytes(T, E) bytes (0: may be NULL), 8-byte aligned; calls
  * that overlap in time must not share it. */
 int64_t aq_route_topk_workspace_bytes(int64_t T, int64_t E);
 int aq_route_topk(const void *logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t k, int renormalize,

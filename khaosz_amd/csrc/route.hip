@@ -25,7 +25,8 @@ struct RouteArgs {
   int64_t ld;  // logits between tokens
   float* weights;
   int32_t *experts, *rows, *tokens, *offsets;
-  uint16_t* counts;  // [chunks][pitch]
+  uint16_t* counts;            // [chunks][pitch]
+  uint32_t *before, *totals;   // [chunks][pitch], [pitch]: many chunks
   int T, E, k, renormalize, passes, chunks;
   int chunk;  // tokens of a chunk
   int group;  // chunks of a workgroup that hands out rows
@@ -237,8 +238,45 @@ __global__ __launch_bounds__(THREADS) void route_choose_kernel(RouteArgs a) {
   }
 }
 
-// Rows for the choices of a group of chunks: the experts' first rows, the choices of the chunks before, the place among the chunk's.  Every
-// workgroup adds up all chunks' counts by itself; its first choices (of 64 tokens: all there are) are on their way meanwhile.
+// Many chunks: each expert's choices in the chunks before, summed once for everybody.  A workgroup has 32 experts, two to a thread, and its 16 rows of
+// threads a run of chunks each.
+constexpr int RT_SUM_THREADS = 256, RT_SUM_E = 32, RT_SUM_RUNS = RT_SUM_THREADS * 2 / RT_SUM_E;
+__global__ __launch_bounds__(RT_SUM_THREADS) void route_sums_kernel(RouteArgs a) {
+  __shared__ uint32_t run_sum[RT_SUM_RUNS][RT_SUM_E];
+  const int e = (int)blockIdx.x * RT_SUM_E + 2 * (threadIdx.x & (RT_SUM_E / 2 - 1)), run = threadIdx.x / (RT_SUM_E / 2), i = e & (RT_SUM_E - 1);
+  const int per = (a.chunks + RT_SUM_RUNS - 1) / RT_SUM_RUNS, c0 = run * per, c1 = c0 + per < a.chunks ? c0 + per : a.chunks;
+  auto counts = [&](int c) { return *reinterpret_cast<const uint32_t*>(a.counts + (int64_t)c * a.pitch + e); };
+  uint32_t lo = 0, hi = 0;
+  if (e < a.E) {
+#pragma unroll 16
+    for (int c = c0; c < c1; ++c) {
+      const uint32_t two = counts(c);
+      lo += two & 0xffffu, hi += two >> 16;
+    }
+  }
+  run_sum[run][i] = lo, run_sum[run][i + 1] = hi;
+  __syncthreads();
+  if (e >= a.E) return;
+  uint32_t at_lo = 0, at_hi = 0, all_lo = 0, all_hi = 0;
+#pragma unroll
+  for (int r = 0; r < RT_SUM_RUNS; ++r) {
+    const uint32_t x = run_sum[r][i], y = run_sum[r][i + 1];
+    if (r < run) at_lo += x, at_hi += y;
+    all_lo += x, all_hi += y;
+  }
+  if (run == 0) *reinterpret_cast<uint2*>(a.totals + e) = make_uint2(all_lo, all_hi);
+#pragma unroll 16
+  for (int c = c0; c < c1; ++c) {
+    const uint32_t two = counts(c);
+    *reinterpret_cast<uint2*>(a.before + (int64_t)c * a.pitch + e) = make_uint2(at_lo, at_hi);
+    at_lo += two & 0xffffu, at_hi += two >> 16;
+  }
+}
+
+// Rows for the choices of a group of chunks: the experts' first rows, the choices of the chunks before, the place among the chunk's.  Few
+// chunks: every workgroup adds up all their counts by itself (256 workgroups, chunks and experts: 15 us, SUMMED 4 and 4).  Its first choices (of 64 tokens:
+// all there are) are on their way meanwhile.
+template <bool SUMMED>
 __global__ __launch_bounds__(RT_THREADS) void route_rows_kernel(RouteArgs a) {
   __shared__ uint32_t total[RT_MAX_E], before[RT_MAX_E], first[RT_MAX_E + 1], base[RT_GROUP][RT_MAX_E];
   const int tid = threadIdx.x, E = a.E;
@@ -248,32 +286,41 @@ __global__ __launch_bounds__(RT_THREADS) void route_rows_kernel(RouteArgs a) {
   int64_t s = from + tid;
   int expert = -1, place = 0;
   if (s < to) expert = a.experts[s], place = a.rows[s];
-  for (int e = tid; e < E; e += RT_THREADS) total[e] = before[e] = 0;
-  __syncthreads();
-  int width = 32;  // threads to a chunk's counts, two experts each
-  while (2 * width < E) width *= 2;
-  const int e = 2 * (tid & (width - 1)), turns = RT_THREADS / width;
-  if (e < E) {
-    uint32_t sum[2] = {0, 0}, early[2] = {0, 0};
-#pragma unroll 16
-    for (int c = tid / width; c < a.chunks; c += turns) {
-      const uint32_t two = *reinterpret_cast<const uint32_t*>(a.counts + (int64_t)c * a.pitch + e);
-      const uint32_t n[2] = {two & 0xffffu, two >> 16};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        sum[i] += n[i];
-        early[i] += c < c0 ? n[i] : 0;
-        if (c >= c0 && c < c0 + a.group && e + i < E) base[c - c0][e + i] = n[i];
-      }
+  if constexpr (SUMMED) {
+    for (int i = tid; i < E; i += RT_THREADS) {
+      total[i] = a.totals[i];
+      before[i] = a.before[(int64_t)blockIdx.x * a.pitch + i];
+      base[0][i] = 0;
     }
+    __syncthreads();
+  } else {
+    for (int i = tid; i < E; i += RT_THREADS) total[i] = before[i] = 0;
+    __syncthreads();
+    int width = 32;  // threads to a chunk's counts, two experts each
+    while (2 * width < E) width *= 2;
+    const int e = 2 * (tid & (width - 1)), turns = RT_THREADS / width;
+    if (e < E) {
+      uint32_t sum[2] = {0, 0}, early[2] = {0, 0};
+#pragma unroll 16
+      for (int c = tid / width; c < a.chunks; c += turns) {
+        const uint32_t two = *reinterpret_cast<const uint32_t*>(a.counts + (int64_t)c * a.pitch + e);
+        const uint32_t n[2] = {two & 0xffffu, two >> 16};
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (e + i < E) {
-        atomicAdd(&total[e + i], sum[i]);  // whole numbers: any order
-        atomicAdd(&before[e + i], early[i]);
+        for (int i = 0; i < 2; ++i) {
+          sum[i] += n[i];
+          early[i] += c < c0 ? n[i] : 0;
+          if (c >= c0 && c < c0 + a.group && e + i < E) base[c - c0][e + i] = n[i];
+        }
       }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (e + i < E) {
+          atomicAdd(&total[e + i], sum[i]);  // whole numbers: any order
+          atomicAdd(&before[e + i], early[i]);
+        }
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (tid < 64) experts_scan(total, first, E, tid);
   __syncthreads();
   for (int i = tid; i < E; i += RT_THREADS) {
@@ -306,6 +353,9 @@ static int route_passes(int64_t T) {
 static int64_t route_chunk(int64_t T) { return T <= RT_FEW_T ? RT_FEW_TOKENS : (int64_t)route_passes(T) * RT_TOKENS; }
 static int64_t route_chunks(int64_t T) { return (T + route_chunk(T) - 1) / route_chunk(T); }
 
+// Whether the counts are summed by a launch of their own (64 experts, 4096 tokens: 10.4 us, without it 7.6; 256 and 16384: 15.3 and 21.8).
+static bool route_sums(int64_t T, int64_t E) { return route_chunks(T) * E > 16384; }
+
 template <bool BF16, int V>
 static void launch_route(const RouteArgs& a, hipStream_t st) {
   if (a.T <= RT_ONE_PASSES * RT_TOKENS) {
@@ -316,7 +366,13 @@ static void launch_route(const RouteArgs& a, hipStream_t st) {
     queue_kernel((route_choose_kernel<BF16, V, RT_FEW_THREADS, false>), dim3((unsigned)a.chunks), dim3(RT_FEW_THREADS), 0, st, a);
   else
     queue_kernel((route_choose_kernel<BF16, V, RT_THREADS, false>), dim3((unsigned)a.chunks), dim3(RT_THREADS), 0, st, a);
-  queue_kernel(route_rows_kernel, dim3((unsigned)((a.chunks + a.group - 1) / a.group)), dim3(RT_THREADS), 0, st, a);
+  const dim3 groups((unsigned)((a.chunks + a.group - 1) / a.group)), threads(RT_THREADS);
+  if (!route_sums(a.T, a.E)) {
+    queue_kernel(route_rows_kernel<false>, groups, threads, 0, st, a);
+  } else {
+    queue_kernel(route_sums_kernel, dim3((unsigned)((a.E + RT_SUM_E - 1) / RT_SUM_E)), dim3(RT_SUM_THREADS), 0, st, a);
+    queue_kernel(route_rows_kernel<true>, groups, threads, 0, st, a);
+  }
 }
 template <bool BF16>
 static void launch_route(const RouteArgs& a, hipStream_t st) {
@@ -400,7 +456,8 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
 
 extern "C" int64_t aq_route_topk_workspace_bytes(int64_t T, int64_t E) {
   if (T <= aq::RT_ONE_PASSES * aq::RT_TOKENS || T > (int64_t)1 << 24 || E <= 0) return 0;
-  return aq::route_chunks(T) * ((E + 1) / 2 * 2) * (int64_t)sizeof(uint16_t);
+  const int64_t chunks = aq::route_chunks(T), pitch = (E + 1) / 2 * 2;
+  return (aq::route_sums(T, E) ? (chunks + 1) * pitch * 4 : 0) + chunks * pitch * 2;
 }
 
 extern "C" int aq_route_topk(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int64_t k, int renormalize, float* weights,
@@ -416,7 +473,7 @@ extern "C" int aq_route_topk(const void* logits, int dtype, int64_t T, int64_t E
   const int64_t need = aq_route_topk_workspace_bytes(T, E);
   if (need > 0 && !workspace) return AQ_E_NULL;
   if (workspace_bytes < need) return AQ_E_WORKSPACE;
-  if (need > 0 && aq::check_ptr(workspace, 4)) return AQ_E_ALIGN;
+  if (need > 0 && aq::check_ptr(workspace, 8)) return AQ_E_ALIGN;
   aq::RouteArgs a{};
   a.logits = logits;
   a.ld = ld;
@@ -425,7 +482,6 @@ extern "C" int aq_route_topk(const void* logits, int dtype, int64_t T, int64_t E
   a.rows = rows;
   a.tokens = tokens;
   a.offsets = offsets;
-  a.counts = static_cast<uint16_t*>(workspace);
   a.T = (int)T;
   a.E = (int)E;
   a.k = (int)k;
@@ -435,6 +491,9 @@ extern "C" int aq_route_topk(const void* logits, int dtype, int64_t T, int64_t E
   a.group = T <= aq::RT_FEW_T ? aq::RT_GROUP : 1;
   a.chunks = T > 0 ? (int)aq::route_chunks(T) : 0;
   a.pitch = (int)((E + 1) / 2 * 2);
+  a.totals = static_cast<uint32_t*>(workspace);  // (many chunks; then their sums, then the counts)
+  a.before = a.totals + a.pitch;
+  a.counts = reinterpret_cast<uint16_t*>(aq::route_sums(T, E) ? a.before + (int64_t)a.chunks * a.pitch : a.totals);
   const int run = E <= 64 ? 4 : E <= 128 ? 8 : E <= 256 ? 16 : 32, unit = dtype == AQ_BF16 ? 8 : 16;  // a lane's logits; bytes of four
   a.whole = E == 16 * run && !aq::check_ptr(logits, unit) && (T <= 1 || ld * (unit / 4) % unit == 0);
   hipStream_t st = static_cast<hipStream_t>(stream);

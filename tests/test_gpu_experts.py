@@ -67,7 +67,7 @@ def _check_route(x, k, renormalize, got):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 64, 6), (2, 3, 3), (7, 8, 2), (63, 60, 4), (64, 65, 5), (65, 16, 16), (256, 17, 3), (257, 64, 6),
-                                   (333, 60, 4), (511, 200, 8), (700, 256, 8), (130, 128, 7), (1500, 512, 16), (4100, 9, 2)])
+                                   (333, 60, 4), (511, 200, 8), (700, 256, 8), (130, 128, 7), (1500, 512, 16), (4100, 9, 2), (3000, 512, 9), (3000, 401, 5), (2100, 64, 6)])
 def test_route(T, E, k, dtype):
     _say("route", T, E, k, dtype)
     g = torch.Generator().manual_seed(T * 1000 + E)
