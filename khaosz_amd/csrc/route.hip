@@ -354,7 +354,8 @@ static int64_t route_chunk(int64_t T) { return T <= RT_FEW_T ? RT_FEW_TOKENS : (
 static int64_t route_chunks(int64_t T) { return (T + route_chunk(T) - 1) / route_chunk(T); }
 
 // Whether the counts are summed by a launch of their own (64 experts, 4096 tokens: 10.4 us, without it 7.6; 256 and 16384: 15.3 and 21.8).
-static bool route_sums(int64_t T, int64_t E) { return route_chunks(T) * E > 16384; }
+// (Its chunks are a workgroup's each: not those of RT_FEW_TOKENS.)
+static bool route_sums(int64_t T, int64_t E) { return T > RT_FEW_T && route_chunks(T) * E > 16384; }
 
 template <bool BF16, int V>
 static void launch_route(const RouteArgs& a, hipStream_t st) {
