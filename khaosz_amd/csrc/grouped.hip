@@ -7,6 +7,7 @@
 #include <cmath>
 
 #include "aq_grouped.h"
+#include "aq_rows.h"
 
 namespace aq {
 
@@ -59,46 +60,84 @@ __device__ __forceinline__ void store_out(void* y, int64_t i, float v) {
   if constexpr (OUT == OUT_BF16) static_cast<uint16_t*>(y)[i] = (uint16_t)f32_to_bf16_bits(v);
   else static_cast<float*>(y)[i] = v;
 }
-// Tiles of 16 rows x 32 weight rows: four wavefronts take every fourth 128-byte line of K, operands straight from memory into registers, the
-// sums meet in LDS.
-constexpr int GF_ROWS = 16, GF_COLS = 32, GF_WAVES = 4;
-template <int OUT, bool SWI>
+// Tiles of 16 rows x 32 weight rows: four wavefronts take every fourth 128-byte line of K, weights straight from memory into registers, the sums
+// meet in LDS.  Rows come as codes, from memory like the weights (IN = CODES), or as they are, and every workgroup quantises its own while its
+// weights are on their way (the row quantiser's arithmetic): a launch less for a few rows.
+enum { IN_CODES = 0, IN_BF16 = 1, IN_F32 = 2 };
+constexpr int GF_ROWS = 16, GF_COLS = 32, GF_WAVES = 4, GF_DEEP = 4;  // GF_DEEP: lines of a wavefront on their way at a time
+// bytes between rows of codes in LDS: 16 of them then begin 4 banks apart
+__host__ __device__ inline int few_pitch(int K) { return (K + 127) / 128 * 128 + 16; }
+
+template <int OUT, bool SWI, int IN, int VPL>
 __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs p) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t xs[];  // IN: the rows' codes
   __shared__ int part[GF_WAVES][2][GF_ROWS][17];
+  __shared__ float scale[GF_ROWS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   RowTile t;
   if (!find_tile<GF_ROWS>(p, blockIdx.y, lane, t)) return;
   const int K = p.K, FH = SWI ? p.N / 2 : p.N;
   const int n0 = (int)blockIdx.x * (SWI ? 16 : GF_COLS);
-  const uint8_t* const w = p.w + t.e * p.w_bytes;
-  const __amdgpu_buffer_rsrc_t Wr = make_rsrc(w, (uint32_t)p.w_bytes), Xr = make_rsrc(p.x, (uint32_t)p.x_rows * (uint32_t)K);
+  const __amdgpu_buffer_rsrc_t Wr = make_rsrc(p.w + t.e * p.w_bytes, (uint32_t)p.w_bytes);
   const int r16 = lane & 15, q16 = (lane >> 4) * 16;
-  const int row = t.first + r16;
-  int tok = -1;
-  if (row < t.end) tok = p.tokens ? p.tokens[row] : row;
-  const bool live = tok >= 0 && tok < p.x_rows;
-  const uint32_t xo = (uint32_t)tok * (uint32_t)K + q16;
   const int na = n0 + r16, nb = SWI ? FH + na : na + 16;
   const bool ina = na < FH, inb = SWI ? ina : nb < FH;
   const uint32_t ao = (uint32_t)na * (uint32_t)K + q16, bo = (uint32_t)nb * (uint32_t)K + q16;
-  v4i acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
   const int lines = (K + 127) / 128;
-  constexpr int DEEP = 4;
-  for (int l0 = wave; l0 < lines; l0 += GF_WAVES * DEEP) {
-    v4i xv[2 * DEEP], av[2 * DEEP], bv[2 * DEEP];
+  auto token = [&](int row) {  // -1: none
+    const int tok = row < t.end ? (p.tokens ? p.tokens[row] : row) : -1;
+    return tok < p.x_rows ? tok : -1;
+  };
+  v4i av[2 * GF_DEEP], bv[2 * GF_DEEP];
+  auto k_of = [&](int l0, int i) { return (l0 + i / 2 * GF_WAVES) * 128 + i % 2 * 64; };
+  auto load_weights = [&](int l0) {
 #pragma unroll
-    for (int i = 0; i < 2 * DEEP; ++i) {
-      const int k = (l0 + i / 2 * GF_WAVES) * 128 + i % 2 * 64;
+    for (int i = 0; i < 2 * GF_DEEP; ++i) {
+      const int k = k_of(l0, i);
       const bool in = k + q16 < K;
       av[i] = __builtin_amdgcn_raw_buffer_load_b128(Wr, in && ina ? ao + k : OOB_OFFSET, 0, 2);
       bv[i] = __builtin_amdgcn_raw_buffer_load_b128(Wr, in && inb ? bo + k : OOB_OFFSET, 0, 2);
-      xv[i] = __builtin_amdgcn_raw_buffer_load_b128(Xr, in && live ? xo + k : OOB_OFFSET, 0, 0);
+    }
+  };
+  load_weights(wave);
+  const int pitch = few_pitch(K);
+  __amdgpu_buffer_rsrc_t Xr = make_rsrc(p.x, IN == IN_CODES ? (uint32_t)p.x_rows * (uint32_t)K : 0u);
+  uint32_t xo = OOB_OFFSET;
+  if constexpr (IN == IN_CODES) {
+    const int tok = token(t.first + r16);
+    if (tok >= 0) xo = (uint32_t)tok * (uint32_t)K + q16;
+  } else {
+    constexpr bool BF16 = IN == IN_BF16;
+    const int rows = t.end - t.first < GF_ROWS ? t.end - t.first : GF_ROWS;
+    for (int m = wave; m < rows; m += GF_WAVES) {
+      const int tok = __builtin_amdgcn_readfirstlane(token(t.first + m));
+      RowsToLds<BF16, 1, VPL> r;
+      r.issue(p.x + (int64_t)(tok < 0 ? 0 : tok) * K * (BF16 ? 2 : 4), tok >= 0, K, K, 0, 1, lane);
+      r.finish(tok >= 0, 1, K, xs + m * pitch, pitch, scale + m, 0, 1, lane);
+      if (tok < 0 && lane == 0) scale[m] = 0.0f;  // a row of zeros
+    }
+    __syncthreads();
+  }
+  v4i acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  for (int l0 = wave; l0 < lines;) {
+    v4i xv[2 * GF_DEEP];
+#pragma unroll
+    for (int i = 0; i < 2 * GF_DEEP; ++i) {
+      const int k = k_of(l0, i);
+      if constexpr (IN == IN_CODES) {
+        xv[i] = __builtin_amdgcn_raw_buffer_load_b128(Xr, k + q16 < K && xo != OOB_OFFSET ? xo + k : OOB_OFFSET, 0, 0);
+      } else {
+        xv[i] = v4i{0, 0, 0, 0};  // (past K the weights are zeros)
+        if (k < K) xv[i] = *reinterpret_cast<const v4i*>(xs + r16 * pitch + k + q16);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 2 * DEEP; ++i) {
+    for (int i = 0; i < 2 * GF_DEEP; ++i) {
       acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv[i], av[i], acc[0], 0, 0, 0);
       acc[1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv[i], bv[i], acc[1], 0, 0, 0);
     }
+    l0 += GF_WAVES * GF_DEEP;
+    if (l0 < lines) load_weights(l0);
   }
 #pragma unroll
   for (int g = 0; g < 2; ++g)
@@ -107,8 +146,13 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
   __syncthreads();
   const int m = tid >> 4, c = tid & 15, out_row = t.first + m;
   if (out_row >= t.end) return;
-  const int otok = p.tokens ? p.tokens[out_row] : out_row;
-  const float sx = otok >= 0 && otok < p.x_rows ? p.sx[otok] : 0.0f;
+  float sx;
+  if constexpr (IN == IN_CODES) {
+    const int tok = token(out_row);
+    sx = tok >= 0 ? p.sx[tok] : 0.0f;
+  } else {
+    sx = scale[m];
+  }
   float y[2];
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
@@ -142,14 +186,38 @@ static int choose_grouped(const GroupedArgs& a) {
   return used * ((a.N + 255) / 256) >= 1.75 * device_cus() || a.R > 24 * a.E ? GROUPED_WALK_256 : GROUPED_FEW;
 }
 
+template <int OUT, bool SWI, int IN, int VPL>
+static int launch_few(const GroupedArgs& a, hipStream_t st) {
+  const int64_t tiles = grouped_most_tiles(a.R, a.E, GF_ROWS), cols = (a.N + GF_COLS - 1) / GF_COLS;
+  if (tiles > 65535 || cols > 0x7fffffff) return AQ_E_RANGE;
+  queue_kernel((grouped_few_kernel<OUT, SWI, IN, VPL>), dim3((unsigned)cols, (unsigned)tiles), dim3(GF_WAVES * 64),
+               IN == IN_CODES ? 0 : GF_ROWS * few_pitch(a.K), st, a);
+  return (int)hipGetLastError();
+}
+
+// Rows as they are (a.x of `dtype`, which is the output's type too), quantised in the launch.
+constexpr int64_t GF_IN_BF16_K = 4096, GF_IN_F32_K = 2048;  // longest rows
+template <bool SWI>
+static int launch_rows(const GroupedArgs& a, int dtype, hipStream_t st) {
+  if (dtype == AQ_BF16)
+    return a.K <= 2048 ? launch_few<OUT_BF16, SWI, IN_BF16, 4>(a, st) : launch_few<OUT_BF16, SWI, IN_BF16, 8>(a, st);
+  return a.K <= 1024 ? launch_few<OUT_F32, SWI, IN_F32, 4>(a, st) : launch_few<OUT_F32, SWI, IN_F32, 8>(a, st);
+}
+// Whether the two products of a layer quantise their rows themselves.
+static bool rows_in_launch(int64_t T, int64_t k, int64_t dim, int64_t F, int dtype) {
+  const int64_t most = dtype == AQ_BF16 ? GF_IN_BF16_K : GF_IN_F32_K;
+  if (dim > most || F > most) return false;
+#ifdef AQ_LAB
+  if (g_forced_grouped) return g_forced_grouped == GROUPED_FEW;
+#endif
+  return T * k <= 16;
+}
+
 template <int OUT, bool SWI>
 static int launch_grouped(const GroupedArgs& a, hipStream_t st) {
   const int kind = choose_grouped(a);
   if (kind != GROUPED_FEW) return grouped_walk_launch<OUT, SWI>(a, kind == GROUPED_WALK_256 ? 256 : kind == GROUPED_WALK_128 ? 128 : 64, st);
-  const int64_t tiles = grouped_most_tiles(a.R, a.E, GF_ROWS), cols = (a.N + GF_COLS - 1) / GF_COLS;
-  if (tiles > 65535 || cols > 0x7fffffff) return AQ_E_RANGE;
-  queue_kernel((grouped_few_kernel<OUT, SWI>), dim3((unsigned)cols, (unsigned)tiles), dim3(GF_WAVES * 64), 0, st, a);
-  return (int)hipGetLastError();
+  return launch_few<OUT, SWI, IN_CODES, 1>(a, st);
 }
 
 static int grouped(const int8_t* xq, const float* sx, int64_t x_rows, const int8_t* wq, const float* sw, const void* bias, int bias_dtype,
@@ -185,9 +253,9 @@ static int grouped(const int8_t* xq, const float* sx, int64_t x_rows, const int8
   return y_dtype == AQ_BF16 ? launch_grouped<OUT_BF16, false>(a, st) : launch_grouped<OUT_F32, false>(a, st);
 }
 
-// Scratch of a whole layer: codes and scales of x, h (later the experts' outputs), codes and scales of h.
+// Scratch of a whole layer: codes and scales of x, h, its codes and scales, the experts' outputs.
 struct ExpertsScratch {
-  int64_t xq, sx, h, hq, sh, bytes;
+  int64_t xq, sx, h, hq, sh, y, bytes;
   ExpertsScratch(int64_t T, int64_t R, int64_t dim, int64_t F, int size) {
     auto take = [&](int64_t n) {
       const int64_t at = bytes;
@@ -197,9 +265,10 @@ struct ExpertsScratch {
     bytes = 0;
     xq = take(T * dim);
     sx = take(T * 4);
-    h = take(R * (F > dim ? F : dim) * size);
+    h = take(R * F * size);
     hq = take(R * F);
     sh = take(R * 4);
+    y = take(R * dim * size);
   }
 };
 
@@ -243,12 +312,40 @@ extern "C" int aq_experts_w8a8(const void* x, int x_dtype, int64_t T, int64_t di
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
   int8_t *const xq = reinterpret_cast<int8_t*>(ws + s.xq), *const hq = reinterpret_cast<int8_t*>(ws + s.hq);
   float *const sx = reinterpret_cast<float*>(ws + s.sx), *const sh = reinterpret_cast<float*>(ws + s.sh);
-  void* const h = ws + s.h;
-  int rc = aq_quant_rowwise_i8(x, x_dtype, T, dim, dim, xq, sx, stream);
-  if (rc == AQ_OK) rc = aq_swiglu_w8a8_grouped(xq, sx, T, up_gate, up_gate_scale, offsets, E, tokens, R, h, x_dtype, F, dim, stream);
-  if (rc == AQ_OK) rc = aq_quant_rowwise_i8(h, x_dtype, R, F, F, hq, sh, stream);
-  if (rc == AQ_OK) rc = aq_linear_w8a8_grouped(hq, sh, R, down, down_scale, nullptr, AQ_F32, offsets, E, nullptr, R, h, x_dtype, dim, F, stream);
-  if (rc == AQ_OK) rc = aq_combine_rows(h, x_dtype, R, dim, rows, weights, T, k, residual, out, stream);
+  void *const h = ws + s.h, *const y = ws + s.y;
+  int rc;
+  if (aq::rows_in_launch(T, k, dim, F, x_dtype)) {
+    aq::GroupedArgs a{};
+    a.x = static_cast<const uint8_t*>(x);
+    a.x_rows = (int)T;
+    a.w = reinterpret_cast<const uint8_t*>(up_gate);
+    a.sw = up_gate_scale;
+    a.offsets = offsets;
+    a.tokens = tokens;
+    a.y = h;
+    a.w_bytes = 2 * F * dim;
+    a.R = (int)R;
+    a.E = (int)E;
+    a.N = (int)(2 * F);
+    a.K = (int)dim;
+    rc = aq::launch_rows<true>(a, x_dtype, static_cast<hipStream_t>(stream));
+    a.x = static_cast<const uint8_t*>(h);
+    a.x_rows = (int)R;
+    a.w = reinterpret_cast<const uint8_t*>(down);
+    a.sw = down_scale;
+    a.tokens = nullptr;
+    a.y = y;
+    a.w_bytes = dim * F;
+    a.N = (int)dim;
+    a.K = (int)F;
+    if (rc == AQ_OK) rc = aq::launch_rows<false>(a, x_dtype, static_cast<hipStream_t>(stream));
+  } else {
+    rc = aq_quant_rowwise_i8(x, x_dtype, T, dim, dim, xq, sx, stream);
+    if (rc == AQ_OK) rc = aq_swiglu_w8a8_grouped(xq, sx, T, up_gate, up_gate_scale, offsets, E, tokens, R, h, x_dtype, F, dim, stream);
+    if (rc == AQ_OK) rc = aq_quant_rowwise_i8(h, x_dtype, R, F, F, hq, sh, stream);
+    if (rc == AQ_OK) rc = aq_linear_w8a8_grouped(hq, sh, R, down, down_scale, nullptr, AQ_F32, offsets, E, nullptr, R, y, x_dtype, dim, F, stream);
+  }
+  if (rc == AQ_OK) rc = aq_combine_rows(y, x_dtype, R, dim, rows, weights, T, k, residual, out, stream);
   return rc;
 }
 
