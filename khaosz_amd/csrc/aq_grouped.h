@@ -41,6 +41,57 @@ inline int64_t grouped_most_tiles(int64_t R, int64_t E, int64_t BM) {
   return used + (R - used) / BM;
 }
 
+// The tiles of BM rows that every expert's rows need, numbered expert by expert.  A workgroup takes the offsets into LDS (off: GP_MAX_E + 1); a
+// wavefront's lanes hold the running count over runs of experts, so that a tile's expert is two ballots away.  Offsets outside 0 .. R, or that fall, count
+// as the nearest that do not: nothing is read or written outside the R rows.
+template <int BM>
+struct GroupTiles {
+  const int32_t* off;
+  int E, per, upto, mine;  // per: experts of a lane; upto: tiles of the lanes up to this one
+  struct At {
+    int e, before, tiles;  // the expert, the tiles of the experts before it, its own
+  };
+  __device__ __forceinline__ int tiles_of(int e) const {
+    const int rows = e < E ? off[e + 1] - off[e] : 0;
+    return rows > 0 ? (rows + BM - 1) / BM : 0;
+  }
+  __device__ __forceinline__ void init(const GroupedArgs& p, int32_t* lds, int tid, int threads) {
+    for (int e = tid; e <= p.E; e += threads) {
+      const int o = p.offsets[e];
+      lds[e] = o < 0 ? 0 : o > p.R ? p.R : o;
+    }
+    __syncthreads();
+    off = lds;
+    E = p.E;
+    per = (E + 63) >> 6;
+    const int lane = tid & 63;
+    mine = 0;
+    for (int i = 0; i < per; ++i) mine += tiles_of(lane * per + i);
+    upto = wave_scan(mine);
+  }
+  // all tiles times `times` (offsets that fall can make it more than was launched for)
+  __device__ __forceinline__ int count(int times) const {
+    const int64_t all = (int64_t)__builtin_amdgcn_readlane(upto, 63) * times;
+    return all < 0x7fffffff ? (int)all : 0x7fffffff;
+  }
+  __device__ __forceinline__ At find(int q, int lane) const {  // q below count(1)
+    const int at = __builtin_ctzll(__ballot(upto > q));
+    const int e0 = at * per, before = __builtin_amdgcn_readlane(upto - mine, at);
+    const int n = lane < per ? tiles_of(e0 + lane) : 0;  // (per <= 8: inside a row of 16 lanes)
+    int in = n;
+    in += __builtin_amdgcn_update_dpp(0, in, 0x111, 0xf, 0xf, false);
+    in += __builtin_amdgcn_update_dpp(0, in, 0x112, 0xf, 0xf, false);
+    in += __builtin_amdgcn_update_dpp(0, in, 0x114, 0xf, 0xf, false);
+    const int sub = __builtin_ctzll(__ballot(lane < per && before + in > q));
+    At a;
+    a.e = e0 + sub;
+    a.tiles = __builtin_amdgcn_readlane(n, sub);
+    a.before = before + __builtin_amdgcn_readlane(in, sub) - a.tiles;
+    return a;
+  }
+};
+static_assert(GP_MAX_E <= 64 * 8, "a lane's run of experts");
+
 // up silu(gate) of fp32 projections, which are rounded to the output's type first.  fp32: the layer's frozen arithmetic.  bf16: the hardware's
 // exponential and reciprocal, 1 step of fp32 each, for a result that is rounded to 2^-8; the difference is below 2^-16 and the exponential's
 // argument its largest part.  (The frozen form takes 35 operations, and the epilogue of a tile of K = 2048 then half as long as its products.)

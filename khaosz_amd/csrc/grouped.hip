@@ -63,12 +63,15 @@ __device__ __forceinline__ void store_out(void* y, int64_t i, float v) {
 // Tiles of 16 rows x 32 weight rows: four wavefronts take every fourth 128-byte line of K, weights straight from memory into registers, the sums
 // meet in LDS.  Rows come as codes, from memory like the weights (IN = CODES), or as they are, and every workgroup quantises its own while its
 // weights are on their way (the row quantiser's arithmetic): a launch less for a few rows.
+constexpr int GP_MAX_TOKEN_K = 64;  // choices of a token
 enum { IN_CODES = 0, IN_BF16 = 1, IN_F32 = 2 };
-constexpr int GF_ROWS = 16, GF_COLS = 32, GF_WAVES = 4, GF_DEEP = 4;  // GF_DEEP: lines of a wavefront on their way at a time
+constexpr int GF_ROWS = 16, GF_COLS = 32, GF_WAVES = 4;
 // bytes between rows of codes in LDS: 16 of them then begin 4 banks apart
 __host__ __device__ inline int few_pitch(int K) { return (K + 127) / 128 * 128 + 16; }
 
-template <int OUT, bool SWI, int IN, int VPL>
+// DEEP: lines of a wavefront on their way at a time, cut to the rows' length class (a load of nothing takes its turn in the address path all the
+// same, and branches around loads make them wait for each other: 24.7 -> 66 us for four tokens' up and gate).
+template <int OUT, bool SWI, int IN, int VPL, int DEEP>
 __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t xs[];  // IN: the rows' codes
   __shared__ int part[GF_WAVES][2][GF_ROWS][17];
@@ -88,11 +91,11 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
     const int tok = row < t.end ? (p.tokens ? p.tokens[row] : row) : -1;
     return tok < p.x_rows ? tok : -1;
   };
-  v4i av[2 * GF_DEEP], bv[2 * GF_DEEP];
+  v4i av[2 * DEEP], bv[2 * DEEP];
   auto k_of = [&](int l0, int i) { return (l0 + i / 2 * GF_WAVES) * 128 + i % 2 * 64; };
   auto load_weights = [&](int l0) {
 #pragma unroll
-    for (int i = 0; i < 2 * GF_DEEP; ++i) {
+    for (int i = 0; i < 2 * DEEP; ++i) {
       const int k = k_of(l0, i);
       const bool in = k + q16 < K;
       av[i] = __builtin_amdgcn_raw_buffer_load_b128(Wr, in && ina ? ao + k : OOB_OFFSET, 0, 2);
@@ -100,6 +103,21 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
     }
   };
   load_weights(wave);
+  // the epilogue's operands, one tile row and two columns (SwiGLU: one) to a thread
+  const int m = tid >> 4, c = tid & 15, out_row = t.first + m;
+  float sw[2], bias[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int n = SWI ? g * FH + n0 + c : n0 + g * 16 + c;
+    const int64_t at = (int64_t)t.e * p.N + (n < p.N ? n : 0);
+    sw[g] = p.sw[at];
+    bias[g] = !SWI && p.bias ? load_bias(p, at) : 0.0f;
+  }
+  float sx = 0.0f;
+  if constexpr (IN == IN_CODES) {
+    const int tok = token(out_row);
+    if (tok >= 0) sx = p.sx[tok];
+  }
   const int pitch = few_pitch(K);
   __amdgpu_buffer_rsrc_t Xr = make_rsrc(p.x, IN == IN_CODES ? (uint32_t)p.x_rows * (uint32_t)K : 0u);
   uint32_t xo = OOB_OFFSET;
@@ -120,9 +138,9 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
   }
   v4i acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
   for (int l0 = wave; l0 < lines;) {
-    v4i xv[2 * GF_DEEP];
+    v4i xv[2 * DEEP];
 #pragma unroll
-    for (int i = 0; i < 2 * GF_DEEP; ++i) {
+    for (int i = 0; i < 2 * DEEP; ++i) {
       const int k = k_of(l0, i);
       if constexpr (IN == IN_CODES) {
         xv[i] = __builtin_amdgcn_raw_buffer_load_b128(Xr, k + q16 < K && xo != OOB_OFFSET ? xo + k : OOB_OFFSET, 0, 0);
@@ -132,11 +150,11 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2 * GF_DEEP; ++i) {
+    for (int i = 0; i < 2 * DEEP; ++i) {
       acc[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv[i], av[i], acc[0], 0, 0, 0);
       acc[1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xv[i], bv[i], acc[1], 0, 0, 0);
     }
-    l0 += GF_WAVES * GF_DEEP;
+    l0 += GF_WAVES * DEEP;
     if (l0 < lines) load_weights(l0);
   }
 #pragma unroll
@@ -144,30 +162,94 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[wave][g][(lane >> 4) * 4 + i][r16] = acc[g][i];
   __syncthreads();
-  const int m = tid >> 4, c = tid & 15, out_row = t.first + m;
   if (out_row >= t.end) return;
-  float sx;
-  if constexpr (IN == IN_CODES) {
-    const int tok = token(out_row);
-    sx = tok >= 0 ? p.sx[tok] : 0.0f;
-  } else {
-    sx = scale[m];
-  }
+  if constexpr (IN != IN_CODES) sx = scale[m];
   float y[2];
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     int s = 0;
 #pragma unroll
     for (int v = 0; v < GF_WAVES; ++v) s += part[v][g][m][c];
-    const int n = SWI ? g * FH + n0 + c : n0 + g * 16 + c;
-    if (n >= p.N) continue;
-    const int64_t at = (int64_t)t.e * p.N + n;
-    y[g] = __fmul_rn(__fmul_rn((float)s, sx), p.sw[at]);
-    if (p.bias) y[g] = __fadd_rn(y[g], load_bias(p, at));
-    if constexpr (!SWI) store_out<OUT>(p.y, (int64_t)out_row * p.N + n, y[g]);
+    y[g] = __fmul_rn(__fmul_rn((float)s, sx), sw[g]);
+    if constexpr (!SWI) {
+      if (p.bias) y[g] = __fadd_rn(y[g], bias[g]);
+      const int n = n0 + g * 16 + c;
+      if (n < FH) store_out<OUT>(p.y, (int64_t)out_row * FH + n, y[g]);
+    }
   }
-  if constexpr (SWI)
-    if (n0 + c < FH) store_out<OUT>(p.y, (int64_t)out_row * FH + n0 + c, grouped_swiglu<OUT>(y[0], y[1]));
+  if constexpr (SWI) store_out<OUT>(p.y, (int64_t)out_row * FH + n0 + c, grouped_swiglu<OUT>(y[0], y[1]));  // (F is a multiple of 16)
+}
+
+// The second product and the weighted sum in one launch, for a few tokens: a workgroup has 16 columns of one token's output, a wavefront one of its
+// choices at a time: it quantises that row of h, multiplies it with its expert's 16 weight rows and leaves the rounded output times its weight in LDS,
+// where the choices are added in their order: the bits of the grouped Linear and combine_rows.  Experts that several tokens chose are read for each.
+constexpr int GT_WAVES = 8, GT_COLS = 16, GT_LINES = 12;  // lines of 128 bytes on their way at a time
+struct TokenArgs {
+  GroupedArgs g;  // x: h [R, K]
+  const int32_t* rows;
+  const float* weights;
+  const void* res;
+  int k;
+};
+template <int OUT, int VPL>
+__global__ __launch_bounds__(GT_WAVES * 64) void grouped_token_kernel(TokenArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t xs[];  // a row of codes per wavefront
+  __shared__ float term[GP_MAX_TOKEN_K][GT_COLS];
+  __shared__ float scale[GT_WAVES];
+  constexpr bool BF16 = OUT == OUT_BF16;
+  const GroupedArgs& p = a.g;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int K = p.K, N = p.N, t = blockIdx.y, n0 = (int)blockIdx.x * GT_COLS, pitch = few_pitch(K);
+  const int r16 = lane & 15, q16 = (lane >> 4) * 16, n = n0 + r16;
+  uint8_t* const mine = xs + wave * pitch;
+  for (int j = wave; j < a.k; j += GT_WAVES) {
+    const int row = __builtin_amdgcn_readfirstlane(a.rows[(int64_t)t * a.k + j]);
+    float y = 0.0f, w = 0.0f;
+    if (row >= 0 && row < p.R) {
+      int e = 0;  // experts whose rows end at or before it
+      for (int i = lane; i < p.E; i += 64) e += __popcll(__ballot(p.offsets[i + 1] <= row));
+      e = __builtin_amdgcn_readfirstlane(e);
+      if (e < p.E) {
+        const __amdgpu_buffer_rsrc_t Wr = make_rsrc(p.w + e * p.w_bytes, (uint32_t)p.w_bytes);
+        const uint32_t wo = (uint32_t)n * (uint32_t)K + q16;
+        w = a.weights[(int64_t)t * a.k + j];
+        const float sw = p.sw[(int64_t)e * N + n];
+        RowsToLds<BF16, 1, VPL> r;
+        r.issue(p.x + (int64_t)row * K * (BF16 ? 2 : 4), 1, K, K, 0, 1, lane);
+        v4i acc = {0, 0, 0, 0};
+        for (int l0 = 0; l0 * 128 < K; l0 += GT_LINES) {
+          v4i wv[2 * GT_LINES];
+#pragma unroll
+          for (int i = 0; i < 2 * GT_LINES; ++i) {
+            const int k = l0 * 128 + i * 64;
+            wv[i] = __builtin_amdgcn_raw_buffer_load_b128(Wr, k + q16 < K ? wo + k : OOB_OFFSET, 0, 2);
+          }
+          if (l0 == 0) {
+            r.finish(1, 1, K, mine, pitch, scale + wave, 0, 1, lane);
+            __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS operations keep their order)
+          }
+#pragma unroll
+          for (int i = 0; i < 2 * GT_LINES; ++i) {
+            const int k = l0 * 128 + i * 64;
+            if (k < K) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(mine + k + q16), wv[i], acc, 0, 0, 0);
+          }
+        }
+        y = __fmul_rn(__fmul_rn((float)acc[0], scale[wave]), sw);  // (every row of the operand is this row)
+        if constexpr (BF16) y = bf16_bits_to_f32(f32_to_bf16_bits(y));
+      }
+    }
+    if (lane < GT_COLS) term[j][lane] = __fmul_rn(w, y);
+  }
+  __syncthreads();
+  if (tid >= GT_COLS) return;
+  float sum = 0.0f;
+  for (int j = 0; j < a.k; ++j) {
+    const int row = a.rows[(int64_t)t * a.k + j];
+    if (row >= 0 && row < p.R) sum = __fadd_rn(sum, term[j][tid]);
+  }
+  const int64_t at = (int64_t)t * N + n0 + tid;
+  if (a.res) sum = __fadd_rn(sum, BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(a.res)[at]) : static_cast<const float*>(a.res)[at]);
+  store_out<OUT>(p.y, at, sum);
 }
 
 #ifdef AQ_LAB
@@ -186,13 +268,18 @@ static int choose_grouped(const GroupedArgs& a) {
   return used * ((a.N + 255) / 256) >= 1.75 * device_cus() || a.R > 24 * a.E ? GROUPED_WALK_256 : GROUPED_FEW;
 }
 
-template <int OUT, bool SWI, int IN, int VPL>
-static int launch_few(const GroupedArgs& a, hipStream_t st) {
+template <int OUT, bool SWI, int IN, int VPL, int DEEP>
+static int launch_few_of(const GroupedArgs& a, hipStream_t st) {
   const int64_t tiles = grouped_most_tiles(a.R, a.E, GF_ROWS), cols = (a.N + GF_COLS - 1) / GF_COLS;
   if (tiles > 65535 || cols > 0x7fffffff) return AQ_E_RANGE;
-  queue_kernel((grouped_few_kernel<OUT, SWI, IN, VPL>), dim3((unsigned)cols, (unsigned)tiles), dim3(GF_WAVES * 64),
+  queue_kernel((grouped_few_kernel<OUT, SWI, IN, VPL, DEEP>), dim3((unsigned)cols, (unsigned)tiles), dim3(GF_WAVES * 64),
                IN == IN_CODES ? 0 : GF_ROWS * few_pitch(a.K), st, a);
   return (int)hipGetLastError();
+}
+
+template <int OUT, bool SWI, int IN, int VPL>
+static int launch_few(const GroupedArgs& a, hipStream_t st) {
+  return a.K <= GF_WAVES * 3 * 128 ? launch_few_of<OUT, SWI, IN, VPL, 3>(a, st) : launch_few_of<OUT, SWI, IN, VPL, 4>(a, st);
 }
 
 // Rows as they are (a.x of `dtype`, which is the output's type too), quantised in the launch.
@@ -211,6 +298,18 @@ static bool rows_in_launch(int64_t T, int64_t k, int64_t dim, int64_t F, int dty
   if (g_forced_grouped) return g_forced_grouped == GROUPED_FEW;
 #endif
   return T * k <= 16;
+}
+
+// The second product with the weighted sum, up to GT_TOKENS tokens (dim is a multiple of 16, and so of GT_COLS).
+constexpr int64_t GT_TOKENS = 2;
+template <int OUT, int VPL>
+static int launch_token(const TokenArgs& a, int64_t T, hipStream_t st) {
+  queue_kernel((grouped_token_kernel<OUT, VPL>), dim3((unsigned)(a.g.N / GT_COLS), (unsigned)T), dim3(GT_WAVES * 64), GT_WAVES * few_pitch(a.g.K), st, a);
+  return (int)hipGetLastError();
+}
+static int launch_tokens(const TokenArgs& a, int64_t T, int dtype, hipStream_t st) {
+  if (dtype == AQ_BF16) return a.g.K <= 2048 ? launch_token<OUT_BF16, 4>(a, T, st) : launch_token<OUT_BF16, 8>(a, T, st);
+  return a.g.K <= 1024 ? launch_token<OUT_F32, 4>(a, T, st) : launch_token<OUT_F32, 8>(a, T, st);
 }
 
 template <int OUT, bool SWI>
@@ -338,6 +437,10 @@ extern "C" int aq_experts_w8a8(const void* x, int x_dtype, int64_t T, int64_t di
     a.w_bytes = dim * F;
     a.N = (int)dim;
     a.K = (int)F;
+    if (rc == AQ_OK && T <= aq::GT_TOKENS) {
+      a.y = out;
+      return aq::launch_tokens(aq::TokenArgs{a, rows, weights, residual, (int)k}, T, x_dtype, static_cast<hipStream_t>(stream));
+    }
     if (rc == AQ_OK) rc = aq::launch_rows<false>(a, x_dtype, static_cast<hipStream_t>(stream));
   } else {
     rc = aq_quant_rowwise_i8(x, x_dtype, T, dim, dim, xq, sx, stream);

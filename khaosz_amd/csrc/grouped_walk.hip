@@ -1,8 +1,7 @@
 // Grouped products of many rows an expert: tiles of 128 rows x 256 weight rows, walked by one workgroup per compute unit whose K loop does not stop
 // between them (as gemm_walk.hip walks the tiles of a single Linear).
 //
-// Every workgroup takes the offsets into LDS, and a wavefront's lanes hold the running count of tiles, so that a tile's expert is two ballots
-// away.  Inside an expert tiles go in groups of 8 by rows, then by columns: the 32 tiles that an XCD works on at a time share 2 MB of rows and 2 MB of
+// Inside an expert tiles go in groups of 8 by rows, then by columns: the 32 tiles that an XCD works on at a time share 2 MB of rows and 2 MB of
 // weights.  The rows' tokens of the next tile are fetched into LDS under this tile's first step, for its first stages are requested in the
 // last steps.
 #include "aq_grouped.h"
@@ -64,21 +63,9 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
   int32_t* const tok_lds = reinterpret_cast<int32_t*>(smem + S::TOK);
   int32_t* const off = reinterpret_cast<int32_t*>(smem + S::OFF);
 
-  for (int e = tid; e <= p.E; e += GW_THREADS) {
-    const int o = p.offsets[e];
-    off[e] = o < 0 ? 0 : o > p.R ? p.R : o;
-  }
-  __syncthreads();
-  const int per = (p.E + 63) >> 6;  // experts of a lane
-  auto tiles_of = [&](int e) {
-    const int rows = e < p.E ? off[e + 1] - off[e] : 0;
-    return rows > 0 ? (rows + GW_BM - 1) / GW_BM : 0;
-  };
-  int mine = 0;
-  for (int i = 0; i < per; ++i) mine += tiles_of(lane * per + i);
-  const int upto = wave_scan(mine);
-  const int64_t all_tiles = (int64_t)__builtin_amdgcn_readlane(upto, 63) * tiles_n;  // (offsets that fall can make it more than was launched for)
-  const int count = all_tiles < 0x7fffffff ? (int)all_tiles : 0x7fffffff;
+  GroupTiles<GW_BM> tiles;
+  tiles.init(p, off, tid, GW_THREADS);
+  const int count = tiles.count(tiles_n);
   int id = blockIdx.x;
   if (id >= count) return;
 
@@ -87,21 +74,13 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
     const int share = count / NUM_XCD, rest = count % NUM_XCD, xcd = pid % NUM_XCD;
     const int t = xcd * share + (xcd < rest ? xcd : rest) + pid / NUM_XCD;
     const int q = (int)by_tiles_n((uint32_t)t);  // tiles of rows before it, of experts before its own for sure
-    const int at = __builtin_ctzll(__ballot(upto > q));
-    const int e0 = at * per, before = __builtin_amdgcn_readlane(upto - mine, at);
-    const int n = lane < per ? tiles_of(e0 + lane) : 0;  // (per <= 8: a row of 16 lanes)
-    int in = n;
-    in += __builtin_amdgcn_update_dpp(0, in, 0x111, 0xf, 0xf, false);
-    in += __builtin_amdgcn_update_dpp(0, in, 0x112, 0xf, 0xf, false);
-    in += __builtin_amdgcn_update_dpp(0, in, 0x114, 0xf, 0xf, false);
-    const int sub = __builtin_ctzll(__ballot(lane < per && before + in > q));
-    const int tiles_m = __builtin_amdgcn_readlane(n, sub);
-    const int rem = t - (before + __builtin_amdgcn_readlane(in, sub) - tiles_m) * tiles_n;
+    const auto expert = tiles.find(q, lane);
+    const int rem = t - expert.before * tiles_n;
     const int group_sz = GW_GROUP * tiles_n, group = rem / group_sz, first_m = group * GW_GROUP;
-    const int gm = tiles_m - first_m < GW_GROUP ? tiles_m - first_m : GW_GROUP, in_group = rem - group * group_sz;
+    const int gm = expert.tiles - first_m < GW_GROUP ? expert.tiles - first_m : GW_GROUP, in_group = rem - group * group_sz;
     const int n_at = in_group / gm;
     WalkTile w;
-    w.e = __builtin_amdgcn_readfirstlane(e0 + sub);
+    w.e = __builtin_amdgcn_readfirstlane(expert.e);
     w.first = __builtin_amdgcn_readfirstlane(off[w.e] + (first_m + in_group - n_at * gm) * GW_BM);
     w.end = __builtin_amdgcn_readfirstlane(off[w.e + 1]);
     w.n0 = __builtin_amdgcn_readfirstlane(n_at * (SWI ? BN / 2 : BN));
