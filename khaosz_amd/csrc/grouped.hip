@@ -49,7 +49,10 @@ __device__ __forceinline__ bool find_tile(const GroupedArgs& p, int idx, int lan
 }
 template <int BM>
 __device__ __forceinline__ bool find_tile(const GroupedArgs& p, int idx, int lane, RowTile& t) {
-  return p.E <= 64 ? find_tile<BM, 1>(p, idx, lane, t) : find_tile<BM, GP_MAX_E / 64>(p, idx, lane, t);
+  return p.E <= 64    ? find_tile<BM, 1>(p, idx, lane, t)
+         : p.E <= 128 ? find_tile<BM, 2>(p, idx, lane, t)
+         : p.E <= 256 ? find_tile<BM, 4>(p, idx, lane, t)
+                      : find_tile<BM, GP_MAX_E / 64>(p, idx, lane, t);
 }
 
 __device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
@@ -183,7 +186,7 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
 // The second product and the weighted sum in one launch, for a few tokens: a workgroup has 16 columns of one token's output, a wavefront one of its
 // choices at a time: it quantises that row of h, multiplies it with its expert's 16 weight rows and leaves the rounded output times its weight in LDS,
 // where the choices are added in their order: the bits of the grouped Linear and combine_rows.  Experts that several tokens chose are read for each.
-constexpr int GT_WAVES = 8, GT_COLS = 16, GT_LINES = 12;  // lines of 128 bytes on their way at a time
+constexpr int GT_WAVES = 8, GT_COLS = 16;
 struct TokenArgs {
   GroupedArgs g;  // x: h [R, K]
   const int32_t* rows;
@@ -191,8 +194,10 @@ struct TokenArgs {
   const void* res;
   int k;
 };
-template <int OUT, int VPL>
-__global__ __launch_bounds__(GT_WAVES * 64) void grouped_token_kernel(TokenArgs a) {
+// LINES: of 128 bytes of each weight row on their way at a time.  12 where a compute unit has one workgroup at most, 4 where it can have two (one token,
+// 2 of 8 experts of 1536 / 2816: 19.0 us, 21.4 with 4; four tokens, 6 of 64 of 2048 / 1408: 47.1, 45.5 with 4).
+template <int OUT, int VPL, int LINES>
+__global__ __launch_bounds__(GT_WAVES * 64, LINES == 4 ? 4 : 2) void grouped_token_kernel(TokenArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t xs[];  // a row of codes per wavefront
   __shared__ float term[GP_MAX_TOKEN_K][GT_COLS];
   __shared__ float scale[GT_WAVES];
@@ -217,10 +222,10 @@ __global__ __launch_bounds__(GT_WAVES * 64) void grouped_token_kernel(TokenArgs 
         RowsToLds<BF16, 1, VPL> r;
         r.issue(p.x + (int64_t)row * K * (BF16 ? 2 : 4), 1, K, K, 0, 1, lane);
         v4i acc = {0, 0, 0, 0};
-        for (int l0 = 0; l0 * 128 < K; l0 += GT_LINES) {
-          v4i wv[2 * GT_LINES];
+        for (int l0 = 0; l0 * 128 < K; l0 += LINES) {
+          v4i wv[2 * LINES];
 #pragma unroll
-          for (int i = 0; i < 2 * GT_LINES; ++i) {
+          for (int i = 0; i < 2 * LINES; ++i) {
             const int k = l0 * 128 + i * 64;
             wv[i] = __builtin_amdgcn_raw_buffer_load_b128(Wr, k + q16 < K ? wo + k : OOB_OFFSET, 0, 2);
           }
@@ -229,7 +234,7 @@ __global__ __launch_bounds__(GT_WAVES * 64) void grouped_token_kernel(TokenArgs 
             __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS operations keep their order)
           }
 #pragma unroll
-          for (int i = 0; i < 2 * GT_LINES; ++i) {
+          for (int i = 0; i < 2 * LINES; ++i) {
             const int k = l0 * 128 + i * 64;
             if (k < K) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(mine + k + q16), wv[i], acc, 0, 0, 0);
           }
@@ -256,7 +261,10 @@ __global__ __launch_bounds__(GT_WAVES * 64) void grouped_token_kernel(TokenArgs 
 static int g_forced_grouped = 0;  // lab build only: 0 = by size
 #endif
 
-// Which kernel: walked tiles where they are at least 7 to 4 compute units (R rows dealt out evenly reach E (1 - e^(-R / E)) experts), or where experts
+// Experts with rows, of E, when R rows are dealt out evenly.
+static double experts_used(int64_t R, int64_t E) { return E * (1.0 - std::exp(-(double)R / E)); }
+
+// Which kernel: walked tiles where they are at least 7 to 4 compute units, or where experts
 // have more rows than the tile of 16.
 enum { GROUPED_FEW = 1, GROUPED_WALK_256 = 2, GROUPED_WALK_128 = 3, GROUPED_WALK_64 = 4 };
 static int choose_grouped(const GroupedArgs& a) {
@@ -264,8 +272,7 @@ static int choose_grouped(const GroupedArgs& a) {
 #ifdef AQ_LAB
   if (g_forced_grouped) return g_forced_grouped;
 #endif
-  const double used = a.E * (1.0 - std::exp(-(double)a.R / a.E));
-  return used * ((a.N + 255) / 256) >= 1.75 * device_cus() || a.R > 24 * a.E ? GROUPED_WALK_256 : GROUPED_FEW;
+  return experts_used(a.R, a.E) * ((a.N + 255) / 256) >= 1.75 * device_cus() || a.R > 24 * a.E ? GROUPED_WALK_256 : GROUPED_FEW;
 }
 
 template <int OUT, bool SWI, int IN, int VPL, int DEEP>
@@ -290,26 +297,37 @@ static int launch_rows(const GroupedArgs& a, int dtype, hipStream_t st) {
     return a.K <= 2048 ? launch_few<OUT_BF16, SWI, IN_BF16, 4>(a, st) : launch_few<OUT_BF16, SWI, IN_BF16, 8>(a, st);
   return a.K <= 1024 ? launch_few<OUT_F32, SWI, IN_F32, 4>(a, st) : launch_few<OUT_F32, SWI, IN_F32, 8>(a, st);
 }
-// Whether the two products of a layer quantise their rows themselves.
-static bool rows_in_launch(int64_t T, int64_t k, int64_t dim, int64_t F, int dtype) {
-  const int64_t most = dtype == AQ_BF16 ? GF_IN_BF16_K : GF_IN_F32_K;
+// Whether the two products of a layer quantise their rows themselves: two launches less, but every workgroup rounds its tile's rows, and tiles of 16 rows
+// stream weights at 5.6 TB/s where walked ones reach 6.3 (us, with | without: 16 tokens' 6 of 64 of 2048 / 1408 91 | 99, 32 tokens' 113 | 109;
+// 16 tokens' 2 of 8 of 1536 / 2816 38 | 41, 32 tokens' 43.5 | 43.6).
+static bool rows_in_launch(int64_t T, int64_t k, int64_t E, int64_t dim, int64_t F, int dtype) {
+  const int64_t most = dtype == AQ_BF16 ? GF_IN_BF16_K : GF_IN_F32_K, R = T * k;
   if (dim > most || F > most) return false;
 #ifdef AQ_LAB
   if (g_forced_grouped) return g_forced_grouped == GROUPED_FEW;
 #endif
-  return T * k <= 16;
+  return experts_used(R, E) * (double)(3 * dim * F) * (1.0 + (double)R / E) <= 1.2e9;
 }
 
-// The second product with the weighted sum, up to GT_TOKENS tokens (dim is a multiple of 16, and so of GT_COLS).
-constexpr int64_t GT_TOKENS = 2;
+// The second product with the weighted sum (dim is a multiple of 16, and so of GT_COLS).
 template <int OUT, int VPL>
 static int launch_token(const TokenArgs& a, int64_t T, hipStream_t st) {
-  queue_kernel((grouped_token_kernel<OUT, VPL>), dim3((unsigned)(a.g.N / GT_COLS), (unsigned)T), dim3(GT_WAVES * 64), GT_WAVES * few_pitch(a.g.K), st, a);
+  const dim3 grid((unsigned)(a.g.N / GT_COLS), (unsigned)T), block(GT_WAVES * 64);
+  const size_t lds = (size_t)GT_WAVES * few_pitch(a.g.K);
+  bool deep = true;
+  if constexpr (VPL == 4) deep = (int64_t)grid.x * T <= device_cus();  // (rows of 8 vectors a lane leave no room for two)
+  if (deep) queue_kernel((grouped_token_kernel<OUT, VPL, 12>), grid, block, lds, st, a);
+  else if constexpr (VPL == 4) queue_kernel((grouped_token_kernel<OUT, VPL, 4>), grid, block, lds, st, a);
   return (int)hipGetLastError();
 }
 static int launch_tokens(const TokenArgs& a, int64_t T, int dtype, hipStream_t st) {
   if (dtype == AQ_BF16) return a.g.K <= 2048 ? launch_token<OUT_BF16, 4>(a, T, st) : launch_token<OUT_BF16, 8>(a, T, st);
   return a.g.K <= 1024 ? launch_token<OUT_F32, 4>(a, T, st) : launch_token<OUT_F32, 8>(a, T, st);
+}
+// Whether it is: what the experts of several tokens cost more, read for each, is then less than the launch saved (us, with | without: 64 tokens' 16 on 256
+// experts of 1024 / 512, 4 MB more, 30.1 | 35.9; 4 tokens' 6 of 64 of 2048 / 1408, 11 MB, 45.5 | 46.3; 6 tokens', 22 MB, 65.6 | 58.7).
+static bool tokens_in_launch(int64_t T, int64_t k, int64_t E, int64_t dim, int64_t F) {
+  return T <= 65535 && ((double)(T * k) - experts_used(T * k, E)) * (double)(dim * F) <= 8e6;
 }
 
 template <int OUT, bool SWI>
@@ -413,7 +431,7 @@ extern "C" int aq_experts_w8a8(const void* x, int x_dtype, int64_t T, int64_t di
   float *const sx = reinterpret_cast<float*>(ws + s.sx), *const sh = reinterpret_cast<float*>(ws + s.sh);
   void *const h = ws + s.h, *const y = ws + s.y;
   int rc;
-  if (aq::rows_in_launch(T, k, dim, F, x_dtype)) {
+  if (aq::rows_in_launch(T, k, E, dim, F, x_dtype)) {
     aq::GroupedArgs a{};
     a.x = static_cast<const uint8_t*>(x);
     a.x_rows = (int)T;
@@ -437,7 +455,7 @@ extern "C" int aq_experts_w8a8(const void* x, int x_dtype, int64_t T, int64_t di
     a.w_bytes = dim * F;
     a.N = (int)dim;
     a.K = (int)F;
-    if (rc == AQ_OK && T <= aq::GT_TOKENS) {
+    if (rc == AQ_OK && aq::tokens_in_launch(T, k, E, dim, F)) {
       a.y = out;
       return aq::launch_tokens(aq::TokenArgs{a, rows, weights, residual, (int)k}, T, x_dtype, static_cast<hipStream_t>(stream));
     }
