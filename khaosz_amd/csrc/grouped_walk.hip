@@ -17,7 +17,7 @@ template <int WM_, int TN_, int NST_>
 struct GroupedShape {
   static constexpr int WM = WM_, WN = 8 / WM_, TM = 4 / WM_, TN = TN_, BN = 32 * TN * WN, NST = NST_;
   static constexpr int STAGE = (GW_BM + BN) * GW_BK;
-  static constexpr int SX = NST * STAGE, TOK = SX + 8 * 64 * 4, OFF = TOK + GW_BM * 4, LDS = OFF + (GP_MAX_E + 1) * 4;
+  static constexpr int SX = NST * STAGE, TOK = SX + 2 * 8 * 64 * 4, OFF = TOK + GW_BM * 4, LDS = OFF + (GP_MAX_E + 1) * 4;
   static_assert(LDS <= 160 * 1024, "LDS of one compute unit");
   static_assert(NST >= 3, "a stage in use, one that lands, one on its way");
 };
@@ -44,7 +44,7 @@ struct WalkTile {
   int e, first, end, n0;  // rows first .. end - 1 (end of the expert's rows) by columns from n0 (SwiGLU: of h)
 };
 
-template <class S, int OUT, bool SWI>
+template <class S, int OUT, bool SWI, bool ODD>
 __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p, int tiles_n, UDiv by_tiles_n) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass drops a kernel in whose generic lambdas it finds the device's operations)
   __shared__ __attribute__((aligned(1024))) uint8_t smem[S::LDS];
@@ -53,13 +53,17 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
   constexpr int BEHIND = (NST - 2) * NLOADS;       // loads behind the next stage's when a step ends
   static_assert(!SWI || TN == 2, "up and gate in one lane");
   constexpr int V = SWI || TN == 1 ? 1 : 2;  // neighbouring outputs of a lane
+  constexpr int ESZ = OUT == OUT_BF16 ? 2 : 4;
+  constexpr int EPI = 4;                     // steps that finish the tile before
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wave_m = wave / S::WN, wave_n = wave % S::WN;
   const int K = p.K, N = p.N, FH = SWI ? N / 2 : N;
-  const int steps = (K + BK - 1) / BK, nk = steps < 2 * AHEAD ? 2 * AHEAD : steps;  // (steps past K are of zeros)
+  const int steps = (K + BK - 1) / BK, least = EPI + AHEAD > 2 * AHEAD ? EPI + AHEAD : 2 * AHEAD;
+  const int nk = steps < least ? least : steps;  // (steps past K are of zeros)
   const int col = lane & 31, rq = (lane >> 5) * 4;
-  float* const sx_lds = reinterpret_cast<float*>(smem + S::SX) + wave * 64;
+  float* sx_lds = reinterpret_cast<float*>(smem + S::SX) + wave * 128;  // row scales of this wavefront, of this tile ..
+  float* sx_done = sx_lds + 64;                                         // .. and of the one before
   int32_t* const tok_lds = reinterpret_cast<int32_t*>(smem + S::TOK);
   int32_t* const off = reinterpret_cast<int32_t*>(smem + S::OFF);
 
@@ -141,17 +145,87 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
     if (is_a) a[idx] = v;
     else b[idx] = v;
   };
-  // One sub-step: its products, the next sub-step's fragment reads and the loads [LD0, LD1) of the requested stage between them
-  auto slot = [&](auto tm_c, auto cur_c, const uint8_t* st_next, int ks_next, int k_ld, int b_ld, auto lo_c, auto hi_c) {
-    constexpr int CUR = decltype(cur_c)::value, LD0 = decltype(lo_c)::value, NLD = decltype(hi_c)::value - LD0;
+  // The tile before, as its sums and what finishes them: every step of the first EPI has two or four of its rows' outputs between its products
+  // (finished in one go, with the matrix core idle, they took a quarter of the time at K = 1408: 48000 rows of 1408 -> 2048 182 us).  Rows that it did
+  // not have fall outside the window.
+  struct Done {
+    v16i acc[TM][TN];
+    float sw[TN], bias[TN];
+    __amdgpu_buffer_rsrc_t out;
+    uint32_t at, at1;  // at1: an odd N's second column, by itself
+  };
+  Done done;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = done.acc[i][j][r] = 0;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) done.sw[j] = done.bias[j] = 0.0f;
+  done.out = make_rsrc(p.y, 0);
+  done.at = done.at1 = OOB_OFFSET;
+  const uint32_t rowb = (uint32_t)FH * ESZ;
+  const bool odd_lane = lane & 1;
+  constexpr int ROW_STORES = V == 1 && OUT == OUT_BF16 && !ODD ? 2 : V == 2 && ODD ? 8 : 4;  // of four rows, per lane
+  v4f sxq;
+  float held = 0.0f;
+  // row q of the four rows 8 g + rq .. of accumulator row i: three rounded operations; bf16 neighbours go as a dword
+  auto finish = [&](int i, int g, int q) {
+    const int r0 = i * 32 + g * 8;
+    if (q == 0) sxq = *reinterpret_cast<const v4f*>(sx_done + r0 + rq);
+    float y[TN], o[V];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      y[j] = __fmul_rn(__fmul_rn((float)done.acc[i][j][g * 4 + q], sxq[q]), done.sw[j]);
+      if constexpr (!SWI) y[j] = __fadd_rn(y[j], done.bias[j]);
+    }
+    if constexpr (SWI) {
+      o[0] = grouped_swiglu<OUT>(y[0], y[1]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) o[v] = y[v];
+    }
+    const uint32_t at = done.at + (r0 + q) * rowb;
+    if constexpr (V == 2 && ODD) {
+      const uint32_t at1 = done.at1 + (r0 + q) * rowb;
+      if constexpr (OUT == OUT_F32) {
+        store_dword<0>(__float_as_uint(o[0]), done.out, at);
+        store_dword<0>(__float_as_uint(o[V - 1]), done.out, at1);
+      } else {
+        store_word(f32_to_bf16_bits(o[0]), done.out, at);
+        store_word(f32_to_bf16_bits(o[V - 1]), done.out, at1);
+      }
+    } else if constexpr (V == 2) {
+      if constexpr (OUT == OUT_F32) store_pair(o[0], o[V - 1], done.out, at);
+      else store_dword(pack_bf16x2(o[0], o[V - 1]), done.out, at);
+    } else if constexpr (OUT == OUT_F32) {
+      store_dword(__float_as_uint(o[0]), done.out, at);
+    } else if constexpr (ODD) {
+      store_word(f32_to_bf16_bits(o[0]), done.out, at);
+    } else {  // two rows of two neighbouring lanes
+      if (q & 1) store_dword(pair_columns(pack_bf16x2(held, o[0]), odd_lane), done.out, at - rowb);
+      held = o[0];
+    }
+  };
+  // One sub-step: its products (FIRST: of a tile), the next sub-step's fragment reads and the loads [LD0, LD1) of the requested stage between them,
+  // and, with ROW >= 0, four rows (part `g`) of accumulator row ROW of the tile before.
+  auto slot = [&](auto tm_c, auto first_c, auto row_c, int g, auto cur_c, const uint8_t* st_next, int ks_next, int k_ld, int b_ld, auto lo_c, auto hi_c) {
+    constexpr int CUR = decltype(cur_c)::value, LD0 = decltype(lo_c)::value, NLD = decltype(hi_c)::value - LD0, ROW = decltype(row_c)::value;
     constexpr int NMMA = decltype(tm_c)::value * TN, NFR = TM + TN;
 #pragma unroll
     for (int m = 0; m < NMMA; ++m) {
-      acc[m / TN][m % TN] = mma<false>(af[CUR][m / TN], bf[CUR][m % TN], acc[m / TN][m % TN]);
+      v16i c = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+      if constexpr (!decltype(first_c)::value) c = acc[m / TN][m % TN];
+      acc[m / TN][m % TN] = mma<false>(af[CUR][m / TN], bf[CUR][m % TN], c);
 #pragma unroll
       for (int f = (m * NFR) / NMMA; f < ((m + 1) * NFR) / NMMA; ++f) load_frag(st_next, ks_next, f, af[CUR ^ 1], bf[CUR ^ 1]);
 #pragma unroll
       for (int q = (m * NLD) / NMMA; q < ((m + 1) * NLD) / NMMA; ++q) issue_load(k_ld, b_ld, LD0 + q);
+      if constexpr (ROW >= 0) {
+#pragma unroll
+        for (int q = (m * 4) / NMMA; q < ((m + 1) * 4) / NMMA; ++q) finish(ROW, g, q);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -162,18 +236,23 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
   using l2 = std::integral_constant<int, NLOADS * 2 / 3>;
   using all = std::integral_constant<int, NLOADS>;
   int b_cur = 0;  // buffer of the current stage
+  using no = std::false_type;
+  using none = std::integral_constant<int, -1>;
   // A K step of a tile with TMV accumulator rows: its first fragments are in af[0].  Requests the stage AHEAD steps on into the buffer that the
-  // step before left, and waits for the next one: `behind` says how.
-  auto step = [&](auto tm_c, int k_ld, auto&& behind) {
+  // step before left, and waits for the next one: `behind` says how.  FIRST: of the tile.  DONE: part `g` of the tile before is finished in it.
+  auto step = [&](auto tm_c, auto first_c, auto done_c, int g, int k_ld, auto&& behind) {
+    constexpr bool DONE = decltype(done_c)::value;
+    using row0 = std::integral_constant<int, DONE ? 0 : -1>;
+    using row1 = std::integral_constant<int, DONE && TM == 2 ? 1 : -1>;
     const int b_next = b_cur == NST - 1 ? 0 : b_cur + 1, b_prev = b_cur == 0 ? NST - 1 : b_cur - 1;
     const uint8_t *st = smem + b_cur * S::STAGE, *st_next = smem + b_next * S::STAGE;
-    slot(tm_c, c0{}, st, 1, k_ld, b_prev, c0{}, l1{});
-    slot(tm_c, c1{}, st, 2, k_ld, b_prev, l1{}, l2{});
-    slot(tm_c, c0{}, st, 3, k_ld, b_prev, l2{}, all{});
+    slot(tm_c, first_c, row0{}, g, c0{}, st, 1, k_ld, b_prev, c0{}, l1{});
+    slot(tm_c, no{}, none{}, g, c1{}, st, 2, k_ld, b_prev, l1{}, l2{});
+    slot(tm_c, no{}, row1{}, g, c0{}, st, 3, k_ld, b_prev, l2{}, all{});
     __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the last fragments of the stage are in registers
     behind();                            // the next stage has landed
     AQ_BARRIER();
-    slot(tm_c, c1{}, st_next, 0, k_ld, b_cur, all{}, all{});
+    slot(tm_c, no{}, none{}, g, c1{}, st_next, 0, k_ld, b_cur, all{}, all{});
     b_cur = b_next;
   };
   static_assert(NKS == 4, "four sub-steps");
@@ -197,18 +276,9 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
 #pragma unroll
   for (int f = 0; f < TM + TN; ++f) load_frag(smem, 0, f, af[0], bf[0]);
 
-  constexpr int ESZ = OUT == OUT_BF16 ? 2 : 4;
-  constexpr int ROW_STORES = V == 1 && OUT == OUT_BF16 ? 8 : 16;  // of an accumulator row, per lane, at least
   const __amdgpu_buffer_rsrc_t Tr = make_rsrc(p.tokens, gather ? (uint32_t)p.R * 4u : 0u);
-  int stores = 0;  // accumulator rows that the tile before stored
   auto tile = [&](auto tm_c) {  // false: it was the last
     constexpr int TMV = decltype(tm_c)::value;
-#pragma unroll
-    for (int i = 0; i < TMV; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
     id += gridDim.x;
     const bool last = id >= count;
     WalkTile next = now;
@@ -217,19 +287,17 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
     if (lane < 16)
       fetch_dword_to_lds(Tr, tok_lds + wave * 16, (uint32_t)(next.first + wave * 16 + lane) * 4u);
     int k0 = AHEAD * BK;
+    // behind the next stage's loads: the step's stores, and in the first step the tokens
+    step(tm_c, std::true_type{}, std::true_type{}, 0, k0, [&]() { AQ_WAIT_VMCNT(BEHIND + 1 + TM * ROW_STORES); });
+    k0 += BK;
 #pragma unroll
-    for (int s = 0; s < NST - 2; ++s, k0 += BK)
-      step(tm_c, k0, [&]() {  // behind the next stage's loads: the stores of the tile before and the tokens, too
-        if (stores == 2) AQ_WAIT_VMCNT(BEHIND + 1 + 2 * ROW_STORES);
-        else if (stores == 1) AQ_WAIT_VMCNT(BEHIND + 1 + ROW_STORES);
-        else AQ_WAIT_VMCNT(BEHIND + 1);
-      });
-    for (int s = NST - 2; s < nk - AHEAD; ++s, k0 += BK) step(tm_c, k0, landed);
+    for (int g = 1; g < EPI; ++g, k0 += BK) step(tm_c, no{}, std::true_type{}, g, k0, [&]() { AQ_WAIT_VMCNT(BEHIND + TM * ROW_STORES); });
+    for (int s = EPI; s < nk - AHEAD; ++s, k0 += BK) step(tm_c, no{}, no{}, 0, k0, landed);
     // the epilogue's operands, then the next tile's first stages
     const int mw = now.first + first_row(now), nt = now.n0, end = now.end;
     const int64_t scales = (int64_t)now.e * N;
     auto my_column = [&](int j) { return nt + (V == 2 ? wave_n * 64 + 2 * col + j : wave_n * 32 + col); };  // of h or y
-    float swn[TN], bn[TN];
+    float swn[TN];
     const __amdgpu_buffer_rsrc_t Wr = make_rsrc(p.sw + scales, (uint32_t)N * 4u);
     if (lane < 32 * TM)
       fetch_dword_to_lds(Sr, sx_lds, my_tok >= 0 ? (uint32_t)my_tok * 4u : OOB_OFFSET);
@@ -259,79 +327,34 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
       for (int i = 0; i < NLOADS; ++i) vo[i] = OOB_OFFSET;
     }
 #pragma unroll
-    for (int s = 0; s < AHEAD - 1; ++s) step(tm_c, s * BK, landed);
-    step(tm_c, (AHEAD - 1) * BK, [&]() {
+    for (int s = 0; s < AHEAD - 1; ++s) step(tm_c, no{}, no{}, 0, s * BK, landed);
+    step(tm_c, no{}, no{}, 0, (AHEAD - 1) * BK, [&]() {
       landed();
       fr_a = next_fr_a;  // (the fragments read behind this step's barrier are the next tile's)
     });
     asm volatile("" ::: "memory");
 
-    // ---- epilogue: three rounded operations, then bf16 rows of neighbouring columns a dword a lane
-    const uint32_t rowb = (uint32_t)FH * ESZ;
+    // what finishes it, under the next tile's first steps
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) done.acc[i][j] = acc[i][j];
     const int rows = end - mw < 32 * TMV ? end - mw : 32 * TMV;
     const uint32_t window = rows > 0 ? (uint32_t)rows * rowb - (uint32_t)nt * ESZ : 0u;
-    const __amdgpu_buffer_rsrc_t Cr =
-        make_rsrc(static_cast<uint8_t*>(p.y) + (rows > 0 ? ((int64_t)mw * FH + nt) * ESZ : 0), window);
+    done.out = make_rsrc(static_cast<uint8_t*>(p.y) + (rows > 0 ? ((int64_t)mw * FH + nt) * ESZ : 0), window);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) bn[j] = !has_bias ? 0.0f : bias_bf16 ? bf16_bits_to_f32(braw[j]) : __uint_as_float(braw[j]);
-    const bool odd = lane & 1, even_n = SWI || (N & 1) == 0;
-    const uint32_t c = (uint32_t)(my_column(0) - nt);
-    uint32_t at = OOB_OFFSET, at1 = OOB_OFFSET;  // at1: an odd N's second column, by itself
-    if (my_column(0) < FH) at = (uint32_t)rq * rowb + (V == 1 && OUT == OUT_BF16 && even_n ? (c & ~1u) * 2 + (odd ? rowb : 0u) : c * ESZ);
-    if (V == 2 && my_column(1) < FH) at1 = (uint32_t)rq * rowb + (c + 1) * ESZ;
-#pragma unroll
-    for (int i = 0; i < TMV; ++i) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int r0 = i * 32 + g * 8;
-        const v4f sxq = *reinterpret_cast<const v4f*>(sx_lds + r0 + rq);
-        float y[TN][4], o[V][4];
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            y[j][q] = __fmul_rn(__fmul_rn((float)acc[i][j][g * 4 + q], sxq[q]), swn[j]);
-            if constexpr (!SWI) y[j][q] = has_bias ? __fadd_rn(y[j][q], bn[j]) : y[j][q];
-          }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if constexpr (SWI) o[0][q] = grouped_swiglu<OUT>(y[0][q], y[1][q]);
-          else
-#pragma unroll
-            for (int v = 0; v < V; ++v) o[v][q] = y[v][q];
-        }
-        if constexpr (V == 1 && OUT == OUT_F32) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) store_dword(__float_as_uint(o[0][q]), Cr, at + (r0 + q) * rowb);
-        } else if constexpr (V == 1) {
-          if (even_n) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) store_dword(pair_columns(pack_bf16x2(o[0][2 * h], o[0][2 * h + 1]), odd), Cr, at + (r0 + 2 * h) * rowb);
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) store_word(f32_to_bf16_bits(o[0][q]), Cr, at + (r0 + q) * rowb);
-          }
-        } else if (even_n) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if constexpr (OUT == OUT_F32) store_pair(o[0][q], o[V - 1][q], Cr, at + (r0 + q) * rowb);
-            else store_dword(pack_bf16x2(o[0][q], o[V - 1][q]), Cr, at + (r0 + q) * rowb);
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if constexpr (OUT == OUT_F32) {
-              store_dword<0>(__float_as_uint(o[0][q]), Cr, at + (r0 + q) * rowb);
-              store_dword<0>(__float_as_uint(o[V - 1][q]), Cr, at1 + (r0 + q) * rowb);
-            } else {
-              store_word(f32_to_bf16_bits(o[0][q]), Cr, at + (r0 + q) * rowb);
-              store_word(f32_to_bf16_bits(o[V - 1][q]), Cr, at1 + (r0 + q) * rowb);
-            }
-          }
-        }
-      }
+    for (int j = 0; j < TN; ++j) {
+      done.sw[j] = swn[j];
+      if constexpr (!SWI) done.bias[j] = !has_bias ? 0.0f : bias_bf16 ? bf16_bits_to_f32(braw[j]) : __uint_as_float(braw[j]);
     }
-    stores = TMV;
+    const uint32_t c = (uint32_t)(my_column(0) - nt);
+    done.at = done.at1 = OOB_OFFSET;
+    if (my_column(0) < FH)  // (two lanes' columns of two rows: the even lane has the first row of the two)
+      done.at = (uint32_t)rq * rowb + (V == 1 && OUT == OUT_BF16 && !ODD ? (c & ~1u) * 2 + (odd_lane ? rowb : 0u) : c * ESZ);
+    if (V == 2 && my_column(1) < FH) done.at1 = (uint32_t)rq * rowb + (c + 1) * ESZ;
+    float* const other = sx_lds;
+    sx_lds = sx_done;
+    sx_done = other;
     return !last;
   };
   if constexpr (TM == 2) {
@@ -339,6 +362,12 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
   } else {
     while (tile(c1{})) {}
   }
+#pragma unroll
+  for (int g = 0; g < EPI; ++g)
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) finish(i, g, q);
   AQ_WAIT_VMCNT(0);  // nothing lands in LDS behind the walk
   AQ_BARRIER();
 #endif
@@ -350,8 +379,15 @@ static int walk_launch(const GroupedArgs& a, hipStream_t st) {
   const int64_t most = grouped_most_tiles(a.R, a.E, GW_BM) * tiles_n;
   if (most > 0x7fffffff) return AQ_E_RANGE;
   const int cus = device_cus();
-  queue_kernel(grouped_walk_kernel<S, OUT, SWI>, dim3((unsigned)(most < cus ? most : cus)), dim3(GW_THREADS), 0, st, a, tiles_n,
-               UDiv::of((uint32_t)tiles_n));
+  const dim3 grid((unsigned)(most < cus ? most : cus)), block(GW_THREADS);
+  const UDiv by_tiles_n = UDiv::of((uint32_t)tiles_n);
+  if constexpr (!SWI) {
+    if (a.N & 1) {
+      queue_kernel(grouped_walk_kernel<S, OUT, SWI, true>, grid, block, 0, st, a, tiles_n, by_tiles_n);
+      return (int)hipGetLastError();
+    }
+  }
+  queue_kernel(grouped_walk_kernel<S, OUT, SWI, false>, grid, block, 0, st, a, tiles_n, by_tiles_n);
   return (int)hipGetLastError();
 }
 template <int OUT, bool SWI>
