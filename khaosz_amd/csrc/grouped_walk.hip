@@ -42,6 +42,7 @@ __device__ __forceinline__ uint32_t pair_columns(uint32_t mine, bool odd) {
 
 struct WalkTile {
   int e, first, end, n0;  // rows first .. end - 1 (end of the expert's rows) by columns from n0 (SwiGLU: of h)
+  int rot;                // the K step it begins with
 };
 
 template <class S, int OUT, bool SWI, bool ODD>
@@ -88,7 +89,14 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
     w.first = __builtin_amdgcn_readfirstlane(off[w.e] + (first_m + in_group - n_at * gm) * GW_BM);
     w.end = __builtin_amdgcn_readfirstlane(off[w.e + 1]);
     w.n0 = __builtin_amdgcn_readfirstlane(n_at * (SWI ? BN / 2 : BN));
+    w.rot = __builtin_amdgcn_readfirstlane((in_group % gm + n_at) % 8 * steps / 8);
     return w;
+  };
+  // K step s of a tile.  Tiles beside each other begin at different steps: what they share is then brought by one of them at a time and found in the L2 by the
+  // others, where all of them in step would wait for each line's way from memory.
+  auto k_of = [&](int s, const WalkTile& t) {
+    const int k = s + t.rot;
+    return (s >= steps ? steps : k >= steps ? k - steps : k) * BK;
   };
 
   const __amdgpu_buffer_rsrc_t Ar = make_rsrc(p.x, (uint32_t)p.x_rows * (uint32_t)K), Sr = make_rsrc(p.sx, (uint32_t)p.x_rows * 4u);
@@ -269,7 +277,7 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
 #pragma unroll
   for (int s = 0; s < AHEAD; ++s)
 #pragma unroll
-    for (int q = 0; q < NLOADS; ++q) issue_load(s * BK, s, q);
+    for (int q = 0; q < NLOADS; ++q) issue_load(k_of(s, now), s, q);
   __builtin_amdgcn_s_waitcnt(0xc07f);  // the tokens are read: the next tile's may come
   AQ_WAIT_VMCNT(BEHIND);               // stage 0 has landed
   AQ_BARRIER();
@@ -286,13 +294,11 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
     // its tokens, 16 rows to a wavefront (one operation of each, counted below); they are there before step AHEAD
     if (lane < 16)
       fetch_dword_to_lds(Tr, tok_lds + wave * 16, (uint32_t)(next.first + wave * 16 + lane) * 4u);
-    int k0 = AHEAD * BK;
     // behind the next stage's loads: the step's stores, and in the first step the tokens
-    step(tm_c, std::true_type{}, std::true_type{}, 0, k0, [&]() { AQ_WAIT_VMCNT(BEHIND + 1 + TM * ROW_STORES); });
-    k0 += BK;
+    step(tm_c, std::true_type{}, std::true_type{}, 0, k_of(AHEAD, now), [&]() { AQ_WAIT_VMCNT(BEHIND + 1 + TM * ROW_STORES); });
 #pragma unroll
-    for (int g = 1; g < EPI; ++g, k0 += BK) step(tm_c, no{}, std::true_type{}, g, k0, [&]() { AQ_WAIT_VMCNT(BEHIND + TM * ROW_STORES); });
-    for (int s = EPI; s < nk - AHEAD; ++s, k0 += BK) step(tm_c, no{}, no{}, 0, k0, landed);
+    for (int g = 1; g < EPI; ++g) step(tm_c, no{}, std::true_type{}, g, k_of(AHEAD + g, now), [&]() { AQ_WAIT_VMCNT(BEHIND + TM * ROW_STORES); });
+    for (int s = EPI; s < nk - AHEAD; ++s) step(tm_c, no{}, no{}, 0, k_of(AHEAD + s, now), landed);
     // the epilogue's operands, then the next tile's first stages
     const int mw = now.first + first_row(now), nt = now.n0, end = now.end;
     const int64_t scales = (int64_t)now.e * N;
@@ -327,8 +333,8 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
       for (int i = 0; i < NLOADS; ++i) vo[i] = OOB_OFFSET;
     }
 #pragma unroll
-    for (int s = 0; s < AHEAD - 1; ++s) step(tm_c, no{}, no{}, 0, s * BK, landed);
-    step(tm_c, no{}, no{}, 0, (AHEAD - 1) * BK, [&]() {
+    for (int s = 0; s < AHEAD - 1; ++s) step(tm_c, no{}, no{}, 0, k_of(s, now), landed);
+    step(tm_c, no{}, no{}, 0, k_of(AHEAD - 1, now), [&]() {
       landed();
       fr_a = next_fr_a;  // (the fragments read behind this step's barrier are the next tile's)
     });
