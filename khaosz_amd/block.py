@@ -432,16 +432,98 @@ class MLP(nn.Module):
         return self.down(self.up(x) * F.silu(self.gate(x)), **kw)
 
 
+class MoE(nn.Module):
+    """Routed experts in the MLP's place (DeepSeekMoE, astrai/model/components/mlp.py:31-93): every token goes through ``n_activated_experts`` of
+    ``n_routed_experts`` MLPs, chosen by the largest logits of ``router`` and weighted by their softmax, and through all ``n_shared_experts``.
+
+    Its plain forward runs the experts one after the other on the rows of their tokens, as the reference does, and so waits for the
+    device to learn how many each has.  ``fuse_experts()`` runs a quantized layer's routing, products and sums on the device, in one call
+    that waits for nothing (and can be captured in a graph): not bit-identical, since h = up * silu(gate) is rounded once and the weights stay in
+    float32."""
+
+    def __init__(self, dim: int, dim_ffn: int, n_routed_experts: int, n_activated_experts: int, n_shared_experts: int = 0):
+        super().__init__()
+        if not 0 < n_activated_experts <= n_routed_experts:
+            raise ValueError(f"{n_activated_experts} of {n_routed_experts} experts cannot be activated")
+        self.n_activated_experts = n_activated_experts
+        self.router = Linear(dim, n_routed_experts)
+        self.routed_experts = nn.ModuleList([MLP(dim, dim_ffn) for _ in range(n_routed_experts)])
+        self.shared_experts = nn.ModuleList([MLP(dim, dim_ffn) for _ in range(n_shared_experts)])
+        self._experts: Optional[Tuple[Tensor, Tensor, Tensor, Tensor]] = None  # set by fuse_experts(): stacked codes and scales
+
+    def fuse_experts(self) -> bool:
+        """Stacks the quantized experts' weights (up on top of gate, and down); the experts' own buffers become slices of the stacks, so
+        that no second copy is kept.  False, and nothing changes, unless every routed expert is quantized (int8, without biases) and the
+        sizes are what ``ops.experts_w8a8`` takes."""
+        if self._experts is not None:
+            return False
+        parts = [(e.up, e.gate, e.down) for e in self.routed_experts]
+        linears = [p for e in parts for p in e]
+        if any(type(p) is not QuantLinear or p.bias is not None or p._shared is not None for p in linears):
+            return False
+        F_, E = parts[0][2].in_dim, len(parts)
+        if F_ % 16 or E > ops.ROUTE_MAX_EXPERTS or self.n_activated_experts > ops.ROUTE_MAX_CHOICES:
+            return False
+        up_gate, up_gate_scale = (torch.stack([torch.cat([getattr(u, n), getattr(g, n)]) for u, g, _ in parts]) for n in ("qweight", "w_scale"))
+        down, down_scale = (torch.stack([getattr(d, n) for _, _, d in parts]) for n in ("qweight", "w_scale"))
+        for i, (expert, (u, g, d)) in enumerate(zip(self.routed_experts, parts)):
+            u.qweight, g.qweight, d.qweight = up_gate[i, :F_], up_gate[i, F_:], down[i]
+            u.w_scale, g.w_scale, d.w_scale = up_gate_scale[i, :F_], up_gate_scale[i, F_:], down_scale[i]
+            if expert._upgate is not None:
+                expert._upgate.qweight, expert._upgate.w_scale = up_gate[i], up_gate_scale[i]
+        self._experts = up_gate, up_gate_scale, down, down_scale
+        return True
+
+    def _apply(self, fn, recurse=True):
+        # a move or a cast of the module goes through the experts' buffers: they are stacked again from there
+        fused, self._experts = self._experts is not None, None
+        super()._apply(fn, recurse)
+        if fused:
+            self.fuse_experts()
+        return self
+
+    def _route(self, x: Tensor) -> Tuple[Tensor, Tensor]:
+        """weights and experts ``[T, k]`` as the reference takes them (mlp.py:72-82)"""
+        probs = torch.softmax(self.router(x).float(), dim=-1).to(x.dtype)
+        w, idx = torch.topk(probs, self.n_activated_experts, dim=-1)
+        return w / w.sum(dim=-1, keepdim=True), idx
+
+    def forward(self, x: Tensor, codes: Optional[Tuple[Tensor, Tensor]] = None, residual: Optional[Tensor] = None, norm=None) -> Tensor:
+        """``residual`` and ``norm`` as for the MLP; the router needs the activations themselves, so ``codes`` are not taken."""
+        if codes is not None:
+            raise ValueError("routed experts take activations, not codes")
+        if norm is not None:
+            x = F.rms_norm(x, (x.shape[-1],), norm[0], norm[1])
+        rows = x.reshape(-1, x.shape[-1])
+        for shared in self.shared_experts:
+            y = shared(x)
+            residual = y if residual is None else residual + y
+        if self._experts is not None and x.is_cuda and not (torch.is_grad_enabled() and x.requires_grad):
+            r = ops.route_topk(self.router(rows), self.n_activated_experts)
+            out = ops.experts_w8a8(rows, r, *self._experts, residual=None if residual is None else residual.reshape(rows.shape))
+            return out.view(x.shape)
+        w, idx = self._route(rows)
+        out = torch.zeros_like(rows)
+        for e, expert in enumerate(self.routed_experts):
+            tok, slot = (idx == e).nonzero(as_tuple=True)
+            if tok.numel():
+                out.index_add_(0, tok, expert(rows[tok]) * w[tok, slot].unsqueeze(-1))
+        out = out.view(x.shape)
+        return out if residual is None else out + residual
+
+
 class DecoderBlock(nn.Module):
-    """``x += attn(norm(x)); x += mlp(norm(x))`` (astrai/model/components/decoder_block.py:12-59)."""
+    """``x += attn(norm(x)); x += mlp(norm(x))`` (astrai/model/components/decoder_block.py:12-59).  With ``n_routed_experts`` the MLP is a layer of routed
+    experts (``MoE``), each ``dim_ffn`` wide."""
 
     def __init__(self, dim: int, n_heads: int, dim_ffn: int, n_kv_heads: int, norm_eps: float = 1e-5,
-                 layer_id: int = 0, use_qk_norm: bool = False, use_gated_attention: bool = False):
+                 layer_id: int = 0, use_qk_norm: bool = False, use_gated_attention: bool = False, n_routed_experts: int = 0,
+                 n_activated_experts: int = 2, n_shared_experts: int = 0):
         super().__init__()
         self.attention = GQA(dim, n_heads, n_kv_heads, layer_id, use_qk_norm, norm_eps, use_gated_attention)
         self.input_norm = RMSNorm(dim, norm_eps)
         self.post_attention_norm = RMSNorm(dim, norm_eps)
-        self.mlp = MLP(dim, dim_ffn)
+        self.mlp = MoE(dim, dim_ffn, n_routed_experts, n_activated_experts, n_shared_experts) if n_routed_experts else MLP(dim, dim_ffn)
         self._norm_quant = False
         self._residual_adds = False
 
@@ -455,7 +537,9 @@ class DecoderBlock(nn.Module):
         per-token quantisation in one launch and never write the normalised activations.  The
         bf16 rounding of the norm output disappears, so outputs move by less than the
         quantisation noise (not bit-identical to the unfused block)."""
-        if self.attention._qkv is not None and self.mlp._upgate is not None:
+        if self.attention._qkv is not None and isinstance(self.mlp, MoE):
+            self._norm_quant = True  # (of the attention's projections: the router reads the other norm's output)
+        elif self.attention._qkv is not None and self.mlp._upgate is not None:
             self._norm_quant = True
             self.mlp._swiglu_quant = True  # likewise: silu * up and the quantisation for `down` in one launch
         return self._norm_quant

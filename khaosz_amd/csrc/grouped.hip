@@ -264,15 +264,31 @@ static int g_forced_grouped = 0;  // lab build only: 0 = by size
 // Experts with rows, of E, when R rows are dealt out evenly.
 static double experts_used(int64_t R, int64_t E) { return E * (1.0 - std::exp(-(double)R / E)); }
 
-// Which kernel: walked tiles where they are at least 7 to 4 compute units, or where experts
-// have more rows than the tile of 16.
+// Which kernel: the one whose estimated time, in us, is least.  Tiles of 16 rows: units of 32 weight rows, four to a compute unit at a time.  Walked
+// tiles: rounds of tiles, each of its steps and a beginning and an end, beside the weights' way from memory.  Fitted to 805 random sizes (1 to 256
+// experts, 1 to 8192 tokens, K 128 to 6912): 1.7 % slower than the best kernel in the mean, one in twenty 11 % or more (always 128 x 256 50 %, always 128 x 128 30 %).
 enum { GROUPED_FEW = 1, GROUPED_WALK_256 = 2, GROUPED_WALK_128 = 3, GROUPED_WALK_64 = 4 };
-static int choose_grouped(const GroupedArgs& a) {
+static double walk_us(const GroupedArgs& a, double used, int width, int least_steps, double launch, double ends, double step, double tb_s, double tail) {
+  const double avg = a.R / used, cus = device_cus(), steps = (a.K + 127) / 128;
+  const double tiles = used * (avg / 128 + tail > 1 ? avg / 128 + tail : 1) * ((a.N + width - 1) / width), part = tiles / cus;
+  const double rounds = part > 0.78 ? part + 0.25 : part;
+  const double c = (rounds > 1 ? rounds : 1) * (ends + step * (steps > least_steps ? steps : least_steps)), m = used * a.N * a.K * 1e-6 / tb_s;
+  return launch + std::sqrt(std::sqrt(c * c * c * c + m * m * m * m));
+}
+static int choose_grouped(const GroupedArgs& a, bool swiglu) {
   if (a.N > (1 << 20)) return GROUPED_FEW;  // (a tile's rows by 32-bit offsets)
 #ifdef AQ_LAB
   if (g_forced_grouped) return g_forced_grouped;
 #endif
-  return experts_used(a.R, a.E) * ((a.N + 255) / 256) >= 1.75 * device_cus() || a.R > 24 * a.E ? GROUPED_WALK_256 : GROUPED_FEW;
+  const double used = experts_used(a.R, a.E), rows = a.R / used / 16 + 0.45;
+  const double units = used * (rows > 1 ? rows : 1) * ((a.N + GF_COLS - 1) / GF_COLS);
+  const double us[] = {units / (4 * device_cus()) * (2.3 + 7.6 * a.K / 1024) + 2.3 * ((a.K + 2047) / 2048),
+                       walk_us(a, used, 256, 6, 4.8, 2.7, 0.47, 5.5, 0.75), walk_us(a, used, 128, 7, 3.4, 2.3, 0.40, 12.0, 0.75),
+                       walk_us(a, used, 64, 10, 2.3, 2.2, 0.26, 5.0, 1.0)};
+  int best = 0;
+  for (int i = 1; i < (swiglu ? 3 : 4); ++i)
+    if (us[i] < us[best]) best = i;
+  return GROUPED_FEW + best;
 }
 
 template <int OUT, bool SWI, int IN, int VPL, int DEEP>
@@ -332,7 +348,7 @@ static bool tokens_in_launch(int64_t T, int64_t k, int64_t E, int64_t dim, int64
 
 template <int OUT, bool SWI>
 static int launch_grouped(const GroupedArgs& a, hipStream_t st) {
-  const int kind = choose_grouped(a);
+  const int kind = choose_grouped(a, SWI);
   if (kind != GROUPED_FEW) return grouped_walk_launch<OUT, SWI>(a, kind == GROUPED_WALK_256 ? 256 : kind == GROUPED_WALK_128 ? 128 : 64, st);
   return launch_few<OUT, SWI, IN_CODES, 1>(a, st);
 }

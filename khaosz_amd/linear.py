@@ -439,7 +439,7 @@ REFERENCE_SHARED_INPUTS = {
 
 
 def fuse_shared_inputs(model: nn.Module, norms: bool = False, decode_attention: bool = False,
-                       residuals: bool = False) -> int:
+                       residuals: bool = False, experts: bool = False) -> int:
     """Call ``fuse_projections()`` on every module that offers it (attention and MLP blocks whose
     projections read one input); returns how many fused modules were built.  Run it after
     ``quantize_model`` and after loading weights: the fused module owns the weight storage from
@@ -452,7 +452,8 @@ def fuse_shared_inputs(model: nn.Module, norms: bool = False, decode_attention: 
     projection run single-token steps on a paged cache through the in-place attention kernels
     (``fuse_decode_attention()``).  ``residuals=True`` lets blocks hand the residual stream to the
     quantized projection that ends each branch (``fuse_residual_adds()``): the add happens in that
-    kernel's epilogue, bit-identical to the separate add."""
+    kernel's epilogue, bit-identical to the separate add.  ``experts=True`` lets layers of routed experts run
+    as grouped products on the device (``fuse_experts()``): not bit-identical to the loop over the experts."""
     n = 0
     for m in model.modules():
         f = getattr(m, "fuse_projections", None)
@@ -476,6 +477,11 @@ def fuse_shared_inputs(model: nn.Module, norms: bool = False, decode_attention: 
     if residuals:
         for m in model.modules():
             f = getattr(m, "fuse_residual_adds", None)
+            if callable(f):
+                f()
+    if experts:
+        for m in model.modules():
+            f = getattr(m, "fuse_experts", None)
             if callable(f):
                 f()
     return n

@@ -5,8 +5,8 @@ token embedding, ``n_layers`` pre-norm blocks sharing one rotary table and one
 paged KV cache, a final RMSNorm and the vocabulary projection.
 
 Only what the benchmark's configurations use is here (grouped-query attention
-with its qk-norm and output-gate options, SwiGLU MLP, optional tied embedding;
-no MoE / MLA).  The attention mask follows ``process_attention_mask``
+with its qk-norm and output-gate options, SwiGLU MLP or routed experts, optional tied
+embedding; no MLA).  The attention mask follows ``process_attention_mask``
 (transformer.py:17-46) for the two cases the benchmark runs -- a prompt from
 position 0 (causal, no mask tensor) and one new token per sequence (a mask of
 zeros) -- without its device-to-host reads, so a step can be captured in a HIP
@@ -42,6 +42,9 @@ class LMConfig:
     tie_weight: bool = False
     use_qk_norm: bool = False
     use_gated_attention: bool = False
+    n_routed_experts: int = 0      # 0: an MLP
+    n_activated_experts: int = 2
+    n_shared_experts: int = 0
 
 
 class Embedding(nn.Module):
@@ -73,7 +76,9 @@ class AutoRegressiveLM(nn.Module):
         self.embed_tokens = Embedding(config.vocab_size, config.dim)
         self.layers = nn.ModuleList([
             DecoderBlock(config.dim, config.n_heads, config.dim_ffn, config.n_kv_heads, config.norm_eps, layer_id=i,
-                         use_qk_norm=config.use_qk_norm, use_gated_attention=config.use_gated_attention)
+                         use_qk_norm=config.use_qk_norm, use_gated_attention=config.use_gated_attention,
+                         n_routed_experts=config.n_routed_experts, n_activated_experts=config.n_activated_experts,
+                         n_shared_experts=config.n_shared_experts)
             for i in range(config.n_layers)])
         self.norm = RMSNorm(config.dim, config.norm_eps)
         self.lm_head = Linear(config.dim, config.vocab_size)

@@ -936,6 +936,10 @@ def compact_pages(page_table: torch.Tensor, refs: torch.Tensor, k_layers: torch.
     return CompactedPages(table, counts, where, live)
 
 
+# what the routed-expert operators take at most
+ROUTE_MAX_EXPERTS, ROUTE_MAX_CHOICES = 512, 16
+
+
 class Routing(NamedTuple):
     """What ``route_topk`` gives for ``T`` tokens and ``k`` choices each: the weights (float32 ``[T, k]``) and the experts (int32 ``[T, k]``, -1: none),
     and the choices in the experts' order: expert e has rows ``offsets[e] .. offsets[e + 1] - 1`` (int32 ``[E + 1]``), ``rows`` (int32 ``[T, k]``) is the row of

@@ -1,0 +1,170 @@
+"""The layer of routed experts (MoE, DeepSeekMoE of mlp.py:31-93) as a module: its plain forward (CPU), and quantized and fused inside a block and a
+model, where routing, products and sums run as the grouped operators (GPU)."""
+import copy
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from khaosz_amd import AutoRegressiveLM, LMConfig, fuse_shared_inputs, ops, quantize_model
+from khaosz_amd.block import DecoderBlock, MLP, MoE, rotary_table
+from khaosz_amd.linear import Linear, QuantLinear
+
+DEV = "cuda:0"
+
+
+def _moe(dim, ffn, E, k, shared=0, seed=0):
+    torch.manual_seed(seed)
+    m = MoE(dim, ffn, E, k, shared)
+    for x in m.modules():
+        if isinstance(x, Linear):
+            x.reset_parameters()
+    return m
+
+
+def test_plain_forward_is_the_sum_over_the_chosen_experts():
+    m = _moe(32, 48, 5, 2, shared=2)
+    x = torch.randn(2, 7, 32)
+    rows = x.view(-1, 32)
+    p = torch.softmax(m.router(rows), -1)
+    w, idx = p.topk(2, -1)
+    want = torch.stack([sum(w[t, j] / w[t].sum() * m.routed_experts[int(idx[t, j])](rows[t:t + 1])[0] for j in range(2)) for t in range(14)])
+    want = want.view(x.shape) + m.shared_experts[0](x) + m.shared_experts[1](x)
+    assert torch.allclose(m(x), want, atol=1e-5)
+    assert torch.allclose(m(x, residual=x), want + x, atol=1e-5)
+    gain = torch.rand(32)
+    assert torch.allclose(m(x, norm=(gain, 1e-5)), m(F.rms_norm(x, (32,), gain, 1e-5)), atol=1e-6)
+
+
+def test_state_dict_keys_and_refusals():
+    b = DecoderBlock(64, 4, 48, 2, n_routed_experts=3, n_activated_experts=2, n_shared_experts=1)
+    keys = set(b.state_dict())
+    assert {"mlp.router.weight", "mlp.routed_experts.2.down.weight", "mlp.shared_experts.0.gate.weight"} <= keys
+    assert type(DecoderBlock(64, 4, 48, 2).mlp) is MLP
+    with pytest.raises(ValueError):
+        MoE(32, 48, 4, 5)
+    with pytest.raises(ValueError):
+        MoE(32, 48, 4, 0)
+    with pytest.raises(ValueError):
+        b.mlp(torch.zeros(1, 64), codes=(torch.zeros(1, 64, dtype=torch.int8), torch.ones(1)))
+    assert not b.mlp.fuse_experts()  # not quantized
+    c = LMConfig(vocab_size=50, dim=64, n_layers=2, n_heads=4, n_kv_heads=2, dim_ffn=48, max_len=64, n_routed_experts=3)
+    assert isinstance(AutoRegressiveLM(c).layers[1].mlp, MoE)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape,E,k,shared", [((1, 1), 8, 2, 0), ((3, 1), 8, 2, 1), ((2, 40), 6, 3, 2), ((4, 150), 64, 4, 0)])
+def test_fused_layer_follows_the_loop_over_the_experts(shape, E, k, shared, dtype):
+    m = _moe(256, 352, E, k, shared, seed=E).to(DEV)
+    m.router.to(dtype)
+    assert quantize_model(m) == 3 * (E + shared)
+    assert fuse_shared_inputs(m) == E + shared
+    x = torch.randn(*shape, 256, device=DEV).to(dtype)
+    with torch.inference_mode():
+        plain = m(x)
+        one = [e(x) for e in m.routed_experts]
+        assert fuse_shared_inputs(m, experts=True) == 0 and m._experts is not None
+        assert all(torch.equal(a, e(x)) for a, e in zip(one, m.routed_experts))  # the experts by themselves are what they were
+        fused = m(x)
+        assert fused.shape == x.shape and fused.dtype == dtype
+        rows = x.view(-1, 256)
+        # The plain layer chooses by probabilities rounded to x's type: a token may take another expert only where the k-th and the next
+        # largest are one number there, or neighbours (each is off by at most half a step).
+        probs = torch.softmax(m.router(rows).float(), -1).sort(-1, descending=True).values
+        mine = ops.route_topk(m.router(rows), k).experts.long().sort(-1).values
+        same = (m._route(rows)[1].sort(-1).values == mine).all(-1)
+        assert (probs[:, k - 1] - probs[:, k] <= torch.finfo(dtype).eps * probs[:, k - 1])[~same].all()
+        # for the others: roundings of h, of the weights and of partial sums to bf16
+        a, b = (v.view(-1, 256)[same].double() for v in (fused, plain))
+        assert float((a - b).norm() / b.norm()) < 3e-2
+        res = None
+        for s in m.shared_experts:
+            res = s(rows) if res is None else res + s(rows)
+        r = ops.route_topk(m.router(rows), k)
+        assert torch.equal(fused.view(-1, 256), ops.experts_w8a8(rows, r, *m._experts, residual=res))
+    assert not m.fuse_experts()
+
+
+@pytest.mark.gpu
+def test_stacked_weights_follow_loads_moves_and_copies():
+    m = _moe(64, 48, 4, 2).to(DEV)
+    quantize_model(m)
+    assert m.fuse_experts()
+    x = torch.randn(9, 64, device=DEV)
+    with torch.inference_mode():
+        before = m(x)
+        other = _moe(64, 48, 4, 2, seed=9).to(DEV)
+        quantize_model(other)
+        m.load_state_dict(other.state_dict())
+        want = other(x)
+        after = m(x)
+        assert not torch.equal(after, before) and (after - want).norm() / want.norm() < 1e-2
+        twin = copy.deepcopy(m)
+        assert torch.equal(twin(x), after)
+        twin.routed_experts[0].down.qweight.zero_()
+        assert not torch.equal(twin(x), after) and torch.equal(m(x), after)
+        m.cpu().to(DEV)
+        assert torch.equal(m(x), after) and m._experts[0].data_ptr() == m.routed_experts[0].up.qweight.data_ptr()
+
+
+@pytest.mark.gpu
+def test_experts_that_cannot_be_stacked_stay_as_they_are():
+    m = _moe(64, 48, 4, 2).to(DEV)
+    quantize_model(m)
+    m.routed_experts[1].down = QuantLinear(48, 64, bias=True, device=DEV)
+    assert not m.fuse_experts() and m._experts is None
+    f = _moe(64, 48, 4, 2).to(DEV)
+    quantize_model(f, mode="fp8")
+    assert not f.fuse_experts()
+    big = _moe(64, 48, 20, 17).to(DEV)
+    quantize_model(big)
+    assert not big.fuse_experts()
+
+
+@pytest.mark.gpu
+def test_block_and_model_with_routed_experts():
+    """Prompt and steps of a small model: every fusion on against none, one captured step replayed, and the launches of a step: nothing waits."""
+    torch.manual_seed(4)
+    c = LMConfig(vocab_size=200, dim=256, n_layers=2, n_heads=4, n_kv_heads=2, dim_ffn=352, max_len=128, n_routed_experts=8, n_activated_experts=2,
+                 n_shared_experts=1)
+    model = AutoRegressiveLM(c).to(torch.bfloat16).to(DEV)
+    quantize_model(model)
+    plain = copy.deepcopy(model)
+    fuse_shared_inputs(model, norms=True, decode_attention=True, residuals=True, experts=True)
+    assert all(layer.mlp._experts is not None and layer._norm_quant for layer in model.layers)
+    ids = torch.randint(0, 200, (3, 20), device=DEV)
+
+    def caches():
+        cache = model.new_cache(8, 64, dtype=torch.bfloat16)
+        cache.bind(torch.arange(6, device=DEV).view(3, 2), 20)
+        return cache
+    with torch.inference_mode():
+        a, b = caches(), caches()
+        y, z = (m(ids, paged_cache=k, start_pos=0)["logits"] for m, k in ((model, a), (plain, b)))
+        # int8 noise of two layers in other places: a token whose router is nearly undecided may take another expert
+        assert (y.double() - z.double()).norm() / z.double().norm() < 0.15
+        step = torch.randint(0, 200, (3, 1), device=DEV)
+        a.bind(a.page_table, 21)
+        want = model(step, paged_cache=a, start_pos=20)["logits"].clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            model(step, paged_cache=a, start_pos=20)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                out = model(step, paged_cache=a, start_pos=20)["logits"]
+        torch.cuda.current_stream().wait_stream(side)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            assert torch.equal(model(step, paged_cache=a, start_pos=20)["logits"], want)
+    block = model.layers[0]
+    x = torch.randn(3, 1, 256, device=DEV, dtype=torch.bfloat16)
+    fr = rotary_table(64, 128, device=DEV)[20:21].unsqueeze(0).expand(3, -1, -1)
+    with torch.inference_mode():
+        got = block(x, fr, None, a)
+        att = block.attention(x, fr, None, a, norm=(block.input_norm.weight, block.input_norm.norm_eps), residual=x)
+        n = block.post_attention_norm
+        assert torch.equal(got, block.mlp(att, norm=(n.weight, n.norm_eps), residual=att))
