@@ -183,10 +183,12 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
   if constexpr (SWI) store_out<OUT>(p.y, (int64_t)out_row * FH + n0 + c, grouped_swiglu<OUT>(y[0], y[1]));  // (F is a multiple of 16)
 }
 
-// The second product and the weighted sum in one launch, for a few tokens: a workgroup has 16 columns of one token's output, a wavefront one of its
-// choices at a time: it quantises that row of h, multiplies it with its expert's 16 weight rows and leaves the rounded output times its weight in LDS,
+// The second product and the weighted sum in one launch, for a few tokens: a workgroup has 8 columns of one token's output, a wavefront one of its
+// choices at a time: it quantises that row of h, multiplies it with its expert's 8 weight rows and leaves the rounded output times its weight in LDS,
 // where the choices are added in their order: the bits of the grouped Linear and combine_rows.  Experts that several tokens chose are read for each.
-constexpr int GT_WAVES = 8, GT_COLS = 16;
+// The matrix core's 16 columns are the 8 weight rows' two halves of K, and rows 0 and 1 of its other operand the same halves of the row: half the
+// loads and products of 16 columns in a row, on twice the compute units (one token, 6 of 64 experts of 2048 / 1408: 9.8 us).
+constexpr int GT_WAVES = 8, GT_COLS = 8;
 struct TokenArgs {
   GroupedArgs g;  // x: h [R, K]
   const int32_t* rows;
@@ -194,10 +196,11 @@ struct TokenArgs {
   const void* res;
   int k;
 };
-// LINES: of 128 bytes of each weight row on their way at a time.  12 where a compute unit has one workgroup at most, 4 where it can have two (one token,
-// 2 of 8 experts of 1536 / 2816: 19.0 us, 21.4 with 4; four tokens, 6 of 64 of 2048 / 1408: 47.1, 45.5 with 4).
-template <int OUT, int VPL, int LINES>
-__global__ __launch_bounds__(GT_WAVES * 64, LINES == 4 ? 4 : 2) void grouped_token_kernel(TokenArgs a) {
+// GT_LINES: of 128 bytes of each half on their way at a time.  With 8 or 12 a compute unit has room for one workgroup, with 4 for two (8 tokens' 8 of 256
+// experts of 1024 / 512, the layer: 38.2, 43.9 and 33.5 us; one token's 6 of 64 of 2048 / 1408: 22.0, 22.8 and 22.3).
+constexpr int GT_LINES = 4;
+template <int OUT, int VPL>
+__global__ __launch_bounds__(GT_WAVES * 64, VPL == 4 ? 4 : 2) void grouped_token_kernel(TokenArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t xs[];  // a row of codes per wavefront
   __shared__ float term[GP_MAX_TOKEN_K][GT_COLS];
   __shared__ float scale[GT_WAVES];
@@ -205,8 +208,10 @@ __global__ __launch_bounds__(GT_WAVES * 64, LINES == 4 ? 4 : 2) void grouped_tok
   const GroupedArgs& p = a.g;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int K = p.K, N = p.N, t = blockIdx.y, n0 = (int)blockIdx.x * GT_COLS, pitch = few_pitch(K);
-  const int r16 = lane & 15, q16 = (lane >> 4) * 16, n = n0 + r16;
+  const int r16 = lane & 15, q16 = (lane >> 4) * 16, n = n0 + (r16 & 7);
+  const int half = (K + 31) / 32 * 16, k_of_lane = (r16 >> 3) * half, k_end = r16 >> 3 ? K - half : half;
   uint8_t* const mine = xs + wave * pitch;
+  const uint8_t* const operand = mine + (r16 & 1) * half + q16;
   for (int j = wave; j < a.k; j += GT_WAVES) {
     const int row = __builtin_amdgcn_readfirstlane(a.rows[(int64_t)t * a.k + j]);
     float y = 0.0f, w = 0.0f;
@@ -216,30 +221,31 @@ __global__ __launch_bounds__(GT_WAVES * 64, LINES == 4 ? 4 : 2) void grouped_tok
       e = __builtin_amdgcn_readfirstlane(e);
       if (e < p.E) {
         const __amdgpu_buffer_rsrc_t Wr = make_rsrc(p.w + e * p.w_bytes, (uint32_t)p.w_bytes);
-        const uint32_t wo = (uint32_t)n * (uint32_t)K + q16;
+        const uint32_t wo = (uint32_t)n * (uint32_t)K + k_of_lane + q16;
         w = a.weights[(int64_t)t * a.k + j];
         const float sw = p.sw[(int64_t)e * N + n];
         RowsToLds<BF16, 1, VPL> r;
         r.issue(p.x + (int64_t)row * K * (BF16 ? 2 : 4), 1, K, K, 0, 1, lane);
         v4i acc = {0, 0, 0, 0};
-        for (int l0 = 0; l0 * 128 < K; l0 += LINES) {
-          v4i wv[2 * LINES];
+        for (int k0 = 0; k0 < half; k0 += GT_LINES * 128) {
+          v4i wv[2 * GT_LINES];
 #pragma unroll
-          for (int i = 0; i < 2 * LINES; ++i) {
-            const int k = l0 * 128 + i * 64;
-            wv[i] = __builtin_amdgcn_raw_buffer_load_b128(Wr, k + q16 < K ? wo + k : OOB_OFFSET, 0, 2);
+          for (int i = 0; i < 2 * GT_LINES; ++i) {
+            const int k = k0 + i * 64;
+            wv[i] = __builtin_amdgcn_raw_buffer_load_b128(Wr, k + q16 < k_end ? wo + k : OOB_OFFSET, 0, 2);
           }
-          if (l0 == 0) {
+          if (k0 == 0) {
             r.finish(1, 1, K, mine, pitch, scale + wave, 0, 1, lane);
             __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS operations keep their order)
           }
 #pragma unroll
-          for (int i = 0; i < 2 * LINES; ++i) {
-            const int k = l0 * 128 + i * 64;
-            if (k < K) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(mine + k + q16), wv[i], acc, 0, 0, 0);
+          for (int i = 0; i < 2 * GT_LINES; ++i) {
+            const int k = k0 + i * 64;
+            if (k < half) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(operand + k), wv[i], acc, 0, 0, 0);
           }
         }
-        y = __fmul_rn(__fmul_rn((float)acc[0], scale[wave]), sw);  // (every row of the operand is this row)
+        const int sum = acc[0] + __builtin_amdgcn_update_dpp(0, acc[1], 0x128 /* row_ror:8 */, 0xf, 0xf, false);  // lanes 0 .. 7: both halves
+        y = __fmul_rn(__fmul_rn((float)sum, scale[wave]), sw);
         if constexpr (BF16) y = bf16_bits_to_f32(f32_to_bf16_bits(y));
       }
     }
@@ -330,20 +336,17 @@ template <int OUT, int VPL>
 static int launch_token(const TokenArgs& a, int64_t T, hipStream_t st) {
   const dim3 grid((unsigned)(a.g.N / GT_COLS), (unsigned)T), block(GT_WAVES * 64);
   const size_t lds = (size_t)GT_WAVES * few_pitch(a.g.K);
-  bool deep = true;
-  if constexpr (VPL == 4) deep = (int64_t)grid.x * T <= device_cus();  // (rows of 8 vectors a lane leave no room for two)
-  if (deep) queue_kernel((grouped_token_kernel<OUT, VPL, 12>), grid, block, lds, st, a);
-  else if constexpr (VPL == 4) queue_kernel((grouped_token_kernel<OUT, VPL, 4>), grid, block, lds, st, a);
+  queue_kernel((grouped_token_kernel<OUT, VPL>), grid, block, lds, st, a);
   return (int)hipGetLastError();
 }
 static int launch_tokens(const TokenArgs& a, int64_t T, int dtype, hipStream_t st) {
   if (dtype == AQ_BF16) return a.g.K <= 2048 ? launch_token<OUT_BF16, 4>(a, T, st) : launch_token<OUT_BF16, 8>(a, T, st);
   return a.g.K <= 1024 ? launch_token<OUT_F32, 4>(a, T, st) : launch_token<OUT_F32, 8>(a, T, st);
 }
-// Whether it is: what the experts of several tokens cost more, read for each, is then less than the launch saved (us, with | without: 64 tokens' 16 on 256
-// experts of 1024 / 512, 4 MB more, 30.1 | 35.9; 4 tokens' 6 of 64 of 2048 / 1408, 11 MB, 45.5 | 46.3; 6 tokens', 22 MB, 65.6 | 58.7).
+// Whether it is: what the experts of several tokens cost more, read for each, is then less than the launch saved (us of the layer, with | without: 64
+// choices of 256 experts of 1024 / 512, 4 MB more, 33.4 | 36.0; 18 of 64 of 2048 / 1408, 7 MB, 42.7 | 40.2; 24 of them, 11 MB, 48.8 | 46.3).
 static bool tokens_in_launch(int64_t T, int64_t k, int64_t E, int64_t dim, int64_t F) {
-  return T <= 65535 && ((double)(T * k) - experts_used(T * k, E)) * (double)(dim * F) <= 8e6;
+  return T <= 65535 && ((double)(T * k) - experts_used(T * k, E)) * (double)(dim * F) <= 5e6;
 }
 
 template <int OUT, bool SWI>
