@@ -281,6 +281,7 @@ static double walk_us(const GroupedArgs& a, double used, int width, int least_st
   const double c = (rounds > 1 ? rounds : 1) * (ends + step * (steps > least_steps ? steps : least_steps)), m = used * a.N * a.K * 1e-6 / tb_s;
   return launch + std::sqrt(std::sqrt(c * c * c * c + m * m * m * m));
 }
+static bool few_fits(int64_t R, int64_t E) { return grouped_most_tiles(R, E, GF_ROWS) <= 65535; }  // (the grid's second axis)
 static int choose_grouped(const GroupedArgs& a, bool swiglu) {
   if (a.N > (1 << 20)) return GROUPED_FEW;  // (a tile's rows by 32-bit offsets)
 #ifdef AQ_LAB
@@ -291,8 +292,8 @@ static int choose_grouped(const GroupedArgs& a, bool swiglu) {
   const double us[] = {units / (4 * device_cus()) * (2.3 + 7.6 * a.K / 1024) + 2.3 * ((a.K + 2047) / 2048),
                        walk_us(a, used, 256, 6, 4.8, 2.7, 0.47, 5.5, 0.75), walk_us(a, used, 128, 7, 3.4, 2.3, 0.40, 12.0, 0.75),
                        walk_us(a, used, 64, 10, 2.3, 2.2, 0.26, 5.0, 1.0)};
-  int best = 0;
-  for (int i = 1; i < (swiglu ? 3 : 4); ++i)
+  int best = few_fits(a.R, a.E) ? 0 : 1;
+  for (int i = best + 1; i < (swiglu ? 3 : 4); ++i)
     if (us[i] < us[best]) best = i;
   return GROUPED_FEW + best;
 }
@@ -300,7 +301,7 @@ static int choose_grouped(const GroupedArgs& a, bool swiglu) {
 template <int OUT, bool SWI, int IN, int VPL, int DEEP>
 static int launch_few_of(const GroupedArgs& a, hipStream_t st) {
   const int64_t tiles = grouped_most_tiles(a.R, a.E, GF_ROWS), cols = (a.N + GF_COLS - 1) / GF_COLS;
-  if (tiles > 65535 || cols > 0x7fffffff) return AQ_E_RANGE;
+  if (tiles > 65535 || cols > 0x7fffffff) return AQ_E_RANGE;  // (more rows of N > 2^20 columns than memory holds)
   queue_kernel((grouped_few_kernel<OUT, SWI, IN, VPL, DEEP>), dim3((unsigned)cols, (unsigned)tiles), dim3(GF_WAVES * 64),
                IN == IN_CODES ? 0 : GF_ROWS * few_pitch(a.K), st, a);
   return (int)hipGetLastError();
@@ -324,7 +325,7 @@ static int launch_rows(const GroupedArgs& a, int dtype, hipStream_t st) {
 // 16 tokens' 2 of 8 of 1536 / 2816 38 | 41, 32 tokens' 43.5 | 43.6).
 static bool rows_in_launch(int64_t T, int64_t k, int64_t E, int64_t dim, int64_t F, int dtype) {
   const int64_t most = dtype == AQ_BF16 ? GF_IN_BF16_K : GF_IN_F32_K, R = T * k;
-  if (dim > most || F > most) return false;
+  if (dim > most || F > most || !few_fits(R, E)) return false;
 #ifdef AQ_LAB
   if (g_forced_grouped) return g_forced_grouped == GROUPED_FEW;
 #endif

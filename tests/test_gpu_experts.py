@@ -203,6 +203,20 @@ def test_grouped_linear_bits(kernel, groups, K, N):
         assert torch.equal(got.cpu(), want), (tokens, dtype)
 
 
+def test_more_rows_than_one_grid_axis_has_tiles():
+    """1.1 million rows are more than 65535 tiles of 16, of narrow layers the few-rows kernel is the quickest for."""
+    R = 1_100_000
+    xq, sx, wq, sw, offsets, tok, _ = _operands([R], 16, 1, 77)
+    y = ops.linear_w8a8_grouped(*_on(xq, sx, wq, sw, offsets), out_dtype=torch.float32)
+    want = (xq.float() @ wq[0].float().t()) * sx[:, None] * sw[0]
+    assert torch.equal(y.cpu(), want)
+    _, _, uq, us, dq, ds = _layer(2, 16, 16, 78)
+    x = torch.randn(R // 2, 16, device=DEV).bfloat16()
+    r = ops.route_topk(torch.randn(R // 2, 2, device=DEV), 2)
+    got = ops.experts_w8a8(x, r, uq, us, dq, ds)
+    assert torch.equal(got, _composed(x, r, uq, us, dq, ds, None))
+
+
 @pytest.mark.parametrize("K,N", [(2048, 272), (4096, 96), (528, 514)])
 def test_grouped_linear_bits_many_rows(kernel, K, N):
     """Enough rows an expert for whole tiles of any kernel."""
