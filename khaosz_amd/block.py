@@ -432,6 +432,20 @@ class MLP(nn.Module):
         return self.down(self.up(x) * F.silu(self.gate(x)), **kw)
 
 
+def _stack_again(moe: "MoE", incompatible_keys) -> None:
+    """After a load that put new tensors in the place of the stacks' slices (``assign=True``)."""
+    if moe._experts is None:
+        return
+    up_gate, up_gate_scale, down, down_scale = moe._experts
+    F_ = down.shape[2]
+    for i, e in enumerate(moe.routed_experts):
+        for p, w, s in ((e.up, up_gate[i], up_gate_scale[i]), (e.gate, up_gate[i, F_:], up_gate_scale[i, F_:]), (e.down, down[i], down_scale[i])):
+            if p.qweight.data_ptr() != w.data_ptr() or p.w_scale.data_ptr() != s.data_ptr():
+                moe._experts = None
+                moe.fuse_experts()
+                return
+
+
 class MoE(nn.Module):
     """Routed experts in the MLP's place (DeepSeekMoE, astrai/model/components/mlp.py:31-93): every token goes through ``n_activated_experts`` of
     ``n_routed_experts`` MLPs, chosen by the largest logits of ``router`` and weighted by their softmax, and through all ``n_shared_experts``.
@@ -439,7 +453,8 @@ class MoE(nn.Module):
     Its plain forward runs the experts one after the other on the rows of their tokens, as the reference does, and so waits for the
     device to learn how many each has.  ``fuse_experts()`` runs a quantized layer's routing, products and sums on the device, in one call
     that waits for nothing (and can be captured in a graph): not bit-identical, since h = up * silu(gate) is rounded once and the weights stay in
-    float32."""
+    float32.  The experts' own forwards (and hooks on them) are not called then.  Where autograd records, through ``x`` or the router's weight, the layer
+    runs the plain forward."""
 
     def __init__(self, dim: int, dim_ffn: int, n_routed_experts: int, n_activated_experts: int, n_shared_experts: int = 0):
         super().__init__()
@@ -450,6 +465,7 @@ class MoE(nn.Module):
         self.routed_experts = nn.ModuleList([MLP(dim, dim_ffn) for _ in range(n_routed_experts)])
         self.shared_experts = nn.ModuleList([MLP(dim, dim_ffn) for _ in range(n_shared_experts)])
         self._experts: Optional[Tuple[Tensor, Tensor, Tensor, Tensor]] = None  # set by fuse_experts(): stacked codes and scales
+        self.register_load_state_dict_post_hook(_stack_again)
 
     def fuse_experts(self) -> bool:
         """Stacks the quantized experts' weights (up on top of gate, and down); the experts' own buffers become slices of the stacks, so
@@ -482,11 +498,14 @@ class MoE(nn.Module):
             self.fuse_experts()
         return self
 
-    def _route(self, x: Tensor) -> Tuple[Tensor, Tensor]:
+    def _choose(self, logits: Tensor, dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
         """weights and experts ``[T, k]`` as the reference takes them (mlp.py:72-82)"""
-        probs = torch.softmax(self.router(x).float(), dim=-1).to(x.dtype)
+        probs = torch.softmax(logits.float(), dim=-1).to(dtype)
         w, idx = torch.topk(probs, self.n_activated_experts, dim=-1)
         return w / w.sum(dim=-1, keepdim=True), idx
+
+    def _route(self, x: Tensor) -> Tuple[Tensor, Tensor]:
+        return self._choose(self.router(x), x.dtype)
 
     def forward(self, x: Tensor, codes: Optional[Tuple[Tensor, Tensor]] = None, residual: Optional[Tensor] = None, norm=None) -> Tensor:
         """``residual`` and ``norm`` as for the MLP; the router needs the activations themselves, so ``codes`` are not taken."""
@@ -498,11 +517,12 @@ class MoE(nn.Module):
         for shared in self.shared_experts:
             y = shared(x)
             residual = y if residual is None else residual + y
-        if self._experts is not None and x.is_cuda and not (torch.is_grad_enabled() and x.requires_grad):
-            r = ops.route_topk(self.router(rows), self.n_activated_experts)
+        logits = self.router(rows)
+        if self._experts is not None and x.is_cuda and not logits.requires_grad:
+            r = ops.route_topk(logits, self.n_activated_experts)
             out = ops.experts_w8a8(rows, r, *self._experts, residual=None if residual is None else residual.reshape(rows.shape))
             return out.view(x.shape)
-        w, idx = self._route(rows)
+        w, idx = self._choose(logits, x.dtype)
         out = torch.zeros_like(rows)
         for e, expert in enumerate(self.routed_experts):
             tok, slot = (idx == e).nonzero(as_tuple=True)

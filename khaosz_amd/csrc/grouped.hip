@@ -66,6 +66,9 @@ __device__ __forceinline__ void store_out(void* y, int64_t i, float v) {
 // Tiles of 16 rows x 32 weight rows: four wavefronts take every fourth 128-byte line of K, weights straight from memory into registers, the sums
 // meet in LDS.  Rows come as codes, from memory like the weights (IN = CODES), or as they are, and every workgroup quantises its own while its
 // weights are on their way (the row quantiser's arithmetic): a launch less for a few rows.
+// What bounds it: HBM (16 tokens' 6 of 64 experts, SwiGLU of 2048 -> 1408 from codes: 293 MB in 49 us, 6.0 TB/s, the launch included); of one token the
+// chain of launch, offsets, row and weights (35 MB in 11 us).  A workgroup that walks units, the next one's weights on their way, is slower (one token
+// 14.6 us, 16 tokens 54): two of its size fit a compute unit where four of these do.
 constexpr int GP_MAX_TOKEN_K = 64;  // choices of a token
 enum { IN_CODES = 0, IN_BF16 = 1, IN_F32 = 2 };
 constexpr int GF_ROWS = 16, GF_COLS = 32, GF_WAVES = 4;
@@ -441,7 +444,7 @@ extern "C" int aq_experts_w8a8(const void* x, int x_dtype, int64_t T, int64_t di
   if (!x || !offsets || !tokens || !rows || !weights || !up_gate || !up_gate_scale || !down || !down_scale || !out || !workspace) return AQ_E_NULL;
   if (aq::check_ptr16(x) || aq::check_ptr16(up_gate) || aq::check_ptr16(down) || aq::check_ptr16(out) || aq::check_ptr16(workspace) ||
       aq::check_ptr(up_gate_scale, 4) || aq::check_ptr(down_scale, 4) || aq::check_ptr(offsets, 4) ||
-      aq::check_ptr(tokens, 4) || aq::check_ptr(rows, 4) || aq::check_ptr(weights, 4))
+      aq::check_ptr(tokens, 4) || aq::check_ptr(rows, 4) || aq::check_ptr(weights, 4) || aq::check_ptr(residual, x_dtype == AQ_BF16 ? 2 : 4))
     return AQ_E_ALIGN;
   if (workspace_bytes < aq_experts_w8a8_workspace_bytes(x_dtype, T, k, dim, F)) return AQ_E_WORKSPACE;
   const int64_t R = T * k;

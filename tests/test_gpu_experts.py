@@ -400,6 +400,33 @@ def test_layer_is_its_parts(T, E, k, dim, F, dtype):
     assert (got.double() - want).norm() / want.norm() < 4e-2
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [1, 5, 40, 700])
+def test_layer_with_infinities_and_nan_in_a_row(T, dtype):
+    """The same bits, or NaN in the same places, whichever launch quantises the rows; the other rows as without them."""
+    _say("odd rows", T, dtype)
+    _, _, uq, us, dq, ds = _layer(8, 256, 352, T)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = torch.randn(T, 256, generator=g, device=DEV).to(dtype)
+    r = ops.route_topk(torch.randn(T, 8, generator=g, device=DEV), 2)
+    clean = ops.experts_w8a8(x, r, uq, us, dq, ds)
+    others = torch.arange(T, device=DEV) != T // 2
+    for odd in (math.inf, -math.inf, math.nan, 3e38):
+        x[T // 2, 7] = odd
+        got, want = ops.experts_w8a8(x, r, uq, us, dq, ds), _composed(x, r, uq, us, dq, ds, None)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+        assert torch.equal(got[others], clean[others])
+
+
+def test_layer_of_no_tokens():
+    _, _, uq, us, dq, ds = _layer(3, 64, 32, 1)
+    r = ops.route_topk(torch.empty(0, 3, device=DEV), 2)
+    x = torch.empty(0, 64, device=DEV)
+    assert ops.experts_w8a8(x, r, uq, us, dq, ds).shape == (0, 64)
+    assert ops.linear_w8a8_grouped(x.to(torch.int8), x[:, 0], uq, us, r.offsets).shape == (0, 64)
+    assert ops.combine_rows(x, r.rows, r.weights).shape == (0, 64)
+
+
 def test_layer_under_a_graph_on_another_stream_and_twice_at_once():
     """One captured pass (routing and experts) replayed over new inputs beside eager work; two streams at once."""
     E, k, dim, F = 16, 4, 256, 128

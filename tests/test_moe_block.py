@@ -109,6 +109,38 @@ def test_stacked_weights_follow_loads_moves_and_copies():
 
 
 @pytest.mark.gpu
+def test_stacked_weights_follow_a_load_that_assigns():
+    m, other = (_moe(64, 48, 4, 2, seed=s).to(DEV) for s in (1, 9))
+    quantize_model(m)
+    quantize_model(other)
+    fuse_shared_inputs(m, experts=True)
+    x = torch.randn(9, 64, device=DEV)
+    with torch.inference_mode():
+        before = m(x)
+        m.load_state_dict({k: v.clone() for k, v in other.state_dict().items()}, assign=True)
+        other.fuse_experts()
+        assert torch.equal(m(x), other(x)) and not torch.equal(m(x), before)
+        assert m._experts[2].data_ptr() == m.routed_experts[0].down.qweight.data_ptr()
+        assert torch.equal(m.routed_experts[3](x), other.routed_experts[3](x))
+
+
+@pytest.mark.gpu
+def test_a_fused_layer_keeps_the_routers_gradient_and_refuses_the_inputs():
+    m = _moe(64, 48, 4, 2).to(DEV)
+    quantize_model(m)
+    m.fuse_experts()
+    x = torch.randn(9, 64, device=DEV)
+    out = m(x)
+    out.sum().backward()
+    assert out.requires_grad and m.router.weight.grad.abs().sum() > 0
+    with pytest.raises(RuntimeError):
+        m(x.clone().requires_grad_())
+    m.router.requires_grad_(False)
+    assert not m(x).requires_grad
+    assert m(x[:0]).shape == (0, 64)
+
+
+@pytest.mark.gpu
 def test_experts_that_cannot_be_stacked_stay_as_they_are():
     m = _moe(64, 48, 4, 2).to(DEV)
     quantize_model(m)
