@@ -75,6 +75,18 @@ constexpr int GF_ROWS = 16, GF_COLS = 32, GF_WAVES = 4;
 // bytes between rows of codes in LDS: 16 of them then begin 4 banks apart
 __host__ __device__ inline int few_pitch(int K) { return (K + 127) / 128 * 128 + 16; }
 
+// A row of x (rows: they are, in its type) on its way into a wavefront's registers; -1: zeros.
+template <bool BF16, int VPL>
+__device__ __forceinline__ void ask_for_row(RowsToLds<BF16, 1, VPL>& r, const uint8_t* x, int K, int row, int lane) {
+  const uint32_t bytes = (uint32_t)K * (BF16 ? 2 : 4);
+  const __amdgpu_buffer_rsrc_t R = make_rsrc(x + (row < 0 ? 0 : row) * (int64_t)bytes, row < 0 ? 0u : bytes);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const v4i v = __builtin_amdgcn_raw_buffer_load_b128(R, (i * 64 + lane) * 16, 0, 0);
+    r.c[0][i] = make_uint4((uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3]);
+  }
+}
+
 // DEEP: lines of a wavefront on their way at a time, cut to the rows' length class (a load of nothing takes its turn in the address path all the
 // same, and branches around loads make them wait for each other: 24.7 -> 66 us for four tokens' up and gate).
 template <int OUT, bool SWI, int IN, int VPL, int DEEP>
@@ -83,6 +95,10 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
   __shared__ int part[GF_WAVES][2][GF_ROWS][17];
   __shared__ float scale[GF_ROWS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // tokens of up to 64 rows come beside the offsets: x is then asked for without another wait
+  const bool near = p.R <= 64;
+  int my_token = -1;
+  if (p.tokens && near) my_token = p.tokens[lane < p.R ? lane : 0];
   RowTile t;
   if (!find_tile<GF_ROWS>(p, blockIdx.y, lane, t)) return;
   const int K = p.K, FH = SWI ? p.N / 2 : p.N;
@@ -94,8 +110,10 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
   const uint32_t ao = (uint32_t)na * (uint32_t)K + q16, bo = (uint32_t)nb * (uint32_t)K + q16;
   const int lines = (K + 127) / 128;
   auto token = [&](int row) {  // -1: none
-    const int tok = row < t.end ? (p.tokens ? p.tokens[row] : row) : -1;
-    return tok < p.x_rows ? tok : -1;
+    int tok = row;
+    if (p.tokens && near) tok = __shfl(my_token, row & 63);
+    else if (p.tokens) tok = row < t.end ? p.tokens[row] : -1;
+    return row < t.end && tok >= 0 && tok < p.x_rows ? tok : -1;
   };
   v4i av[2 * DEEP], bv[2 * DEEP];
   auto k_of = [&](int l0, int i) { return (l0 + i / 2 * GF_WAVES) * 128 + i % 2 * 64; };
@@ -108,6 +126,16 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
       bv[i] = __builtin_amdgcn_raw_buffer_load_b128(Wr, in && inb ? bo + k : OOB_OFFSET, 0, 2);
     }
   };
+  // The first row of each wavefront before the weights, as it is rounded while they come (behind them if its token takes a wait of its own).
+  constexpr bool BF16 = IN == IN_BF16;
+  const int rows = t.end - t.first < GF_ROWS ? t.end - t.first : GF_ROWS;
+  const bool known = !p.tokens || near;
+  int tok = -1;
+  [[maybe_unused]] RowsToLds<BF16, 1, VPL> ahead;
+  if constexpr (IN != IN_CODES) {
+    if (known) tok = __builtin_amdgcn_readfirstlane(token(t.first + wave));
+    ask_for_row<BF16>(ahead, p.x, K, tok, lane);
+  }
   load_weights(wave);
   // the epilogue's operands, one tile row and two columns (SwiGLU: one) to a thread
   const int m = tid >> 4, c = tid & 15, out_row = t.first + m;
@@ -131,14 +159,16 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
     const int tok = token(t.first + r16);
     if (tok >= 0) xo = (uint32_t)tok * (uint32_t)K + q16;
   } else {
-    constexpr bool BF16 = IN == IN_BF16;
-    const int rows = t.end - t.first < GF_ROWS ? t.end - t.first : GF_ROWS;
-    for (int m = wave; m < rows; m += GF_WAVES) {
+    auto round_row = [&](RowsToLds<BF16, 1, VPL>& r, int m, int tok) {
+      r.finish(1, 1, K, xs + m * pitch, pitch, scale + m, 0, 1, lane);
+      if (tok < 0 && lane == 0) scale[m] = 0.0f;  // a row of zeros
+    };
+    if (known && wave < rows) round_row(ahead, wave, tok);
+    for (int m = known ? wave + GF_WAVES : wave; m < rows; m += GF_WAVES) {
       const int tok = __builtin_amdgcn_readfirstlane(token(t.first + m));
       RowsToLds<BF16, 1, VPL> r;
-      r.issue(p.x + (int64_t)(tok < 0 ? 0 : tok) * K * (BF16 ? 2 : 4), tok >= 0, K, K, 0, 1, lane);
-      r.finish(tok >= 0, 1, K, xs + m * pitch, pitch, scale + m, 0, 1, lane);
-      if (tok < 0 && lane == 0) scale[m] = 0.0f;  // a row of zeros
+      ask_for_row<BF16>(r, p.x, K, tok, lane);
+      round_row(r, m, tok);
     }
     __syncthreads();
   }
