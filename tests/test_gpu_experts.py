@@ -401,6 +401,22 @@ def test_layer_is_its_parts(T, E, k, dim, F, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,k", [(63, 1), (64, 1), (65, 1), (32, 2), (33, 2), (16, 4)])
+def test_layer_whose_tokens_fit_a_wavefront_and_do_not(T, k, dtype):
+    """63 to 66 rows of 3 experts, tiles of up to 16: the tokens beside the offsets, or read row by row; and a row of a token that there is not."""
+    _, _, uq, us, dq, ds = _layer(3 + k, 144, 80, T)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = torch.randn(T, 144, generator=g, device=DEV).to(dtype)
+    r = ops.route_topk(torch.randn(T, 3 + k, generator=g, device=DEV), k)
+    assert torch.equal(ops.experts_w8a8(x, r, uq, us, dq, ds), _composed(x, r, uq, us, dq, ds, None))
+    tokens = r.tokens.clone()
+    tokens[0], tokens[T // 2], tokens[-1] = -1, T, 1 << 30
+    odd = r._replace(tokens=tokens)
+    got = ops.experts_w8a8(x, odd, uq, us, dq, ds)
+    assert torch.equal(got, _composed(x, odd, uq, us, dq, ds, None))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("T", [1, 5, 40, 700])
 def test_layer_with_infinities_and_nan_in_a_row(T, dtype):
     """The same bits, or NaN in the same places, whichever launch quantises the rows; the other rows as without them."""
