@@ -33,12 +33,13 @@ __device__ __forceinline__ void fetch_dword_to_lds(__amdgpu_buffer_rsrc_t r, voi
 }
 __device__ __forceinline__ uint32_t load_dword(__amdgpu_buffer_rsrc_t r, uint32_t at) { return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)at, 0, 0); }
 __device__ __forceinline__ uint32_t load_word(__amdgpu_buffer_rsrc_t r, uint32_t at) { return (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)at, 0, 0); }
-template <int POLICY = STORE_WT>
+template <int POLICY>
 __device__ __forceinline__ void store_dword(uint32_t v, __amdgpu_buffer_rsrc_t r, uint32_t at) { __builtin_amdgcn_raw_buffer_store_b32(v, r, at, 0, POLICY); }
 __device__ __forceinline__ void store_word(uint32_t v, __amdgpu_buffer_rsrc_t r, uint32_t at) { __builtin_amdgcn_raw_buffer_store_b16((uint16_t)v, r, at, 0, 0); }
+template <int POLICY>
 __device__ __forceinline__ void store_pair(float a, float b, __amdgpu_buffer_rsrc_t r, uint32_t at) {
   const v2i_t two = {__float_as_int(a), __float_as_int(b)};
-  __builtin_amdgcn_raw_buffer_store_b64(two, r, at, 0, STORE_WT);
+  __builtin_amdgcn_raw_buffer_store_b64(two, r, at, 0, POLICY);
 }
 // Values of rows a (low half) and b of this lane's column and its neighbour's -> the even lane both columns of row a, the odd one of row b
 __device__ __forceinline__ uint32_t pair_columns(uint32_t mine, bool odd) {
@@ -51,7 +52,12 @@ struct WalkTile {
   int rot;                // the K step it begins with
 };
 
-template <class S, int OUT, bool SWI, bool ODD>
+// Rows of the output: whole 128-byte lines, whole dwords (with bf16: an even number), or neither.  Parts of lines stay in the L2 until the rest is there;
+// written through, they go to memory by themselves (43000 rows of 608 -> 3060: 191 us, 244 written through; whole lines 1 % faster written through
+// where the next launch reads them, 4096 tokens' 6 of 64 320.6 and 322.2).
+enum { ROWS_LINES, ROWS_DWORDS, ROWS_ODD };
+
+template <class S, int OUT, bool SWI, int ROWS>
 __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p, int tiles_n, UDiv by_tiles_n) {
 #ifdef __HIP_DEVICE_COMPILE__  // (the host pass drops a kernel in whose generic lambdas it finds the device's operations)
   __shared__ __attribute__((aligned(1024))) uint8_t smem[S::LDS];
@@ -62,6 +68,8 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
   constexpr int V = SWI || TN == 1 ? 1 : 2;  // neighbouring outputs of a lane
   constexpr int ESZ = OUT == OUT_BF16 ? 2 : 4;
   constexpr int EPI = 4;                     // steps that finish the tile before
+  constexpr bool ODD = ROWS == ROWS_ODD;
+  constexpr int POLICY = ROWS == ROWS_LINES ? STORE_WT : 0;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wave_m = wave / S::WN, wave_n = wave % S::WN;
@@ -204,21 +212,21 @@ __global__ __launch_bounds__(GW_THREADS) void grouped_walk_kernel(GroupedArgs p,
     if constexpr (V == 2 && ODD) {
       const uint32_t at1 = done.at1 + (r0 + q) * rowb;
       if constexpr (OUT == OUT_F32) {
-        store_dword<0>(__float_as_uint(o[0]), done.out, at);
-        store_dword<0>(__float_as_uint(o[V - 1]), done.out, at1);
+        store_dword<POLICY>(__float_as_uint(o[0]), done.out, at);
+        store_dword<POLICY>(__float_as_uint(o[V - 1]), done.out, at1);
       } else {
         store_word(f32_to_bf16_bits(o[0]), done.out, at);
         store_word(f32_to_bf16_bits(o[V - 1]), done.out, at1);
       }
     } else if constexpr (V == 2) {
-      if constexpr (OUT == OUT_F32) store_pair(o[0], o[V - 1], done.out, at);
-      else store_dword(pack_bf16x2(o[0], o[V - 1]), done.out, at);
+      if constexpr (OUT == OUT_F32) store_pair<POLICY>(o[0], o[V - 1], done.out, at);
+      else store_dword<POLICY>(pack_bf16x2(o[0], o[V - 1]), done.out, at);
     } else if constexpr (OUT == OUT_F32) {
-      store_dword(__float_as_uint(o[0]), done.out, at);
+      store_dword<POLICY>(__float_as_uint(o[0]), done.out, at);
     } else if constexpr (ODD) {
       store_word(f32_to_bf16_bits(o[0]), done.out, at);
     } else {  // two rows of two neighbouring lanes
-      if (q & 1) store_dword(pair_columns(pack_bf16x2(held, o[0]), odd_lane), done.out, at - rowb);
+      if (q & 1) store_dword<POLICY>(pair_columns(pack_bf16x2(held, o[0]), odd_lane), done.out, at - rowb);
       held = o[0];
     }
   };
@@ -393,13 +401,14 @@ static int walk_launch(const GroupedArgs& a, hipStream_t st) {
   const int cus = device_cus();
   const dim3 grid((unsigned)(most < cus ? most : cus)), block(GW_THREADS);
   const UDiv by_tiles_n = UDiv::of((uint32_t)tiles_n);
-  if constexpr (!SWI) {
-    if (a.N & 1) {
-      queue_kernel(grouped_walk_kernel<S, OUT, SWI, true>, grid, block, 0, st, a, tiles_n, by_tiles_n);
-      return (int)hipGetLastError();
-    }
+  const bool lines = (SWI ? a.N / 2 : a.N) * (OUT == OUT_BF16 ? 2 : 4) % 128 == 0;
+  if (lines) {
+    queue_kernel((grouped_walk_kernel<S, OUT, SWI, ROWS_LINES>), grid, block, 0, st, a, tiles_n, by_tiles_n);
+  } else if (SWI || a.N % 2 == 0) {
+    queue_kernel((grouped_walk_kernel<S, OUT, SWI, ROWS_DWORDS>), grid, block, 0, st, a, tiles_n, by_tiles_n);
+  } else if constexpr (!SWI) {
+    queue_kernel((grouped_walk_kernel<S, OUT, SWI, ROWS_ODD>), grid, block, 0, st, a, tiles_n, by_tiles_n);
   }
-  queue_kernel(grouped_walk_kernel<S, OUT, SWI, false>, grid, block, 0, st, a, tiles_n, by_tiles_n);
   return (int)hipGetLastError();
 }
 template <int OUT, bool SWI>
