@@ -23,6 +23,7 @@ struct GroupedArgs {
   int x_rows, R, E;
   int N;            // weight rows of an expert (SwiGLU: up and gate)
   int K;
+  int held;         // rows that a workgroup has room for in LDS, where it quantises them
 };
 
 // Inclusive sum over the 64 lanes

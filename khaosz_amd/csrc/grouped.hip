@@ -90,7 +90,7 @@ __device__ __forceinline__ void ask_for_row(RowsToLds<BF16, 1, VPL>& r, const ui
 // DEEP: lines of a wavefront on their way at a time, cut to the rows' length class (a load of nothing takes its turn in the address path all the
 // same, and branches around loads make them wait for each other: 24.7 -> 66 us for four tokens' up and gate).
 template <int OUT, bool SWI, int IN, int VPL, int DEEP>
-__global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs p) {
+__global__ __launch_bounds__(GF_WAVES * 64, VPL == 8 ? 3 : VPL == 16 ? 2 : 1) void grouped_few_kernel(GroupedArgs p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t xs[];  // IN: the rows' codes
   __shared__ int part[GF_WAVES][2][GF_ROWS][17];
   __shared__ float scale[GF_ROWS];
@@ -153,6 +153,7 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
     if (tok >= 0) sx = p.sx[tok];
   }
   const int pitch = few_pitch(K);
+  [[maybe_unused]] const uint8_t* const held = xs + (r16 < p.held ? r16 : 0) * pitch;  // (rows past the tile's: any)
   __amdgpu_buffer_rsrc_t Xr = make_rsrc(p.x, IN == IN_CODES ? (uint32_t)p.x_rows * (uint32_t)K : 0u);
   uint32_t xo = OOB_OFFSET;
   if constexpr (IN == IN_CODES) {
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(GF_WAVES * 64) void grouped_few_kernel(GroupedArgs 
         xv[i] = __builtin_amdgcn_raw_buffer_load_b128(Xr, k + q16 < K && xo != OOB_OFFSET ? xo + k : OOB_OFFSET, 0, 0);
       } else {
         xv[i] = v4i{0, 0, 0, 0};  // (past K the weights are zeros)
-        if (k < K) xv[i] = *reinterpret_cast<const v4i*>(xs + r16 * pitch + k + q16);
+        if (k < K) xv[i] = *reinterpret_cast<const v4i*>(held + k + q16);
       }
     }
 #pragma unroll
@@ -336,46 +337,67 @@ static int launch_few_of(const GroupedArgs& a, hipStream_t st) {
   const int64_t tiles = grouped_most_tiles(a.R, a.E, GF_ROWS), cols = (a.N + GF_COLS - 1) / GF_COLS;
   if (tiles > 65535 || cols > 0x7fffffff) return AQ_E_RANGE;  // (more rows of N > 2^20 columns than memory holds)
   queue_kernel((grouped_few_kernel<OUT, SWI, IN, VPL, DEEP>), dim3((unsigned)cols, (unsigned)tiles), dim3(GF_WAVES * 64),
-               IN == IN_CODES ? 0 : GF_ROWS * few_pitch(a.K), st, a);
+               IN == IN_CODES ? 0 : a.held * few_pitch(a.K), st, a);
   return (int)hipGetLastError();
 }
 
+// VPL: 16-byte vectors of a row in a lane (rows as they are), 4, 8 or 16: rows of the length class below are not its own.
 template <int OUT, bool SWI, int IN, int VPL>
 static int launch_few(const GroupedArgs& a, hipStream_t st) {
-  return a.K <= GF_WAVES * 3 * 128 ? launch_few_of<OUT, SWI, IN, VPL, 3>(a, st) : launch_few_of<OUT, SWI, IN, VPL, 4>(a, st);
+  constexpr int DEEP_3 = GF_WAVES * 3 * 128, MOST = IN == IN_CODES ? 1 << 30 : VPL * 64 * (IN == IN_BF16 ? 8 : 4), LEAST = VPL <= 4 ? 0 : MOST / 2;
+  if constexpr (LEAST < DEEP_3)
+    if (a.K <= DEEP_3) return launch_few_of<OUT, SWI, IN, VPL, 3>(a, st);
+  if constexpr (MOST > DEEP_3) return launch_few_of<OUT, SWI, IN, VPL, 4>(a, st);
+  return AQ_E_RANGE;
 }
 
-// Rows as they are (a.x of `dtype`, which is the output's type too), quantised in the launch.
-constexpr int64_t GF_IN_BF16_K = 4096, GF_IN_F32_K = 2048;  // longest rows
-template <bool SWI>
-static int launch_rows(const GroupedArgs& a, int dtype, hipStream_t st) {
-  if (dtype == AQ_BF16)
-    return a.K <= 2048 ? launch_few<OUT_BF16, SWI, IN_BF16, 4>(a, st) : launch_few<OUT_BF16, SWI, IN_BF16, 8>(a, st);
-  return a.K <= 1024 ? launch_few<OUT_F32, SWI, IN_F32, 4>(a, st) : launch_few<OUT_F32, SWI, IN_F32, 8>(a, st);
+// Rows as they are (a.x of `dtype`, which is the output's type too), quantised in the launch.  A workgroup has their codes in LDS: up to 16 rows of 4096,
+// or fewer of up to 8192, so that a compute unit has room for two.
+static int64_t most_in_launch(int dtype) { return dtype == AQ_BF16 ? 8192 : 4096; }  // of 16 vectors a lane
+static int rows_held(int64_t R) { return R < GF_ROWS ? (int)R : GF_ROWS; }
+static bool rows_fit(int64_t K, int64_t R) { return rows_held(R) * few_pitch((int)K) <= GF_ROWS * few_pitch(4096); }
+template <int OUT, int IN, bool SWI>
+static int launch_rows_of(const GroupedArgs& a, hipStream_t st) {
+  constexpr int CLASS = 256 * (IN == IN_BF16 ? 8 : 4);
+  return a.K <= CLASS       ? launch_few<OUT, SWI, IN, 4>(a, st)
+         : a.K <= 2 * CLASS ? launch_few<OUT, SWI, IN, 8>(a, st)
+                            : launch_few<OUT, SWI, IN, 16>(a, st);
 }
-// Whether the two products of a layer quantise their rows themselves: two launches less, but every workgroup rounds its tile's rows, and tiles of 16 rows
-// stream weights at 5.6 TB/s where walked ones reach 6.3 (us, with | without: 16 tokens' 6 of 64 of 2048 / 1408 91 | 99, 32 tokens' 113 | 109;
-// 16 tokens' 2 of 8 of 1536 / 2816 38 | 41, 32 tokens' 43.5 | 43.6).
-static bool rows_in_launch(int64_t T, int64_t k, int64_t E, int64_t dim, int64_t F, int dtype) {
-  const int64_t most = dtype == AQ_BF16 ? GF_IN_BF16_K : GF_IN_F32_K, R = T * k;
-  if (dim > most || F > most || !few_fits(R, E)) return false;
+template <bool SWI>
+static int launch_rows(GroupedArgs a, int dtype, hipStream_t st) {
+  a.held = rows_held(a.R);
+  return dtype == AQ_BF16 ? launch_rows_of<OUT_BF16, IN_BF16, SWI>(a, st) : launch_rows_of<OUT_F32, IN_F32, SWI>(a, st);
+}
+// Whether a product of a layer quantises its rows itself: a launch less, but every workgroup reads and rounds its tile's rows, one after the other in a
+// wavefront, holds up to 16 of them in LDS and longer ones in more registers.  So the weights times 1 + rows an expert have a limit by the rows' length
+// (us of the layer, with | without.  Up to 2048: 16 tokens' 6 of 64 of 2048 / 1408, x 93.1 | 95.8, then h 89.8 | 93.1; 16 tokens' 4 of 16 of 2048 / 5632, x 123.2 | 121.5.  Up
+// to 4096: 4 tokens' 2 of 8 of 3584 / 4096, x 63.2 | 69.8, 8 tokens' 80.5 | 77.7.  Up to 8192: one token's 2 of 8 of 1536 / 6912, h 25.6 | 35.0, of 4096 / 8192 67.8 | 65.7,
+// 4 tokens' 143 | 123), and rows an expert by themselves (32 tokens' 8 of 16 of 5120 / 144, h 50.0 | 43.4).  At 106 sizes 1.2 % slower than the best choice
+// in the mean.
+static bool rows_in_launch(int64_t R, int64_t E, int64_t N, int64_t K, int dtype) {
+  if (K > most_in_launch(dtype) || !few_fits(R, E)) return false;
 #ifdef AQ_LAB
   if (g_forced_grouped) return g_forced_grouped == GROUPED_FEW;
 #endif
-  return experts_used(R, E) * (double)(3 * dim * F) * (1.0 + (double)R / E) <= 1.2e9;
+  const double limit = 4 * K <= most_in_launch(dtype) ? 8e8 : 2 * K <= most_in_launch(dtype) ? 3e8 : 1.2e8;
+  return R <= 8 * E && experts_used(R, E) * (double)(N * K) * (1.0 + (double)R / E) <= limit;
 }
 
 // The second product with the weighted sum (dim is a multiple of 16, and so of GT_COLS).
 template <int OUT, int VPL>
 static int launch_token(const TokenArgs& a, int64_t T, hipStream_t st) {
   const dim3 grid((unsigned)(a.g.N / GT_COLS), (unsigned)T), block(GT_WAVES * 64);
-  const size_t lds = (size_t)GT_WAVES * few_pitch(a.g.K);
+  const size_t lds = (size_t)(a.k < GT_WAVES ? a.k : GT_WAVES) * few_pitch(a.g.K);
   queue_kernel((grouped_token_kernel<OUT, VPL>), grid, block, lds, st, a);
   return (int)hipGetLastError();
 }
+template <int OUT>
+static int launch_tokens_of(const TokenArgs& a, int64_t T, hipStream_t st) {
+  constexpr int CLASS = 256 * (OUT == OUT_BF16 ? 8 : 4);
+  return a.g.K <= CLASS ? launch_token<OUT, 4>(a, T, st) : a.g.K <= 2 * CLASS ? launch_token<OUT, 8>(a, T, st) : launch_token<OUT, 16>(a, T, st);
+}
 static int launch_tokens(const TokenArgs& a, int64_t T, int dtype, hipStream_t st) {
-  if (dtype == AQ_BF16) return a.g.K <= 2048 ? launch_token<OUT_BF16, 4>(a, T, st) : launch_token<OUT_BF16, 8>(a, T, st);
-  return a.g.K <= 1024 ? launch_token<OUT_F32, 4>(a, T, st) : launch_token<OUT_F32, 8>(a, T, st);
+  return dtype == AQ_BF16 ? launch_tokens_of<OUT_BF16>(a, T, st) : launch_tokens_of<OUT_F32>(a, T, st);
 }
 // Whether it is: what the experts of several tokens cost more, read for each, is then less than the launch saved (us of the layer, with | without: 64
 // choices of 256 experts of 1024 / 512, 4 MB more, 33.4 | 36.0; 18 of 64 of 2048 / 1408, 7 MB, 42.7 | 40.2; 24 of them, 11 MB, 48.8 | 46.3).
@@ -483,40 +505,43 @@ extern "C" int aq_experts_w8a8(const void* x, int x_dtype, int64_t T, int64_t di
   int8_t *const xq = reinterpret_cast<int8_t*>(ws + s.xq), *const hq = reinterpret_cast<int8_t*>(ws + s.hq);
   float *const sx = reinterpret_cast<float*>(ws + s.sx), *const sh = reinterpret_cast<float*>(ws + s.sh);
   void *const h = ws + s.h, *const y = ws + s.y;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  aq::GroupedArgs a{};
+  a.offsets = offsets;
+  a.R = (int)R;
+  a.E = (int)E;
   int rc;
-  if (aq::rows_in_launch(T, k, E, dim, F, x_dtype)) {
-    aq::GroupedArgs a{};
+  if (aq::rows_in_launch(R, E, 2 * F, dim, x_dtype) && aq::rows_fit(dim, R)) {
     a.x = static_cast<const uint8_t*>(x);
     a.x_rows = (int)T;
     a.w = reinterpret_cast<const uint8_t*>(up_gate);
     a.sw = up_gate_scale;
-    a.offsets = offsets;
     a.tokens = tokens;
     a.y = h;
     a.w_bytes = 2 * F * dim;
-    a.R = (int)R;
-    a.E = (int)E;
     a.N = (int)(2 * F);
     a.K = (int)dim;
-    rc = aq::launch_rows<true>(a, x_dtype, static_cast<hipStream_t>(stream));
+    rc = aq::launch_rows<true>(a, x_dtype, st);
+  } else {
+    rc = aq_quant_rowwise_i8(x, x_dtype, T, dim, dim, xq, sx, stream);
+    if (rc == AQ_OK) rc = aq_swiglu_w8a8_grouped(xq, sx, T, up_gate, up_gate_scale, offsets, E, tokens, R, h, x_dtype, F, dim, stream);
+  }
+  if (rc != AQ_OK) return rc;
+  const bool few = aq::rows_in_launch(R, E, dim, F, x_dtype), token = few && aq::tokens_in_launch(T, k, E, dim, F);
+  if (token || (few && aq::rows_fit(F, R))) {
     a.x = static_cast<const uint8_t*>(h);
     a.x_rows = (int)R;
     a.w = reinterpret_cast<const uint8_t*>(down);
     a.sw = down_scale;
     a.tokens = nullptr;
-    a.y = y;
+    a.y = token ? out : y;
     a.w_bytes = dim * F;
     a.N = (int)dim;
     a.K = (int)F;
-    if (rc == AQ_OK && aq::tokens_in_launch(T, k, E, dim, F)) {
-      a.y = out;
-      return aq::launch_tokens(aq::TokenArgs{a, rows, weights, residual, (int)k}, T, x_dtype, static_cast<hipStream_t>(stream));
-    }
-    if (rc == AQ_OK) rc = aq::launch_rows<false>(a, x_dtype, static_cast<hipStream_t>(stream));
+    if (token) return aq::launch_tokens(aq::TokenArgs{a, rows, weights, residual, (int)k}, T, x_dtype, st);
+    rc = aq::launch_rows<false>(a, x_dtype, st);
   } else {
-    rc = aq_quant_rowwise_i8(x, x_dtype, T, dim, dim, xq, sx, stream);
-    if (rc == AQ_OK) rc = aq_swiglu_w8a8_grouped(xq, sx, T, up_gate, up_gate_scale, offsets, E, tokens, R, h, x_dtype, F, dim, stream);
-    if (rc == AQ_OK) rc = aq_quant_rowwise_i8(h, x_dtype, R, F, F, hq, sh, stream);
+    rc = aq_quant_rowwise_i8(h, x_dtype, R, F, F, hq, sh, stream);
     if (rc == AQ_OK) rc = aq_linear_w8a8_grouped(hq, sh, R, down, down_scale, nullptr, AQ_F32, offsets, E, nullptr, R, y, x_dtype, dim, F, stream);
   }
   if (rc == AQ_OK) rc = aq_combine_rows(y, x_dtype, R, dim, rows, weights, T, k, residual, out, stream);

@@ -417,6 +417,19 @@ def test_layer_whose_tokens_fit_a_wavefront_and_do_not(T, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,E,k,dim,F", [(1, 4, 2, 128, 6912), (1, 2, 1, 8192, 48), (1, 2, 1, 8208, 48), (2, 4, 4, 64, 8192), (2, 4, 4, 64, 8208), (3, 4, 3, 4112, 4112),
+                                         (4, 8, 2, 64, 6912), (5, 8, 2, 6912, 64), (7, 4, 2, 96, 4128), (16, 4, 4, 4112, 32), (16, 4, 4, 32, 4112), (40, 4, 1, 2064, 2064)])
+def test_layer_of_long_rows(T, E, k, dim, F, dtype):
+    """Rows of x or of h of more than 4096 (fp32: 2048) are quantised in the products' launches while a workgroup has room for them."""
+    _say("long rows", T, E, k, dim, F, dtype)
+    _, _, uq, us, dq, ds = _layer(E, dim, F, T)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x, res = (torch.randn(T, dim, generator=g, device=DEV).to(dtype) for _ in range(2))
+    r = ops.route_topk(torch.randn(T, E, generator=g, device=DEV), k)
+    assert torch.equal(ops.experts_w8a8(x, r, uq, us, dq, ds, residual=res), _composed(x, r, uq, us, dq, ds, res))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("T", [1, 5, 40, 700])
 def test_layer_with_infinities_and_nan_in_a_row(T, dtype):
     """The same bits, or NaN in the same places, whichever launch quantises the rows; the other rows as without them."""
