@@ -305,13 +305,17 @@ static int g_forced_grouped = 0;  // lab build only: 0 = by size
 static double experts_used(int64_t R, int64_t E) { return E * (1.0 - std::exp(-(double)R / E)); }
 
 // Which kernel: the one whose estimated time, in us, is least.  Tiles of 16 rows: units of 32 weight rows, four to a compute unit at a time.  Walked
-// tiles: rounds of tiles, each of its steps and a beginning and an end, beside the weights' way from memory.  Fitted to 805 random sizes (1 to 256
-// experts, 1 to 8192 tokens, K 128 to 6912): 1.7 % slower than the best kernel in the mean, one in twenty 11 % or more (always 128 x 256 50 %, always 128 x 128 30 %).
+// tiles: rounds of tiles (mostly whole ones: the last takes as long), each of its steps and a beginning and an end, beside the weights' way from memory.
+// Fitted to 900 random sizes of experts that are asked for alike (1 to 256 experts, 1 to 8192 tokens, K 128 to 6912), 400 of uneven ones (2 to 128 experts, 20 to
+// 600 rows each) and 350 with 0.2 to 300 rows each: 1.5, 0.9 and 1.4 % slower than the best kernel in the mean, one in twenty 12, 6 and 11 % or more (on the
+// first always 128 x 256 50 %, always 128 x 128 30 %).
+// Chosen by the launch itself, from the tiles that there are, the width was 0.3 % off on the second, but three widths in one kernel cost 1 to 2 % and the
+// choice 0.5 to 1 us.
 enum { GROUPED_FEW = 1, GROUPED_WALK_256 = 2, GROUPED_WALK_128 = 3, GROUPED_WALK_64 = 4 };
-static double walk_us(const GroupedArgs& a, double used, int width, int least_steps, double launch, double ends, double step, double tb_s, double tail) {
-  const double avg = a.R / used, cus = device_cus(), steps = (a.K + 127) / 128;
-  const double tiles = used * (avg / 128 + tail > 1 ? avg / 128 + tail : 1) * ((a.N + width - 1) / width), part = tiles / cus;
-  const double rounds = part > 0.78 ? part + 0.25 : part;
+static double walk_us(const GroupedArgs& a, double used, int width, int least_steps, double launch, double ends, double step, double tb_s, double tail, double even) {
+  const double avg = a.R / used / 128 + tail, steps = (a.K + 127) / 128;
+  const double part = used * (avg > 1 ? avg : 1) * ((a.N + width - 1) / width) / device_cus();
+  const double rounds = even * part + (1 - even) * std::ceil(part);
   const double c = (rounds > 1 ? rounds : 1) * (ends + step * (steps > least_steps ? steps : least_steps)), m = used * a.N * a.K * 1e-6 / tb_s;
   return launch + std::sqrt(std::sqrt(c * c * c * c + m * m * m * m));
 }
@@ -321,11 +325,11 @@ static int choose_grouped(const GroupedArgs& a, bool swiglu) {
 #ifdef AQ_LAB
   if (g_forced_grouped) return g_forced_grouped;
 #endif
-  const double used = experts_used(a.R, a.E), rows = a.R / used / 16 + 0.45;
+  const double used = experts_used(a.R, a.E), rows = a.R / used / 16 + 0.58;
   const double units = used * (rows > 1 ? rows : 1) * ((a.N + GF_COLS - 1) / GF_COLS);
-  const double us[] = {units / (4 * device_cus()) * (2.3 + 7.6 * a.K / 1024) + 2.3 * ((a.K + 2047) / 2048),
-                       walk_us(a, used, 256, 6, 4.8, 2.7, 0.47, 5.5, 0.75), walk_us(a, used, 128, 7, 3.4, 2.3, 0.40, 12.0, 0.75),
-                       walk_us(a, used, 64, 10, 2.3, 2.2, 0.26, 5.0, 1.0)};
+  const double us[] = {units / (4 * device_cus()) * (2.24 + 12.82 * a.K / 1024) + 1.80 * ((a.K + 2047) / 2048),
+                       walk_us(a, used, 256, 6, 1.49, 3.80, 1.085, 4.53, 0.544, 0.127), walk_us(a, used, 128, 7, 3.55, 2.36, 0.626, 4.84, 0.527, 0.205),
+                       walk_us(a, used, 64, 10, 3.36, 0.335, 0.507, 6.36, 0.532, 0.217)};
   int best = few_fits(a.R, a.E) ? 0 : 1;
   for (int i = best + 1; i < (swiglu ? 3 : 4); ++i)
     if (us[i] < us[best]) best = i;
