@@ -943,7 +943,7 @@ ROUTE_MAX_EXPERTS, ROUTE_MAX_CHOICES = 512, 16
 class Routing(NamedTuple):
     """What ``route_topk`` gives for ``T`` tokens and ``k`` choices each: the weights (float32 ``[T, k]``) and the experts (int32 ``[T, k]``, -1: none),
     and the choices in the experts' order: expert e has rows ``offsets[e] .. offsets[e + 1] - 1`` (int32 ``[E + 1]``), ``rows`` (int32 ``[T, k]``) is the row of
-    each choice (-1: none) and ``tokens`` (int32 ``[T k]``) the token of each row (-1 past the last one in use)."""
+    each choice (-1: none) and ``tokens`` (int32 ``[T k]``) the token of each row (-1 past the last one in use).  The five may share one storage."""
     weights: torch.Tensor
     experts: torch.Tensor
     rows: torch.Tensor
@@ -1010,7 +1010,7 @@ def linear_w8a8_grouped(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw
     """``linear_w8a8`` of several experts at once, ``wq`` int8 ``[E, N, K]``, ``sw`` ``[E, N]``, ``bias`` ``[E, N]``: rows ``offsets[e] .. offsets[e + 1] - 1``
     (int32 ``[E + 1]``, on the device; a group may be empty) of the result ``[R, N]`` are expert e's Linear on rows ``tokens[r]`` (int32 ``[R]``) of ``xq`` ``[T, K]``, or,
     without ``tokens``, on the same rows of ``xq`` ``[R, K]``: the bits of the single calls.  Rows past ``offsets[E]`` are not written.  A token
-    outside ``0 .. T - 1`` counts as a row of zeros.  ``E`` at most 512."""
+    outside ``0 .. T - 1`` counts as a row of zeros.  ``E`` at most 512, ``R`` 2^25, ``T K`` and ``N K`` below 2^31 - 16."""
     y = (_host or _native()).linear_w8a8_grouped(xq, sx, wq, sw, offsets, tokens, bias, out_dtype)
     if y is not None:
         return y
@@ -1086,7 +1086,8 @@ def experts_w8a8(x: torch.Tensor, routing: Routing, up_gate: torch.Tensor, up_ga
     """The routed experts' MLP on ``x`` ``[T, dim]``: each token's rows through its experts' up, gate, SwiGLU and down, weighted and summed
     (``residual`` ``[T, dim]`` added).  ``up_gate`` int8 ``[E, 2F, dim]`` with scales ``[E, 2F]``, ``down`` int8 ``[E, dim, F]`` with scales ``[E, dim]``.  The bits of
     ``quant_rowwise_i8``, ``swiglu_w8a8_grouped``, ``quant_rowwise_i8``, ``linear_w8a8_grouped`` and ``combine_rows`` one after the other (what
-    DeepSeekMoE.forward, mlp.py:83-91, does expert by expert), in one call that waits for nothing."""
+    DeepSeekMoE.forward, mlp.py:83-91, does expert by expert), in one call that waits for nothing.  At most 64 choices a token; ``T dim``, ``T k F`` and
+    ``2 F dim`` below 2^31 - 16: a longer batch is handed over in parts."""
     out = (_host or _native()).experts_w8a8(x, routing, up_gate, up_gate_scale, down, down_scale, residual)
     if out is not None:
         return out
