@@ -336,6 +336,50 @@ def test_combine(T, k, N, dtype):
         assert ((got.double() - want).abs() <= (k + 2) * HALF[torch.float32] * size + HALF[dtype] * want.abs() + 1e-40).all()
 
 
+@pytest.mark.parametrize("kernel_of", [2, 3, 4])
+def test_outputs_past_32_bits(kernel_of):
+    """1.1 million rows of 2056 bf16 values are 4.5 GB: products that write them, and sums that read the last of them."""
+    from khaosz_amd import _abi
+    R, K, N = 1_100_000, 16, 2056
+    g = torch.Generator().manual_seed(1)
+    xq = torch.randint(-127, 128, (64, K), generator=g, dtype=torch.int8)
+    wq = torch.randint(-127, 128, (2, N, K), generator=g, dtype=torch.int8)
+    sx, sw = torch.rand(64, generator=g), torch.rand(2, N, generator=g)
+    tok = (torch.arange(R, dtype=torch.int32) * 7) % 64
+    offsets = torch.tensor([0, 1_000_003, R], dtype=torch.int32)
+    with _abi.lab_library() as lab:
+        lab.aq_lab_set_grouped_kernel(kernel_of)
+        y = ops.linear_w8a8_grouped(*_on(xq, sx, wq, sw, offsets, tok))
+    each = torch.stack([((xq.float() @ wq[e].float().t()) * sx[:, None]) * sw[e] for e in range(2)]).to(torch.bfloat16)
+    for lo, hi in ((0, 500), (1_000_000, 1_000_500), (1_044_000, 1_045_500), (R - 700, R)):
+        at = torch.arange(lo, hi)
+        assert torch.equal(y[lo:hi].cpu(), each[(at >= 1_000_003).long(), tok[at].long()])
+    rows = torch.tensor([[R - 1, 0], [R - 2, 1_044_500], [-1, R - 3]], dtype=torch.int32)
+    got = ops.combine_rows(y, rows.to(DEV), torch.ones(3, 2, device=DEV))
+    last = lambda r: y[r].float().cpu()
+    assert torch.equal(got.cpu(), torch.stack([last(R - 1) + last(0), last(R - 2) + last(1_044_500), last(R - 3)]).to(torch.bfloat16))
+
+
+def test_weights_past_32_bits(kernel):
+    """260 experts of 4096 x 4096 codes: the last one's begin 4.3 GB behind the first's."""
+    E, K, N = 260, 4096, 4096
+    g = torch.Generator(device=DEV).manual_seed(2)
+    wq = torch.zeros(E, N, K, dtype=torch.int8, device=DEV)
+    wq[0], wq[-1] = (torch.randint(-127, 128, (N, K), generator=g, dtype=torch.int8, device=DEV) for _ in range(2))
+    sw = torch.rand(E, N, generator=g, device=DEV) * 1e-4
+    xq, sx = torch.randint(-127, 128, (5, K), generator=g, dtype=torch.int8, device=DEV), torch.rand(5, generator=g, device=DEV)
+    offsets = torch.full((E + 1,), 2, dtype=torch.int32, device=DEV)
+    offsets[0], offsets[-1] = 0, 5
+    y = ops.linear_w8a8_grouped(xq, sx, wq, sw, offsets, out_dtype=torch.float32)
+    h = ops.swiglu_w8a8_grouped(xq, sx, wq, sw, offsets, out_dtype=torch.float32)
+    for lo, hi, e in ((0, 2, 0), (2, 5, -1)):
+        one = ops.linear_w8a8(xq[lo:hi], sx[lo:hi], wq[e], sw[e], out_dtype=torch.float32)
+        assert torch.equal(y[lo:hi], one)
+        up, gate = one.double().chunk(2, 1)
+        want = up * gate / (1 + torch.exp(-gate))
+        assert ((h[lo:hi].double() - want).abs() <= 8 * HALF[torch.float32] * want.abs() + 1e-34 * up.abs() + 1e-38).all()  # (as above)
+
+
 def test_combine_ignores_what_no_row_names():
     y = torch.full((6, 64), math.nan, device=DEV)
     y[4] = 1.0
