@@ -115,14 +115,10 @@ struct Key<false> {
   }
 };
 
-// exp(x - most), most the largest of them: 1 for it, infinite or not.  2^(t log2 e), the product's rounding taken back to first order, by the hardware's
-// exponential (one step).
+// exp(x - most), most the largest of them: 1 for it, infinite or not.
 __device__ __forceinline__ float exp_below(float x, float most) {
-  const float t = fmaxf(x - most, -150.0f);  // (2^-216 is 0)
-  const float y = t * 1.44269502e0f;
-  const float rest = __builtin_fmaf(t, 1.92596303e-8f, __builtin_fmaf(t, 1.44269502e0f, -y));
-  const float e = __builtin_amdgcn_exp2f(y);
-  return x == most ? 1.0f : __builtin_fmaf(e * 0.693147182f, rest, e);
+  const float e = exp_hw(fmaxf(x - most, -150.0f));  // (2^-216 is 0)
+  return x == most ? 1.0f : e;
 }
 
 // The choices of token t by the 16 lanes that hold it: lane j has choice j < k (expert -1: there is none) and its weight.

@@ -308,6 +308,31 @@ def test_grouped_swiglu(kernel, groups, K, F):
         assert ((got.cpu().double() - want).abs() <= tol * want.abs() + 1e-34 * up.abs() + 1e-38).all()
 
 
+def test_grouped_swiglu_over_every_gate(kernel):
+    """Every bf16 gate, each beside 256 ups, in bf16: nothing but the 7 half steps of fp32 that the layer's frozen form takes (the exponential's two steps, a sum, a
+    quotient, a product) before the rounding of h.  Gates below -87 have the exponential of 87."""
+    F = 256
+    gates = torch.arange(65536, device=DEV, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    gates = gates[gates.abs() < 1e18]  # (beyond, a product with an up overflows; what is not finite: below)
+    R = gates.numel()
+    g = torch.Generator(device=DEV).manual_seed(11)
+    xq, wq = torch.zeros(R, 16, dtype=torch.int8, device=DEV), torch.zeros(1, 2 * F, 16, dtype=torch.int8, device=DEV)
+    xq[:, 0], wq[:, :, 0] = 1, 1
+    sw = torch.ones(1, 2 * F, device=DEV)
+    sw[0, :F] = 1.0 + torch.rand(F, generator=g, device=DEV)
+    sx = gates.float()
+    offsets = torch.tensor([0, R], dtype=torch.int32, device=DEV)
+    got = ops.swiglu_w8a8_grouped(xq, sx, wq, sw, offsets).double()
+    up, gate = (sx[:, None] * sw[:, :F]).to(torch.bfloat16).double(), gates.double()[:, None]
+    want = up * gate / (1.0 + torch.exp(-gate.clamp(min=-87.0)))
+    tol = HALF[torch.bfloat16] + 7 * HALF[torch.float32]
+    assert ((got - want).abs() <= tol * want.abs() + 1e-37).all()  # (1e-37: of numbers below fp32's normal ones)
+    # what is not finite, as a division has it
+    sx = torch.tensor([math.inf, -math.inf, math.nan], device=DEV)
+    odd = ops.swiglu_w8a8_grouped(xq[:3], sx, wq, sw, torch.tensor([0, 3], dtype=torch.int32, device=DEV))
+    assert odd[:2].eq(math.inf).all() and odd[2].isnan().all()
+
+
 # ---- the weighted sum -----------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
