@@ -453,8 +453,8 @@ class MoE(nn.Module):
     Its plain forward runs the experts one after the other on the rows of their tokens, as the reference does, and so waits for the
     device to learn how many each has.  ``fuse_experts()`` runs a quantized layer's routing, products and sums on the device, in one call
     that waits for nothing (and can be captured in a graph): not bit-identical, since h = up * silu(gate) is rounded once and the weights stay in
-    float32.  The experts' own forwards (and hooks on them) are not called then.  Where autograd records, through ``x`` or the router's weight, the layer
-    runs the plain forward."""
+    float32.  The experts' own forwards (and hooks on them) are not called then.  Where autograd records, through ``x``, the router's weight, the
+    shared experts or ``residual``, the layer runs the plain forward."""
 
     def __init__(self, dim: int, dim_ffn: int, n_routed_experts: int, n_activated_experts: int, n_shared_experts: int = 0):
         super().__init__()
@@ -518,7 +518,8 @@ class MoE(nn.Module):
             y = shared(x)
             residual = y if residual is None else residual + y
         logits = self.router(rows)
-        if self._experts is not None and x.is_cuda and not logits.requires_grad:
+        records = logits.requires_grad or residual is not None and residual.requires_grad and torch.is_grad_enabled()
+        if self._experts is not None and x.is_cuda and not records:
             r = ops.route_topk(logits, self.n_activated_experts)
             out = ops.experts_w8a8(rows, r, *self._experts, residual=None if residual is None else residual.reshape(rows.shape))
             return out.view(x.shape)

@@ -141,6 +141,41 @@ def test_a_fused_layer_keeps_the_routers_gradient_and_refuses_the_inputs():
 
 
 @pytest.mark.gpu
+def test_a_fused_layer_keeps_the_gradients_of_shared_experts_and_residual():
+    """The router is frozen and x records nothing; shared experts in floating point, and the residual, do."""
+    m = _moe(64, 48, 4, 2, shared=2).to(DEV)
+    quantize_model(m.routed_experts)
+    assert m.fuse_experts()
+    m.router.requires_grad_(False)
+    x, down = torch.randn(9, 64, device=DEV), torch.randn(9, 64, device=DEV)
+    with torch.no_grad():
+        y = m(x)
+        assert not y.requires_grad
+    m(x).backward(down)
+    got = [p.grad.clone() for p in m.shared_experts.parameters()]
+    m.shared_experts.zero_grad()
+    (m.shared_experts[0](x) + m.shared_experts[1](x)).backward(down)  # the output is a sum, of which these are terms
+    assert all(torch.equal(a, p.grad) and a.abs().sum() > 0 for a, p in zip(got, m.shared_experts.parameters()))
+    # the formula's gradient against a difference: along a direction of the first shared expert's down, in which the layer is linear
+    first, d = m.shared_experts[0], torch.randn(64, 48, device=DEV)
+    with torch.no_grad():
+        h = (first.up(x) * F.silu(first.gate(x))).abs()
+        size = h @ (first.down.weight.abs() + d.abs()).t() + y.abs()
+        first.down.weight.add_(d)
+        z = m(x)
+        size = float((down.abs() * (size + z.abs())).sum())
+    # each output is off by a half step for every product and addition behind it: 48 of them, the weight's, and the sums of experts and residual
+    assert abs(float(((z.double() - y.double()) * down.double()).sum() - (got[2].double() * d.double()).sum())) <= 64 * 2.0 ** -24 * 2 * size
+    m.shared_experts.requires_grad_(False)
+    r = torch.randn(9, 64, device=DEV, requires_grad=True)
+    m(x, residual=r).backward(down)
+    assert torch.equal(r.grad, down)
+    assert not m(x, residual=r.detach()).requires_grad
+    with torch.inference_mode():
+        assert m(x, residual=r).shape == x.shape
+
+
+@pytest.mark.gpu
 def test_experts_that_cannot_be_stacked_stay_as_they_are():
     m = _moe(64, 48, 4, 2).to(DEV)
     quantize_model(m)
