@@ -434,16 +434,30 @@ class MLP(nn.Module):
 
 def _stack_again(moe: "MoE", incompatible_keys) -> None:
     """After a load that put new tensors in the place of the stacks' slices (``assign=True``)."""
-    if moe._experts is None:
-        return
-    up_gate, up_gate_scale, down, down_scale = moe._experts
-    F_ = down.shape[2]
-    for i, e in enumerate(moe.routed_experts):
-        for p, w, s in ((e.up, up_gate[i], up_gate_scale[i]), (e.gate, up_gate[i, F_:], up_gate_scale[i, F_:]), (e.down, down[i], down_scale[i])):
-            if p.qweight.data_ptr() != w.data_ptr() or p.w_scale.data_ptr() != s.data_ptr():
-                moe._experts = None
-                moe.fuse_experts()
-                return
+    moe._stacked()
+
+
+def _are_rows(whole: QuantLinear, parts) -> bool:
+    """Whether these are quantized layers whose codes and scales are the fused one's rows, one after the other (none has a bias)."""
+    codes, scales = whole.qweight.data_ptr(), whole.w_scale.data_ptr()
+    for p in parts:
+        if type(p) is not QuantLinear or p.bias is not None or (p.qweight.data_ptr(), p.w_scale.data_ptr()) != (codes, scales):
+            return False
+        codes, scales = codes + p.qweight.numel(), scales + 4 * p.w_scale.numel()
+    return True
+
+
+class _Seen:
+    """What native code remembers of a layer's experts (``MoE._stacked``): of this layer alone, so that a copy or a pickle of it begins with nothing."""
+
+    def __init__(self):
+        self.look = None
+
+    def __deepcopy__(self, memo):
+        return _Seen()
+
+    def __reduce__(self):
+        return _Seen, ()
 
 
 class MoE(nn.Module):
@@ -465,6 +479,7 @@ class MoE(nn.Module):
         self.routed_experts = nn.ModuleList([MLP(dim, dim_ffn) for _ in range(n_routed_experts)])
         self.shared_experts = nn.ModuleList([MLP(dim, dim_ffn) for _ in range(n_shared_experts)])
         self._experts: Optional[Tuple[Tensor, Tensor, Tensor, Tensor]] = None  # set by fuse_experts(): stacked codes and scales
+        self._seen = _Seen()
         self.register_load_state_dict_post_hook(_stack_again)
 
     def fuse_experts(self) -> bool:
@@ -473,22 +488,56 @@ class MoE(nn.Module):
         sizes are what ``ops.experts_w8a8`` takes."""
         if self._experts is not None:
             return False
-        parts = [(e.up, e.gate, e.down) for e in self.routed_experts]
-        linears = [p for e in parts for p in e]
-        if any(type(p) is not QuantLinear or p.bias is not None or p._shared is not None for p in linears):
+        parts = self._projections()
+        if parts is None:
             return False
         F_, E = parts[0][2].in_dim, len(parts)
         if F_ % 16 or E > ops.ROUTE_MAX_EXPERTS or self.n_activated_experts > ops.ROUTE_MAX_CHOICES:
             return False
-        up_gate, up_gate_scale = (torch.stack([torch.cat([getattr(u, n), getattr(g, n)]) for u, g, _ in parts]) for n in ("qweight", "w_scale"))
-        down, down_scale = (torch.stack([getattr(d, n) for _, _, d in parts]) for n in ("qweight", "w_scale"))
-        for i, (expert, (u, g, d)) in enumerate(zip(self.routed_experts, parts)):
-            u.qweight, g.qweight, d.qweight = up_gate[i, :F_], up_gate[i, F_:], down[i]
-            u.w_scale, g.w_scale, d.w_scale = up_gate_scale[i, :F_], up_gate_scale[i, F_:], down_scale[i]
-            if expert._upgate is not None:
-                expert._upgate.qweight, expert._upgate.w_scale = up_gate[i], up_gate_scale[i]
+        with torch.inference_mode(False), torch.no_grad():  # (of tensors that a later load outside of inference mode may write to)
+            up_gate, up_gate_scale = (torch.stack([torch.cat([getattr(u, n), getattr(g, n)]) for u, g, _ in parts]) for n in ("qweight", "w_scale"))
+            down, down_scale = (torch.stack([getattr(d, n) for _, _, d in parts]) for n in ("qweight", "w_scale"))
+            for i, (expert, (u, g, d)) in enumerate(zip(self.routed_experts, parts)):
+                u.qweight, g.qweight, d.qweight = up_gate[i, :F_], up_gate[i, F_:], down[i]
+                u.w_scale, g.w_scale, d.w_scale = up_gate_scale[i, :F_], up_gate_scale[i, F_:], down_scale[i]
+                if expert._upgate is not None:
+                    expert._upgate.qweight, expert._upgate.w_scale = up_gate[i], up_gate_scale[i]
         self._experts = up_gate, up_gate_scale, down, down_scale
         return True
+
+    def _projections(self) -> Optional[list]:
+        """(up, gate, down) of every routed expert, or None unless all are MLPs of plain quantized layers (int8, no bias) of the same sizes, each in
+        one place only."""
+        if not len(self.routed_experts) or any(type(e) is not MLP for e in self.routed_experts):
+            return None
+        parts = [(e.up, e.gate, e.down) for e in self.routed_experts]
+        linears = [p for e in parts for p in e]
+        if (any(type(p) is not QuantLinear or p.bias is not None or p._shared is not None for p in linears) or len({id(p) for p in linears}) < len(linears)
+                or len({(u.qweight.shape, g.qweight.shape, d.qweight.shape) for u, g, d in parts}) > 1
+                or len({(p.qweight.device, p.w_scale.dtype) for p in linears}) > 1):
+            return None
+        (u, g, d), dim = parts[0], parts[0][0].in_dim
+        return parts if u.qweight.shape == g.qweight.shape == d.qweight.shape[::-1] and d.out_dim == dim else None
+
+    def _stacked(self) -> bool:
+        """Whether the stacks are the experts' weights.  They are looked at for every forward (64 experts: 1.5 us): a load into a child, an expert or a projection put in
+        another's place and ``fuse_projections()`` leave storage of their own.  It is stacked again then; where it cannot be (another kind of
+        layer in one's place), the layer is back to its plain forward until ``fuse_experts()`` is called again."""
+        if self._experts is None:
+            return False
+        _native()
+        self._seen.look = linear_native().experts_stacked(self._seen.look, self.routed_experts._modules, *self._experts)
+        if self._seen.look is not None:
+            return True
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the routed experts' weights are no longer those that fuse_experts() stacked: call the layer once before it is captured")
+        self._experts = None
+        if self.fuse_experts():
+            return True
+        for e in self.routed_experts:  # nor need what an expert fused by itself be the projections that it has now
+            if type(e) is MLP and e._upgate is not None and not _are_rows(e._upgate, (e.up, e.gate)):
+                e._upgate = None
+        return False
 
     def _apply(self, fn, recurse=True):
         # a move or a cast of the module goes through the experts' buffers: they are stacked again from there
@@ -519,7 +568,7 @@ class MoE(nn.Module):
             residual = y if residual is None else residual + y
         logits = self.router(rows)
         records = logits.requires_grad or residual is not None and residual.requires_grad and torch.is_grad_enabled()
-        if self._experts is not None and x.is_cuda and not records:
+        if x.is_cuda and not records and self._stacked() and logits.shape[1] == len(self.routed_experts):
             r = ops.route_topk(logits, self.n_activated_experts)
             out = ops.experts_w8a8(rows, r, *self._experts, residual=None if residual is None else residual.reshape(rows.shape))
             return out.view(x.shape)
