@@ -89,6 +89,16 @@ def _bias_of(m: nn.Module) -> Optional[Tensor]:
     return b if b is not None else m.__dict__.get("bias")
 
 
+def _joined(parts: Sequence[Tensor]) -> Tensor:
+    """``torch.cat(parts)``, without a copy where they are rows of one storage, one part behind the other."""
+    first, end = parts[0], parts[0].data_ptr()
+    for t in parts:
+        if not t.is_contiguous() or t.data_ptr() != end or t.untyped_storage().data_ptr() != first.untyped_storage().data_ptr():
+            return torch.cat(list(parts), dim=0)
+        end += t.numel() * t.element_size()
+    return first.as_strided((sum(t.shape[0] for t in parts), *first.shape[1:]), first.stride())
+
+
 class _SharedInput:
     """Sibling projections that a module's forward applies to ONE input tensor, run as one concatenated
     projection (``QuantLinear.concat``: one activation quantisation, one launch, bit-identical columns)
@@ -212,7 +222,8 @@ class QuantLinear(_NativeCall):
         once and the weights are streamed by one launch.  Per-channel weight scales and per-token
         activation scales make every output element the same arithmetic as in its own module, so
         the result is bit-identical.  Afterwards the parts' ``qweight`` / ``w_scale`` (and bias)
-        are row slices of the fused buffers: no second copy of the weights is kept."""
+        are row slices of the fused buffers: no second copy of the weights is kept.  (Parts that lie one behind the other already, as in the stacks of
+        fused experts, stay there.)"""
         parts = list(parts)
         if not parts or any(not isinstance(p, QuantLinear) for p in parts):
             raise ValueError("concat needs QuantLinear modules")
@@ -220,8 +231,8 @@ class QuantLinear(_NativeCall):
             raise ValueError("parts must share in_dim and all have, or all lack, a bias")
         dev = parts[0].qweight.device
         fused = cls(parts[0].in_dim, sum(p.out_dim for p in parts), bias=parts[0].bias is not None, device=dev)
-        fused.qweight = torch.cat([p.qweight for p in parts], dim=0)
-        fused.w_scale = torch.cat([p.w_scale for p in parts], dim=0)
+        fused.qweight = _joined([p.qweight for p in parts])
+        fused.w_scale = _joined([p.w_scale for p in parts])
         if fused.bias is not None:
             fused.bias = nn.Parameter(torch.cat([p.bias.detach() for p in parts], dim=0), requires_grad=False)
         row = 0

@@ -142,6 +142,32 @@ def test_the_stacks_follow(how, projections):
     assert m._stacked() and m._experts[0][1, FFN:].eq(7).all() and (m.routed_experts[1]._upgate is None or m.routed_experts[1]._upgate.qweight[FFN:].eq(7).all())
 
 
+def test_projections_fused_behind_the_stacks_keep_no_second_copy():
+    torch.manual_seed(0)
+    m = MoE(DIM, FFN, E, 2)
+    for i in range(E):
+        m.routed_experts[i] = _quantized(i, "cpu")
+    assert m.fuse_experts()
+    stacks = m._experts
+    codes = [[e.up.qweight.clone(), e.gate.qweight.clone(), e.up.w_scale.clone(), e.gate.w_scale.clone()] for e in m.routed_experts]
+    assert fuse_shared_inputs(m) == E
+    for i, (e, (u, g, us, gs)) in enumerate(zip(m.routed_experts, codes)):
+        fused = e._upgate
+        assert fused.qweight.data_ptr() == stacks[0][i].data_ptr() and fused.w_scale.data_ptr() == stacks[1][i].data_ptr()
+        assert torch.equal(fused.qweight, torch.cat([u, g])) and torch.equal(fused.w_scale, torch.cat([us, gs]))
+        assert torch.equal(e.up.qweight, u) and torch.equal(e.gate.qweight, g)
+    assert m._stacked() and m._experts is stacks
+    m.load_state_dict(_all(m, "cpu"))
+    assert torch.equal(stacks[0][2, :FFN], _quantized(82, "cpu").up.qweight)  # through the child, without a forward in between
+    # parts elsewhere, in another order or with a gap are copied
+    a, b = _quantized(1, "cpu"), _quantized(2, "cpu")
+    whole = QuantLinear.concat([a.up, a.gate])
+    for parts in ([a.gate, a.up], [a.up, b.up], [b.up, b.gate]):
+        want = torch.cat([p.qweight for p in parts])
+        again = QuantLinear.concat(parts)
+        assert torch.equal(again.qweight, want) and again.qweight.data_ptr() != whole.qweight.data_ptr()
+
+
 @pytest.mark.parametrize("how", list(APART))
 def test_experts_that_no_longer_fit_take_the_layer_apart(how):
     m = _layer("cpu")
