@@ -547,6 +547,19 @@ class MoE(nn.Module):
             self.fuse_experts()
         return self
 
+    def _run_stacked(self, rows: Tensor, logits: Tensor, residual: Optional[Tensor]) -> Tensor:
+        """Routing and experts by the grouped operators, in parts of as many tokens as those take at a time (each token's output has the same bits
+        in any)."""
+        k, (T, dim) = self.n_activated_experts, rows.shape
+        most = min(ops.EXPERTS_MAX_TOKENS, ops.EXPERTS_MAX_ROWS // k, ops.EXPERTS_MAX_VALUES // max(dim, k * self._experts[2].shape[2]))
+        if T <= most:
+            return ops.experts_w8a8(rows, ops.route_topk(logits, k), *self._experts, residual=residual)
+        out = torch.empty_like(rows)
+        for at in range(0, T, most):
+            part = slice(at, at + most)
+            out[part] = ops.experts_w8a8(rows[part], ops.route_topk(logits[part], k), *self._experts, residual=None if residual is None else residual[part])
+        return out
+
     def _choose(self, logits: Tensor, dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
         """weights and experts ``[T, k]`` as the reference takes them (mlp.py:72-82)"""
         probs = torch.softmax(logits.float(), dim=-1).to(dtype)
@@ -569,9 +582,7 @@ class MoE(nn.Module):
         logits = self.router(rows)
         records = logits.requires_grad or residual is not None and residual.requires_grad and torch.is_grad_enabled()
         if x.is_cuda and not records and self._stacked() and logits.shape[1] == len(self.routed_experts):
-            r = ops.route_topk(logits, self.n_activated_experts)
-            out = ops.experts_w8a8(rows, r, *self._experts, residual=None if residual is None else residual.reshape(rows.shape))
-            return out.view(x.shape)
+            return self._run_stacked(rows, logits, None if residual is None else residual.reshape(rows.shape)).view(x.shape)
         w, idx = self._choose(logits, x.dtype)
         out = torch.zeros_like(rows)
         for e, expert in enumerate(self.routed_experts):

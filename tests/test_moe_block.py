@@ -176,6 +176,39 @@ def test_a_fused_layer_keeps_the_gradients_of_shared_experts_and_residual():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("limit,value", [("EXPERTS_MAX_TOKENS", 7), ("EXPERTS_MAX_ROWS", 45), ("EXPERTS_MAX_VALUES", 64 * 11), ("EXPERTS_MAX_VALUES", 2 * 48 * 9), ("EXPERTS_MAX_TOKENS", 1)])
+def test_a_batch_in_parts_has_the_bits_of_the_whole(limit, value, monkeypatch):
+    m = _moe(64, 48, 4, 2, shared=1).to(DEV)
+    quantize_model(m)
+    m.fuse_experts()
+    x = torch.randn(3, 17, 64, device=DEV)
+    with torch.inference_mode():
+        want, with_residual = m(x), m(x, residual=x)
+        calls = []
+        route = ops.route_topk
+        monkeypatch.setattr(ops, "route_topk", lambda logits, k: calls.append(logits.shape[0]) or route(logits, k))
+        monkeypatch.setattr(ops, limit, value)
+        assert torch.equal(m(x), want) and torch.equal(m(x, residual=x), with_residual)
+        assert len(calls) > 2 and sum(calls) == 2 * 51 and m(x[:0]).shape == (0, 17, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E,k", [((1 << 24) + 100, 2, 1), (1 << 24, 4, 3)])
+def test_batches_past_what_one_call_takes(T, E, k):
+    """More tokens, and more rows, than the operators take at a time."""
+    m = _moe(16, 16, E, k).to(DEV)
+    quantize_model(m)
+    assert m.fuse_experts()
+    m.router.to(torch.bfloat16)
+    x = torch.randn(T, 16, device=DEV, dtype=torch.bfloat16)
+    with torch.inference_mode():
+        y, logits = m(x), m.router(x)
+        for at in (0, (1 << 25) // k - 50, (1 << 24) - 50, T - 90):
+            part = slice(max(0, min(at, T - 90)), min(at, T - 90) + 90)
+            assert torch.equal(y[part], ops.experts_w8a8(x[part], ops.route_topk(logits[part], k), *m._experts)), at
+
+
+@pytest.mark.gpu
 def test_experts_that_cannot_be_stacked_stay_as_they_are():
     m = _moe(64, 48, 4, 2).to(DEV)
     quantize_model(m)
