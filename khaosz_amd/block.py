@@ -491,8 +491,9 @@ class MoE(nn.Module):
         parts = self._projections()
         if parts is None:
             return False
-        F_, E = parts[0][2].in_dim, len(parts)
-        if F_ % 16 or E > ops.ROUTE_MAX_EXPERTS or self.n_activated_experts > ops.ROUTE_MAX_CHOICES:
+        dim, F_, E = parts[0][0].in_dim, parts[0][2].in_dim, len(parts)
+        if (dim % 16 or F_ % 16 or 2 * F_ * dim > ops.EXPERTS_MAX_VALUES or max(dim, F_) > ops.EXPERTS_MAX_WIDTH or E > ops.ROUTE_MAX_EXPERTS
+                or self.n_activated_experts > ops.ROUTE_MAX_CHOICES):
             return False
         with torch.inference_mode(False), torch.no_grad():  # (of tensors that a later load outside of inference mode may write to)
             up_gate, up_gate_scale = (torch.stack([torch.cat([getattr(u, n), getattr(g, n)]) for u, g, _ in parts]) for n in ("qweight", "w_scale"))

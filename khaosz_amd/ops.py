@@ -936,10 +936,10 @@ def compact_pages(page_table: torch.Tensor, refs: torch.Tensor, k_layers: torch.
     return CompactedPages(table, counts, where, live)
 
 
-# what the routed-expert operators take at most: experts and choices of a token, tokens, rows, and values of x, of h and of an expert's weights (codes
-# by 31-bit offsets)
+# what the routed-expert operators take at most: experts and choices of a token, tokens, rows, values in one of them, and values of x, of h and of an
+# expert's weights (codes by 31-bit offsets)
 ROUTE_MAX_EXPERTS, ROUTE_MAX_CHOICES = 512, 16
-EXPERTS_MAX_TOKENS, EXPERTS_MAX_ROWS, EXPERTS_MAX_VALUES = 1 << 24, 1 << 25, (1 << 31) - 17
+EXPERTS_MAX_TOKENS, EXPERTS_MAX_ROWS, EXPERTS_MAX_WIDTH, EXPERTS_MAX_VALUES = 1 << 24, 1 << 25, 1 << 24, (1 << 31) - 17
 
 
 class Routing(NamedTuple):

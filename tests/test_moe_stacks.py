@@ -184,6 +184,36 @@ def test_a_load_on_a_layer_with_a_float_expert():
     assert m._experts is None
 
 
+@pytest.mark.parametrize("dim,ffn,fits", [(32768, 32752, True), (32768, 32768, False), (16, 1 << 24, True), (32, (1 << 24) + 16, False), (1 << 25, 16, False), (64, 40, False), (40, 64, False)])
+def test_experts_of_sizes_that_the_operators_do_not_take_are_not_stacked(dim, ffn, fits):
+    """What the operators would refuse at every call (2 F dim past 31 bits, rows past 2^24, not whole pieces of 16) stays a loop."""
+    from khaosz_amd import _abi
+    with torch.device("meta"):
+        m = MoE(dim, ffn, 2, 1)
+        for e in m.routed_experts:
+            e.up, e.gate, e.down = QuantLinear(dim, ffn, device="meta"), QuantLinear(dim, ffn, device="meta"), QuantLinear(ffn, dim, device="meta")
+    assert m.fuse_experts() == fits
+    p = 1 << 20  # a fake, aligned pointer: what is taken ends at the workspace's size, before any launch
+    rc = _abi.load().aq_experts_w8a8(p, 1, 1, dim, p, 2, p, p, p, 1, p, p, p, p, ffn, None, p, p, 0, None)
+    assert (rc == -5) == fits and rc in (-2, -5, -6)
+
+
+def test_limits_of_a_batch_are_the_librarys():
+    """The largest batches that the layer hands over in one call are taken, and one more of each is not."""
+    from khaosz_amd import _abi, ops
+    p = 1 << 20
+
+    def experts(T, k, dim, ffn):
+        return _abi.load().aq_experts_w8a8(p, 1, T, dim, p, 2, p, p, p, k, p, p, p, p, ffn, None, p, p, 0, None)
+    assert experts(ops.EXPERTS_MAX_TOKENS, 1, 16, 16) == -5 and experts(ops.EXPERTS_MAX_TOKENS + 1, 1, 16, 16) == -6
+    assert experts(ops.EXPERTS_MAX_ROWS // 16, 16, 16, 16) == -5 and experts(ops.EXPERTS_MAX_ROWS // 16 + 1, 16, 16, 16) == -6
+    for k, dim, ffn in ((2, 2048, 14336), (1, 4096, 16), (6, 2048, 1408)):
+        most = ops.EXPERTS_MAX_VALUES // max(dim, k * ffn)
+        assert experts(most, k, dim, ffn) == -5 and experts(most + 2, k, dim, ffn) == -6
+    route = lambda T: _abi.load().aq_route_topk(p, 1, T, 8, 8, 2, 1, p, p, p, p, p, p, 0, None)
+    assert route(ops.EXPERTS_MAX_TOKENS) == -5 and route(ops.EXPERTS_MAX_TOKENS + 1) == -6
+
+
 def test_stacks_of_copies_are_their_own():
     m = _layer("cpu")
     twin = copy.deepcopy(m)
