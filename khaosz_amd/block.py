@@ -468,7 +468,9 @@ class MoE(nn.Module):
     device to learn how many each has.  ``fuse_experts()`` runs a quantized layer's routing, products and sums on the device, in one call
     that waits for nothing (and can be captured in a graph): not bit-identical, since h = up * silu(gate) is rounded once and the weights stay in
     float32.  The experts' own forwards (and hooks on them) are not called then.  Where autograd records, through ``x``, the router's weight, the
-    shared experts or ``residual``, the layer runs the plain forward."""
+    shared experts or ``residual``, the layer runs the plain forward.  A token whose logits are all -inf or NaN goes to no expert of the fused layer (which
+    gives its shared experts and ``residual`` alone) and single ones that are NaN are never chosen, where the plain forward gives NaN: a router that has gone
+    wrong shows in the logits, not in the fused layer's output."""
 
     def __init__(self, dim: int, dim_ffn: int, n_routed_experts: int, n_activated_experts: int, n_shared_experts: int = 0):
         super().__init__()

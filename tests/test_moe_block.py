@@ -209,6 +209,32 @@ def test_batches_past_what_one_call_takes(T, E, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [5, 200])
+def test_tokens_whose_logits_are_no_numbers(T, dtype):
+    """NaN and -inf in a token's activations, and a row of NaN in the router's weight: the other tokens as without them, those by what is documented."""
+    m = _moe(64, 48, 4, 2, shared=1).to(DEV)
+    m.router.to(dtype)
+    quantize_model(m)
+    m.fuse_experts()
+    x, res = (torch.randn(T, 64, device=DEV).to(dtype) for _ in range(2))
+    with torch.inference_mode():
+        want = m(x, residual=res)
+        odd = x.clone()
+        odd[3, 9] = float("nan")  # every logit of it
+        got = m(odd, residual=res)
+        others = torch.arange(T, device=DEV) != 3
+        assert torch.equal(got[others], want[others])
+        alone = m.shared_experts[0](odd) + res
+        assert torch.equal(got[3].isnan(), alone[3].isnan()) and torch.equal(got[3].nan_to_num(), alone[3].nan_to_num())
+        m.router.weight[2] = float("nan")
+        got, r = m(x, residual=res), ops.route_topk(m.router(x), 2)
+        assert not r.experts.eq(2).any() and r.experts.ge(0).all() and not got.isnan().any()
+        m.router.weight.fill_(float("nan"))
+        assert torch.equal(m(x, residual=res), m.shared_experts[0](x) + res)
+
+
+@pytest.mark.gpu
 def test_experts_that_cannot_be_stacked_stay_as_they_are():
     m = _moe(64, 48, 4, 2).to(DEV)
     quantize_model(m)
