@@ -563,14 +563,12 @@ class MoE(nn.Module):
             out[part] = ops.experts_w8a8(rows[part], ops.route_topk(logits[part], k), *self._experts, residual=None if residual is None else residual[part])
         return out
 
-    def _choose(self, logits: Tensor, dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
-        """weights and experts ``[T, k]`` as the reference takes them (mlp.py:72-82)"""
-        probs = torch.softmax(logits.float(), dim=-1).to(dtype)
+    def _route(self, x: Tensor, logits: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+        """weights and experts ``[T, k]`` as the reference takes them (mlp.py:72-82); ``logits``: the router's, where they are in hand"""
+        logits = self.router(x) if logits is None else logits
+        probs = torch.softmax(logits.float(), dim=-1).to(x.dtype)
         w, idx = torch.topk(probs, self.n_activated_experts, dim=-1)
         return w / w.sum(dim=-1, keepdim=True), idx
-
-    def _route(self, x: Tensor) -> Tuple[Tensor, Tensor]:
-        return self._choose(self.router(x), x.dtype)
 
     def forward(self, x: Tensor, codes: Optional[Tuple[Tensor, Tensor]] = None, residual: Optional[Tensor] = None, norm=None) -> Tensor:
         """``residual`` and ``norm`` as for the MLP; the router needs the activations themselves, so ``codes`` are not taken."""
@@ -586,7 +584,7 @@ class MoE(nn.Module):
         records = logits.requires_grad or residual is not None and residual.requires_grad and torch.is_grad_enabled()
         if x.is_cuda and not records and self._stacked() and logits.shape[1] == len(self.routed_experts):
             return self._run_stacked(rows, logits, None if residual is None else residual.reshape(rows.shape)).view(x.shape)
-        w, idx = self._choose(logits, x.dtype)
+        w, idx = self._route(rows, logits)
         out = torch.zeros_like(rows)
         for e, expert in enumerate(self.routed_experts):
             tok, slot = (idx == e).nonzero(as_tuple=True)
