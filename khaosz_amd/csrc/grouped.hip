@@ -17,6 +17,9 @@ struct RowTile {
 
 // Tile `idx` of the list that has ceil(rows / BM) tiles of every expert: every lane looks at a run of experts.  false: there is none.
 // Offsets outside 0 .. R, or that fall, count as the nearest that do not: nothing is read or written outside the R rows.
+// (GroupTiles answers the same of offsets in LDS, for workgroups that ask again and again.  Of one question this is the shorter chain, without a store, a
+// barrier and reads of LDS: 16 tokens' 6 of 64 experts, the layer 90.0 us, by GroupTiles 93.8; one token's 21.2 and 21.6; 10 rows of 8 experts 4.9 and 5.2.  Of 512
+// experts, eight to a lane, it is the longer one: 64 rows of 512 -> 512 10.6 and 9.3.)
 template <int BM, int PER>
 __device__ __forceinline__ bool find_tile(const GroupedArgs& p, int idx, int lane, RowTile& t) {
   int o[PER + 1], n = 0, mine[PER];
