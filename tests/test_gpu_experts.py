@@ -128,6 +128,43 @@ def test_route_of_a_large_batch_against_torch():
     assert torch.equal(got.offsets, torch.searchsorted(group, torch.arange(E + 1, device=DEV)).int())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k", [(32768, 64, 3), (32769, 64, 3), (40000, 64, 4), (70000, 255, 7), (33000, 512, 2)])
+def test_route_of_chunks_of_several_passes_whose_counts_are_summed_apart(T, E, k, dtype):
+    """More than 32768 tokens are two passes or more to a chunk; more than 16384 chunks times experts, and the counts have a launch of their own."""
+    _say("large route", T, E, k, dtype)
+    g = torch.Generator(device=DEV).manual_seed(T + E)
+    x = torch.randn(T, E, generator=g, device=DEV).to(dtype)
+    x[:, E // 3] += 1.0  # one that is asked often
+    x[torch.rand(T, generator=g, device=DEV) < 0.1] = -math.inf
+    got = ops.route_topk(x, k)
+    top, at = torch.sort(x.float(), dim=1, descending=True, stable=True)
+    experts = torch.where(top[:, :k] > -math.inf, at[:, :k], -1)
+    assert torch.equal(got.experts, experts.int())
+    group, order = torch.sort(torch.where(experts < 0, E, experts).reshape(-1), stable=True)
+    rows = torch.empty_like(order)
+    rows[order] = torch.arange(T * k, device=DEV)
+    assert torch.equal(got.rows, torch.where(experts < 0, -1, rows.view(T, k)).int())
+    assert torch.equal(got.tokens, torch.where(group < E, order // k, -1).int())
+    assert torch.equal(got.offsets, torch.searchsorted(group, torch.arange(E + 1, device=DEV)).int())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("E", [64, 128, 256, 512])
+@pytest.mark.parametrize("T", [1, 2, 100, 300, 2500])
+def test_route_of_whole_vectors_in_strided_and_shifted_views(T, E, dtype):
+    """Logits whose rows are whole vectors of a lane, at every stride and base: read as vectors where both are aligned."""
+    g = torch.Generator(device=DEV).manual_seed(T + E)
+    buf = torch.randn((T + 2) * (E + 24), generator=g, device=DEV).to(dtype)
+    k = 6
+    for stride in (E, E + 4, E + 8, E + 1, E + 2, E + 7):
+        for base in (0, 1, 2, 4, 8, 5):
+            view = buf[base:].as_strided((T, E), (stride, 1))
+            got, want = ops.route_topk(view, k), ops.route_topk(view.clone(memory_format=torch.contiguous_format), k)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (stride, base)
+    _check_route(view[:300], k, True, ops.route_topk(view[:300], k))
+
+
 # ---- grouped products -----------------------------------------------------------------------------------------------
 
 def _operands(counts, K, N, seed, tokens=None, dtype=torch.bfloat16, bias=None, loud=False):
