@@ -554,6 +554,8 @@ class MoE(nn.Module):
         """Routing and experts by the grouped operators, in parts of as many tokens as those take at a time (each token's output has the same bits
         in any)."""
         k, (T, dim) = self.n_activated_experts, rows.shape
+        if rows.data_ptr() % 16:
+            rows = rows.clone()  # (the loop gathers rows; the operators take x where it lies, in pieces of 16 bytes)
         most = min(ops.EXPERTS_MAX_TOKENS, ops.EXPERTS_MAX_ROWS // k, ops.EXPERTS_MAX_VALUES // max(dim, k * self._experts[2].shape[2]))
         if T <= most:
             return ops.experts_w8a8(rows, ops.route_topk(logits, k), *self._experts, residual=residual)

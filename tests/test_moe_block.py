@@ -235,6 +235,22 @@ def test_tokens_whose_logits_are_no_numbers(T, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_activations_and_residual_at_any_address(dtype):
+    m = _moe(64, 48, 4, 2).to(DEV)
+    m.router.to(dtype)
+    quantize_model(m)
+    m.fuse_experts()
+    buf = torch.randn(2, 9 * 64 + 8, device=DEV).to(dtype)
+    with torch.inference_mode():
+        for at in range(8):
+            x, res = buf[0, at:at + 9 * 64].view(9, 64), buf[1, at:at + 9 * 64].view(9, 64)
+            logits = m.router(x)
+            want = ops.experts_w8a8(x.clone(), ops.route_topk(logits, 2), *m._experts, residual=res.clone())
+            assert torch.equal(m(x, residual=res), want), at
+
+
+@pytest.mark.gpu
 def test_experts_that_cannot_be_stacked_stay_as_they_are():
     m = _moe(64, 48, 4, 2).to(DEV)
     quantize_model(m)
