@@ -536,6 +536,18 @@ def test_layer_of_long_rows(T, E, k, dim, F, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,E,k,dim,F", [(1, 64, 8, 64, 8192), (1, 64, 16, 64, 8192), (2, 128, 9, 16, 8192), (1, 64, 8, 64, 4096), (3, 256, 16, 32, 4096), (1, 64, 16, 8192, 16)])
+def test_layer_of_long_rows_and_many_choices(T, E, k, dim, F, dtype):
+    """A row of codes for each of eight wavefronts: more than 64 KB of a compute unit's LDS."""
+    _say("long rows, many choices", T, E, k, dim, F, dtype)
+    _, _, uq, us, dq, ds = _layer(E, dim, F, T)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x, res = (torch.randn(T, dim, generator=g, device=DEV).to(dtype) for _ in range(2))
+    r = ops.route_topk(torch.randn(T, E, generator=g, device=DEV), k)
+    assert torch.equal(ops.experts_w8a8(x, r, uq, us, dq, ds, residual=res), _composed(x, r, uq, us, dq, ds, res))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("T", [1, 5, 40, 700])
 def test_layer_with_infinities_and_nan_in_a_row(T, dtype):
     """The same bits, or NaN in the same places, whichever launch quantises the rows; the other rows as without them."""
