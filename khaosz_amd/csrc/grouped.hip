@@ -407,9 +407,12 @@ static int launch_tokens(const TokenArgs& a, int64_t T, int dtype, hipStream_t s
   return dtype == AQ_BF16 ? launch_tokens_of<OUT_BF16>(a, T, st) : launch_tokens_of<OUT_F32>(a, T, st);
 }
 // Whether it is: what the experts of several tokens cost more, read for each, is then less than the launch saved (us of the layer, with | without: 64
-// choices of 256 experts of 1024 / 512, 4 MB more, 33.4 | 36.0; 18 of 64 of 2048 / 1408, 7 MB, 42.7 | 40.2; 24 of them, 11 MB, 48.8 | 46.3).
+// choices of 256 experts of 1024 / 512, 4 MB more, 33.4 | 36.0; 18 of 64 of 2048 / 1408, 7 MB, 42.7 | 40.2; 24 of them, 11 MB, 48.8 | 46.3).  And its workgroups, of a
+// token's 8 columns each, are on the device at once, four to a compute unit: of wide layers with narrow experts there are many with little to do (54 tokens' 1 of 128 of
+// 3568 / 80 112.7 | 31.1; 8 tokens' 1 of 60 of 5200 / 80 35.5 | 22.1; 7 tokens' 8 of 64 of 592 / 256 14.9 | 16.0).  At 835 sizes 0.8 % slower than the better of the two in
+// the mean, one in twenty 4 % (without the second condition 5.2 and 32 %).
 static bool tokens_in_launch(int64_t T, int64_t k, int64_t E, int64_t dim, int64_t F) {
-  return T <= 65535 && ((double)(T * k) - experts_used(T * k, E)) * (double)(dim * F) <= 5e6;
+  return T * (dim / GT_COLS) <= 4 * device_cus() && ((double)(T * k) - experts_used(T * k, E)) * (double)(dim * F) <= 5e6;
 }
 
 template <int OUT, bool SWI>

@@ -547,6 +547,40 @@ def test_layer_of_long_rows_and_many_choices(T, E, k, dim, F, dtype):
     assert torch.equal(ops.experts_w8a8(x, r, uq, us, dq, ds, residual=res), _composed(x, r, uq, us, dq, ds, res))
 
 
+@pytest.mark.parametrize("T,E,k,dim,F", [(54, 128, 1, 3568, 80), (16, 60, 1, 1936, 80), (2, 16, 2, 4096, 48), (2, 16, 2, 4112, 48), (512, 2, 1, 16, 16), (513, 2, 1, 16, 16)])
+def test_layer_of_many_columns_and_narrow_experts(T, E, k, dim, F):
+    """The second product and the sum in one launch, or not: the same bits; and never in a launch of so many workgroups that the layer takes far longer than its parts
+    one after the other (the first of these took three times as long)."""
+    _say("many columns", T, E, k, dim, F)
+    _, _, uq, us, dq, ds = _layer(E, dim, F, T)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = torch.randn(T, dim, generator=g, device=DEV).bfloat16()
+    r = ops.route_topk(torch.randn(T, E, generator=g, device=DEV), k)
+
+    def parts():
+        xq, sx = ops.quant_rowwise_i8(x)
+        hq, sh = ops.quant_rowwise_i8(ops.swiglu_w8a8_grouped(xq, sx, uq, us, r.offsets, r.tokens))
+        return ops.combine_rows(ops.linear_w8a8_grouped(hq, sh, dq, ds, r.offsets), r.rows, r.weights)
+    assert torch.equal(ops.experts_w8a8(x, r, uq, us, dq, ds), parts())
+    us_of = []
+    for call in (lambda: ops.experts_w8a8(x, r, uq, us, dq, ds), parts):
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(10):
+                call()
+        times = []
+        for _ in range(8):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            graph.replay()
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b) * 100)
+        us_of.append(min(times))
+    assert us_of[0] < 1.8 * us_of[1], us_of
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("T", [1, 5, 40, 700])
 def test_layer_with_infinities_and_nan_in_a_row(T, dtype):
