@@ -522,25 +522,29 @@ class MoE(nn.Module):
         (u, g, d), dim = parts[0], parts[0][0].in_dim
         return parts if u.qweight.shape == g.qweight.shape == d.qweight.shape[::-1] and d.out_dim == dim else None
 
-    def _stacked(self) -> bool:
-        """Whether the stacks are the experts' weights.  They are looked at for every forward (64 experts: 1.5 us): a load into a child, an expert or a projection put in
-        another's place and ``fuse_projections()`` leave storage of their own.  It is stacked again then; where it cannot be (another kind of
-        layer in one's place), the layer is back to its plain forward until ``fuse_experts()`` is called again."""
-        if self._experts is None:
-            return False
+    def _stacked(self) -> Optional[Tuple[Tensor, Tensor, Tensor, Tensor]]:
+        """The stacks, where the layer has them: the experts' weights as those are now.  They are looked at for every forward (64 experts: 2.7 us): a
+        load into a child, an expert or a projection put in another's place and ``fuse_projections()`` leave storage of their own.  It is stacked
+        again then; where it cannot be (another kind of layer in one's place), the layer is back to its plain forward until ``fuse_experts()`` is
+        called again."""
+        stacks = self._experts
+        if stacks is None:
+            return None
         _native()
-        self._seen.look = linear_native().experts_stacked(self._seen.look, self.routed_experts._modules, *self._experts)
-        if self._seen.look is not None:
-            return True
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        look = linear_native().experts_stacked(self._seen.look, self.routed_experts._modules, *stacks)
+        self._seen.look = look
+        if look is not None:
+            return stacks
+        if stacks[0].is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the routed experts' weights are no longer those that fuse_experts() stacked: call the layer once before it is captured")
         self._experts = None
-        if self.fuse_experts():
-            return True
+        self.fuse_experts()
         for e in self.routed_experts:  # nor need what an expert fused by itself be the projections that it has now
             if type(e) is MLP and e._upgate is not None and not _are_rows(e._upgate, (e.up, e.gate)):
                 e._upgate = None
-        return False
+        if stacks[0].is_cuda:
+            torch.cuda.synchronize(stacks[0].device)  # calls on other streams may still read the stacks that go, and read the new ones next
+        return self._experts
 
     def _apply(self, fn, recurse=True):
         # a move or a cast of the module goes through the experts' buffers: they are stacked again from there
@@ -550,19 +554,19 @@ class MoE(nn.Module):
             self.fuse_experts()
         return self
 
-    def _run_stacked(self, rows: Tensor, logits: Tensor, residual: Optional[Tensor]) -> Tensor:
+    def _run_stacked(self, stacks, rows: Tensor, logits: Tensor, residual: Optional[Tensor]) -> Tensor:
         """Routing and experts by the grouped operators, in parts of as many tokens as those take at a time (each token's output has the same bits
         in any)."""
         k, (T, dim) = self.n_activated_experts, rows.shape
         if rows.data_ptr() % 16:
             rows = rows.clone()  # (the loop gathers rows; the operators take x where it lies, in pieces of 16 bytes)
-        most = min(ops.EXPERTS_MAX_TOKENS, ops.EXPERTS_MAX_ROWS // k, ops.EXPERTS_MAX_VALUES // max(dim, k * self._experts[2].shape[2]))
+        most = min(ops.EXPERTS_MAX_TOKENS, ops.EXPERTS_MAX_ROWS // k, ops.EXPERTS_MAX_VALUES // max(dim, k * stacks[2].shape[2]))
         if T <= most:
-            return ops.experts_w8a8(rows, ops.route_topk(logits, k), *self._experts, residual=residual)
+            return ops.experts_w8a8(rows, ops.route_topk(logits, k), *stacks, residual=residual)
         out = torch.empty_like(rows)
         for at in range(0, T, most):
             part = slice(at, at + most)
-            out[part] = ops.experts_w8a8(rows[part], ops.route_topk(logits[part], k), *self._experts, residual=None if residual is None else residual[part])
+            out[part] = ops.experts_w8a8(rows[part], ops.route_topk(logits[part], k), *stacks, residual=None if residual is None else residual[part])
         return out
 
     def _route(self, x: Tensor, logits: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
@@ -584,8 +588,9 @@ class MoE(nn.Module):
             residual = y if residual is None else residual + y
         logits = self.router(rows)
         records = logits.requires_grad or residual is not None and residual.requires_grad and torch.is_grad_enabled()
-        if x.is_cuda and not records and self._stacked() and logits.shape[1] == len(self.routed_experts):
-            return self._run_stacked(rows, logits, None if residual is None else residual.reshape(rows.shape)).view(x.shape)
+        stacks = self._stacked() if x.is_cuda and not records else None
+        if stacks is not None and logits.shape[1] == stacks[0].shape[0]:
+            return self._run_stacked(stacks, rows, logits, None if residual is None else residual.reshape(rows.shape)).view(x.shape)
         w, idx = self._route(rows, logits)
         out = torch.zeros_like(rows)
         for e, expert in enumerate(self.routed_experts):

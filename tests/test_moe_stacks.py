@@ -315,3 +315,60 @@ def test_moved_weights_are_refused_under_capture():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want) and torch.equal(m(x), want)
+
+
+@pytest.mark.gpu
+def test_a_compiled_layer_and_threads_that_share_one():
+    import threading
+    m = _layer(DEV)
+    x = torch.randn(11, DIM, device=DEV)
+    with torch.inference_mode():
+        want = m(x)
+        torch._dynamo.reset()
+        compiled = torch.compile(m, backend="eager")
+        assert torch.equal(compiled(x), want)
+        STACKED["codes set"](m, DEV)
+        after = compiled(x)
+        assert torch.equal(after, m(x)) and not torch.equal(after, want)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()), torch.inference_mode():
+            for i in range(50):
+                if i % 10 == 0:
+                    m.routed_experts[1].train(i % 20 == 0)  # (looked through again)
+                if not torch.equal(m(x), after):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.gpu
+def test_a_layer_on_one_stream_behind_a_change_seen_on_another():
+    """The call that stacks the weights again does so on its stream; a call on another stream, with nothing between the two, reads whole stacks."""
+    m, other = _layer(DEV), _layer(DEV, False)
+    x = torch.randn(11, DIM, device=DEV)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.inference_mode():
+        for i in range(5):
+            for e in range(E):
+                m.routed_experts[e].load_state_dict(_dict(DEV, 200 + 10 * i + e), assign=True)
+            other.load_state_dict({k: v.clone() for k, v in m.state_dict().items()})
+            other._experts = None
+            assert other.fuse_experts()
+            want = other(x)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(a):
+                big = torch.randn(4096, 4096, device=DEV)
+                for _ in range(8):
+                    big = big @ big  # the stream is busy
+                one = m(x)
+            with torch.cuda.stream(b):
+                two = m(x)
+            torch.cuda.synchronize()
+            assert torch.equal(one, want) and torch.equal(two, want)
