@@ -310,8 +310,8 @@ static double experts_used(int64_t R, int64_t E) { return E * (1.0 - std::exp(-(
 // Which kernel: the one whose estimated time, in us, is least.  Tiles of 16 rows: units of 32 weight rows, four to a compute unit at a time.  Walked
 // tiles: rounds of tiles (mostly whole ones: the last takes as long), each of its steps and a beginning and an end, beside the weights' way from memory.
 // Fitted to 900 random sizes of experts that are asked for alike (1 to 256 experts, 1 to 8192 tokens, K 128 to 6912), 400 of uneven ones (2 to 128 experts, 20 to
-// 600 rows each) and 350 with 0.2 to 300 rows each: 1.5, 0.9 and 1.4 % slower than the best kernel in the mean, one in twenty 12, 6 and 11 % or more (on the
-// first always 128 x 256 50 %, always 128 x 128 30 %).
+// 600 rows each) and 350 with 0.2 to 300 rows each: 1.5, 0.9 and 1.4 % slower than the best kernel in the mean, one in twenty 12, 6 and 11 % or more.  At 200
+// other sizes, asked for as routers ask, 3.8 % in the mean, one in twenty 20 % or more (always 128 x 256 59 %, always 128 x 128 36 %).
 // Chosen by the launch itself, from the tiles that there are, the width was 0.3 % off on the second, but three widths in one kernel cost 1 to 2 % and the
 // choice 0.5 to 1 us.
 enum { GROUPED_FEW = 1, GROUPED_WALK_256 = 2, GROUPED_WALK_128 = 3, GROUPED_WALK_64 = 4 };
@@ -379,8 +379,8 @@ static int launch_rows(GroupedArgs a, int dtype, hipStream_t st) {
 // wavefront, holds up to 16 of them in LDS and longer ones in more registers.  So the weights times 1 + rows an expert have a limit by the rows' length
 // (us of the layer, with | without.  Up to 2048: 16 tokens' 6 of 64 of 2048 / 1408, x 93.1 | 95.8, then h 89.8 | 93.1; 16 tokens' 4 of 16 of 2048 / 5632, x 123.2 | 121.5.  Up
 // to 4096: 4 tokens' 2 of 8 of 3584 / 4096, x 63.2 | 69.8, 8 tokens' 80.5 | 77.7.  Up to 8192: one token's 2 of 8 of 1536 / 6912, h 25.6 | 35.0, of 4096 / 8192 67.8 | 65.7,
-// 4 tokens' 143 | 123), and rows an expert by themselves (32 tokens' 8 of 16 of 5120 / 144, h 50.0 | 43.4).  At 106 sizes 1.2 % slower than the best choice
-// in the mean.
+// 4 tokens' 143 | 123), and rows an expert by themselves (32 tokens' 8 of 16 of 5120 / 144, h 50.0 | 43.4).  At 200 sizes, with the rule
+// of the sum below, 2.0 % slower than the best of the three ways in the mean, one in twenty 11 %; always apart 33 %, always in the launch 13 %.
 static bool rows_in_launch(int64_t R, int64_t E, int64_t N, int64_t K, int dtype) {
   if (K > most_in_launch(dtype) || !few_fits(R, E)) return false;
 #ifdef AQ_LAB
@@ -408,9 +408,9 @@ static int launch_tokens(const TokenArgs& a, int64_t T, int dtype, hipStream_t s
 }
 // Whether it is: what the experts of several tokens cost more, read for each, is then less than the launch saved (us of the layer, with | without: 64
 // choices of 256 experts of 1024 / 512, 4 MB more, 33.4 | 36.0; 18 of 64 of 2048 / 1408, 7 MB, 42.7 | 40.2; 24 of them, 11 MB, 48.8 | 46.3).  And its workgroups, of a
-// token's 8 columns each, are on the device at once, four to a compute unit: of wide layers with narrow experts there are many with little to do (54 tokens' 1 of 128 of
-// 3568 / 80 112.7 | 31.1; 8 tokens' 1 of 60 of 5200 / 80 35.5 | 22.1; 7 tokens' 8 of 64 of 592 / 256 14.9 | 16.0).  At 835 sizes 0.8 % slower than the better of the two in
-// the mean, one in twenty 4 % (without the second condition 5.2 and 32 %).
+// token's 8 columns each, are at most four to a compute unit, which has room for one or two at a time: of wide layers with narrow experts there are many with little
+// to do (54 tokens' 1 of 128 of 3568 / 80 112.7 | 31.1; 8 tokens' 1 of 60 of 5200 / 80 35.5 | 22.1; 7 tokens' 8 of 64 of 592 / 256 14.9 | 16.0).  At 835 sizes 0.8 % slower than
+// the better of the two in the mean, one in twenty 4 % or more (without the second condition 5.2 and 32 %).
 static bool tokens_in_launch(int64_t T, int64_t k, int64_t E, int64_t dim, int64_t F) {
   return T * (dim / GT_COLS) <= 4 * device_cus() && ((double)(T * k) - experts_used(T * k, E)) * (double)(dim * F) <= 5e6;
 }

@@ -5,10 +5,11 @@
 // weights.  The rows' tokens of the next tile are fetched into LDS under this tile's first step, for its first stages are requested in the
 // last steps.
 //
-// What bounds it, and what was measured: many rows an expert, the matrix core at the clock that random codes leave (48000 rows of 64 experts, 1408 ->
-// 2048: 170 us, 1.6 POP/s of the 2.36 that torch's product of 8192 x 8192 x 8192 reaches on this card; without its stores 148, with loads that all hit
-// the L2 147); a few dozen rows, the weights (96 of 60 experts, SwiGLU of 2048 -> 1408: 280 MB in 50 us, 5.6 TB/s, the launch included); a few
-// hundred, both (12000 of 64 experts, SwiGLU: 314 MB in 91 us, 1.14 POP/s).  A ragged last round is left as it is: its tiles' columns dealt out
+// What bounds it, and what was measured.  Many rows an expert: the clock that power leaves and, of its cycles, the loads (48000 rows of 64 experts, 1408 ->
+// 2048: 171 us, 1.6 POP/s of the 2.36 that torch's product of 8192 x 8192 x 8192 reaches on this card; 1.64 GHz of 2.4, the matrix core at work in 51 % of the
+// cycles; on codes of zeros, the same instructions and bytes, 145; without its stores 148, with loads that all hit the L2 147).  A few dozen rows: the weights (96 of 60
+// experts, SwiGLU of 2048 -> 1408: 280 MB in 50 us, 5.6 TB/s, the launch included).  A few hundred: both (12000 of 64 experts, SwiGLU of 1536 -> 1408: 342 MB in 94 us,
+// 1.1 POP/s, the matrix core 38 % of the cycles; on zeros 88).  A ragged last round is left as it is: its tiles' columns dealt out
 // to two or four workgroups each take as many K steps (500 tokens' 2 of 8, SwiGLU: 73 us, 79 that way).
 #include "aq_grouped.h"
 

@@ -454,7 +454,7 @@ def fuse_shared_inputs(model: nn.Module, norms: bool = False, decode_attention: 
     """Call ``fuse_projections()`` on every module that offers it (attention and MLP blocks whose
     projections read one input); returns how many fused modules were built.  Run it after
     ``quantize_model`` and after loading weights: the fused module owns the weight storage from
-    then on.  Outputs stay bit-identical.  Modules of the reference itself (its GQA, MLA and MLP classes,
+    then on (a later load reaches it where it copies, not with ``assign=True``).  Outputs stay bit-identical.  Modules of the reference itself (its GQA, MLA and MLP classes,
     recognised by name) get the same single launch behind their own unchanged forward (``share_inputs``).
     ``norms=True`` additionally lets blocks compute
     RMSNorm and the quantisation of its output in one launch (``fuse_norm_quant()``), which
@@ -463,8 +463,9 @@ def fuse_shared_inputs(model: nn.Module, norms: bool = False, decode_attention: 
     projection run single-token steps on a paged cache through the in-place attention kernels
     (``fuse_decode_attention()``).  ``residuals=True`` lets blocks hand the residual stream to the
     quantized projection that ends each branch (``fuse_residual_adds()``): the add happens in that
-    kernel's epilogue, bit-identical to the separate add.  ``experts=True`` lets layers of routed experts run
-    as grouped products on the device (``fuse_experts()``): not bit-identical to the loop over the experts."""
+    kernel's epilogue, bit-identical to the separate add.  ``experts=True`` lets this package's layers of routed
+    experts (``MoE``) run as grouped products on the device (``fuse_experts()``): not bit-identical to the loop over the
+    experts, which those with FP8 layers or biases, and the reference's own class, keep."""
     n = 0
     for m in model.modules():
         f = getattr(m, "fuse_projections", None)
