@@ -548,7 +548,7 @@ class MoE(nn.Module):
 
     def _apply(self, fn, recurse=True):
         # a move or a cast of the module goes through the experts' buffers: they are stacked again from there
-        fused, self._experts = self._experts is not None, None
+        fused, self._experts, self._seen.look = self._experts is not None, None, None  # (a look holds what it saw)
         super()._apply(fn, recurse)
         if fused:
             self.fuse_experts()

@@ -1,6 +1,9 @@
 """A fused layer of routed experts computes with the weights that its experts have, however those got there: loads into a child, experts and projections put in
 another's place, tensors that were set.  The stacks themselves on the CPU; what the layer then computes on the GPU."""
 import copy
+import gc
+import io
+import weakref
 
 import pytest
 import torch
@@ -220,6 +223,22 @@ def test_stacks_of_copies_are_their_own():
     assert twin._stacked() and m._stacked()
     twin.routed_experts[0].up.qweight.fill_(3)
     assert twin._experts[0][0, :FFN].eq(3).all() and not m._experts[0][0, :FFN].eq(3).all()
+    buf = io.BytesIO()
+    torch.save(m, buf)  # (after a look: what native code remembers is not the layer's state)
+    buf.seek(0)
+    again = torch.load(buf, weights_only=False)
+    assert again._stacked() and torch.equal(again._experts[0], m._experts[0])
+    again.routed_experts[2].down.qweight.fill_(5)
+    assert again._stacked()[2][2].eq(5).all()
+
+
+def test_a_moved_layer_keeps_nothing_of_the_stacks_it_had():
+    m = _layer("cpu")
+    assert m._stacked()
+    old, slices = [weakref.ref(t) for t in m._experts], [weakref.ref(e.up.qweight) for e in m.routed_experts]
+    m.double().float()
+    gc.collect()
+    assert all(r() is None for r in old + slices) and m._stacked()
 
 
 def test_stacks_made_in_inference_mode_can_be_written_outside():
