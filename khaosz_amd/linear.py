@@ -90,10 +90,11 @@ def _bias_of(m: nn.Module) -> Optional[Tensor]:
 
 
 def _joined(parts: Sequence[Tensor]) -> Tensor:
-    """``torch.cat(parts)``, without a copy where they are rows of one storage, one part behind the other."""
+    """``torch.cat(parts)``, without a copy where they are rows of one storage, one part behind the other, that begin where the kernels read (at
+    pieces of 16 bytes: a slice of a checkpoint need not)."""
     first, end = parts[0], parts[0].data_ptr()
     for t in parts:
-        if not t.is_contiguous() or t.data_ptr() != end or t.untyped_storage().data_ptr() != first.untyped_storage().data_ptr():
+        if first.data_ptr() % 16 or not t.is_contiguous() or t.data_ptr() != end or t.untyped_storage().data_ptr() != first.untyped_storage().data_ptr():
             return torch.cat(list(parts), dim=0)
         end += t.numel() * t.element_size()
     return first.as_strided((sum(t.shape[0] for t in parts), *first.shape[1:]), first.stride())

@@ -162,6 +162,10 @@ def test_projections_fused_behind_the_stacks_keep_no_second_copy():
     assert m._stacked() and m._experts is stacks
     m.load_state_dict(_all(m, "cpu"))
     assert torch.equal(stacks[0][2, :FFN], _quantized(82, "cpu").up.qweight)  # through the child, without a forward in between
+    # parts that lie where the kernels cannot read are copied
+    flat, c = torch.randint(-127, 128, (2 * FFN * DIM + 4,), dtype=torch.int8), _quantized(3, "cpu")  # (its base is at a multiple of 64)
+    c.up.qweight, c.gate.qweight = flat[4:].view(2, FFN, DIM)
+    assert c.up.qweight.data_ptr() % 16 and QuantLinear.concat([c.up, c.gate]).qweight.data_ptr() % 16 == 0
     # parts elsewhere, in another order or with a gap are copied
     a, b = _quantized(1, "cpu"), _quantized(2, "cpu")
     whole = QuantLinear.concat([a.up, a.gate])
