@@ -206,6 +206,34 @@ class PagedKV:
         return k[:, :self.total_len], v[:, :self.total_len]
 
 
+_rows_are = None  # the native check, once it is loaded
+
+
+def _settled(module: nn.Module, name: str, parts: Tuple[str, ...]) -> Optional[QuantLinear]:
+    """``module``'s fused projection ``name``, while its rows are the codes, scales and biases of ``parts``.  They are looked at for every forward: a load
+    that assigns, another projection in one's place or a tensor that was set leave storage of their own.  They are fused again then, or, where they no
+    longer can be (an adapter in one's place), run one by one until ``fuse_projections()`` is called again."""
+    global _rows_are
+    whole = module.__dict__[name]
+    if whole is None:
+        return None
+    if _rows_are is None:
+        _rows_are = linear_native().rows_are
+    if _rows_are(whole, module._modules, parts):
+        return whole
+    cuda = whole.qweight.is_cuda
+    if cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the weights of a fused projection are no longer those that were fused: call the module once before it is captured")
+    object.__setattr__(module, name, None)
+    try:
+        module.fuse_projections()
+    except ValueError:  # (one got a bias, or another width)
+        pass
+    if cuda:
+        torch.cuda.synchronize(whole.qweight.device)  # calls on other streams may still read the rows that go, and read the new ones next
+    return module.__dict__[name]
+
+
 class GQA(nn.Module):
     """Grouped-query attention (astrai/model/components/attention.py:32-109), with its two
     options: RMSNorm over the head dimension of q and k after the rotation (``use_qk_norm``,
@@ -291,6 +319,8 @@ class GQA(nn.Module):
         return self.o_proj(out) + residual
 
     def _project_qkv(self, x: Tensor, codes, norm) -> Tensor:
+        if self._qkv is None:
+            return torch.cat([self.q_proj(x), self.k_proj(x), self.v_proj(x)], dim=-1)
         if codes is not None:
             return self._qkv.forward_codes(codes[0], codes[1], x.dtype).view(*x.shape[:-1], -1)
         return self._qkv(x) if norm is None else self._qkv(x, norm=norm)
@@ -303,6 +333,8 @@ class GQA(nn.Module):
         un-normalised stream and the norm runs inside the fused q/k/v projection.  ``residual``:
         added to the output (in o_proj's epilogue when it is quantized)."""
         B, S, _ = x.shape
+        if _settled(self, "_qkv", ("q_proj", "k_proj", "v_proj")) is None and codes is not None:
+            raise ValueError("a pre-quantised input needs the fused q/k/v projection")
         if norm is not None and self._qkv is None:
             x, norm = F.rms_norm(x, (x.shape[-1],), norm[0], norm[1]), None
         # The paged decode kernels know two masks: none, and per-sequence lengths (``cache.seq_lens``).  Any
@@ -405,23 +437,25 @@ class MLP(nn.Module):
     def forward(self, x: Tensor, codes: Optional[Tuple[Tensor, Tensor]] = None,
                 residual: Optional[Tensor] = None, norm=None) -> Tensor:
         """``codes`` / ``norm``: as for the attention block (the input of up and gate)."""
-        if norm is not None and self._upgate is None:
+        ug = _settled(self, "_upgate", ("up", "gate"))
+        if codes is not None and ug is None:
+            raise ValueError("a pre-quantised input needs the fused up/gate projection")
+        if norm is not None and ug is None:
             x, norm = F.rms_norm(x, (x.shape[-1],), norm[0], norm[1]), None
         if residual is not None and not isinstance(self.down, QuantLinear):
             return self.forward(x, codes, norm=norm) + residual
         kw = {} if residual is None else {"residual": residual}
-        if self._upgate is not None:
+        if ug is not None:
             if (self._swiglu_quant and codes is None and isinstance(self.down, QuantLinear)
-                    and ops.gemv_swiglu_ok(x, self._upgate.qweight.shape[0] // 2)):
+                    and ops.gemv_swiglu_ok(x, ug.qweight.shape[0] // 2)):
                 # decode step: up, gate and the activation in one launch (the [M, 2F] projections are never
                 # written), then `down`, which quantises the few rows of h itself
-                ug = self._upgate
                 h = ops.gemv_w8a8_decode_swiglu(x, ug.qweight, ug.w_scale, ug.bias, out_dtype=x.dtype, norm=norm)
                 return self.down(h.view(*x.shape[:-1], -1), **kw)
             if codes is not None:
-                ug = self._upgate.forward_codes(codes[0], codes[1], x.dtype).view(*x.shape[:-1], -1)
+                ug = ug.forward_codes(codes[0], codes[1], x.dtype).view(*x.shape[:-1], -1)
             else:
-                ug = self._upgate(x) if norm is None else self._upgate(x, norm=norm)
+                ug = ug(x) if norm is None else ug(x, norm=norm)
             if (self._swiglu_quant and isinstance(self.down, QuantLinear) and ug.is_cuda
                     and ug.shape[-1] // 2 <= ops.SWIGLU_QUANT_MAX_F.get(ug.dtype, 0)):
                 # activation, product and the down projection's quantisation in one launch
@@ -435,16 +469,6 @@ class MLP(nn.Module):
 def _stack_again(moe: "MoE", incompatible_keys) -> None:
     """After a load that put new tensors in the place of the stacks' slices (``assign=True``)."""
     moe._stacked()
-
-
-def _are_rows(whole: QuantLinear, parts) -> bool:
-    """Whether these are quantized layers whose codes and scales are the fused one's rows, one after the other (none has a bias)."""
-    codes, scales = whole.qweight.data_ptr(), whole.w_scale.data_ptr()
-    for p in parts:
-        if type(p) is not QuantLinear or p.bias is not None or (p.qweight.data_ptr(), p.w_scale.data_ptr()) != (codes, scales):
-            return False
-        codes, scales = codes + p.qweight.numel(), scales + 4 * p.w_scale.numel()
-    return True
 
 
 class _Seen:
@@ -539,9 +563,6 @@ class MoE(nn.Module):
             raise RuntimeError("the routed experts' weights are no longer those that fuse_experts() stacked: call the layer once before it is captured")
         self._experts = None
         self.fuse_experts()
-        for e in self.routed_experts:  # nor need what an expert fused by itself be the projections that it has now
-            if type(e) is MLP and e._upgate is not None and not _are_rows(e._upgate, (e.up, e.gate)):
-                e._upgate = None
         if stacks[0].is_cuda:
             torch.cuda.synchronize(stacks[0].device)  # calls on other streams may still read the stacks that go, and read the new ones next
         return self._experts

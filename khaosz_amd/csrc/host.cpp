@@ -724,7 +724,7 @@ PyObject *k_modules, *k_buffers, *k_parameters, *k_qweight, *k_w_scale, *k_bias,
     *k_fwd_pre_hooks, *k_compiled, *k_attention, *k_mlp, *k_input_norm, *k_post_norm, *k_qkv, *k_upgate, *k_o_proj, *k_down, *k_q_norm,
     *k_k_norm, *k_decode_attention, *k_use_qk_norm, *k_use_gate, *k_n_heads, *k_n_kv_heads, *k_head_dim, *k_layer_id, *k_swiglu_quant,
     *k_norm_quant, *k_residual_adds, *k_k_layers, *k_v_layers, *k_page_table, *k_total_len, *k_seq_lens, *k_invalid, *k_page_size, *k_shared_len,
-    *k_shared, *k_residual, *k_norm, *k_call, *k_decode_rows, *k_forward_codes, *k_forward_attn, *k_up, *k_gate;
+    *k_shared, *k_residual, *k_norm, *k_call, *k_decode_rows, *k_forward_codes, *k_forward_attn, *k_up, *k_gate, *k_q_proj, *k_k_proj, *k_v_proj;
 
 PyObject* dict_of(PyObject* o) {  // borrowed; null if it has none
   PyObject** d = _PyObject_GetDictPtr(o);
@@ -865,6 +865,49 @@ bool proj_of(PyObject* m, int dev, Proj* p) {
   p->w = static_cast<const int8_t*>(w->const_data_ptr());
   p->s = static_cast<const float*>(s->const_data_ptr());
   return true;
+}
+
+// Whether a fused projection's codes, scales and bias are those of these modules, one module's rows behind the other's, as QuantLinear.concat leaves
+// them.  Looked at before each call that reads them (0.5 us for a block's two): nothing else tells when a module got another tensor, or its parent another module.
+bool rows_are(PyObject* whole, std::initializer_list<PyObject*> parts) {
+  struct At {
+    const char *w = nullptr, *s = nullptr, *b = nullptr;
+    int64_t N = 0, K = 0, bias_bytes = 0;
+  };
+  auto at = [](PyObject* m, At* a) {
+    PyObject *d = m ? dict_of(m) : nullptr, *buffers = get(d, k_buffers), *bias = nested(d, k_parameters, k_bias);
+    if (!bias) bias = get(d, k_bias);
+    const Tensor *w = unpack(get(buffers, k_qweight)), *s = unpack(get(buffers, k_w_scale)), *b = bias && bias != Py_None ? unpack(bias) : nullptr;
+    if (!w || !s || w->dim() != 2 || !w->is_contiguous() || w->scalar_type() != ScalarType::Char || s->scalar_type() != ScalarType::Float ||
+        (bias && bias != Py_None && !b))
+      return false;
+    a->N = w->size(0), a->K = w->size(1);
+    a->w = static_cast<const char*>(w->const_data_ptr()), a->s = static_cast<const char*>(s->const_data_ptr());
+    if (b) a->b = static_cast<const char*>(b->const_data_ptr()), a->bias_bytes = a->N * static_cast<int64_t>(b->element_size());
+    return s->numel() == a->N && (!b || b->numel() == a->N);
+  };
+  At all, part;
+  if (!at(whole, &all)) return false;
+  int64_t rows = 0;
+  for (PyObject* m : parts) {
+    part = At();
+    if (!at(m, &part) || part.K != all.K || part.w != all.w || part.s != all.s || part.b != all.b) return false;
+    rows += part.N;
+    all.w += part.N * part.K, all.s += 4 * part.N;
+    if (all.b) all.b += part.bias_bytes;
+  }
+  return rows == all.N;
+}
+
+// rows_are(fused projection, {name: module} of its parent, (name, ..)) -> bool
+PyObject* rows_are(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS AQ_ARGS(3);
+  if (!PyTuple_CheckExact(args[2])) return PyErr_Format(PyExc_TypeError, "expected the modules' names");
+  const Py_ssize_t n = PyTuple_GET_SIZE(args[2]);
+  auto part = [&](Py_ssize_t i) { return get(args[1], PyTuple_GET_ITEM(args[2], i)); };
+  const bool are = n == 2 ? rows_are(args[0], {part(0), part(1)}) : n == 3 && rows_are(args[0], {part(0), part(1), part(2)});
+  return PyBool_FromLong(are);
+  END_HANDLE_TH_ERRORS
 }
 
 // Whether a module is a QuantLinear that keeps just this: N x K codes and N scales at these addresses, no bias, no shared input.
@@ -1256,6 +1299,9 @@ bool Block::read(PyObject* block, PyObject* px, PyObject* protary, PyObject* cac
     return false;
   if (qk_norm && (!gain_of(nested(ad, k_modules, k_q_norm), D, c.dev, &qn) || !gain_of(nested(ad, k_modules, k_k_norm), D, c.dev, &kn)))
     return false;
+  PyObject *am = get(ad, k_modules), *mm = get(md, k_modules);
+  if (!rows_are(get(ad, k_qkv), {get(am, k_q_proj), get(am, k_k_proj), get(am, k_v_proj)}) || !rows_are(get(md, k_upgate), {get(mm, k_up), get(mm, k_gate)}))
+    return false;  // (fused again on the step-by-step path)
   F = ug.N / 2;
   if (qkv.K != dim || qkv.N != (Hq + 2 * Hkv) * D || o.K != Hq * D || o.N != dim || ug.K != dim || ug.N % 2 || F % 16 ||
       F > limit_of(types.swiglu_max_f) || down.K != F || down.N != dim)
@@ -1525,6 +1571,7 @@ PyMethodDef methods[] = {
     AQ_METHOD(combine_rows),
     AQ_METHOD(experts_w8a8),
     AQ_METHOD(experts_stacked),
+    {"rows_are", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(static_cast<PyObject* (*)(PyObject*, PyObject* const*, Py_ssize_t)>(rows_are))), METH_FASTCALL, nullptr},
     AQ_METHOD(block_forward),
     {nullptr, nullptr, 0, nullptr},
 };
@@ -1553,7 +1600,8 @@ PyMODINIT_FUNC PyInit__host() {
               {&k_shared, "_shared"},         {&k_residual, "residual"},        {&k_norm, "norm"},
               {&k_call, "__call__"},          {&k_decode_rows, "DECODE_MAX_ROWS"},
               {&k_forward_codes, "forward_codes"}, {&k_forward_attn, "forward_attn"},
-              {&k_up, "up"},                  {&k_gate, "gate"}};
+              {&k_up, "up"},                  {&k_gate, "gate"},                {&k_q_proj, "q_proj"},
+              {&k_k_proj, "k_proj"},          {&k_v_proj, "v_proj"}};
   for (const auto& k : keys)
     if (!(*k.key = PyUnicode_InternFromString(k.name))) return nullptr;
   return PyModule_Create(&module);

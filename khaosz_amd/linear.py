@@ -116,6 +116,7 @@ class _SharedInput:
         self._x = self._y = None
         self._version = None
         self._served: set = set()
+        self._gone: set = set()  # siblings that run by themselves
 
     @staticmethod
     def _version_of(x: Tensor):
@@ -124,6 +125,19 @@ class _SharedInput:
         except RuntimeError:  # inference tensors carry no version counter
             return None
 
+    def holds(self, part: "QuantLinear", index: int) -> bool:
+        """Whether the sibling's codes, scales and bias are its rows of the concatenated projection: a load that assigns, a move or a tensor that was set
+        leave it storage of its own, and it runs by itself (and nothing is kept for it)."""
+        lo, whole = self.bounds[index][0], self.fused
+        for mine, rows in ((part._buffers["qweight"], whole._buffers["qweight"]), (part._buffers["w_scale"], whole._buffers["w_scale"]),
+                           (_bias_of(part), _bias_of(whole))):
+            if mine is not rows and (mine is None or rows is None or mine.dtype != rows.dtype
+                                     or mine.data_ptr() != rows.data_ptr() + lo * rows.stride(0) * rows.element_size()):
+                self._gone.add(index)
+                return False
+        self._gone.discard(index)
+        return True
+
     def output(self, x: Tensor, index: int) -> Tensor:
         if self._x is not x or self._version != self._version_of(x) or index in self._served:
             self._y = self.fused(x)
@@ -131,7 +145,7 @@ class _SharedInput:
         lo, hi = self.bounds[index]
         y = self._y[..., lo:hi]
         self._served.add(index)
-        if len(self._served) == len(self.bounds):
+        if len(self._served | self._gone) == len(self.bounds):
             self._x = self._y = None
             self._served = set()
         return y
@@ -294,7 +308,7 @@ class QuantLinear(_NativeCall):
         ``ops.rmsnorm_quant_rowwise_i8``)."""
         if x.requires_grad:
             _no_grad_guard(x)
-        if self._shared is not None and residual is None and norm is None:
+        if self._shared is not None and residual is None and norm is None and self._shared[0].holds(self, self._shared[1]):
             return self._shared[0].output(x, self._shared[1])
         # straight from where nn.Module keeps them: its __getattr__ costs half a microsecond a name
         wq, sw, bias = self._buffers["qweight"], self._buffers["w_scale"], _bias_of(self)
@@ -455,7 +469,8 @@ def fuse_shared_inputs(model: nn.Module, norms: bool = False, decode_attention: 
     """Call ``fuse_projections()`` on every module that offers it (attention and MLP blocks whose
     projections read one input); returns how many fused modules were built.  Run it after
     ``quantize_model`` and after loading weights: the fused module owns the weight storage from
-    then on (a later load reaches it where it copies, not with ``assign=True``).  Outputs stay bit-identical.  Modules of the reference itself (its GQA, MLA and MLP classes,
+    then on.  Weights that come otherwise later (a load with ``assign=True``, another projection in one's place) are noticed by
+    the next forward.  Outputs stay bit-identical.  Modules of the reference itself (its GQA, MLA and MLP classes,
     recognised by name) get the same single launch behind their own unchanged forward (``share_inputs``).
     ``norms=True`` additionally lets blocks compute
     RMSNorm and the quantisation of its output in one launch (``fuse_norm_quant()``), which
