@@ -226,7 +226,8 @@ def _settled(module: nn.Module, name: str, parts: Tuple[str, ...]) -> Optional[Q
         raise RuntimeError("the weights of a fused projection are no longer those that were fused: call the module once before it is captured")
     object.__setattr__(module, name, None)
     try:
-        module.fuse_projections()
+        with torch.inference_mode(False), torch.no_grad():  # (of tensors that a later load outside of inference mode may write to)
+            module.fuse_projections()
     except ValueError:  # (one got a bias, or another width)
         pass
     if cuda:

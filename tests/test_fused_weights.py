@@ -74,6 +74,17 @@ def test_fused_rows_follow_their_parts(how, which, make, bias):
     assert whole.qweight[lo:lo + now[which].out_dim].eq(9).all()
 
 
+@pytest.mark.parametrize("make", [_gqa, _mlp])
+def test_rows_fused_in_inference_mode_can_be_written_outside(make):
+    m, name, parts = make("cpu", True)
+    m.fuse_projections()
+    CHANGES["another part"](m, parts[1])
+    with torch.inference_mode():
+        whole = _settled(m, name, parts)
+    m.load_state_dict({k: torch.ones_like(v) for k, v in m.state_dict().items()})
+    assert whole.qweight.eq(1).all() and whole.bias.eq(1).all() and _settled(m, name, parts) is whole
+
+
 class Doubled(nn.Module):
     def __init__(self, base):
         super().__init__()
