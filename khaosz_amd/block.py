@@ -231,7 +231,7 @@ def _settled(module: nn.Module, name: str, parts: Tuple[str, ...]) -> Optional[Q
     except ValueError:  # (one got a bias, or another width)
         pass
     if cuda:
-        torch.cuda.synchronize(whole.qweight.device)  # calls on other streams may still read the rows that go, and read the new ones next
+        torch.cuda.synchronize(whole.qweight.device)  # calls on other streams may still read the rows that go
     return module.__dict__[name]
 
 
@@ -319,12 +319,12 @@ class GQA(nn.Module):
             return self.o_proj(out, residual=residual)
         return self.o_proj(out) + residual
 
-    def _project_qkv(self, x: Tensor, codes, norm) -> Tensor:
-        if self._qkv is None:
+    def _project_qkv(self, whole: Optional[QuantLinear], x: Tensor, codes, norm) -> Tensor:
+        if whole is None:
             return torch.cat([self.q_proj(x), self.k_proj(x), self.v_proj(x)], dim=-1)
         if codes is not None:
-            return self._qkv.forward_codes(codes[0], codes[1], x.dtype).view(*x.shape[:-1], -1)
-        return self._qkv(x) if norm is None else self._qkv(x, norm=norm)
+            return whole.forward_codes(codes[0], codes[1], x.dtype).view(*x.shape[:-1], -1)
+        return whole(x) if norm is None else whole(x, norm=norm)
 
     def forward(self, x: Tensor, rotary_emb: Tensor, attn_mask: Optional[Tensor] = None,
                 cache=None, codes: Optional[Tuple[Tensor, Tensor]] = None,
@@ -334,9 +334,10 @@ class GQA(nn.Module):
         un-normalised stream and the norm runs inside the fused q/k/v projection.  ``residual``:
         added to the output (in o_proj's epilogue when it is quantized)."""
         B, S, _ = x.shape
-        if _settled(self, "_qkv", ("q_proj", "k_proj", "v_proj")) is None and codes is not None:
+        whole = _settled(self, "_qkv", ("q_proj", "k_proj", "v_proj"))  # (one look: another thread may fuse it again meanwhile)
+        if whole is None and codes is not None:
             raise ValueError("a pre-quantised input needs the fused q/k/v projection")
-        if norm is not None and self._qkv is None:
+        if norm is not None and whole is None:
             x, norm = F.rms_norm(x, (x.shape[-1],), norm[0], norm[1]), None
         # The paged decode kernels know two masks: none, and per-sequence lengths (``cache.seq_lens``).  Any
         # mask TENSOR -- padding, or a caller's own -- goes to the stock attention below: the kernels would
@@ -344,7 +345,7 @@ class GQA(nn.Module):
         # different positions the caller binds ``seq_lens`` instead, as ``AutoRegressiveLM.forward`` does.)
         if (self._decode_attention and S == 1 and attn_mask is None and isinstance(cache, PagedKV) and x.is_cuda
                 and x.dtype == torch.bfloat16):
-            qkv = self._project_qkv(x, codes, norm)
+            qkv = self._project_qkv(whole, x, codes, norm)
             if cache.shared_len > 0 and ops.paged_attn_shared_positions(B, self.n_heads, self.n_kv_heads, self.head_dim, cache.total_len,
                                                                         cache.shared_len, True) > 0:
                 # the first positions of all sequences are the same pages: read once
@@ -373,7 +374,7 @@ class GQA(nn.Module):
             # or a table with unmapped pages, the one that reads everything through the page table.  A mask
             # tensor (padding) goes to the stock attention.
             nq, nkv = self.n_heads * self.head_dim, self.n_kv_heads * self.head_dim
-            qkv = self._project_qkv(x, codes, norm)
+            qkv = self._project_qkv(whole, x, codes, norm)
             start = cache.total_len - S
             direct = start == 0 and cache.all_mapped
             kc, vc = cache.k_layers[self.layer_id], cache.v_layers[self.layer_id]
@@ -393,9 +394,9 @@ class GQA(nn.Module):
             out = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), attn_mask,
                                                  enable_gqa=self.n_heads != self.n_kv_heads)
             return self._out(self._gated(out.transpose(1, 2).reshape(B, S, -1), x, norm, codes), residual)
-        if self._qkv is not None:
+        if whole is not None:
             nq, nkv = self.n_heads * self.head_dim, self.n_kv_heads * self.head_dim
-            qkv = self._project_qkv(x, codes, norm)
+            qkv = self._project_qkv(whole, x, codes, norm)
             q, k, v = qkv.split((nq, nkv, nkv), dim=-1)
         else:
             q, k, v = self.q_proj(x), self.k_proj(x), self.v_proj(x)
@@ -525,6 +526,8 @@ class MoE(nn.Module):
         with torch.inference_mode(False), torch.no_grad():  # (of tensors that a later load outside of inference mode may write to)
             up_gate, up_gate_scale = (torch.stack([torch.cat([getattr(u, n), getattr(g, n)]) for u, g, _ in parts]) for n in ("qweight", "w_scale"))
             down, down_scale = (torch.stack([getattr(d, n) for _, _, d in parts]) for n in ("qweight", "w_scale"))
+            if down.is_cuda:
+                torch.cuda.synchronize(down.device)  # whoever reads the slices next, on any stream, reads them whole
             for i, (expert, (u, g, d)) in enumerate(zip(self.routed_experts, parts)):
                 u.qweight, g.qweight, d.qweight = up_gate[i, :F_], up_gate[i, F_:], down[i]
                 u.w_scale, g.w_scale, d.w_scale = up_gate_scale[i, :F_], up_gate_scale[i, F_:], down_scale[i]
@@ -565,7 +568,7 @@ class MoE(nn.Module):
         self._experts = None
         self.fuse_experts()
         if stacks[0].is_cuda:
-            torch.cuda.synchronize(stacks[0].device)  # calls on other streams may still read the stacks that go, and read the new ones next
+            torch.cuda.synchronize(stacks[0].device)  # calls on other streams may still read the stacks that go
         return self._experts
 
     def _apply(self, fn, recurse=True):

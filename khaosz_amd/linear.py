@@ -250,6 +250,8 @@ class QuantLinear(_NativeCall):
         fused.w_scale = _joined([p.w_scale for p in parts])
         if fused.bias is not None:
             fused.bias = nn.Parameter(torch.cat([p.bias.detach() for p in parts], dim=0), requires_grad=False)
+        if fused.qweight.is_cuda:
+            torch.cuda.synchronize(fused.qweight.device)  # whoever reads the slices next, on any stream, reads them whole
         row = 0
         for p in parts:
             n = p.out_dim

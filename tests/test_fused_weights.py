@@ -221,3 +221,40 @@ def test_siblings_behind_a_shared_input_follow(how):
                 assert torch.equal(p(x), alone(x)), n
             if how != "another part":
                 assert group._x is None and group._y is None
+
+
+@pytest.mark.gpu
+def test_threads_that_share_a_block_whose_weights_move():
+    """Every call, fused or projection by projection (the same bits without fused norms), has each projection's old weights or its new ones, whole."""
+    import threading
+
+    def replace(m, n, p):
+        setattr(getattr(m, n[0]), n[1], p)
+    b, allowed = _block(False), []
+    for mask in range(16):  # any of the four replaced or not yet
+        c = _block(False)
+        for i, n in enumerate(PARTS):
+            if mask >> i & 1:
+                replace(c, n, _new(getattr(getattr(c, n[0]), n[1])))
+        allowed.append(_run(c, 3, 1, 40, False))
+    wrong, stop = [], threading.Event()
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            while not stop.is_set():
+                y = _run(b, 3, 1, 40, False)
+                if not any(torch.equal(y, a) for a in allowed):
+                    wrong.append(min(float((y.double() - a.double()).norm() / a.double().norm()) for a in allowed))
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for n in PARTS:
+        p = _new(getattr(getattr(b, n[0]), n[1]))
+        torch.cuda.synchronize()
+        replace(b, n, p)
+        _run(b, 3, 1, 40, False)
+    stop.set()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+    assert torch.equal(_run(b, 3, 1, 40, False), allowed[15])
