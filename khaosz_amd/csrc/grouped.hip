@@ -310,8 +310,8 @@ static double experts_used(int64_t R, int64_t E) { return E * (1.0 - std::exp(-(
 // Which kernel: the one whose estimated time, in us, is least.  Tiles of 16 rows: units of 32 weight rows, four to a compute unit at a time.  Walked
 // tiles: rounds of tiles (mostly whole ones: the last takes as long), each of its steps and a beginning and an end, beside the weights' way from memory.
 // Fitted to 900 random sizes of experts that are asked for alike (1 to 256 experts, 1 to 8192 tokens, K 128 to 6912), 400 of uneven ones (2 to 128 experts, 20 to
-// 600 rows each) and 350 with 0.2 to 300 rows each: 1.5, 0.9 and 1.4 % slower than the best kernel in the mean, one in twenty 12, 6 and 11 % or more.  At 200
-// other sizes, asked for as routers ask, 3.8 % in the mean, one in twenty 20 % or more (always 128 x 256 59 %, always 128 x 128 36 %).
+// 600 rows each) and 350 with 0.2 to 300 rows each: 1.5, 0.9 and 1.4 % slower than the best kernel in the mean, one in twenty 12, 6 and 11 % or more.  At 199
+// other sizes, asked for as routers ask, 3.9 % in the mean, one in twenty 20 % or more (always 128 x 256 59 %, always 128 x 128 36 %).
 // Chosen by the launch itself, from the tiles that there are, the width was 0.3 % off on the second, but three widths in one kernel cost 1 to 2 % and the
 // choice 0.5 to 1 us.
 enum { GROUPED_FEW = 1, GROUPED_WALK_256 = 2, GROUPED_WALK_128 = 3, GROUPED_WALK_64 = 4 };
